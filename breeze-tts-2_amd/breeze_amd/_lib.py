@@ -1,5 +1,5 @@
-"""ctypes binding of libbzgemv.so (the C ABI declared in include/bz_gemv.h and
-include/bz_attn.h).
+"""ctypes binding of libbzgemv.so (the C ABI declared in the headers under
+include/).
 
 torch is imported before the library is opened: both link the HIP runtime by
 its SONAME (libamdhip64.so.7), so the library binds to the runtime torch has
@@ -28,6 +28,7 @@ W_INT4_TILED, W_INT4_TILED_PAIRED, W_FP8_TILED, W_FP8_TILED_PAIRED = 4, 5, 6, 7
 EPI_NONE, EPI_SILU_GATE, EPI_RESIDUAL = 0, 1, 2
 DT_BF16, DT_F32 = 0, 1
 MASK_BOOL = 2  # include/bz_attn.h
+KV_E4M3 = 3  # include/bz_paged.h
 STEP_INV_BF16 = 256  # added to bz_step_tables' dtype
 
 EXPORTS = (
@@ -54,6 +55,9 @@ EXPORTS = (
     "bz_attn_step",
     "bz_attn_workspace",
     "bz_attn_default_split",
+    "bz_paged_rope_cache",
+    "bz_paged_attn",
+    "bz_paged_attn_workspace",
     "bz_sample_cfg",
     "bz_sample_next",
     "bz_stream_read",
@@ -108,6 +112,41 @@ def gemv_desc(*values) -> GemvDesc:
     """A descriptor from its fields' values in order (pointers as integers, 0
     for NULL)."""
     return GemvDesc.from_buffer_copy(_GEMV_RECORD.pack(*values))
+
+
+class PagedKv(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "abi_version", "T", "B", "HQ", "HKV", "D", "kv_dtype", "page_size", "num_pages", "table_width", "groups",
+        "prefix_width")] + [
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("k_page", ctypes.c_int64),
+        ("k_head", ctypes.c_int64),
+        ("k_pos", ctypes.c_int64),
+        ("v_page", ctypes.c_int64),
+        ("v_head", ctypes.c_int64),
+        ("v_pos", ctypes.c_int64),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("ld_table", ctypes.c_int64),
+        ("kv_lens", ctypes.c_void_p),
+        ("q_starts", ctypes.c_void_p),
+        ("prefix_table", ctypes.c_void_p),
+        ("ld_prefix", ctypes.c_int64),
+        ("prefix_lens", ctypes.c_void_p),
+        ("prefix_seqs", ctypes.c_void_p),
+    ]
+
+
+_PAGED_RECORD = struct.Struct("@" + "".join(_CODES[t] for _, t in PagedKv._fields_))
+assert _PAGED_RECORD.size == ctypes.sizeof(PagedKv)
+
+
+def paged_kv(*values) -> PagedKv:
+    """A bz_paged_kv from its fields' values in order (pointers as integers, 0
+    for NULL)."""
+    return PagedKv.from_buffer_copy(_PAGED_RECORD.pack(*values))
 
 
 class BzError(RuntimeError):
@@ -171,6 +210,13 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.bz_attn_workspace.argtypes = [i32, i32, i32, i32, i32]
     lib.bz_attn_default_split.restype = ctypes.c_int32
     lib.bz_attn_default_split.argtypes = [i32]
+    lib.bz_paged_rope_cache.restype = ctypes.c_int
+    lib.bz_paged_rope_cache.argtypes = [ctypes.POINTER(PagedKv), vp, i64, vp, vp, f32, vp, vp, i32, i64, i64, vp, vp,
+                                        i64, vp]
+    lib.bz_paged_attn.restype = ctypes.c_int
+    lib.bz_paged_attn.argtypes = [ctypes.POINTER(PagedKv), vp, i64, f32, vp, ctypes.c_size_t, vp, i64, vp]
+    lib.bz_paged_attn_workspace.restype = ctypes.c_size_t
+    lib.bz_paged_attn_workspace.argtypes = [ctypes.POINTER(PagedKv)]
     lib.bz_stream_read.restype = ctypes.c_int
     lib.bz_stream_read.argtypes = [vp, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_uint32, vp, vp]
     lib.bz_shared_read.restype = ctypes.c_int

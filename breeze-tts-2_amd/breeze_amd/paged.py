@@ -1,0 +1,310 @@
+"""Operators over a paged key/value cache (include/bz_paged.h).
+
+A server that runs requests of different lengths keeps their keys and values in
+pages of one pool instead of a static [B, HKV, S, D] cache each:
+
+``paged_rope_cache``         q/k RMSNorm + RoPE of the new tokens, their keys and
+                             values into the pages, rotated queries out
+``paged_attention``          attention of each sequence's newest rows over its pages
+``shared_prefix_attention``  the same where sequences begin with a shared prompt (a
+                             voice), whose pages are stored and read once
+
+Common arguments:
+
+k_pages, v_pages  [pages, HKV, page_size, D] bf16, or float8_e4m3fn with k_scale /
+                  v_scale (fp32 [HKV]: a code stands for code * scale).  Any strides with
+                  contiguous D, so a [pages, page_size, HKV, D] pool is passed as its
+                  transpose(1, 2).  page_size a power of two, 16 .. 4096.
+block_table       int32 [B, W]: position j of sequence b lies in page
+                  block_table[b, j // page_size].  Entries past a sequence's length are not
+                  read; one outside [0, pages) is a page that is not there (not written,
+                  not attended).
+kv_lens           int32 [B], the new rows included
+q_starts          int32 [B + 1]: sequence b has the rows q_starts[b] .. q_starts[b + 1] - 1,
+                  its newest positions in order; None: one row each.  Rows of no sequence
+                  are not touched: in a tensor that the call allocates they hold anything.
+
+Lengths, tables and starts are read on the device: no call synchronizes, and a
+captured graph follows them.  Calls may run on several streams at once; a
+workspace belongs to its call.
+"""
+
+from __future__ import annotations
+
+import functools
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import DT_BF16, DT_F32, KV_E4M3
+
+__all__ = ["paged_rope_cache", "paged_attention", "shared_prefix_attention"]
+
+_KV = {torch.bfloat16: DT_BF16, torch.float8_e4m3fn: KV_E4M3}
+_CS = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
+
+
+def _gpu(name: str, t: torch.Tensor, index: int) -> None:
+    at = t.get_device()  # -1 on the CPU
+    if at == index and at >= 0:
+        return
+    if at < 0:
+        raise RuntimeError(f"{name} must be a GPU tensor (got {t.device}); the HIP path has no CPU fallback")
+    raise RuntimeError(f"{name} is on {t.device}, expected cuda:{index}")
+
+
+def _ints(name: str, t: torch.Tensor, shape: tuple, index: int) -> int:
+    """The pointer of an int32 tensor of this shape with unit stride in its last dimension."""
+    _gpu(name, t, index)
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name} must have unit stride in its last dimension")
+    return t.data_ptr()
+
+
+def _table(name: str, t: torch.Tensor, index: int) -> tuple:
+    """(rows, width, pointer, row stride) of a page table."""
+    if t.dim() != 2 or t.shape[1] < 1:
+        raise ValueError(f"{name} must be [rows, pages] with at least one page, got {list(t.shape)}")
+    p = _ints(name, t, t.shape, index)
+    rows, width = t.shape
+    ld = t.stride(0) if rows > 1 else width
+    if ld < width:
+        raise ValueError(f"{name} must not have overlapping rows")
+    return rows, width, p, ld
+
+
+def _strides(t: torch.Tensor) -> tuple:
+    """Element strides of a pool; those of dimensions of size 1 are not used and count as D."""
+    if t.stride(3) != 1:
+        raise ValueError("a position's D elements must be contiguous")
+    return tuple(s if n > 1 else t.shape[3] for s, n in zip(t.stride()[:3], t.shape))
+
+
+def _cache(T: int, HQ: int, k_pages, v_pages, k_scale, v_scale, block_table, kv_lens, q_starts, index: int) -> tuple:
+    """The fields of bz_paged_kv without the prefixes', checked."""
+    _gpu("k_pages", k_pages, index)
+    _gpu("v_pages", v_pages, index)
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+        raise ValueError("k_pages and v_pages must both be [pages, HKV, page_size, D] of one dtype")
+    kind = _KV.get(k_pages.dtype)
+    if kind is None:
+        raise TypeError(f"pages must be bfloat16 or float8_e4m3fn, got {k_pages.dtype}")
+    pages, HKV, ps, D = k_pages.shape
+    if kind == KV_E4M3:
+        if k_scale is None or v_scale is None:
+            raise ValueError("an e4m3 cache comes with k_scale and v_scale")
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            _gpu(name, t, index)
+            if t.dtype != torch.float32 or t.shape != (HKV,) or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous float32 [{HKV}] tensor")
+        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+    else:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError("a bf16 cache has no scales")
+        ks = vs = 0
+    B, width, table, ld = _table("block_table", block_table, index)
+    lens = _ints("kv_lens", kv_lens, (B,), index)
+    if q_starts is not None:
+        starts = _ints("q_starts", q_starts, (B + 1,), index)
+    elif T == B:
+        starts = 0
+    else:
+        raise ValueError(f"{T} rows for {B} sequences: q_starts says which are whose")
+    return ((_lib.ABI_VERSION, T, B, HQ, HKV, D, kind, ps, pages, width),
+            (k_pages.data_ptr(), v_pages.data_ptr(), *_strides(k_pages), *_strides(v_pages), ks, vs, table, ld, lens,
+             starts))
+
+
+_NO_PREFIX = (0, 0), (0, 0, 0, 0)
+
+
+def _prefixes(table, lens, seqs, B: int, index: int) -> tuple:
+    if table.dim() == 1:
+        table = table.unsqueeze(0)
+    groups, width, p, ld = _table("prefix_table", table, index)
+    if groups < 1:
+        raise ValueError("prefix_table needs at least one prefix")
+    n = _ints("prefix_lens", lens, (groups,), index)
+    if seqs is not None:
+        at = _ints("prefix_seqs", seqs, (groups + 1,), index)
+    elif groups == 1:
+        at = 0
+    else:
+        raise ValueError("prefix_seqs says which sequences begin with which prefix")
+    return (groups, width), (p, ld, n, at)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(sizes: tuple) -> int:
+    d = _lib.paged_kv(*sizes, *(0,) * 18)
+    return int(_lib.lib().bz_paged_attn_workspace(d))
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy whose rows begin at multiples of 16 bytes and do not overlap."""
+    if t.data_ptr() % 16 or (t.shape[0] > 1 and (t.stride(0) * t.element_size() % 16 or t.stride(0) < t.shape[1])):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _heads(name: str, t: torch.Tensor) -> torch.Tensor:
+    """[T, HQ, D] -> [T, HQ * D] with unit column stride."""
+    if t.dim() != 3 or t.dtype != torch.bfloat16:
+        raise ValueError(f"{name} must be a bf16 [rows, HQ, D] tensor")
+    if (t.stride(2) != 1 and t.shape[2] > 1) or (t.stride(1) != t.shape[2] and t.shape[1] > 1):
+        t = t.contiguous()
+    return t.as_strided((t.shape[0], t.shape[1] * t.shape[2]), (t.stride(0), 1))
+
+
+def _result(name: str, t: Optional[torch.Tensor], shape: tuple, dev, index: int, *inputs) -> torch.Tensor:
+    if t is None:
+        return torch.empty(shape, device=dev, dtype=torch.bfloat16)
+    _gpu(name, t, index)
+    inner = 1
+    for n, s in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if n > 1 and s != inner:
+            raise ValueError(f"{name} must have contiguous rows")
+        inner *= n
+    if t.dtype != torch.bfloat16 or t.shape != shape:
+        raise ValueError(f"{name} must be a bf16 {list(shape)} tensor")
+    if t.data_ptr() % 16 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < inner)):
+        raise ValueError(f"{name} needs rows at multiples of 16 bytes that do not overlap")
+    if t.numel():
+        end = t.data_ptr() + 2 * ((t.shape[0] - 1) * t.stride(0) + inner)
+        for x in inputs:
+            if x.numel() and x.data_ptr() < end and t.data_ptr() < x.data_ptr() + x.element_size() * (
+                    (x.shape[0] - 1) * x.stride(0) + x[0].numel()):
+                raise ValueError(f"{name} must not overlap the input")
+    return t
+
+
+def _call(index: int, f, *args) -> None:
+    """f(*args, stream) with the tensors' device current."""
+    if torch._C._cuda_getDevice() == index:
+        rc = f(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = f(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        raise _lib.BzError(rc, f.__name__)
+
+
+def paged_rope_cache(qkv, cos, sin, k_pages, v_pages, block_table, kv_lens, HQ: int, q_starts=None, *, positions=None,
+                     q_norm_w=None, k_norm_w=None, eps: float = 1e-6, k_scale=None, v_scale=None,
+                     q_out=None) -> torch.Tensor:
+    """Per-head q/k RMSNorm and rotate-half RoPE of the rows' qkv (bf16
+    [T, (HQ + 2 HKV) D], q heads, k heads, v heads); their keys and values into
+    the pages (e4m3: rounded once, saturated); q as bf16 [T, HQ, D] (returned).
+    What qkv_rope_cache does for a static cache, for any number of rows of
+    each sequence.
+
+    cos, sin: bf16 or fp32 [P, D], the rotary table.  Row t uses row positions[t]
+    (int64 [T]), or without positions its own position in the sequence's pages; behind
+    a shared prefix pass positions.  A row outside the table is written to no page
+    and its q is zero."""
+    index = qkv.get_device()
+    _gpu("qkv", qkv, index)
+    if qkv.dim() != 2 or qkv.dtype != torch.bfloat16:
+        raise ValueError("qkv must be a bf16 [rows, (HQ + 2 HKV) D] tensor")
+    T = qkv.shape[0]
+    sizes, refs = _cache(T, HQ, k_pages, v_pages, k_scale, v_scale, block_table, kv_lens, q_starts, index)
+    HKV, D = sizes[4], sizes[5]
+    if HQ < 1 or qkv.shape[1] != (HQ + 2 * HKV) * D:
+        raise ValueError(f"qkv width {qkv.shape[1]} is not ({HQ} + 2 * {HKV}) heads of {D}")
+    if qkv.stride(1) != 1:
+        qkv = qkv.contiguous()
+    qkv = _rows16(qkv)
+    for name, t in (("cos", cos), ("sin", sin)):
+        _gpu(name, t, index)
+    if cos.dim() == 3 and cos.shape[0] == 1:
+        cos, sin = cos[0], sin[0] if sin.dim() == 3 else sin
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.shape[1] != D or cos.shape[0] < 1:
+        raise ValueError(f"cos and sin must both be [positions, {D}] of one dtype")
+    cs = _CS.get(cos.dtype)
+    if cs is None:
+        raise TypeError(f"cos and sin must be bfloat16 or float32, got {cos.dtype}")
+    if cos.stride() != sin.stride() or cos.stride(1) != 1 or (cos.shape[0] > 1 and cos.stride(0) % 8) \
+            or cos.data_ptr() % 16 or sin.data_ptr() % 16:
+        cos, sin = (t.clone(memory_format=torch.contiguous_format) for t in (cos, sin))
+    at = 0
+    if positions is not None:
+        _gpu("positions", positions, index)
+        if positions.dtype != torch.int64 or positions.shape != (T,) or not positions.is_contiguous():
+            raise ValueError(f"positions must be a contiguous int64 [{T}] tensor")
+        at = positions.data_ptr()
+    if (q_norm_w is None) != (k_norm_w is None):
+        raise ValueError("q_norm_w and k_norm_w come together")
+    qn = kn = None
+    if q_norm_w is not None:
+        qn, kn = q_norm_w, k_norm_w
+        for name, t in (("q_norm_w", qn), ("k_norm_w", kn)):
+            _gpu(name, t, index)
+            if t.numel() != D:
+                raise ValueError(f"{name} must have {D} elements")
+        qn, kn = (w if w.dtype == torch.bfloat16 and w.is_contiguous() and w.data_ptr() % 16 == 0
+                  else w.to(torch.bfloat16).clone(memory_format=torch.contiguous_format) for w in (qn, kn))
+    q = _result("q_out", q_out, (T, HQ, D), qkv.device, index, qkv)
+    if T == 0 or sizes[2] == 0:
+        return q
+    d = _lib.paged_kv(*sizes, *_NO_PREFIX[0], *refs, *_NO_PREFIX[1])
+    _call(index, _lib.lib().bz_paged_rope_cache, d, qkv.data_ptr(), _ld(qkv), None if qn is None else qn.data_ptr(),
+          None if kn is None else kn.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), cs,
+          cos.stride(0) if cos.shape[0] > 1 else D, cos.shape[0], at, q.data_ptr(),
+          q.stride(0) if T > 1 else HQ * D)
+    return q
+
+
+def _attention(q, k_pages, v_pages, block_table, kv_lens, q_starts, prefix, scale, k_scale, v_scale, out):
+    index = q.get_device()
+    _gpu("q", q, index)
+    dev = q.device
+    q2 = _rows16(_heads("q", q))
+    T, HQ, D = q.shape
+    sizes, refs = _cache(T, HQ, k_pages, v_pages, k_scale, v_scale, block_table, kv_lens, q_starts, index)
+    if D != sizes[5]:
+        raise ValueError(f"q has heads of {D}, the pages of {sizes[5]}")
+    psizes, prefs = _NO_PREFIX if prefix is None else _prefixes(*prefix, sizes[2], index)
+    out = _result("out", out, (T, HQ * D), dev, index, q2)
+    if T == 0 or sizes[2] == 0:
+        return out
+    sizes += psizes
+    n = _workspace_bytes(sizes)
+    ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
+    _call(index, _lib.lib().bz_paged_attn, _lib.paged_kv(*sizes, *refs, *prefs), q2.data_ptr(), _ld(q2),
+          D ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), n, out.data_ptr(), _ld(out))
+    return out
+
+
+def paged_attention(q, k_pages, v_pages, block_table, kv_lens, q_starts=None, *, scale: Optional[float] = None,
+                    k_scale=None, v_scale=None, out=None) -> torch.Tensor:
+    """softmax(scale q k^T) v of every row over its sequence's positions up to the
+    row's own: q bf16 [T, HQ, D], rotated -> bf16 [T, HQ * D].  Query head h
+    reads key/value head h // (HQ / HKV).  One row per sequence is a decode step,
+    several are drafted tokens, a prompt or a chunk of one.  scale: D ** -0.5
+    unless given, positive.  A row that attends nothing is zero; keys and values that
+    a row does not attend have no part in it, whatever they hold."""
+    return _attention(q, k_pages, v_pages, block_table, kv_lens, q_starts, None, scale, k_scale, v_scale, out)
+
+
+def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_lens, block_table, kv_lens, q_starts=None,
+                            prefix_seqs=None, *, scale: Optional[float] = None, k_scale=None, v_scale=None,
+                            out=None) -> torch.Tensor:
+    """paged_attention for sequences that begin with a shared prefix: prefix g, of
+    prefix_lens[g] positions (int32 [groups]) in the pages prefix_table[g] (int32
+    [groups, W'], or [W'] for one), comes before the own positions of the
+    sequences prefix_seqs[g] .. prefix_seqs[g + 1] - 1 (int32 [groups + 1]; None with one
+    prefix: of all).  Every row attends its whole prefix, then its sequence's own
+    positions as in paged_attention; kv_lens and block_table are about the own
+    positions alone, and kv_lens may leave a row none of them.  The prefix's keys and
+    values are read once for all rows of its sequences."""
+    return _attention(q, k_pages, v_pages, block_table, kv_lens, q_starts, (prefix_table, prefix_lens, prefix_seqs),
+                      scale, k_scale, v_scale, out)
