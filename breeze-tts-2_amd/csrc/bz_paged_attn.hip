@@ -1,110 +1,118 @@
 // Attention of each sequence's newest rows over a paged key/value cache
-// (include/bz_paged.h), with shared prefixes.
-//
-//   s_j = scale q . k_j,  out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  m = max_j s_j
-//
-// over the keys a row attends, in one pass: with m the maximum so far, the sum l
-// and the accumulator are rescaled by e^(m_old - m) as m grows (kept as exponents
-// of 2, scale log2(e) s).  The simple form: a wave per (row, query head), a key
-// per lane for the scores, D / 64 columns per lane for the values.
-#include "bz_paged_kv.h"
+// (include/bz_paged.h), with shared prefixes: the launches.
+#include "bz_paged_attn.h"
+#include "bz_paged_stream.h"
 
 namespace bz {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kPagedWorkgroups = 1024;  // that the keys are cut for
 
-template <int D, bool F8>
-__global__ void __launch_bounds__(256) paged_attn_bf16_row(PagedKv c, const uint16_t* q, int64_t ld_q, float scale,
-                                                           uint16_t* out, int64_t ld_out) {
-    constexpr int DL = D / 64;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int t = blockIdx.x, h = blockIdx.y * 4 + wave;
+// The chunks' parts of a row, merged in the keys' order: its prefix's, then its
+// own.  Four columns of a head to a thread.
+template <int D>
+__global__ void __launch_bounds__(256) paged_attn_bf16_join(PagedKv c, PagedAttn a, int M, bool f8) {
+    const int t = blockIdx.x, lane = threadIdx.x & 63;
     const int b = seq_of_row(c, t, lane);
     if (b >= c.B) return;
-    const RowRange r = seq_rows(c, b);
-    if (t < r.first || t >= r.end || h >= c.HQ) return;
+    const PagedSeg own = paged_seg(c, b);
+    const int row = t - own.first;
+    if (row < 0 || row >= own.rows) return;
+    const int pre = prefix_of_seq(c, b, lane);
+    const int item = blockIdx.y * 256 + threadIdx.x;
+    const int h = item / (D / 4), d = 4 * (item - h * (D / 4));
+    if (h >= c.HQ) return;
     const int head = h / c.G;
-    const int pos = max(c.kv_lens[b], 0) - (r.end - t);
-    int group = -1;
-    if (c.groups > 0) {
-        int g = 0;
-        if (c.prefix_seqs)
-            for (; g < c.groups; ++g)
-                if (c.prefix_seqs[g] <= b && b < c.prefix_seqs[g + 1]) break;
-        if (g < c.groups) group = g;
-    }
-    const float ks = F8 ? c.k_scale[head] : 1.0f;
-    const uint16_t* qr = q + (int64_t)t * ld_q + (int64_t)h * D;
-    float m = -INFINITY, l = 0.0f, acc[DL] = {};
-    bool seen = false;
-    for (int part = 0; part < 2; ++part) {
-        const int32_t* table = part ? c.table + (int64_t)b * c.ld_table : c.prefix_table + (int64_t)group * c.ld_prefix;
-        int n = 0;
-        if (part)
-            n = min(pos + 1, c.width << c.shift);
-        else if (group >= 0)
-            n = min(c.prefix_lens[group], c.prefix_width << c.shift);
-        for (int j0 = 0; j0 < n; j0 += 64) {
-            const int j = j0 + lane;
-            const int page = j < n ? table[j >> c.shift] : -1;
-            const bool there = (unsigned)page < (unsigned)c.num_pages;
-            const int at = j & ((1 << c.shift) - 1);
-            float s = -INFINITY;
-            if (there) {
-                const char* kr = c.k + page * c.k_page + head * c.k_head + at * c.k_pos;
-                s = 0.0f;
-                for (int d = 0; d < D; ++d) {
-                    float kv;
-                    if constexpr (F8)
-                        kv = __builtin_amdgcn_cvt_f32_fp8((int)reinterpret_cast<const uint8_t*>(kr)[d], 0);
-                    else
-                        kv = bf16_to_f32(reinterpret_cast<const uint16_t*>(kr)[d]);
-                    s += bf16_to_f32(qr[d]) * kv;
-                }
-                s = s * ks * scale * kLog2e;
+
+    float m = -INFINITY, l = 0.0f, o[4] = {};
+    for (int part = pre >= 0 ? 0 : 1; part < 2; ++part) {
+        const PagedSeg g = part ? own : paged_seg(c, c.B + pre);
+        const int k = (t - g.first) * c.G + (h - head * c.G), tile = k / M;
+        const int2 note = a.notes[tile_note(c, g, tile, M)];
+        if (c.groups == 0 && g.keys <= note.y) return;  // written by its only slot
+        const int limit = row_limit(g, part ? max(c.kv_lens[b], 0) : 0, part, row);
+        const int n = max(1, (int)(((unsigned)limit + note.y - 1) / (unsigned)note.y));
+        const int64_t at = ((int64_t)note.x * c.HKV + head) * M + (k - tile * M), step = (int64_t)c.HKV * M;
+        constexpr int U = 4;
+        for (int s0 = 0; s0 < n; s0 += U) {
+            float2 x[U];
+            float4 v[U];
+#pragma unroll
+            for (int e = 0; e < U; ++e) {
+                const int64_t i = at + min(s0 + e, n - 1) * step;
+                x[e] = a.ml[i];
+                v[e] = *reinterpret_cast<const float4*>(a.part + i * D + d);
             }
-            const float mn = fmaxf(m, wave_max(s));
+            float mn = m;
+#pragma unroll
+            for (int e = 0; e < U; ++e) mn = fmaxf(mn, x[e].x);
             const float ms = mn == -INFINITY ? 0.0f : mn;
-            const float f = exp2f(m - ms), p = there ? exp2f(s - ms) : 0.0f;
+            const float f = mn == -INFINITY ? 1.0f : pg_exp2(m - ms);
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] *= f;
             m = mn;
-            l = l * f + wave_sum(p);
-            for (int e = 0; e < DL; ++e) acc[e] *= f;
-            uint64_t live = __ballot(there);
-            seen |= live != 0;
-            for (; live; live &= live - 1) {
-                const int k = __builtin_ctzll(live);
-                const float pk = __shfl(p, k, 64);
-                const int pg = __shfl(page, k, 64), ak = (j0 + k) & ((1 << c.shift) - 1);
-                const char* vr = c.v + pg * c.v_page + head * c.v_head + ak * c.v_pos;
-                for (int e = 0; e < DL; ++e) {
-                    float v;
-                    if constexpr (F8)
-                        v = __builtin_amdgcn_cvt_f32_fp8((int)reinterpret_cast<const uint8_t*>(vr)[DL * lane + e], 0);
-                    else
-                        v = bf16_to_f32(reinterpret_cast<const uint16_t*>(vr)[DL * lane + e]);
-                    acc[e] += pk * v;
-                }
+#pragma unroll
+            for (int e = 0; e < U; ++e) {
+                if (s0 + e >= n) break;
+                const float w = mn == -INFINITY ? 1.0f : pg_exp2(x[e].x - ms);
+                l += x[e].y * w;
+                o[0] += v[e].x * w;
+                o[1] += v[e].y * w;
+                o[2] += v[e].z * w;
+                o[3] += v[e].w * w;
             }
         }
     }
-    const float vs = F8 ? c.v_scale[head] : 1.0f;
-    for (int e = 0; e < DL; ++e)
-        out[(int64_t)t * ld_out + (int64_t)h * D + DL * lane + e] = f32_to_bf16(seen ? acc[e] / l * vs : 0.0f);
+    const float f = m == -INFINITY ? (l > 0.0f ? __builtin_nanf("") : 0.0f) : 1.0f / l * (f8 ? c.v_scale[head] : 1.0f);
+    *reinterpret_cast<uint2*>(a.out + (int64_t)t * a.ld_out + (int64_t)h * D + d) =
+        make_uint2(pack_bf16x2(o[0] * f, o[1] * f), pack_bf16x2(o[2] * f, o[3] * f));
 }
 
-template <bool F8>
-static void launch_paged(int D, const PagedKv& c, const uint16_t* q, int64_t ld_q, float scale, uint16_t* out,
-                         int64_t ld_out, hipStream_t st) {
-    const dim3 grid(c.T, (c.HQ + 3) / 4), block(256);
-    switch (D) {
-        case 64:
-            hipLaunchKernelGGL((paged_attn_bf16_row<64, F8>), grid, block, 0, st, c, q, ld_q, scale, out, ld_out);
-            break;
-        case 128:
-            hipLaunchKernelGGL((paged_attn_bf16_row<128, F8>), grid, block, 0, st, c, q, ld_q, scale, out, ld_out);
-            break;
-        default:
-            hipLaunchKernelGGL((paged_attn_bf16_row<256, F8>), grid, block, 0, st, c, q, ld_q, scale, out, ld_out);
+struct PagedPlan {
+    int M;       // rows of a tile
+    int target;  // slots of one key/value head
+    int64_t slots, notes;
+    bool join;
+    size_t ml_at, notes_at, bytes;  // of the workspace
+};
+
+// Rows of a tile by what a segment has on average.
+static PagedPlan paged_plan(const bz_paged_kv* d) {
+    PagedPlan p = {};
+    const int G = d->HQ / d->HKV;
+    const int64_t segs = d->groups > 0 ? std::min(d->B, d->groups) : d->B;
+    const int64_t rows = ((int64_t)d->T + segs - 1) / segs * G;
+    p.M = rows <= 16 || d->D == 256 ? 16 : 32;
+    p.target = std::max(1, kPagedWorkgroups / d->HKV);
+    const PagedBounds b = paged_bounds(d, p.M, p.target);
+    p.notes = b.notes;
+    p.join = d->groups > 0 || (int64_t)d->table_width * d->page_size > kMinChunk;
+    p.slots = p.join ? b.slots : b.notes;
+    const size_t rows_all = (size_t)p.slots * d->HKV * p.M;
+    p.ml_at = p.join ? rows_all * d->D * sizeof(float) : 0;
+    p.notes_at = p.ml_at + (p.join ? rows_all * sizeof(float2) : 0);
+    p.bytes = p.notes_at + (size_t)p.notes * sizeof(int2);
+    return p;
+}
+
+template <int D, bool F8>
+static void launch_stream(const PagedKv& c, const PagedAttn& a, int M, hipStream_t st) {
+    const dim3 grid((unsigned)(a.slots * c.HKV)), block(64 * kStreamWaves);
+    if (M == 16)
+        hipLaunchKernelGGL((paged_attn_bf16_stream<D, F8, 1>), grid, block, 0, st, c, a);
+    else if constexpr (D < 256)
+        hipLaunchKernelGGL((paged_attn_bf16_stream<D, F8, 2>), grid, block, 0, st, c, a);
+}
+
+template <int D>
+static void launch_attn(const PagedKv& c, const PagedAttn& a, const PagedPlan& p, bool f8, hipStream_t st) {
+    if (f8)
+        launch_stream<D, true>(c, a, p.M, st);
+    else
+        launch_stream<D, false>(c, a, p.M, st);
+    if (p.join) {
+        const int per = c.HQ * (D / 4);
+        hipLaunchKernelGGL((paged_attn_bf16_join<D>), dim3(c.T, (per + 255) / 256), dim3(256), 0, st, c, a, p.M, f8);
     }
 }
 
@@ -113,8 +121,7 @@ static void launch_paged(int D, const PagedKv& c, const uint16_t* q, int64_t ld_
 using namespace bz;
 
 extern "C" size_t bz_paged_attn_workspace(const bz_paged_kv* kv) {
-    if (paged_check_sizes(kv) != BZ_OK) return 0;
-    return 0;
+    return paged_check_sizes(kv) == BZ_OK ? paged_plan(kv).bytes : 0;
 }
 
 extern "C" int bz_paged_attn(const bz_paged_kv* kv, const void* q, int64_t ld_q, float scale, void* workspace,
@@ -125,16 +132,28 @@ extern "C" int bz_paged_attn(const bz_paged_kv* kv, const void* q, int64_t ld_q,
     if (!q || !out || !(scale > 0.0f) || scale > 3.0e38f) return BZ_ERR_INVALID_ARG;
     const int D = kv->D;
     if (ld_q < (int64_t)c.HQ * D || ld_out < (int64_t)c.HQ * D) return BZ_ERR_SHAPE;
-    if (!aligned_to(q, 16) || !aligned_to(out, 16) || ld_q % 8 || ld_out % 8) return BZ_ERR_ALIGNMENT;
-    const size_t need = bz_paged_attn_workspace(kv);
-    if (need && (!workspace || workspace_bytes < need)) return BZ_ERR_INVALID_ARG;
-    if (!aligned_to(workspace, 16)) return BZ_ERR_ALIGNMENT;
+    if (!aligned_to(q, 16) || !aligned_to(out, 16) || ld_q % 8 || ld_out % 8 || !aligned_to(workspace, 16))
+        return BZ_ERR_ALIGNMENT;
+    const PagedPlan p = paged_plan(kv);
+    if (p.slots * c.HKV > 0x7FFFFFFF) return BZ_ERR_UNSUPPORTED;
+    if (!workspace || workspace_bytes < p.bytes) return BZ_ERR_INVALID_ARG;
+    char* ws = static_cast<char*>(workspace);
+    const PagedAttn a = {static_cast<const uint16_t*>(q),
+                         ld_q,
+                         scale,
+                         static_cast<uint16_t*>(out),
+                         ld_out,
+                         (float)p.target,
+                         p.slots,
+                         reinterpret_cast<float*>(ws),
+                         reinterpret_cast<float2*>(ws + p.ml_at),
+                         reinterpret_cast<int2*>(ws + p.notes_at)};
+    const bool f8 = kv->kv_dtype == BZ_KV_E4M3;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const uint16_t* qp = static_cast<const uint16_t*>(q);
-    uint16_t* op = static_cast<uint16_t*>(out);
-    if (kv->kv_dtype == BZ_KV_E4M3)
-        launch_paged<true>(D, c, qp, ld_q, scale, op, ld_out, st);
-    else
-        launch_paged<false>(D, c, qp, ld_q, scale, op, ld_out, st);
+    switch (D) {
+        case 64: launch_attn<64>(c, a, p, f8, st); break;
+        case 128: launch_attn<128>(c, a, p, f8, st); break;
+        default: launch_attn<256>(c, a, p, f8, st); break;
+    }
     return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
 }
