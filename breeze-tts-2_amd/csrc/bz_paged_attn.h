@@ -25,6 +25,16 @@ __device__ __forceinline__ pg_f32x4 pg_mfma16(u32x4 a, u32x4 b, pg_f32x4 c) {
                                                   0, 0, 0);
 }
 
+typedef float pg_f32x16 __attribute__((ext_vector_type(16)));
+
+// D = A B + C, 32x32x16: A[i][k] in lane i + 32 (k/8) element k%8, B[k][j] in
+// lane j + 32 (k/8) element k%8, D[i][j] in lane j + 32 ((i/4)%2) element
+// 4 (i/8) + i%4.
+__device__ __forceinline__ pg_f32x16 pg_mfma32(u32x4 a, u32x4 b, pg_f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(pg_bf16x8, a), __builtin_bit_cast(pg_bf16x8, b), c,
+                                                  0, 0, 0);
+}
+
 // 2^x with the hardware instruction alone (below 2^-126 it gives zero).
 __device__ __forceinline__ float pg_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -47,6 +57,30 @@ __device__ __forceinline__ int row_limit(const PagedSeg& g, int kv_len, bool own
     return own ? min(max(kv_len - g.rows + row + 1, 0), g.keys) : g.keys;
 }
 
+// A workgroup's part of the work: a slot with the keys of its chunk that its rows attend.
+struct PagedWork {
+    PagedSlot u;
+    bool own;     // a sequence's own positions, not a shared prefix
+    int kv_len;
+    int rows;     // query rows of the tile, head by head
+    int begin, end;  // keys of the chunk that a row of the tile attends
+    int all;      // the keys before it are attended by all rows
+};
+__device__ __forceinline__ bool paged_work(const PagedKv& c, int M, float target, int slot, int lane, PagedWork& w) {
+    w.u = paged_slot(c, M, target, slot, lane);
+    if (!w.u.any) return false;
+    const PagedSeg& g = w.u.seg;
+    w.own = g.seq < c.B;
+    w.kv_len = w.own ? max(c.kv_lens[g.seq], 0) : 0;
+    const int first = w.u.tile * M;
+    w.rows = min(g.rows * c.G - first, M);
+    const int tile_end = row_limit(g, w.kv_len, w.own, (first + w.rows - 1) / c.G);
+    w.begin = w.u.split * w.u.chunk;
+    w.end = min(w.begin + w.u.chunk, tile_end);
+    w.all = row_limit(g, w.kv_len, w.own, first / c.G);
+    return w.u.split == 0 || w.begin < tile_end;  // else a chunk behind the tile's last row
+}
+
 // One 16-position piece of a segment's keys, none of whose rows is read beyond `n`.
 struct PagedPiece {
     __amdgpu_buffer_rsrc_t k, v;
@@ -67,10 +101,9 @@ __device__ __forceinline__ PagedPiece paged_piece(const PagedKv& c, const char* 
     return p;
 }
 
-// Sixteen e4m3 codes as bf16 (exact).
-__device__ __forceinline__ void f8_widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    lo = fp8x2_bf16<false>(w);
-    hi = fp8x2_bf16<true>(w);
+// Eight e4m3 codes as bf16 (exact).
+__device__ __forceinline__ u32x4 f8_widen(uint32_t lo, uint32_t hi) {
+    return u32x4{fp8x2_bf16<false>(lo), fp8x2_bf16<true>(lo), fp8x2_bf16<false>(hi), fp8x2_bf16<true>(hi)};
 }
 
 // Whether one of two bf16 is infinite or NaN.
@@ -79,20 +112,65 @@ __device__ __forceinline__ bool not_finite2(uint32_t w) {
 }
 // Whether one of four e4m3 codes is NaN (they have no infinities).
 __device__ __forceinline__ bool nan_f8x4(uint32_t w) { return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0; }
-// The halves of w that `f` holds for (a function of 16 bits), as ones; else zeros.
-template <typename F>
-__device__ __forceinline__ uint32_t ones2(uint32_t w, F f) {
-    return (f(w & 0xFFFFu) ? 0x3F80u : 0u) | (f(w >> 16) ? 0x3F800000u : 0u);
-}
-__device__ __forceinline__ uint32_t finite2(uint32_t w) {
-    return ((w & 0x7F80u) == 0x7F80u ? 0u : w & 0xFFFFu) | ((w & 0x7F800000u) == 0x7F800000u ? 0u : w & 0xFFFF0000u);
-}
-
-// What infinities and NaN among the attended values of a column make of its sum,
-// given how many there are of each.
-__device__ __forceinline__ float taint(float nan, float pos, float neg) {
-    if (nan > 0.0f || (pos > 0.0f && neg > 0.0f)) return __builtin_nanf("");
-    return pos > 0.0f ? INFINITY : (neg > 0.0f ? -INFINITY : 0.0f);
+// The rows of a workgroup's tile one by one, a wave to a row and a key to a lane: for a
+// tile in which a value that is not finite belongs to a key that only some of the rows
+// attend (0 times it is NaN, so a matrix product would carry it into the others).
+// Not fast; such a batch has a broken sequence in it.
+template <int D, bool F8>
+__device__ __forceinline__ void paged_rows_apart(const PagedKv& c, const PagedAttn& a, const PagedWork& w, int slot,
+                                                 int head, int M, int wave, int waves, int lane) {
+    constexpr int DL = D / 64;
+    const PagedSeg& g = w.u.seg;
+    const int32_t* table = w.own ? c.table + (int64_t)g.seq * c.ld_table
+                                 : c.prefix_table + (int64_t)(g.seq - c.B) * c.ld_prefix;
+    const float sc = a.scale * kPagedLog2e * (F8 ? c.k_scale[head] : 1.0f), vs = F8 ? c.v_scale[head] : 1.0f;
+    const bool whole = w.u.splits == 1 && c.groups == 0;
+    for (int rr = wave; rr < w.rows; rr += waves) {
+        const int k = w.u.tile * M + rr, row = k / c.G, h = head * c.G + (k - row * c.G);
+        const uint16_t* q = a.q + (int64_t)(g.first + row) * a.ld_q + (int64_t)h * D;
+        const int end = min(w.end, row_limit(g, w.kv_len, w.own, row));
+        float m = -INFINITY, l = 0.0f, acc[DL] = {};
+        bool seen = false;
+        for (int j0 = w.begin; j0 < end; j0 += 64) {
+            const int j = j0 + lane;
+            const int page = j < end ? table[j >> c.shift] : -1;
+            const bool there = (unsigned)page < (unsigned)c.num_pages;
+            const int at = j & ((1 << c.shift) - 1);
+            float s = -INFINITY;
+            if (there) {
+                const char* kr = c.k + page * c.k_page + head * c.k_head + at * c.k_pos;
+                s = 0.0f;
+                for (int d = 0; d < D; ++d)
+                    s += bf16_to_f32(q[d]) * (F8 ? __builtin_amdgcn_cvt_f32_fp8((int)reinterpret_cast<const uint8_t*>(kr)[d], 0)
+                                                 : bf16_to_f32(reinterpret_cast<const uint16_t*>(kr)[d]));
+                s *= sc;
+            }
+            const float mn = fmaxf(m, wave_max(s)), ms = mn == -INFINITY ? 0.0f : mn;
+            const float f = pg_exp2(m - ms), p = there ? pg_exp2(s - ms) : 0.0f;
+            m = mn;
+            l = l * f + wave_sum(p);
+            for (int e = 0; e < DL; ++e) acc[e] *= f;
+            uint64_t live = __ballot(there);
+            seen |= live != 0;
+            for (; live; live &= live - 1) {
+                const int i = __builtin_ctzll(live);
+                const float pi = __shfl(p, i, 64);
+                const int pg = __shfl(page, i, 64), ai = (j0 + i) & ((1 << c.shift) - 1);
+                const char* vr = c.v + pg * c.v_page + head * c.v_head + ai * c.v_pos;
+                for (int e = 0; e < DL; ++e)
+                    acc[e] += pi * (F8 ? __builtin_amdgcn_cvt_f32_fp8((int)reinterpret_cast<const uint8_t*>(vr)[DL * lane + e], 0)
+                                       : bf16_to_f32(reinterpret_cast<const uint16_t*>(vr)[DL * lane + e]));
+            }
+        }
+        if (whole) {
+            uint16_t* o = a.out + (int64_t)(g.first + row) * a.ld_out + (int64_t)h * D + DL * lane;
+            for (int e = 0; e < DL; ++e) o[e] = f32_to_bf16(seen ? acc[e] / l * vs : 0.0f);
+        } else {
+            const int64_t to = ((int64_t)slot * c.HKV + head) * M + rr;
+            for (int e = 0; e < DL; ++e) a.part[to * D + DL * lane + e] = acc[e];
+            if (lane == 0) a.ml[to] = make_float2(m, m == -INFINITY ? (seen ? 1.0f : 0.0f) : l);
+        }
+    }
 }
 
 }  // namespace bz

@@ -2,6 +2,7 @@
 // (include/bz_paged.h), with shared prefixes: the launches.
 #include "bz_paged_attn.h"
 #include "bz_paged_stream.h"
+#include "bz_paged_tile.h"
 
 namespace bz {
 
@@ -82,7 +83,7 @@ static PagedPlan paged_plan(const bz_paged_kv* d) {
     const int G = d->HQ / d->HKV;
     const int64_t segs = d->groups > 0 ? std::min(d->B, d->groups) : d->B;
     const int64_t rows = ((int64_t)d->T + segs - 1) / segs * G;
-    p.M = rows <= 16 || d->D == 256 ? 16 : 32;
+    p.M = rows <= 16 ? 16 : (rows <= 32 && d->D < 256 ? 32 : (rows <= 64 ? 64 : 128));
     p.target = std::max(1, kPagedWorkgroups / d->HKV);
     const PagedBounds b = paged_bounds(d, p.M, p.target);
     p.notes = b.notes;
@@ -100,6 +101,10 @@ static void launch_stream(const PagedKv& c, const PagedAttn& a, int M, hipStream
     const dim3 grid((unsigned)(a.slots * c.HKV)), block(64 * kStreamWaves);
     if (M == 16)
         hipLaunchKernelGGL((paged_attn_bf16_stream<D, F8, 1>), grid, block, 0, st, c, a);
+    else if (M == 128)
+        hipLaunchKernelGGL((paged_attn_bf16_tile<D, F8, 4>), grid, block, 0, st, c, a);
+    else if (M == 64)
+        hipLaunchKernelGGL((paged_attn_bf16_tile<D, F8, 2>), grid, block, 0, st, c, a);
     else if constexpr (D < 256)
         hipLaunchKernelGGL((paged_attn_bf16_stream<D, F8, 2>), grid, block, 0, st, c, a);
 }

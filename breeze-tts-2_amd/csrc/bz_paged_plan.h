@@ -89,7 +89,8 @@ __device__ __forceinline__ PagedSlot paged_slot(const PagedKv& c, int M, float t
         work += (float)tiles_of(c, g.rows, M) * (float)g.keys;
     }
     work = wave_sum(work);
-    const int chunk = max(kMinChunk, ((int)ceilf(fminf(work / target, 1073741824.0f)) + 31) & ~31);
+    const int chunk = __builtin_amdgcn_readfirstlane(
+        max(kMinChunk, ((int)ceilf(fminf(work / target, 1073741824.0f)) + 31) & ~31));
     PagedSlot r = {};
     r.chunk = chunk;
     int base = 0;

@@ -79,25 +79,19 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT <= 128 ? 2 : 1) page
     using S = StreamStep<D, F8>;
     constexpr int M = 16 * RT, T = D / 32, NT = D / 16;
     constexpr int kRow = D + 4;
+    __shared__ int st_apart[kStreamWaves];
     __shared__ float st_m[kStreamWaves][M], st_l[kStreamWaves][M];
     __shared__ __attribute__((aligned(16))) float st_acc[kStreamWaves][16][kRow];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int slot = blockIdx.x / c.HKV, head = blockIdx.x - slot * c.HKV;
 
-    const PagedSlot u = paged_slot(c, M, a.target, slot, lane);
-    if (!u.any) return;
+    PagedWork w;
+    if (!paged_work(c, M, a.target, slot, lane, w)) return;
+    const PagedSlot& u = w.u;
     const PagedSeg& g = u.seg;
-    const bool own = g.seq < c.B;
-    const int kv_len = own ? max(c.kv_lens[g.seq], 0) : 0;
-    const int nrow = min(g.rows * c.G - u.tile * M, M);  // rows of the tile
-    // the chunk's keys that a row of the tile attends
-    const int last_row = (u.tile * M + nrow - 1) / c.G;
-    const int begin = u.split * u.chunk;
-    const int tile_end = row_limit(g, kv_len, own, last_row);
-    const int end = min(begin + u.chunk, tile_end);
-    if (u.split > 0 && begin >= tile_end) return;  // a chunk behind the tile's last row
-    const int tile_min = row_limit(g, kv_len, own, (u.tile * M) / c.G);  // what all rows attend
+    const bool own = w.own;
+    const int nrow = w.rows, begin = w.begin, end = w.end;
 
     // queries: B operands, and each row's limit (behind the tile's rows, its last one again)
     u32x4 q[RT][T];
@@ -106,7 +100,7 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT <= 128 ? 2 : 1) page
     for (int rt = 0; rt < RT; ++rt) {
         const int i = u.tile * M + min(16 * rt + col, nrow - 1);
         const int row = i / c.G, h = head * c.G + (i - row * c.G);
-        limit[rt] = row_limit(g, kv_len, own, row);
+        limit[rt] = row_limit(g, w.kv_len, own, row);
         const uint16_t* p = a.q + (int64_t)(g.first + row) * a.ld_q + (int64_t)h * D;
 #pragma unroll
         for (int t = 0; t < T; ++t)
@@ -155,9 +149,21 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT <= 128 ? 2 : 1) page
         s.load_k(h, piece[h], c.k_pos, col, grp);
         s.load_v(h, piece[h], c.v_pos, col, grp);
     }
+    bool apart = false;
     for (int step = 0; step < steps; ++step, at += kStride) {
         const int there[2] = {piece[0].n, piece[1].n};
-        const bool mask = at + kStep > tile_min || there[0] < 16 || there[1] < 16;
+        const bool mask = at + kStep > w.all || there[0] < 16 || there[1] < 16;
+        if (mask && w.all < end) {  // (behind all rows' limits zeros were loaded)
+            bool odd = false;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int i = 0; i < S::VW; ++i) odd |= F8 ? nan_f8x4(s.v[h][e][i]) : not_finite2(s.v[h][e][i]);
+            apart = __ballot(odd) != 0;
+            if (apart) break;
+        }
         pg_f32x4 score[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) score[rt][0] = score[rt][1] = pg_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -167,10 +173,7 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT <= 128 ? 2 : 1) page
             for (int h = 0; h < 2; ++h) {
                 u32x4 kk;
                 if constexpr (F8) {
-                    uint32_t w[4];
-                    f8_widen(s.k[h][t >> 1][2 * (t & 1)], w[0], w[1]);
-                    f8_widen(s.k[h][t >> 1][2 * (t & 1) + 1], w[2], w[3]);
-                    kk = u32x4{w[0], w[1], w[2], w[3]};
+                    kk = f8_widen(s.k[h][t >> 1][2 * (t & 1)], s.k[h][t >> 1][2 * (t & 1) + 1]);
                 } else {
                     kk = s.k[h][t];
                 }
@@ -186,11 +189,9 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT <= 128 ? 2 : 1) page
         }
 
         uint32_t pb[RT][2][4];
-        uint32_t vis_bits[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             pg_f32x4(&sv)[2] = score[rt];
-            uint32_t vis = 0xFFu;
             if (mask) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -199,11 +200,11 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT <= 128 ? 2 : 1) page
                         const int j = 16 * h + 4 * grp + r;
                         const bool ok = at + j < limit[rt] && 4 * grp + r < there[h];
                         sv[h][r] = ok ? sv[h][r] : -INFINITY;
-                        vis &= ok ? ~0u : ~(1u << (4 * h + r));
+                        seen[rt] |= ok;
                     }
+            } else {
+                seen[rt] = true;
             }
-            vis_bits[rt] = vis;
-            seen[rt] |= vis != 0;
             float mx = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])),
                              fmaxf(fmaxf(sv[1][0], sv[1][1]), fmaxf(sv[1][2], sv[1][3])));
             mx = pg_across(mx, [](float x, float y) { return fmaxf(x, y); });
@@ -256,58 +257,15 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT <= 128 ? 2 : 1) page
             }
             return r;
         };
-        // A value that is not finite of a key that some rows of the tile do not attend: 0 times it
-        // is NaN in their sums.  Its finite part goes the ordinary way, and what the
-        // rest makes of a sum follows from how many of each kind a row attends.
-        bool odd = false;
-        const bool differ = mask && tile_min < end;  // (behind all rows' limits zeros were loaded)
-        if (differ) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int i = 0; i < S::VW; ++i) odd |= F8 ? nan_f8x4(s.v[h][e][i]) : not_finite2(s.v[h][e][i]);
-        }
-        if (differ && __ballot(odd)) {
+        for (int t = 0; t < NT; ++t) {
+            const u32x4 w = column(t);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                u32x4 ones;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    ones[i] = ((vis_bits[rt] >> (2 * i)) & 1 ? 0x3F80u : 0u) | ((vis_bits[rt] >> (2 * i + 1)) & 1 ? 0x3F800000u : 0u);
                 const u32x4 b0 = {pb[rt][0][0], pb[rt][0][1], pb[rt][0][2], pb[rt][0][3]};
                 const u32x4 b1 = {pb[rt][1][0], pb[rt][1][1], pb[rt][1][2], pb[rt][1][3]};
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const u32x4 w = column(t);
-                    u32x4 fin, nan, pos, neg;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        fin[i] = finite2(w[i]);
-                        nan[i] = ones2(w[i], [](uint32_t x) { return (x & 0x7FFFu) > 0x7F80u; });
-                        pos[i] = ones2(w[i], [](uint32_t x) { return x == 0x7F80u; });
-                        neg[i] = ones2(w[i], [](uint32_t x) { return x == 0xFF80u; });
-                    }
-                    const pg_f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
-                    const pg_f32x4 n0 = pg_mfma16(nan, ones, z), n1 = pg_mfma16(pos, ones, z), n2 = pg_mfma16(neg, ones, z);
-                    acc[rt][t] = pg_mfma16(fin, b1, pg_mfma16(fin, b0, acc[rt][t]));
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[rt][t][r] += taint(n0[r], n1[r], n2[r]);
-                    __builtin_amdgcn_sched_barrier(0);  // (one tile's operands in registers, not all)
-                }
-            }
-        } else {
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const u32x4 w = column(t);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const u32x4 b0 = {pb[rt][0][0], pb[rt][0][1], pb[rt][0][2], pb[rt][0][3]};
-                    const u32x4 b1 = {pb[rt][1][0], pb[rt][1][1], pb[rt][1][2], pb[rt][1][3]};
-                    acc[rt][t] = pg_mfma16(w, b0, acc[rt][t]);
-                    acc[rt][t] = pg_mfma16(w, b1, acc[rt][t]);
-                }
+                acc[rt][t] = pg_mfma16(w, b0, acc[rt][t]);
+                acc[rt][t] = pg_mfma16(w, b1, acc[rt][t]);
             }
         }
 #pragma unroll
@@ -325,6 +283,7 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT <= 128 ? 2 : 1) page
             st_l[wave][16 * rt + col] = ls;
         }
     }
+    if (lane == 0) st_apart[wave] = apart;
     const bool whole = u.splits == 1 && c.groups == 0;  // no other slot has keys of these rows
     const float vs = F8 ? c.v_scale[head] : 1.0f;
     const int64_t to = ((int64_t)slot * c.HKV + head) * M;
@@ -338,6 +297,10 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT <= 128 ? 2 : 1) page
 #pragma unroll
             for (int r = 0; r < 4; ++r) st_acc[wave][col][stream_col<D, F8>(t, 4 * grp + r)] = acc[rt][t][r];
         __syncthreads();
+        if (rt == 0 && __builtin_amdgcn_readfirstlane(st_apart[0] | st_apart[1] | st_apart[2] | st_apart[3])) {
+            paged_rows_apart<D, F8>(c, a, w, slot, head, M, wave, kStreamWaves, lane);
+            return;
+        }
         for (int i = tid; i < 4 * D; i += 64 * kStreamWaves) {  // 16 rows of D / 4 pieces
             const int r = i / (D / 4), d = 4 * (i % (D / 4)), rr = 16 * rt + r;
             if (rr >= nrow) continue;
