@@ -25,8 +25,8 @@ q_starts          int32 [B + 1]: sequence b has the rows q_starts[b] .. q_starts
                   are not touched: in a tensor that the call allocates they hold anything.
 
 Lengths, tables and starts are read on the device: no call synchronizes, and a
-captured graph follows them.  Calls may run on several streams at once; a
-workspace belongs to its call.
+captured graph follows them.  Calls may run on several streams at once, and graphs on
+any: each stream and each capture has a workspace of its own.
 """
 
 from __future__ import annotations
@@ -40,6 +40,11 @@ from . import _lib
 from ._lib import DT_BF16, DT_F32, KV_E4M3
 
 __all__ = ["paged_rope_cache", "paged_attention", "shared_prefix_attention"]
+
+# One zeroed workspace for each device and stream, and for each graph capture
+# under way: the kernels leave its counters at zero.
+_WS: dict[tuple, torch.Tensor] = {}
+_WS_RETIRED: list = []
 
 _KV = {torch.bfloat16: DT_BF16, torch.float8_e4m3fn: KV_E4M3}
 _CS = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
@@ -56,23 +61,26 @@ def _gpu(name: str, t: torch.Tensor, index: int) -> None:
 
 def _ints(name: str, t: torch.Tensor, shape: tuple, index: int) -> int:
     """The pointer of an int32 tensor of this shape with unit stride in its last dimension."""
-    _gpu(name, t, index)
-    if t.dtype != torch.int32:
-        raise TypeError(f"{name} must be int32, got {t.dtype}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{name} must have unit stride in its last dimension")
+    if not (t.dtype is torch.int32 and t.shape == shape and t.get_device() == index and index >= 0
+            and (t.stride()[-1] == 1 or shape[-1] <= 1)):
+        _gpu(name, t, index)
+        if t.dtype != torch.int32:
+            raise TypeError(f"{name} must be int32, got {t.dtype}")
+        if t.shape != shape:
+            raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+        if t.stride(-1) != 1 and shape[-1] > 1:
+            raise ValueError(f"{name} must have unit stride in its last dimension")
     return t.data_ptr()
 
 
 def _table(name: str, t: torch.Tensor, index: int) -> tuple:
     """(rows, width, pointer, row stride) of a page table."""
-    if t.dim() != 2 or t.shape[1] < 1:
-        raise ValueError(f"{name} must be [rows, pages] with at least one page, got {list(t.shape)}")
-    p = _ints(name, t, t.shape, index)
-    rows, width = t.shape
-    ld = t.stride(0) if rows > 1 else width
+    shape = t.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"{name} must be [rows, pages] with at least one page, got {list(shape)}")
+    p = _ints(name, t, shape, index)
+    rows, width = shape
+    ld = t.stride()[0] if rows > 1 else width
     if ld < width:
         raise ValueError(f"{name} must not have overlapping rows")
     return rows, width, p, ld
@@ -80,33 +88,47 @@ def _table(name: str, t: torch.Tensor, index: int) -> tuple:
 
 def _strides(t: torch.Tensor) -> tuple:
     """Element strides of a pool; those of dimensions of size 1 are not used and count as D."""
-    if t.stride(3) != 1:
+    a, b, c, d = t.stride()
+    if d != 1:
         raise ValueError("a position's D elements must be contiguous")
-    return tuple(s if n > 1 else t.shape[3] for s, n in zip(t.stride()[:3], t.shape))
+    pages, heads, _, D = t.shape
+    return a if pages > 1 else D, b if heads > 1 else D, c
 
 
-def _cache(T: int, HQ: int, k_pages, v_pages, k_scale, v_scale, block_table, kv_lens, q_starts, index: int) -> tuple:
-    """The fields of bz_paged_kv without the prefixes', checked."""
+def _check_cache(k_pages, v_pages, index: int) -> None:
+    """Raises what is wrong with the pools."""
     _gpu("k_pages", k_pages, index)
     _gpu("v_pages", v_pages, index)
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
         raise ValueError("k_pages and v_pages must both be [pages, HKV, page_size, D] of one dtype")
-    kind = _KV.get(k_pages.dtype)
-    if kind is None:
+    if k_pages.dtype not in _KV:
         raise TypeError(f"pages must be bfloat16 or float8_e4m3fn, got {k_pages.dtype}")
-    pages, HKV, ps, D = k_pages.shape
+
+
+def _scale(name: str, t, HKV: int, index: int) -> int:
+    if t is None:
+        raise ValueError("an e4m3 cache comes with k_scale and v_scale")
+    _gpu(name, t, index)
+    if t.dtype != torch.float32 or t.shape != (HKV,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 [{HKV}] tensor")
+    return t.data_ptr()
+
+
+def _cache(T: int, HQ: int, k_pages, v_pages, k_scale, v_scale, block_table, kv_lens, q_starts, index: int) -> tuple:
+    """The fields of bz_paged_kv without the prefixes', checked."""
+    shape, dtype = k_pages.shape, k_pages.dtype
+    kind = _KV.get(dtype)
+    # one expression for what is nearly always so; what it is not is found out afterwards
+    if not (kind is not None and k_pages.get_device() == index and v_pages.get_device() == index and index >= 0
+            and len(shape) == 4 and v_pages.shape == shape and v_pages.dtype == dtype):
+        _check_cache(k_pages, v_pages, index)
+    pages, HKV, ps, D = shape
     if kind == KV_E4M3:
-        if k_scale is None or v_scale is None:
-            raise ValueError("an e4m3 cache comes with k_scale and v_scale")
-        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            _gpu(name, t, index)
-            if t.dtype != torch.float32 or t.shape != (HKV,) or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous float32 [{HKV}] tensor")
-        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
-    else:
-        if k_scale is not None or v_scale is not None:
-            raise ValueError("a bf16 cache has no scales")
+        ks, vs = _scale("k_scale", k_scale, HKV, index), _scale("v_scale", v_scale, HKV, index)
+    elif k_scale is None and v_scale is None:
         ks = vs = 0
+    else:
+        raise ValueError("a bf16 cache has no scales")
     B, width, table, ld = _table("block_table", block_table, index)
     lens = _ints("kv_lens", kv_lens, (B,), index)
     if q_starts is not None:
@@ -116,8 +138,8 @@ def _cache(T: int, HQ: int, k_pages, v_pages, k_scale, v_scale, block_table, kv_
     else:
         raise ValueError(f"{T} rows for {B} sequences: q_starts says which are whose")
     return ((_lib.ABI_VERSION, T, B, HQ, HKV, D, kind, ps, pages, width),
-            (k_pages.data_ptr(), v_pages.data_ptr(), *_strides(k_pages), *_strides(v_pages), ks, vs, table, ld, lens,
-             starts))
+            (k_pages.data_ptr(), v_pages.data_ptr()) + _strides(k_pages) + _strides(v_pages)
+            + (ks, vs, table, ld, lens, starts))
 
 
 _NO_PREFIX = (0, 0), (0, 0, 0, 0)
@@ -145,29 +167,20 @@ def _workspace_bytes(sizes: tuple) -> int:
     return int(_lib.lib().bz_paged_attn_workspace(d))
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy whose rows begin at multiples of 16 bytes and do not overlap."""
-    if t.data_ptr() % 16 or (t.shape[0] > 1 and (t.stride(0) * t.element_size() % 16 or t.stride(0) < t.shape[1])):
-        return t.clone(memory_format=torch.contiguous_format)
+def _heads(name: str, t: torch.Tensor) -> torch.Tensor:
+    """[T, HQ, D] bf16 whose rows are contiguous, begin at multiples of 16 bytes and do not overlap."""
+    shape = t.shape
+    if len(shape) != 3 or t.dtype != torch.bfloat16:
+        raise ValueError(f"{name} must be a bf16 [rows, HQ, D] tensor")
+    a, b, c = t.stride()
+    T, HQ, D = shape
+    if t.data_ptr() % 16 or (c != 1 and D > 1) or (b != D and HQ > 1) or (T > 1 and (a % 8 or a < HQ * D)):
+        t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _heads(name: str, t: torch.Tensor) -> torch.Tensor:
-    """[T, HQ, D] -> [T, HQ * D] with unit column stride."""
-    if t.dim() != 3 or t.dtype != torch.bfloat16:
-        raise ValueError(f"{name} must be a bf16 [rows, HQ, D] tensor")
-    if (t.stride(2) != 1 and t.shape[2] > 1) or (t.stride(1) != t.shape[2] and t.shape[1] > 1):
-        t = t.contiguous()
-    return t.as_strided((t.shape[0], t.shape[1] * t.shape[2]), (t.stride(0), 1))
-
-
-def _result(name: str, t: Optional[torch.Tensor], shape: tuple, dev, index: int, *inputs) -> torch.Tensor:
-    if t is None:
-        return torch.empty(shape, device=dev, dtype=torch.bfloat16)
+def _result(name: str, t: torch.Tensor, shape: tuple, index: int, x: torch.Tensor) -> torch.Tensor:
+    """A caller's output, checked, apart from the input x."""
     _gpu(name, t, index)
     inner = 1
     for n, s in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
@@ -178,13 +191,22 @@ def _result(name: str, t: Optional[torch.Tensor], shape: tuple, dev, index: int,
         raise ValueError(f"{name} must be a bf16 {list(shape)} tensor")
     if t.data_ptr() % 16 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < inner)):
         raise ValueError(f"{name} needs rows at multiples of 16 bytes that do not overlap")
-    if t.numel():
+    if t.numel() and x.numel():
         end = t.data_ptr() + 2 * ((t.shape[0] - 1) * t.stride(0) + inner)
-        for x in inputs:
-            if x.numel() and x.data_ptr() < end and t.data_ptr() < x.data_ptr() + x.element_size() * (
-                    (x.shape[0] - 1) * x.stride(0) + x[0].numel()):
-                raise ValueError(f"{name} must not overlap the input")
+        if x.data_ptr() < end and t.data_ptr() < x.data_ptr() + 2 * ((x.shape[0] - 1) * x.stride(0) + x[0].numel()):
+            raise ValueError(f"{name} must not overlap the input")
     return t
+
+
+def _norm(name: str, w: torch.Tensor, D: int, index: int) -> torch.Tensor:
+    """Norm weights as an aligned bf16 [D]."""
+    if w.get_device() != index:
+        _gpu(name, w, index)
+    if w.numel() != D:
+        raise ValueError(f"{name} must have {D} elements")
+    if w.dtype != torch.bfloat16 or not w.is_contiguous() or w.data_ptr() % 16:
+        w = w.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
+    return w
 
 
 def _call(index: int, f, *args) -> None:
@@ -212,75 +234,78 @@ def paged_rope_cache(qkv, cos, sin, k_pages, v_pages, block_table, kv_lens, HQ: 
     a shared prefix pass positions.  A row outside the table is written to no page
     and its q is zero."""
     index = qkv.get_device()
-    _gpu("qkv", qkv, index)
-    if qkv.dim() != 2 or qkv.dtype != torch.bfloat16:
+    shape = qkv.shape
+    if index < 0:
+        _gpu("qkv", qkv, index)
+    if len(shape) != 2 or qkv.dtype != torch.bfloat16:
         raise ValueError("qkv must be a bf16 [rows, (HQ + 2 HKV) D] tensor")
-    T = qkv.shape[0]
+    T, width = shape
     sizes, refs = _cache(T, HQ, k_pages, v_pages, k_scale, v_scale, block_table, kv_lens, q_starts, index)
     HKV, D = sizes[4], sizes[5]
-    if HQ < 1 or qkv.shape[1] != (HQ + 2 * HKV) * D:
-        raise ValueError(f"qkv width {qkv.shape[1]} is not ({HQ} + 2 * {HKV}) heads of {D}")
-    if qkv.stride(1) != 1:
-        qkv = qkv.contiguous()
-    qkv = _rows16(qkv)
-    for name, t in (("cos", cos), ("sin", sin)):
-        _gpu(name, t, index)
+    if HQ < 1 or width != (HQ + 2 * HKV) * D:
+        raise ValueError(f"qkv width {width} is not ({HQ} + 2 * {HKV}) heads of {D}")
+    ld, inner = qkv.stride()
+    if inner != 1 or qkv.data_ptr() % 16 or (T > 1 and (ld % 8 or ld < width)):
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+        ld = width
     if cos.dim() == 3 and cos.shape[0] == 1:
         cos, sin = cos[0], sin[0] if sin.dim() == 3 else sin
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.shape[1] != D or cos.shape[0] < 1:
-        raise ValueError(f"cos and sin must both be [positions, {D}] of one dtype")
-    cs = _CS.get(cos.dtype)
-    if cs is None:
+    shape, cs = cos.shape, _CS.get(cos.dtype)
+    if not (cos.get_device() == index and sin.get_device() == index and len(shape) == 2 and sin.shape == shape
+            and sin.dtype == cos.dtype and shape[1] == D and shape[0] > 0 and cs is not None):
+        for name, t in (("cos", cos), ("sin", sin)):
+            _gpu(name, t, index)
+        if cos.dim() != 2 or shape != sin.shape or cos.dtype != sin.dtype or shape[1] != D or shape[0] < 1:
+            raise ValueError(f"cos and sin must both be [positions, {D}] of one dtype")
         raise TypeError(f"cos and sin must be bfloat16 or float32, got {cos.dtype}")
-    if cos.stride() != sin.stride() or cos.stride(1) != 1 or (cos.shape[0] > 1 and cos.stride(0) % 8) \
+    ld_cs, inner = cos.stride()
+    if sin.stride() != (ld_cs, inner) or inner != 1 or (shape[0] > 1 and (ld_cs % 8 or ld_cs < D)) \
             or cos.data_ptr() % 16 or sin.data_ptr() % 16:
         cos, sin = (t.clone(memory_format=torch.contiguous_format) for t in (cos, sin))
+        ld_cs = D
     at = 0
     if positions is not None:
         _gpu("positions", positions, index)
         if positions.dtype != torch.int64 or positions.shape != (T,) or not positions.is_contiguous():
             raise ValueError(f"positions must be a contiguous int64 [{T}] tensor")
         at = positions.data_ptr()
-    if (q_norm_w is None) != (k_norm_w is None):
-        raise ValueError("q_norm_w and k_norm_w come together")
     qn = kn = None
-    if q_norm_w is not None:
-        qn, kn = q_norm_w, k_norm_w
-        for name, t in (("q_norm_w", qn), ("k_norm_w", kn)):
-            _gpu(name, t, index)
-            if t.numel() != D:
-                raise ValueError(f"{name} must have {D} elements")
-        qn, kn = (w if w.dtype == torch.bfloat16 and w.is_contiguous() and w.data_ptr() % 16 == 0
-                  else w.to(torch.bfloat16).clone(memory_format=torch.contiguous_format) for w in (qn, kn))
-    q = _result("q_out", q_out, (T, HQ, D), qkv.device, index, qkv)
+    if q_norm_w is not None and k_norm_w is not None:
+        qn, kn = _norm("q_norm_w", q_norm_w, D, index), _norm("k_norm_w", k_norm_w, D, index)
+    elif q_norm_w is not None or k_norm_w is not None:
+        raise ValueError("q_norm_w and k_norm_w come together")
+    q = qkv.new_empty((T, HQ, D)) if q_out is None else _result("q_out", q_out, (T, HQ, D), index, qkv)
     if T == 0 or sizes[2] == 0:
         return q
-    d = _lib.paged_kv(*sizes, *_NO_PREFIX[0], *refs, *_NO_PREFIX[1])
-    _call(index, _lib.lib().bz_paged_rope_cache, d, qkv.data_ptr(), _ld(qkv), None if qn is None else qn.data_ptr(),
-          None if kn is None else kn.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), cs,
-          cos.stride(0) if cos.shape[0] > 1 else D, cos.shape[0], at, q.data_ptr(),
-          q.stride(0) if T > 1 else HQ * D)
+    _call(index, _lib.lib().bz_paged_rope_cache, _lib.paged_kv(*sizes, 0, 0, *refs, 0, 0, 0, 0), qkv.data_ptr(),
+          ld if T > 1 else width, None if qn is None else qn.data_ptr(), None if kn is None else kn.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), cs,
+          ld_cs if shape[0] > 1 else D, shape[0], at, q.data_ptr(), q.stride()[0] if T > 1 else HQ * D)
     return q
 
 
 def _attention(q, k_pages, v_pages, block_table, kv_lens, q_starts, prefix, scale, k_scale, v_scale, out):
     index = q.get_device()
-    _gpu("q", q, index)
-    dev = q.device
-    q2 = _rows16(_heads("q", q))
+    if index < 0:
+        _gpu("q", q, index)
+    q = _heads("q", q)
     T, HQ, D = q.shape
     sizes, refs = _cache(T, HQ, k_pages, v_pages, k_scale, v_scale, block_table, kv_lens, q_starts, index)
     if D != sizes[5]:
         raise ValueError(f"q has heads of {D}, the pages of {sizes[5]}")
     psizes, prefs = _NO_PREFIX if prefix is None else _prefixes(*prefix, sizes[2], index)
-    out = _result("out", out, (T, HQ * D), dev, index, q2)
+    width = HQ * D
+    if out is None:
+        out, ld = q.new_empty((T, width)), width
+    else:
+        out = _result("out", out, (T, width), index, q)
+        ld = out.stride()[0] if T > 1 else width
     if T == 0 or sizes[2] == 0:
         return out
     sizes += psizes
     n = _workspace_bytes(sizes)
-    ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
-    _call(index, _lib.lib().bz_paged_attn, _lib.paged_kv(*sizes, *refs, *prefs), q2.data_ptr(), _ld(q2),
-          D ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), n, out.data_ptr(), _ld(out))
+    ws = _lib.stream_workspace(_WS, (index,), n, q.device, torch._C._cuda_getCurrentRawStream(index), _WS_RETIRED)
+    _call(index, _lib.lib().bz_paged_attn, _lib.paged_kv(*sizes, *refs, *prefs), q.data_ptr(),
+          q.stride()[0] if T > 1 else width, D ** -0.5 if scale is None else scale, ws.data_ptr(), n, out.data_ptr(), ld)
     return out
 
 

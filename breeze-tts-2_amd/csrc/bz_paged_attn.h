@@ -49,12 +49,19 @@ struct PagedAttn {
     float* part;   // [slots][HKV][M][D] accumulators
     float2* ml;    // [slots][HKV][M] (m, l)
     int2* notes;   // [notes] (first slot, keys of a chunk) of a tile
+    // [notes][HKV] arrivals of a tile's parts, zero between calls; the last to arrive
+    // joins them.  NULL: a launch of its own does.
+    unsigned* arrived;
 };
 
 // The position behind the last key that a row attends in its segment: row i of n of a
 // sequence is position kv_len - n + i; of a shared prefix every row attends all.
 __device__ __forceinline__ int row_limit(const PagedSeg& g, int kv_len, bool own, int row) {
     return own ? min(max(kv_len - g.rows + row + 1, 0), g.keys) : g.keys;
+}
+
+__device__ __forceinline__ int parts_of(int keys, int chunk) {
+    return max(1, (int)(((unsigned)keys + chunk - 1) / (unsigned)chunk));
 }
 
 // A workgroup's part of the work: a slot with the keys of its chunk that its rows attend.
@@ -65,6 +72,7 @@ struct PagedWork {
     int rows;     // query rows of the tile, head by head
     int begin, end;  // keys of the chunk that a row of the tile attends
     int all;      // the keys before it are attended by all rows
+    int parts;    // chunks that have keys of the tile (or one that has none)
 };
 __device__ __forceinline__ bool paged_work(const PagedKv& c, int M, float target, int slot, int lane, PagedWork& w) {
     w.u = paged_slot(c, M, target, slot, lane);
@@ -75,10 +83,11 @@ __device__ __forceinline__ bool paged_work(const PagedKv& c, int M, float target
     const int first = w.u.tile * M;
     w.rows = min(g.rows * c.G - first, M);
     const int tile_end = row_limit(g, w.kv_len, w.own, (first + w.rows - 1) / c.G);
+    w.parts = parts_of(tile_end, w.u.chunk);
     w.begin = w.u.split * w.u.chunk;
     w.end = min(w.begin + w.u.chunk, tile_end);
     w.all = row_limit(g, w.kv_len, w.own, first / c.G);
-    return w.u.split == 0 || w.begin < tile_end;  // else a chunk behind the tile's last row
+    return w.u.split < w.parts;  // else a chunk behind the tile's last row
 }
 
 // One 16-position piece of a segment's keys, none of whose rows is read beyond `n`.
@@ -112,6 +121,139 @@ __device__ __forceinline__ bool not_finite2(uint32_t w) {
 }
 // Whether one of four e4m3 codes is NaN (they have no infinities).
 __device__ __forceinline__ bool nan_f8x4(uint32_t w) { return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0; }
+// The parts that one workgroup leaves: [M][D] accumulators and [M] (m, l).  Where the
+// last workgroup of a tile joins them they are stored to the point at which all XCDs meet
+// (as agent-scope atomics are); for a launch of its own the end of this one does that
+// (those stores past the L2 took prompt tiles 8% longer).
+struct PagedParts {
+    __amdgpu_buffer_rsrc_t acc, ml;
+    bool agent;
+    __device__ __forceinline__ PagedParts(const PagedAttn& a, const PagedKv& c, int slot, int head, int M, int D) {
+        const int64_t at = ((int64_t)slot * c.HKV + head) * M;
+        acc = buffer_rsrc(a.part + at * D, (uint32_t)(M * D) * 4u);
+        ml = buffer_rsrc(a.ml + at, (uint32_t)M * 8u);
+        agent = a.arrived != nullptr;
+    }
+    __device__ __forceinline__ void put(int i, float v) const {
+        if (agent)
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), acc, i * 4, 0, kCpolAgent);
+        else
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), acc, i * 4, 0, 0);
+    }
+    __device__ __forceinline__ void put4(int i, float x, float y, float z, float w) const {
+        const u32x4 v = {__float_as_uint(x), __float_as_uint(y), __float_as_uint(z), __float_as_uint(w)};
+        if (agent)
+            __builtin_amdgcn_raw_buffer_store_b128(v, acc, i * 4, 0, kCpolAgent);
+        else
+            __builtin_amdgcn_raw_buffer_store_b128(v, acc, i * 4, 0, 0);
+    }
+    __device__ __forceinline__ void put_ml(int r, float m, float l) const {
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        const u32x2 v = {__float_as_uint(m), __float_as_uint(l)};
+        if (agent)
+            __builtin_amdgcn_raw_buffer_store_b64(v, ml, r * 8, 0, kCpolAgent);
+        else
+            __builtin_amdgcn_raw_buffer_store_b64(v, ml, r * 8, 0, 0);
+    }
+};
+
+// A row's sums of four columns, joined from parts.
+struct PagedSum {
+    float m = -INFINITY, l = 0.0f, o[4] = {};
+    // factors that bring a part with maximum x, and this sum, to the larger maximum
+    __device__ __forceinline__ void add(float mx, float lx, float4 v) {
+        const float mn = fmaxf(m, mx);
+        const float f = mn == -INFINITY ? 1.0f : pg_exp2(m - mn), g = mn == -INFINITY ? 1.0f : pg_exp2(mx - mn);
+        m = mn;
+        l = l * f + lx * g;
+        o[0] = o[0] * f + v.x * g;
+        o[1] = o[1] * f + v.y * g;
+        o[2] = o[2] * f + v.z * g;
+        o[3] = o[3] * f + v.w * g;
+    }
+    // parts first, first + stride, .. of n; part i is the row at + i step of [M] rows
+    template <bool AGENT>
+    __device__ __forceinline__ void add_parts(const PagedAttn& a, int64_t at, int64_t step, int n, int first, int stride,
+                                              int D, int d) {
+        constexpr int U = 8;  // loads under way at a time
+        for (int s0 = first; s0 < n; s0 += U * stride) {
+            float2 x[U];
+            float4 v[U];
+#pragma unroll
+            for (int e = 0; e < U; ++e) {
+                const int64_t i = at + min(s0 + e * stride, n - 1) * step;
+                if constexpr (AGENT) {
+                    const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t*>(a.ml + i), __ATOMIC_RELAXED,
+                                                         __HIP_MEMORY_SCOPE_AGENT);
+                    x[e] = make_float2(__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32)));
+                    const uint64_t* p = reinterpret_cast<const uint64_t*>(a.part + i * D + d);
+                    const uint64_t w0 = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    const uint64_t w1 = __hip_atomic_load(p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    v[e] = make_float4(__uint_as_float((uint32_t)w0), __uint_as_float((uint32_t)(w0 >> 32)),
+                                       __uint_as_float((uint32_t)w1), __uint_as_float((uint32_t)(w1 >> 32)));
+                } else {
+                    x[e] = a.ml[i];
+                    v[e] = *reinterpret_cast<const float4*>(a.part + i * D + d);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < U; ++e)
+                if (s0 + e * stride < n) add(x[e].x, x[e].y, v[e]);
+        }
+    }
+    // sums of P threads, `apart` threads from each other, into the first's, through LDS [256][8]
+    __device__ __forceinline__ void across(float (*st)[8], int tid, int P, int apart, bool lead) {
+        if (P == 1) return;
+        float* s = st[tid];
+        s[0] = o[0], s[1] = o[1], s[2] = o[2], s[3] = o[3], s[4] = m, s[5] = l;
+        __syncthreads();
+        if (lead)
+            for (int p = 1; p < P; ++p) {
+                const float* x = st[tid + p * apart];
+                add(x[4], x[5], make_float4(x[0], x[1], x[2], x[3]));
+            }
+    }
+    __device__ __forceinline__ void store(uint16_t* p, float vs) const {
+        const float f = m == -INFINITY ? (l > 0.0f ? __builtin_nanf("") : 0.0f) : 1.0f / l * vs;
+        *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(o[0] * f, o[1] * f), pack_bf16x2(o[2] * f, o[3] * f));
+    }
+};
+
+// The last of a tile's workgroups (256 threads) joins the parts; all have been stored.
+// st: LDS of 256 rows of 8.
+template <int D, bool F8>
+__device__ __forceinline__ void paged_join_last(const PagedKv& c, const PagedAttn& a, const PagedWork& w, int head, int M,
+                                                int tid, float (*st)[8], int* last) {
+    const PagedSeg& g = w.u.seg;
+    // every thread's stores have arrived before the workgroup counts itself in
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    unsigned* count = a.arrived + (int64_t)tile_note(c, g, w.u.tile, M) * c.HKV + head;
+    if (tid == 0)
+        *last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)w.parts - 1u;
+    __syncthreads();
+    if (!*last) return;
+    if (tid == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const float vs = F8 ? c.v_scale[head] : 1.0f;
+    const int64_t at0 = ((int64_t)w.u.first_slot * c.HKV + head) * M, step = (int64_t)c.HKV * M;
+    const int items = w.rows * (D / 4);
+    // few items: several threads to each, taking parts in turn
+    int P = 1;
+    while (2 * P * items <= 256 && P < w.parts) P *= 2;
+    for (int i0 = 0; i0 < items; i0 += 256) {
+        const int p = P > 1 ? tid / items : 0, i = i0 + tid - p * items;
+        PagedSum sum;
+        const bool on = P > 1 ? p < P : i < items;
+        const int r = on ? i / (D / 4) : 0, d = 4 * (i % (D / 4));
+        if (on) sum.add_parts<true>(a, at0 + r, step, w.parts, p, P, D, d);
+        sum.across(st, tid, P, items, on && p == 0);
+        if (on && p == 0) {
+            const int k = w.u.tile * M + r, row = k / c.G, h = head * c.G + (k - row * c.G);
+            sum.store(a.out + (int64_t)(g.first + row) * a.ld_out + (int64_t)h * D + d, vs);
+        }
+    }
+}
+
 // The rows of a workgroup's tile one by one, a wave to a row and a key to a lane: for a
 // tile in which a value that is not finite belongs to a key that only some of the rows
 // attend (0 times it is NaN, so a matrix product would carry it into the others).
@@ -124,7 +266,8 @@ __device__ __forceinline__ void paged_rows_apart(const PagedKv& c, const PagedAt
     const int32_t* table = w.own ? c.table + (int64_t)g.seq * c.ld_table
                                  : c.prefix_table + (int64_t)(g.seq - c.B) * c.ld_prefix;
     const float sc = a.scale * kPagedLog2e * (F8 ? c.k_scale[head] : 1.0f), vs = F8 ? c.v_scale[head] : 1.0f;
-    const bool whole = w.u.splits == 1 && c.groups == 0;
+    const bool whole = w.parts == 1 && c.groups == 0;
+    const PagedParts parts(a, c, slot, head, M, D);
     for (int rr = wave; rr < w.rows; rr += waves) {
         const int k = w.u.tile * M + rr, row = k / c.G, h = head * c.G + (k - row * c.G);
         const uint16_t* q = a.q + (int64_t)(g.first + row) * a.ld_q + (int64_t)h * D;
@@ -166,9 +309,8 @@ __device__ __forceinline__ void paged_rows_apart(const PagedKv& c, const PagedAt
             uint16_t* o = a.out + (int64_t)(g.first + row) * a.ld_out + (int64_t)h * D + DL * lane;
             for (int e = 0; e < DL; ++e) o[e] = f32_to_bf16(seen ? acc[e] / l * vs : 0.0f);
         } else {
-            const int64_t to = ((int64_t)slot * c.HKV + head) * M + rr;
-            for (int e = 0; e < DL; ++e) a.part[to * D + DL * lane + e] = acc[e];
-            if (lane == 0) a.ml[to] = make_float2(m, m == -INFINITY ? (seen ? 1.0f : 0.0f) : l);
+            for (int e = 0; e < DL; ++e) parts.put(rr * D + DL * lane + e, acc[e]);
+            if (lane == 0) parts.put_ml(rr, m, m == -INFINITY ? (seen ? 1.0f : 0.0f) : l);
         }
     }
 }

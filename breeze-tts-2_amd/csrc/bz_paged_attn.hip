@@ -8,74 +8,61 @@ namespace bz {
 
 constexpr int kPagedWorkgroups = 1024;  // that the keys are cut for
 
-// The chunks' parts of a row, merged in the keys' order: its prefix's, then its
-// own.  Four columns of a head to a thread.
-template <int D>
+// The parts of a row joined in a launch of its own: its prefix's, then its own.
+// Four columns of a head to P threads, which take its parts in turn.
+template <int D, int P>
 __global__ void __launch_bounds__(256) paged_attn_bf16_join(PagedKv c, PagedAttn a, int M, bool f8) {
-    const int t = blockIdx.x, lane = threadIdx.x & 63;
+    constexpr int kItems = 256 / P;
+    __shared__ float st[P > 1 ? 256 : 1][8];
+    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int b = seq_of_row(c, t, lane);
     if (b >= c.B) return;
     const PagedSeg own = paged_seg(c, b);
     const int row = t - own.first;
     if (row < 0 || row >= own.rows) return;
     const int pre = prefix_of_seq(c, b, lane);
-    const int item = blockIdx.y * 256 + threadIdx.x;
+    const int item = blockIdx.y * kItems + tid % kItems, p = tid / kItems;
     const int h = item / (D / 4), d = 4 * (item - h * (D / 4));
-    if (h >= c.HQ) return;
-    const int head = h / c.G;
+    const bool on = h < c.HQ;
+    const int head = min(h, c.HQ - 1) / c.G;
 
-    float m = -INFINITY, l = 0.0f, o[4] = {};
-    for (int part = pre >= 0 ? 0 : 1; part < 2; ++part) {
+    int64_t at[2] = {};
+    int n[2] = {};
+    bool whole = false;  // written by the only workgroup that has keys of the row's tile
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+        if (!part && pre < 0) continue;
         const PagedSeg g = part ? own : paged_seg(c, c.B + pre);
-        const int k = (t - g.first) * c.G + (h - head * c.G), tile = k / M;
+        const int k = (t - g.first) * c.G + (min(h, c.HQ - 1) - head * c.G), tile = k / M;
         const int2 note = a.notes[tile_note(c, g, tile, M)];
-        if (c.groups == 0 && g.keys <= note.y) return;  // written by its only slot
-        const int limit = row_limit(g, part ? max(c.kv_lens[b], 0) : 0, part, row);
-        const int n = max(1, (int)(((unsigned)limit + note.y - 1) / (unsigned)note.y));
-        const int64_t at = ((int64_t)note.x * c.HKV + head) * M + (k - tile * M), step = (int64_t)c.HKV * M;
-        constexpr int U = 4;
-        for (int s0 = 0; s0 < n; s0 += U) {
-            float2 x[U];
-            float4 v[U];
-#pragma unroll
-            for (int e = 0; e < U; ++e) {
-                const int64_t i = at + min(s0 + e, n - 1) * step;
-                x[e] = a.ml[i];
-                v[e] = *reinterpret_cast<const float4*>(a.part + i * D + d);
-            }
-            float mn = m;
-#pragma unroll
-            for (int e = 0; e < U; ++e) mn = fmaxf(mn, x[e].x);
-            const float ms = mn == -INFINITY ? 0.0f : mn;
-            const float f = mn == -INFINITY ? 1.0f : pg_exp2(m - ms);
-            l *= f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] *= f;
-            m = mn;
-#pragma unroll
-            for (int e = 0; e < U; ++e) {
-                if (s0 + e >= n) break;
-                const float w = mn == -INFINITY ? 1.0f : pg_exp2(x[e].x - ms);
-                l += x[e].y * w;
-                o[0] += v[e].x * w;
-                o[1] += v[e].y * w;
-                o[2] += v[e].z * w;
-                o[3] += v[e].w * w;
-            }
+        const int kv_len = part ? max(c.kv_lens[b], 0) : 0;
+        at[part] = ((int64_t)note.x * c.HKV + head) * M + (k - tile * M);
+        n[part] = parts_of(row_limit(g, kv_len, part, row), note.y);
+        if (c.groups == 0) {
+            const int last = min(g.rows * c.G, (tile + 1) * M) - 1;
+            whole = parts_of(row_limit(g, kv_len, true, last / c.G), note.y) == 1;
         }
     }
-    const float f = m == -INFINITY ? (l > 0.0f ? __builtin_nanf("") : 0.0f) : 1.0f / l * (f8 ? c.v_scale[head] : 1.0f);
-    *reinterpret_cast<uint2*>(a.out + (int64_t)t * a.ld_out + (int64_t)h * D + d) =
-        make_uint2(pack_bf16x2(o[0] * f, o[1] * f), pack_bf16x2(o[2] * f, o[3] * f));
+    PagedSum sum;
+    if (on && !whole)
+        for (int part = 0; part < 2; ++part) sum.add_parts<false>(a, at[part], (int64_t)c.HKV * M, n[part], p, P, D, d);
+    sum.across(st, tid, P, kItems, on && p == 0);
+    if (on && !whole && p == 0)
+        sum.store(a.out + (int64_t)t * a.ld_out + (int64_t)h * D + d, f8 ? c.v_scale[head] : 1.0f);
 }
 
 struct PagedPlan {
     int M;       // rows of a tile
     int target;  // slots of one key/value head
     int64_t slots, notes;
-    bool join;
-    size_t ml_at, notes_at, bytes;  // of the workspace
+    bool join;   // a tile may have several parts
+    bool inside; // which the last of its workgroups joins
+    size_t part_at, ml_at, notes_at, bytes;  // of the workspace, whose first bytes are the counters
 };
+
+// Arrival counters, at the front of every workspace whatever the sizes of a call: they stay
+// zero between calls of different sizes.
+constexpr int kPagedCounters = 16384;
 
 // Rows of a tile by what a segment has on average.
 static PagedPlan paged_plan(const bz_paged_kv* d) {
@@ -89,9 +76,11 @@ static PagedPlan paged_plan(const bz_paged_kv* d) {
     p.notes = b.notes;
     p.join = d->groups > 0 || (int64_t)d->table_width * d->page_size > kMinChunk;
     p.slots = p.join ? b.slots : b.notes;
-    const size_t rows_all = (size_t)p.slots * d->HKV * p.M;
-    p.ml_at = p.join ? rows_all * d->D * sizeof(float) : 0;
-    p.notes_at = p.ml_at + (p.join ? rows_all * sizeof(float2) : 0);
+    p.inside = p.join && p.M <= 32 && d->groups == 0 && b.notes * d->HKV <= kPagedCounters && d->HKV <= 256;
+    const size_t rows_all = p.join ? (size_t)p.slots * d->HKV * p.M : 0;
+    p.part_at = kPagedCounters * sizeof(unsigned);
+    p.ml_at = p.part_at + rows_all * d->D * sizeof(float);
+    p.notes_at = p.ml_at + rows_all * sizeof(float2);
     p.bytes = p.notes_at + (size_t)p.notes * sizeof(int2);
     return p;
 }
@@ -115,9 +104,13 @@ static void launch_attn(const PagedKv& c, const PagedAttn& a, const PagedPlan& p
         launch_stream<D, true>(c, a, p.M, st);
     else
         launch_stream<D, false>(c, a, p.M, st);
-    if (p.join) {
-        const int per = c.HQ * (D / 4);
-        hipLaunchKernelGGL((paged_attn_bf16_join<D>), dim3(c.T, (per + 255) / 256), dim3(256), 0, st, c, a, p.M, f8);
+    if (p.join && !p.inside) {
+        const int items = c.HQ * (D / 4);
+        constexpr int P = 1024 / D > 8 ? 8 : 1024 / D;
+        if ((int64_t)c.T * items <= 65536)
+            hipLaunchKernelGGL((paged_attn_bf16_join<D, P>), dim3(c.T, (items * P + 255) / 256), dim3(256), 0, st, c, a, p.M, f8);
+        else
+            hipLaunchKernelGGL((paged_attn_bf16_join<D, 1>), dim3(c.T, (items + 255) / 256), dim3(256), 0, st, c, a, p.M, f8);
     }
 }
 
@@ -150,9 +143,10 @@ extern "C" int bz_paged_attn(const bz_paged_kv* kv, const void* q, int64_t ld_q,
                          ld_out,
                          (float)p.target,
                          p.slots,
-                         reinterpret_cast<float*>(ws),
+                         reinterpret_cast<float*>(ws + p.part_at),
                          reinterpret_cast<float2*>(ws + p.ml_at),
-                         reinterpret_cast<int2*>(ws + p.notes_at)};
+                         reinterpret_cast<int2*>(ws + p.notes_at),
+                         p.inside ? reinterpret_cast<unsigned*>(ws) : nullptr};
     const bool f8 = kv->kv_dtype == BZ_KV_E4M3;
     hipStream_t st = static_cast<hipStream_t>(stream);
     switch (D) {

@@ -284,10 +284,10 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT <= 128 ? 2 : 1) page
         }
     }
     if (lane == 0) st_apart[wave] = apart;
-    const bool whole = u.splits == 1 && c.groups == 0;  // no other slot has keys of these rows
+    const bool whole = w.parts == 1 && c.groups == 0;  // no other slot has keys of these rows
+    const PagedParts parts(a, c, slot, head, M, D);
     const float vs = F8 ? c.v_scale[head] : 1.0f;
-    const int64_t to = ((int64_t)slot * c.HKV + head) * M;
-    if (u.split == 0 && head == 0 && tid == 0) a.notes[tile_note(c, g, u.tile, M)] = make_int2(slot, u.chunk);
+    if (!a.arrived && u.split == 0 && head == 0 && tid == 0) a.notes[tile_note(c, g, u.tile, M)] = make_int2(slot, u.chunk);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         if (16 * rt >= nrow) break;
@@ -299,36 +299,29 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT <= 128 ? 2 : 1) page
         __syncthreads();
         if (rt == 0 && __builtin_amdgcn_readfirstlane(st_apart[0] | st_apart[1] | st_apart[2] | st_apart[3])) {
             paged_rows_apart<D, F8>(c, a, w, slot, head, M, wave, kStreamWaves, lane);
-            return;
+            break;
         }
         for (int i = tid; i < 4 * D; i += 64 * kStreamWaves) {  // 16 rows of D / 4 pieces
             const int r = i / (D / 4), d = 4 * (i % (D / 4)), rr = 16 * rt + r;
             if (rr >= nrow) continue;
-            float mt = st_m[0][rr];
+            PagedSum sum;
 #pragma unroll
-            for (int w = 1; w < kStreamWaves; ++w) mt = fmaxf(mt, st_m[w][rr]);
-            const float ms = mt == -INFINITY ? 0.0f : mt;
-            float lt = 0.0f, o[4] = {};
-#pragma unroll
-            for (int w = 0; w < kStreamWaves; ++w) {
-                const float f = mt == -INFINITY ? 1.0f : pg_exp2(st_m[w][rr] - ms);
-                lt += st_l[w][rr] * f;
-                const float4 x = *reinterpret_cast<const float4*>(&st_acc[w][r][d]);
-                o[0] += x.x * f;
-                o[1] += x.y * f;
-                o[2] += x.z * f;
-                o[3] += x.w * f;
+            for (int k = 0; k < kStreamWaves; ++k) {
+                const float4 x = *reinterpret_cast<const float4*>(&st_acc[k][r][d]);
+                sum.add(st_m[k][rr], st_l[k][rr], x);
             }
             if (whole) {
                 const int k = u.tile * M + rr, row = k / c.G, h = head * c.G + (k - row * c.G);
-                const float f = mt == -INFINITY ? (lt > 0.0f ? __builtin_nanf("") : 0.0f) : 1.0f / lt * vs;
-                uint16_t* p = a.out + (int64_t)(g.first + row) * a.ld_out + (int64_t)h * D + d;
-                *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(o[0] * f, o[1] * f), pack_bf16x2(o[2] * f, o[3] * f));
+                sum.store(a.out + (int64_t)(g.first + row) * a.ld_out + (int64_t)h * D + d, vs);
             } else {
-                *reinterpret_cast<float4*>(a.part + (to + rr) * D + d) = make_float4(o[0], o[1], o[2], o[3]);
-                if (d == 0) a.ml[to + rr] = make_float2(mt, lt);
+                parts.put4(rr * D + d, sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
+                if (d == 0) parts.put_ml(rr, sum.m, sum.l);
             }
         }
+    }
+    if (!whole && a.arrived) {
+        __syncthreads();  // (st_acc is used again)
+        paged_join_last<D, F8>(c, a, w, head, M, tid, reinterpret_cast<float(*)[8]>(&st_acc[0][0][0]), &st_apart[0]);
     }
 }
 

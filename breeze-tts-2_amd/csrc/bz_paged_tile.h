@@ -77,17 +77,18 @@ struct TileStage {
         }
     }
     // bf16 straight into LDS, 16 bytes a lane one after the other: lane l writes piece
-    // l % LR of its row, so it reads the piece that belongs there
+    // l % LR of its row, so it reads the piece that belongs there.  A load's rows are in
+    // its scalar offset; a lane's offsets differ between loads only by the exchange of
+    // pieces, which repeats.
     template <typename X>
     __device__ __forceinline__ static void load_lds(__amdgpu_buffer_rsrc_t r, uint32_t pos, char* tile, int key0, int lane,
                                                     X swap) {
+        constexpr int rows = 64 / LR;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int key = i * (64 / LR) + lane / LR;
+        for (int i = 0; i < N; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                r, (__attribute__((address_space(3))) void*)(tile + (key0 + i * (64 / LR)) * (2 * D)), 16,
-                (uint32_t)key * pos + 16 * ((lane % LR) ^ swap(key0 + key)), 0, 0, 0);
-        }
+                r, (__attribute__((address_space(3))) void*)(tile + (key0 + i * rows) * (2 * D)), 16,
+                (uint32_t)(lane / LR) * pos + 16 * ((lane % LR) ^ swap(i * rows + lane / LR)), i * rows * pos, 0, 0);
     }
     __device__ __forceinline__ bool odd() const {
         bool o = false;
@@ -175,6 +176,17 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) paged_attn_bf16_tile(Pa
     };
     if (tiles > 0) fetch(0, lds);
 
+    // where this lane reads: its key's pieces 2 t + half (t of 0..3, then 8 pieces on), and its columns of keys
+    // 4 half + 0..3 (of an even and an odd block of 32 columns, then 8 pieces on)
+    uint32_t k_at[4], v_at[2];
+    {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) k_at[t] = col * (2 * D) + 16 * ((2 * t + half) ^ k_swap(col));
+        const int i16 = lane & 15, key = 4 * half + (i16 >> 2), piece = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) v_at[t] = key * (2 * D) + 8 * (i16 & 1) + 16 * ((4 * t + piece) ^ v_swap(key));
+    }
+
     for (int tile = 0; tile < tiles; ++tile) {
         const int at = w.begin + kTileKeys * tile;
         char* kt = lds + (tile & 1) * (2 * kTileBytes);
@@ -226,11 +238,10 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) paged_attn_bf16_tile(Pa
 #pragma unroll
             for (int b = 0; b < GB; ++b) {
                 s[b] = pg_f32x16{};
-                const int key = 32 * (b0 + b) + col;
-                const char* kr = kt + key * (2 * D);
+                const char* kr = kt + 32 * (b0 + b) * (2 * D);
 #pragma unroll
                 for (int t = 0; t < T; ++t)
-                    s[b] = pg_mfma32(*reinterpret_cast<const u32x4*>(kr + 16 * ((2 * t + half) ^ k_swap(key))), q[t], s[b]);
+                    s[b] = pg_mfma32(*reinterpret_cast<const u32x4*>(kr + k_at[t & 3] + 128 * (t >> 2)), q[t], s[b]);
             }
             if (mask) {
 #pragma unroll
@@ -273,17 +284,15 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) paged_attn_bf16_tile(Pa
                     pb[b][r / 2] = pack_bf16x2(p0, p1);
                 }
 
-            // values: the lane's columns of keys 16 j + 4 half + 0..3 and + 8
-            const int i16 = lane & 15, in_key = i16 >> 2, piece = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
 #pragma unroll
             for (int b = 0; b < GB; ++b)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const u32x4 pj = {pb[b][4 * j], pb[b][4 * j + 1], pb[b][4 * j + 2], pb[b][4 * j + 3]};
-                    const char* vr = vt + (32 * (b0 + b) + 16 * j + 4 * half + in_key) * (2 * D) + 8 * (i16 & 1);
+                    const char* vr = vt + (32 * (b0 + b) + 16 * j) * (2 * D);
 #pragma unroll
                     for (int t = 0; t < ND; ++t) {
-                        const char* x = vr + 16 * ((4 * t + piece) ^ v_swap(in_key));
+                        const char* x = vr + v_at[t & 1] + 128 * (t >> 1);
                         const uint2 lo = lds_column4(x), hi = lds_column4(x + 8 * (2 * D));
                         acc[t] = pg_mfma32(u32x4{lo.x, lo.y, hi.x, hi.y}, pj, acc[t]);
                     }
@@ -333,13 +342,13 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) paged_attn_bf16_tile(Pa
             }
     }
 
-    const bool whole = u.splits == 1 && c.groups == 0;  // no other slot has keys of these rows
+    const bool whole = w.parts == 1 && c.groups == 0;  // no other slot has keys of these rows
     if (32 * wr + col >= w.rows) return;
-    const int64_t to = ((int64_t)slot * c.HKV + head) * M + 32 * wr + col;
+    const PagedParts parts(a, c, slot, head, M, D);
+    const int rr = 32 * wr + col;
     const float f = m == -INFINITY ? (l > 0.0f ? __builtin_nanf("") : 0.0f) : 1.0f / l * (F8 ? c.v_scale[head] : 1.0f);
     uint16_t* o = a.out + (int64_t)(g.first + row) * a.ld_out + (int64_t)qh * D + 4 * half;
-    float* part = a.part + to * D + 4 * half;
-    if (!whole && half == 0) a.ml[to] = make_float2(m, l);
+    if (!whole && half == 0) parts.put_ml(rr, m, l);
 #pragma unroll
     for (int t = 0; t < ND; ++t)
 #pragma unroll
@@ -348,8 +357,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) paged_attn_bf16_tile(Pa
                 *reinterpret_cast<uint2*>(o + 32 * t + 2 * r) =
                     make_uint2(pack_bf16x2(acc[t][r] * f, acc[t][r + 1] * f), pack_bf16x2(acc[t][r + 2] * f, acc[t][r + 3] * f));
             else
-                *reinterpret_cast<float4*>(part + 32 * t + 2 * r) =
-                    make_float4(acc[t][r], acc[t][r + 1], acc[t][r + 2], acc[t][r + 3]);
+                parts.put4(rr * D + 4 * half + 32 * t + 2 * r, acc[t][r], acc[t][r + 1], acc[t][r + 2], acc[t][r + 3]);
         }
 }
 

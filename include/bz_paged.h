@@ -95,9 +95,9 @@ int bz_paged_rope_cache(const bz_paged_kv* kv, const void* qkv, int64_t ld_qkv,
  * head h / (HQ / HKV).  q bf16 [T][ld_q], out bf16 [T][ld_out] (must not overlap
  * q), head h at columns h D ..  A row that attends nothing is zero.  Keys and
  * values that a row does not attend have no part in it, whatever they hold.
- * scale > 0.  workspace: bz_paged_attn_workspace bytes, 16-byte aligned, its
- * contents irrelevant before and after; calls that overlap in time need one
- * each. */
+ * scale > 0.  workspace: bz_paged_attn_workspace bytes, 16-byte aligned, zeroed
+ * once before its first use (the kernels leave the counters at its front at zero
+ * again, whatever the sizes of the calls); calls that share one must not overlap. */
 int bz_paged_attn(const bz_paged_kv* kv, const void* q, int64_t ld_q,
                   float scale, void* workspace, size_t workspace_bytes,
                   void* out, int64_t ld_out, void* stream);

@@ -72,6 +72,7 @@ def no_gpu(monkeypatch):
         raise AssertionError("reached the library")
 
     monkeypatch.setattr(paged, "_call", reached)
+    monkeypatch.setattr(paged, "_workspace_bytes", reached)
 
 
 def _args(kv="bf16", **kw):
