@@ -45,6 +45,7 @@ struct PagedAttn {
     uint16_t* out;
     int64_t ld_out;
     float target;  // slots of one key/value head that the keys are cut for
+    int min_chunk;
     int64_t slots;
     float* part;   // [slots][HKV][M][D] accumulators
     float2* ml;    // [slots][HKV][M] (m, l)
@@ -74,8 +75,8 @@ struct PagedWork {
     int all;      // the keys before it are attended by all rows
     int parts;    // chunks that have keys of the tile (or one that has none)
 };
-__device__ __forceinline__ bool paged_work(const PagedKv& c, int M, float target, int slot, int lane, PagedWork& w) {
-    w.u = paged_slot(c, M, target, slot, lane);
+__device__ __forceinline__ bool paged_work(const PagedKv& c, const PagedAttn& a, int M, int slot, int lane, PagedWork& w) {
+    w.u = paged_slot(c, M, a.target, a.min_chunk, slot, lane);
     if (!w.u.any) return false;
     const PagedSeg& g = w.u.seg;
     w.own = g.seq < c.B;
@@ -171,34 +172,49 @@ struct PagedSum {
         o[2] = o[2] * f + v.z * g;
         o[3] = o[3] * f + v.w * g;
     }
-    // parts first, first + stride, .. of n; part i is the row at + i step of [M] rows
+    // U parts: s, s + stride, .. (behind n the last again, not added)
+    template <bool AGENT, int U>
+    __device__ __forceinline__ void add_batch(const PagedAttn& a, int64_t at, int64_t step, int n, int s, int stride, int D,
+                                              int d) {
+        float2 x[U];
+        float4 v[U];
+#pragma unroll
+        for (int e = 0; e < U; ++e) {
+            const int64_t i = at + min(s + e * stride, n - 1) * step;
+            if constexpr (AGENT) {
+                const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t*>(a.ml + i), __ATOMIC_RELAXED,
+                                                     __HIP_MEMORY_SCOPE_AGENT);
+                x[e] = make_float2(__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32)));
+                const uint64_t* p = reinterpret_cast<const uint64_t*>(a.part + i * D + d);
+                const uint64_t w0 = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                const uint64_t w1 = __hip_atomic_load(p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                v[e] = make_float4(__uint_as_float((uint32_t)w0), __uint_as_float((uint32_t)(w0 >> 32)),
+                                   __uint_as_float((uint32_t)w1), __uint_as_float((uint32_t)(w1 >> 32)));
+            } else {
+                x[e] = a.ml[i];
+                v[e] = *reinterpret_cast<const float4*>(a.part + i * D + d);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < U; ++e)
+            if (s + e * stride < n) add(x[e].x, x[e].y, v[e]);
+    }
+    // parts first, first + stride, .. of n; part i is the row at + i step of [M] rows.  As many
+    // under way at a time as are left, up to 16: a round trip to the parts takes about 2 us.
     template <bool AGENT>
     __device__ __forceinline__ void add_parts(const PagedAttn& a, int64_t at, int64_t step, int n, int first, int stride,
                                               int D, int d) {
-        constexpr int U = 8;  // loads under way at a time
-        for (int s0 = first; s0 < n; s0 += U * stride) {
-            float2 x[U];
-            float4 v[U];
-#pragma unroll
-            for (int e = 0; e < U; ++e) {
-                const int64_t i = at + min(s0 + e * stride, n - 1) * step;
-                if constexpr (AGENT) {
-                    const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t*>(a.ml + i), __ATOMIC_RELAXED,
-                                                         __HIP_MEMORY_SCOPE_AGENT);
-                    x[e] = make_float2(__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32)));
-                    const uint64_t* p = reinterpret_cast<const uint64_t*>(a.part + i * D + d);
-                    const uint64_t w0 = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    const uint64_t w1 = __hip_atomic_load(p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    v[e] = make_float4(__uint_as_float((uint32_t)w0), __uint_as_float((uint32_t)(w0 >> 32)),
-                                       __uint_as_float((uint32_t)w1), __uint_as_float((uint32_t)(w1 >> 32)));
-                } else {
-                    x[e] = a.ml[i];
-                    v[e] = *reinterpret_cast<const float4*>(a.part + i * D + d);
-                }
+        for (int s = first; s < n;) {
+            if (n - s > 8 * stride) {
+                add_batch<AGENT, 16>(a, at, step, n, s, stride, D, d);
+                s += 16 * stride;
+            } else if (n - s > 2 * stride) {
+                add_batch<AGENT, 8>(a, at, step, n, s, stride, D, d);
+                s += 8 * stride;
+            } else {
+                add_batch<AGENT, 2>(a, at, step, n, s, stride, D, d);
+                s += 2 * stride;
             }
-#pragma unroll
-            for (int e = 0; e < U; ++e)
-                if (s0 + e * stride < n) add(x[e].x, x[e].y, v[e]);
         }
     }
     // sums of P threads, `apart` threads from each other, into the first's, through LDS [256][8]

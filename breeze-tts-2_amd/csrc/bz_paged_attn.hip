@@ -6,7 +6,12 @@
 
 namespace bz {
 
-constexpr int kPagedWorkgroups = 1024;  // that the keys are cut for
+// Workgroups that the keys are cut for: as many as run at once, so that none starts late.
+static int paged_workgroups(int D, bool f8, int M) {
+    if (M > 32) return 1024;
+    if (D == 256) return (f8 ? 512 : 256);
+    return (D == 64 ? (M == 16 ? 1024 : 768) : (M == 16 ? 768 : 512));
+}
 
 // The parts of a row joined in a launch of its own: its prefix's, then its own.
 // Four columns of a head to P threads, which take its parts in turn.
@@ -54,6 +59,7 @@ __global__ void __launch_bounds__(256) paged_attn_bf16_join(PagedKv c, PagedAttn
 struct PagedPlan {
     int M;       // rows of a tile
     int target;  // slots of one key/value head
+    int min_chunk;
     int64_t slots, notes;
     bool join;   // a tile may have several parts
     bool inside; // which the last of its workgroups joins
@@ -71,10 +77,14 @@ static PagedPlan paged_plan(const bz_paged_kv* d) {
     const int64_t segs = d->groups > 0 ? std::min(d->B, d->groups) : d->B;
     const int64_t rows = ((int64_t)d->T + segs - 1) / segs * G;
     p.M = rows <= 16 ? 16 : (rows <= 32 && d->D < 256 ? 32 : (rows <= 64 ? 64 : 128));
-    p.target = std::max(1, kPagedWorkgroups / d->HKV);
+    p.target = std::max(1, paged_workgroups(d->D, d->kv_dtype != BZ_DT_BF16, p.M) / d->HKV);
+    // a step for each of four waves; two where a part has more rows to be joined (verification
+    // of 5 tokens, 16 sequences of up to 2043 positions, 8 / 2 heads of 128: 20.4 us with 128 and 17.2
+    // with 256; one token, 2 of 610, 16 / 8 heads: 9.4 and 9.9)
+    p.min_chunk = p.M == 16 ? 128 : 256;
     const PagedBounds b = paged_bounds(d, p.M, p.target);
     p.notes = b.notes;
-    p.join = d->groups > 0 || (int64_t)d->table_width * d->page_size > kMinChunk;
+    p.join = d->groups > 0 || (int64_t)d->table_width * d->page_size > p.min_chunk;
     p.slots = p.join ? b.slots : b.notes;
     p.inside = p.join && p.M <= 32 && d->groups == 0 && b.notes * d->HKV <= kPagedCounters && d->HKV <= 256;
     const size_t rows_all = p.join ? (size_t)p.slots * d->HKV * p.M : 0;
@@ -142,6 +152,7 @@ extern "C" int bz_paged_attn(const bz_paged_kv* kv, const void* q, int64_t ld_q,
                          static_cast<uint16_t*>(out),
                          ld_out,
                          (float)p.target,
+                         p.min_chunk,
                          p.slots,
                          reinterpret_cast<float*>(ws + p.part_at),
                          reinterpret_cast<float2*>(ws + p.ml_at),

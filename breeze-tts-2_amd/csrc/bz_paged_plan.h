@@ -8,14 +8,12 @@
 // the device alone, so every workgroup works out the slots by itself from the
 // lengths (64 segments at a time, one wave scan each).  C is the same for all segments, so
 // that workgroups have like amounts however ragged the batch is: about
-// 1 / target of all keys, at least kMinChunk.
+// 1 / target of all keys, at least min_chunk.
 #pragma once
 
 #include "bz_paged_kv.h"
 
 namespace bz {
-
-constexpr int kMinChunk = 128;
 
 struct PagedSeg {
     int first, rows;  // rows of q and out
@@ -80,7 +78,8 @@ struct PagedSlot {
 
 __device__ __forceinline__ int tiles_of(const PagedKv& c, int rows, int M) { return (rows * c.G + M - 1) / M; }
 
-__device__ __forceinline__ PagedSlot paged_slot(const PagedKv& c, int M, float target, int slot, int lane) {
+__device__ __forceinline__ PagedSlot paged_slot(const PagedKv& c, int M, float target, int min_chunk, int slot,
+                                                int lane) {
     const int n = c.B + c.groups;
     float work = 0.0f;
     PagedSeg g = {};
@@ -90,7 +89,7 @@ __device__ __forceinline__ PagedSlot paged_slot(const PagedKv& c, int M, float t
     }
     work = wave_sum(work);
     const int chunk = __builtin_amdgcn_readfirstlane(
-        max(kMinChunk, ((int)ceilf(fminf(work / target, 1073741824.0f)) + 31) & ~31));
+        max(min_chunk, ((int)ceilf(fminf(work / target, 1073741824.0f)) + 31) & ~31));
     PagedSlot r = {};
     r.chunk = chunk;
     int base = 0;

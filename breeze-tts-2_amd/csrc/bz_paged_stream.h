@@ -75,7 +75,7 @@ __device__ __forceinline__ int stream_col(int t, int i) {
 
 // RT row tiles of 16.
 template <int D, bool F8, int RT>
-__global__ void __launch_bounds__(64 * kStreamWaves, D * RT <= 128 ? 2 : 1) paged_attn_bf16_stream(PagedKv c, PagedAttn a) {
+__global__ void __launch_bounds__(64 * kStreamWaves, D * RT < 256 || F8 || D == 128 ? 2 : 1) paged_attn_bf16_stream(PagedKv c, PagedAttn a) {
     using S = StreamStep<D, F8>;
     constexpr int M = 16 * RT, T = D / 32, NT = D / 16;
     constexpr int kRow = D + 4;
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT <= 128 ? 2 : 1) page
     const int slot = blockIdx.x / c.HKV, head = blockIdx.x - slot * c.HKV;
 
     PagedWork w;
-    if (!paged_work(c, M, a.target, slot, lane, w)) return;
+    if (!paged_work(c, a, M, slot, lane, w)) return;
     const PagedSlot& u = w.u;
     const PagedSeg& g = u.seg;
     const bool own = w.own;

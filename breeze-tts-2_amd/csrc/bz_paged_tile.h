@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) paged_attn_bf16_tile(Pa
     const int slot = blockIdx.x / c.HKV, head = blockIdx.x - slot * c.HKV;
 
     PagedWork w;
-    if (!paged_work(c, M, a.target, slot, lane, w)) return;
+    if (!paged_work(c, a, M, slot, lane, w)) return;
     const PagedSlot& u = w.u;
     const PagedSeg& g = u.seg;
 
