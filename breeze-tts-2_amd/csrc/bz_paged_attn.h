@@ -38,18 +38,22 @@ __device__ __forceinline__ pg_f32x16 pg_mfma32(u32x4 a, u32x4 b, pg_f32x16 c) {
 // 2^x with the hardware instruction alone (below 2^-126 it gives zero).
 __device__ __forceinline__ float pg_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The parts of one launch's slots, to be joined.
+struct PagedPartsAt {
+    float* part;          // [slots][HKV][M][D] accumulators
+    float2* ml;           // [slots][HKV][M] (m, l)
+    int2* notes;          // (first slot, keys of a chunk) of a sequence's tile
+    int2* prefix_notes;   // and of a prefix's
+};
+
 struct PagedAttn {
     const uint16_t* q;
     int64_t ld_q;
     float scale;
     uint16_t* out;
     int64_t ld_out;
-    float target;  // slots of one key/value head that the keys are cut for
-    int min_chunk;
-    int64_t slots;
-    float* part;   // [slots][HKV][M][D] accumulators
-    float2* ml;    // [slots][HKV][M] (m, l)
-    int2* notes;   // [notes] (first slot, keys of a chunk) of a tile
+    PagedCut cut;
+    PagedPartsAt to;
     // [notes][HKV] arrivals of a tile's parts, zero between calls; the last to arrive
     // joins them.  NULL: a launch of its own does.
     unsigned* arrived;
@@ -76,7 +80,7 @@ struct PagedWork {
     int parts;    // chunks that have keys of the tile (or one that has none)
 };
 __device__ __forceinline__ bool paged_work(const PagedKv& c, const PagedAttn& a, int M, int slot, int lane, PagedWork& w) {
-    w.u = paged_slot(c, M, a.target, a.min_chunk, slot, lane);
+    w.u = paged_slot(c, a.cut, slot, lane);
     if (!w.u.any) return false;
     const PagedSeg& g = w.u.seg;
     w.own = g.seq < c.B;
@@ -88,7 +92,11 @@ __device__ __forceinline__ bool paged_work(const PagedKv& c, const PagedAttn& a,
     w.begin = w.u.split * w.u.chunk;
     w.end = min(w.begin + w.u.chunk, tile_end);
     w.all = row_limit(g, w.kv_len, w.own, first / c.G);
-    return w.u.split < w.parts;  // else a chunk behind the tile's last row
+    return w.u.split < w.parts;
+}
+// The tile's first slot, noted by the workgroup that has it (of one head).
+__device__ __forceinline__ void note_tile(const PagedKv& c, const PagedAttn& a, const PagedWork& w, int M, int slot) {
+    (w.own ? a.to.notes : a.to.prefix_notes)[tile_note(c, w.u.seg, w.u.tile, M)] = make_int2(slot, w.u.chunk);
 }
 
 // One 16-position piece of a segment's keys, none of whose rows is read beyond `n`.
@@ -131,8 +139,8 @@ struct PagedParts {
     bool agent;
     __device__ __forceinline__ PagedParts(const PagedAttn& a, const PagedKv& c, int slot, int head, int M, int D) {
         const int64_t at = ((int64_t)slot * c.HKV + head) * M;
-        acc = buffer_rsrc(a.part + at * D, (uint32_t)(M * D) * 4u);
-        ml = buffer_rsrc(a.ml + at, (uint32_t)M * 8u);
+        acc = buffer_rsrc(a.to.part + at * D, (uint32_t)(M * D) * 4u);
+        ml = buffer_rsrc(a.to.ml + at, (uint32_t)M * 8u);
         agent = a.arrived != nullptr;
     }
     __device__ __forceinline__ void put(int i, float v) const {
@@ -174,7 +182,7 @@ struct PagedSum {
     }
     // U parts: s, s + stride, .. (behind n the last again, not added)
     template <bool AGENT, int U>
-    __device__ __forceinline__ void add_batch(const PagedAttn& a, int64_t at, int64_t step, int n, int s, int stride, int D,
+    __device__ __forceinline__ void add_batch(const PagedPartsAt& a, int64_t at, int64_t step, int n, int s, int stride, int D,
                                               int d) {
         float2 x[U];
         float4 v[U];
@@ -202,7 +210,7 @@ struct PagedSum {
     // parts first, first + stride, .. of n; part i is the row at + i step of [M] rows.  As many
     // under way at a time as are left, up to 16: a round trip to the parts takes about 2 us.
     template <bool AGENT>
-    __device__ __forceinline__ void add_parts(const PagedAttn& a, int64_t at, int64_t step, int n, int first, int stride,
+    __device__ __forceinline__ void add_parts(const PagedPartsAt& a, int64_t at, int64_t step, int n, int first, int stride,
                                               int D, int d) {
         for (int s = first; s < n;) {
             if (n - s > 8 * stride) {
@@ -261,7 +269,7 @@ __device__ __forceinline__ void paged_join_last(const PagedKv& c, const PagedAtt
         PagedSum sum;
         const bool on = P > 1 ? p < P : i < items;
         const int r = on ? i / (D / 4) : 0, d = 4 * (i % (D / 4));
-        if (on) sum.add_parts<true>(a, at0 + r, step, w.parts, p, P, D, d);
+        if (on) sum.add_parts<true>(a.to, at0 + r, step, w.parts, p, P, D, d);
         sum.across(st, tid, P, items, on && p == 0);
         if (on && p == 0) {
             const int k = w.u.tile * M + r, row = k / c.G, h = head * c.G + (k - row * c.G);
@@ -299,6 +307,7 @@ __device__ __forceinline__ void paged_rows_apart(const PagedKv& c, const PagedAt
             if (there) {
                 const char* kr = c.k + page * c.k_page + head * c.k_head + at * c.k_pos;
                 s = 0.0f;
+#pragma unroll 4
                 for (int d = 0; d < D; ++d)
                     s += bf16_to_f32(q[d]) * (F8 ? __builtin_amdgcn_cvt_f32_fp8((int)reinterpret_cast<const uint8_t*>(kr)[d], 0)
                                                  : bf16_to_f32(reinterpret_cast<const uint16_t*>(kr)[d]));

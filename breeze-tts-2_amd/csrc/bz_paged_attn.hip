@@ -8,7 +8,7 @@ namespace bz {
 
 // Workgroups that the keys are cut for: as many as run at once, so that none starts late.
 static int paged_workgroups(int D, bool f8, int M) {
-    if (M > 32) return 1024;
+    if (M > 32) return 384;
     if (D == 256) return (f8 ? 512 : 256);
     return (D == 64 ? (M == 16 ? 1024 : 768) : (M == 16 ? 768 : 512));
 }
@@ -16,10 +16,10 @@ static int paged_workgroups(int D, bool f8, int M) {
 // The parts of a row joined in a launch of its own: its prefix's, then its own.
 // Four columns of a head to P threads, which take its parts in turn.
 template <int D, int P>
-__global__ void __launch_bounds__(256) paged_attn_bf16_join(PagedKv c, PagedAttn a, int M, bool f8) {
+__global__ void __launch_bounds__(256) paged_attn_bf16_join(PagedKv c, PagedAttn a, bool f8) {
     constexpr int kItems = 256 / P;
     __shared__ float st[P > 1 ? 256 : 1][8];
-    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, M = a.cut.M;
     const int b = seq_of_row(c, t, lane);
     if (b >= c.B) return;
     const PagedSeg own = paged_seg(c, b);
@@ -38,8 +38,8 @@ __global__ void __launch_bounds__(256) paged_attn_bf16_join(PagedKv c, PagedAttn
     for (int part = 0; part < 2; ++part) {
         if (!part && pre < 0) continue;
         const PagedSeg g = part ? own : paged_seg(c, c.B + pre);
-        const int k = (t - g.first) * c.G + (min(h, c.HQ - 1) - head * c.G), tile = k / M;
-        const int2 note = a.notes[tile_note(c, g, tile, M)];
+        const int k = (t - g.first) * c.G + (min(h, c.HQ - 1) - head * c.G), tile = k >> a.cut.log2_M;
+        const int2 note = (part ? a.to.notes : a.to.prefix_notes)[tile_note(c, g, tile, M)];
         const int kv_len = part ? max(c.kv_lens[b], 0) : 0;
         at[part] = ((int64_t)note.x * c.HKV + head) * M + (k - tile * M);
         n[part] = parts_of(row_limit(g, kv_len, part, row), note.y);
@@ -50,78 +50,103 @@ __global__ void __launch_bounds__(256) paged_attn_bf16_join(PagedKv c, PagedAttn
     }
     PagedSum sum;
     if (on && !whole)
-        for (int part = 0; part < 2; ++part) sum.add_parts<false>(a, at[part], (int64_t)c.HKV * M, n[part], p, P, D, d);
+        for (int part = 0; part < 2; ++part) sum.add_parts<false>(a.to, at[part], (int64_t)c.HKV * M, n[part], p, P, D, d);
     sum.across(st, tid, P, kItems, on && p == 0);
     if (on && !whole && p == 0)
         sum.store(a.out + (int64_t)t * a.ld_out + (int64_t)h * D + d, f8 ? c.v_scale[head] : 1.0f);
 }
 
 struct PagedPlan {
-    int M;       // rows of a tile
-    int target;  // slots of one key/value head
-    int min_chunk;
-    int64_t slots, notes;
-    bool join;   // a tile may have several parts
-    bool inside; // which the last of its workgroups joins
-    size_t part_at, ml_at, notes_at, bytes;  // of the workspace, whose first bytes are the counters
+    PagedCut cut;
+    int64_t slots;
+    bool join;    // a tile may have several parts
+    bool inside;  // which the last of its workgroups joins
+    size_t part_at, ml_at, notes_at, prefix_notes_at;  // in the workspace, whose first bytes are the counters
+    size_t bytes;
 };
 
 // Arrival counters, at the front of every workspace whatever the sizes of a call: they stay
 // zero between calls of different sizes.
 constexpr int kPagedCounters = 16384;
 
-// Rows of a tile by what a segment has on average.
+// Rows of a tile for segments of `rows` query rows.
+static int paged_tile_rows(int64_t rows, int D, bool f8) {
+    if (rows <= 16) return 16;
+    if (D == 256) return rows <= 64 || f8 ? 64 : 128;  // (eight waves of e4m3 on its way do not fit the registers)
+    return rows <= 32 ? 32 : (rows <= 64 ? 64 : 128);
+}
+
 static PagedPlan paged_plan(const bz_paged_kv* d) {
     PagedPlan p = {};
     const int G = d->HQ / d->HKV;
+    const bool f8 = d->kv_dtype != BZ_DT_BF16;
+    // by what a segment has on average, a prefix's or a sequence's
     const int64_t segs = d->groups > 0 ? std::min(d->B, d->groups) : d->B;
-    const int64_t rows = ((int64_t)d->T + segs - 1) / segs * G;
-    p.M = rows <= 16 ? 16 : (rows <= 32 && d->D < 256 ? 32 : (rows <= 64 ? 64 : 128));
-    p.target = std::max(1, paged_workgroups(d->D, d->kv_dtype != BZ_DT_BF16, p.M) / d->HKV);
+    const int M = paged_tile_rows(((int64_t)d->T + segs - 1) / segs * G, d->D, f8);
+    const int target = std::max(1, paged_workgroups(d->D, f8, M) / d->HKV);
+    p.cut.M = M;
+    p.cut.log2_M = __builtin_ctz(M);
+    p.cut.target = (float)target;
     // a step for each of four waves; two where a part has more rows to be joined (verification
     // of 5 tokens, 16 sequences of up to 2043 positions, 8 / 2 heads of 128: 20.4 us with 128 and 17.2
     // with 256; one token, 2 of 610, 16 / 8 heads: 9.4 and 9.9)
-    p.min_chunk = p.M == 16 ? 128 : 256;
-    const PagedBounds b = paged_bounds(d, p.M, p.target);
-    p.notes = b.notes;
-    p.join = d->groups > 0 || (int64_t)d->table_width * d->page_size > p.min_chunk;
-    p.slots = p.join ? b.slots : b.notes;
-    p.inside = p.join && p.M <= 32 && d->groups == 0 && b.notes * d->HKV <= kPagedCounters && d->HKV <= 256;
-    const size_t rows_all = p.join ? (size_t)p.slots * d->HKV * p.M : 0;
-    p.part_at = kPagedCounters * sizeof(unsigned);
-    p.ml_at = p.part_at + rows_all * d->D * sizeof(float);
-    p.notes_at = p.ml_at + rows_all * sizeof(float2);
-    p.bytes = p.notes_at + (size_t)p.notes * sizeof(int2);
+    p.cut.min_chunk = M == 16 ? 128 : 256;
+    // tiles that there can be, and with them notes
+    const int64_t notes = (int64_t)d->T * G / M + d->B, prefix_notes = d->groups > 0 ? (int64_t)d->T * G / M + d->groups : 0;
+    p.join = d->groups > 0 || (int64_t)d->table_width * d->page_size > p.cut.min_chunk;
+    p.inside = p.join && M <= 32 && d->groups == 0 && notes * d->HKV <= kPagedCounters && d->HKV <= 256;
+    p.slots = p.join ? paged_slots(notes + prefix_notes, target) : notes;
+    p.bytes = kPagedCounters * sizeof(unsigned);
+    auto take = [&](size_t n) {
+        const size_t at = p.bytes;
+        p.bytes += (n + 15) & ~(size_t)15;
+        return at;
+    };
+    const size_t rows = p.join ? (size_t)p.slots * d->HKV * M : 0;
+    p.part_at = take(rows * d->D * sizeof(float));
+    p.ml_at = take(rows * sizeof(float2));
+    p.notes_at = take((size_t)notes * sizeof(int2));
+    p.prefix_notes_at = take((size_t)prefix_notes * sizeof(int2));
     return p;
 }
 
 template <int D, bool F8>
-static void launch_stream(const PagedKv& c, const PagedAttn& a, int M, hipStream_t st) {
-    const dim3 grid((unsigned)(a.slots * c.HKV)), block(64 * kStreamWaves);
-    if (M == 16)
-        hipLaunchKernelGGL((paged_attn_bf16_stream<D, F8, 1>), grid, block, 0, st, c, a);
-    else if (M == 128)
-        hipLaunchKernelGGL((paged_attn_bf16_tile<D, F8, 4>), grid, block, 0, st, c, a);
-    else if (M == 64)
-        hipLaunchKernelGGL((paged_attn_bf16_tile<D, F8, 2>), grid, block, 0, st, c, a);
-    else if constexpr (D < 256)
-        hipLaunchKernelGGL((paged_attn_bf16_stream<D, F8, 2>), grid, block, 0, st, c, a);
+static void launch_tiles(const PagedKv& c, const PagedAttn& a, int64_t slots, hipStream_t st) {
+    const dim3 grid((unsigned)(slots * c.HKV));
+    switch (a.cut.M) {
+        case 16:
+            hipLaunchKernelGGL((paged_attn_bf16_stream<D, F8, 1>), grid, dim3(256), 0, st, c, a);
+            break;
+        case 32:
+            if constexpr (D < 256) hipLaunchKernelGGL((paged_attn_bf16_stream<D, F8, 2>), grid, dim3(256), 0, st, c, a);
+            break;
+        case 64:
+            hipLaunchKernelGGL((paged_attn_bf16_tile<D, F8, 4, true>), grid, dim3(256), 0, st, c, a);
+            break;
+        default:
+            if constexpr (D == 256 && !F8)
+                hipLaunchKernelGGL((paged_attn_bf16_tile<D, F8, 8, true>), grid, dim3(512), 0, st, c, a);
+            else if constexpr (D < 256)
+                hipLaunchKernelGGL((paged_attn_bf16_tile<D, F8, 4, false>), grid, dim3(256), 0, st, c, a);
+    }
 }
 
 template <int D>
-static void launch_attn(const PagedKv& c, const PagedAttn& a, const PagedPlan& p, bool f8, hipStream_t st) {
+static void launch_attn(const PagedKv& c, PagedAttn a, const PagedPlan& p, char* ws, bool f8, hipStream_t st) {
+    a.cut = p.cut;
+    a.to = {reinterpret_cast<float*>(ws + p.part_at), reinterpret_cast<float2*>(ws + p.ml_at),
+            reinterpret_cast<int2*>(ws + p.notes_at), reinterpret_cast<int2*>(ws + p.prefix_notes_at)};
     if (f8)
-        launch_stream<D, true>(c, a, p.M, st);
+        launch_tiles<D, true>(c, a, p.slots, st);
     else
-        launch_stream<D, false>(c, a, p.M, st);
-    if (p.join && !p.inside) {
-        const int items = c.HQ * (D / 4);
-        constexpr int P = 1024 / D > 8 ? 8 : 1024 / D;
-        if ((int64_t)c.T * items <= 65536)
-            hipLaunchKernelGGL((paged_attn_bf16_join<D, P>), dim3(c.T, (items * P + 255) / 256), dim3(256), 0, st, c, a, p.M, f8);
-        else
-            hipLaunchKernelGGL((paged_attn_bf16_join<D, 1>), dim3(c.T, (items + 255) / 256), dim3(256), 0, st, c, a, p.M, f8);
-    }
+        launch_tiles<D, false>(c, a, p.slots, st);
+    if (!p.join || p.inside) return;
+    const int items = c.HQ * (D / 4);
+    constexpr int P = 1024 / D > 8 ? 8 : 1024 / D;
+    if ((int64_t)c.T * items <= 65536)
+        hipLaunchKernelGGL((paged_attn_bf16_join<D, P>), dim3(c.T, (items * P + 255) / 256), dim3(256), 0, st, c, a, f8);
+    else
+        hipLaunchKernelGGL((paged_attn_bf16_join<D, 1>), dim3(c.T, (items + 255) / 256), dim3(256), 0, st, c, a, f8);
 }
 
 }  // namespace bz
@@ -145,25 +170,20 @@ extern "C" int bz_paged_attn(const bz_paged_kv* kv, const void* q, int64_t ld_q,
     const PagedPlan p = paged_plan(kv);
     if (p.slots * c.HKV > 0x7FFFFFFF) return BZ_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < p.bytes) return BZ_ERR_INVALID_ARG;
-    char* ws = static_cast<char*>(workspace);
-    const PagedAttn a = {static_cast<const uint16_t*>(q),
-                         ld_q,
-                         scale,
-                         static_cast<uint16_t*>(out),
-                         ld_out,
-                         (float)p.target,
-                         p.min_chunk,
-                         p.slots,
-                         reinterpret_cast<float*>(ws + p.part_at),
-                         reinterpret_cast<float2*>(ws + p.ml_at),
-                         reinterpret_cast<int2*>(ws + p.notes_at),
-                         p.inside ? reinterpret_cast<unsigned*>(ws) : nullptr};
+    PagedAttn a = {};
+    a.q = static_cast<const uint16_t*>(q);
+    a.ld_q = ld_q;
+    a.scale = scale;
+    a.out = static_cast<uint16_t*>(out);
+    a.ld_out = ld_out;
+    a.arrived = p.inside ? static_cast<unsigned*>(workspace) : nullptr;
     const bool f8 = kv->kv_dtype == BZ_KV_E4M3;
+    char* ws = static_cast<char*>(workspace);
     hipStream_t st = static_cast<hipStream_t>(stream);
     switch (D) {
-        case 64: launch_attn<64>(c, a, p, f8, st); break;
-        case 128: launch_attn<128>(c, a, p, f8, st); break;
-        default: launch_attn<256>(c, a, p, f8, st); break;
+        case 64: launch_attn<64>(c, a, p, ws, f8, st); break;
+        case 128: launch_attn<128>(c, a, p, ws, f8, st); break;
+        default: launch_attn<256>(c, a, p, ws, f8, st); break;
     }
     return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
 }

@@ -1,14 +1,14 @@
-// How the work of one attention call over a paged cache is cut (device side).
+// How the work of one attention launch over a paged cache is cut (device side).
 //
 // A segment is a set of rows and the keys they attend together: sequence b's rows
 // and its own positions (segment b), or a shared prefix and the rows of all its
 // sequences (segment B + g).  A segment's rows, one for each query head of a
-// key/value head, go in tiles of M; its keys in chunks of C; a (tile, chunk) is a
-// slot, and a workgroup takes a slot of one key/value head.  Lengths are known on
-// the device alone, so every workgroup works out the slots by itself from the
-// lengths (64 segments at a time, one wave scan each).  C is the same for all segments, so
-// that workgroups have like amounts however ragged the batch is: about
-// 1 / target of all keys, at least min_chunk.
+// key/value head, go in tiles of M; the keys that a tile attends in chunks of C; a
+// (tile, chunk) is a slot, and a workgroup takes a slot of one key/value head.
+// Lengths are known on the device alone, so every workgroup works out the slots by
+// itself from the lengths (64 segments at a time, one wave scan each).  C is the
+// same for all segments, so that workgroups have like amounts however ragged the batch
+// is: about 1 / target of all keys, at least min_chunk.
 #pragma once
 
 #include "bz_paged_kv.h"
@@ -21,6 +21,7 @@ struct PagedSeg {
     int seq;    // the sequence, or B + the prefix
 };
 
+// Segment B + p: prefix p.
 __device__ __forceinline__ PagedSeg paged_seg(const PagedKv& c, int s) {
     PagedSeg g = {0, 0, 0, s};
     if (s < c.B) {
@@ -28,7 +29,7 @@ __device__ __forceinline__ PagedSeg paged_seg(const PagedKv& c, int s) {
         g.first = r.first;
         g.rows = r.end - r.first;
         g.keys = min(max(c.kv_lens[s], 0), c.width << c.shift);
-    } else if (s < c.B + c.groups) {
+    } else {
         const int p = s - c.B;
         int lo = 0, hi = c.B;
         if (c.prefix_seqs) {
@@ -70,33 +71,77 @@ __device__ __forceinline__ int wave_scan(int v) {
 
 struct PagedSlot {
     PagedSeg seg;
-    int tile, split, splits;  // splits of its segment
-    int chunk;                // keys of a chunk
-    int first_slot;           // of its tile
+    int tile, split;
+    int chunk;       // keys of a chunk
+    int first_slot;  // of its tile
     bool any;
 };
 
-__device__ __forceinline__ int tiles_of(const PagedKv& c, int rows, int M) { return (rows * c.G + M - 1) / M; }
+struct PagedCut {
+    int M, log2_M;
+    float target;  // slots of one key/value head that the keys are cut for
+    int min_chunk;
+};
 
-__device__ __forceinline__ PagedSlot paged_slot(const PagedKv& c, int M, float target, int min_chunk, int slot,
-                                                int lane) {
-    const int n = c.B + c.groups;
+// How a segment's tiles are cut: tile t has 1 + (number of i >= 1 with from(i) <= t) chunks.
+struct SegCut {
+    int tiles, whole, most;  // chunks that all tiles have, that any has
+    int behind;              // keys before the first row's own position (all attend them)
+    int chunk, G, log2_M;
+    // the first tile with more than i chunks, i >= whole: that of row i chunk - behind
+    __device__ __forceinline__ int from(int i) const {
+        return (int)min(((int64_t)i * chunk - behind) * G >> log2_M, (int64_t)tiles);
+    }
+    __device__ __forceinline__ int slots() const {
+        int n = tiles * whole;
+        for (int i = whole; i < most; ++i) n += tiles - from(i);
+        return n;
+    }
+};
+__device__ __forceinline__ SegCut seg_cut(const PagedKv& c, const PagedSeg& g, int chunk, const PagedCut& cut) {
+    SegCut k;
+    k.tiles = (g.rows * c.G + cut.M - 1) >> cut.log2_M;
+    k.chunk = chunk;
+    k.G = c.G;
+    k.log2_M = cut.log2_M;
+    k.most = max(1, (int)(((unsigned)g.keys + chunk - 1) / (unsigned)chunk));
+    // row i of a sequence attends behind + i + 1 keys
+    k.behind = g.seq < c.B ? max(c.kv_lens[min(g.seq, c.B - 1)], 0) - g.rows : g.keys;
+    k.whole = k.most;
+    if (g.seq < c.B && g.rows > 1) k.whole = min(k.most, k.behind >= 0 ? (int)((unsigned)k.behind / (unsigned)chunk) + 1 : 1);
+    return k;
+}
+
+// Slot `slot`: the prefixes' come first, and of a sequence its last tiles' (whose rows
+// attend most), so that long pieces start early.
+__device__ __forceinline__ PagedSlot paged_slot(const PagedKv& c, const PagedCut& cut, int slot, int lane) {
+    const int n = c.groups + c.B;
+    auto seg = [&](int i) {
+        PagedSeg g = {0, 0, 0, 0};
+        if (i < n) g = paged_seg(c, i < c.groups ? c.B + i : i - c.groups);
+        return g;
+    };
     float work = 0.0f;
     PagedSeg g = {};
     for (int i = 0; i < n; i += 64) {
-        g = paged_seg(c, i + lane);
-        work += (float)tiles_of(c, g.rows, M) * (float)g.keys;
+        g = seg(i + lane);
+        float keys = (float)g.keys;
+        if (g.seq < c.B && g.rows > 1) {  // of a tile on average, or more (a row attends half of the new ones)
+            const float kv = (float)max(c.kv_lens[g.seq], 0);
+            keys = fminf(keys, fmaxf(kv - 0.5f * (float)g.rows, 0.5f * kv) + (float)cut.M / (float)c.G + 1.0f);
+        }
+        work += (float)((g.rows * c.G + cut.M - 1) >> cut.log2_M) * keys;
     }
     work = wave_sum(work);
     const int chunk = __builtin_amdgcn_readfirstlane(
-        max(min_chunk, ((int)ceilf(fminf(work / target, 1073741824.0f)) + 31) & ~31));
+        max(cut.min_chunk, ((int)ceilf(fminf(work / cut.target, 1073741824.0f)) + 31) & ~31));
     PagedSlot r = {};
     r.chunk = chunk;
     int base = 0;
     for (int i = 0; i < n; i += 64) {
-        if (n > 64) g = paged_seg(c, i + lane);
-        const int splits = max(1, (int)(((unsigned)g.keys + chunk - 1) / (unsigned)chunk));
-        const int mine = tiles_of(c, g.rows, M) * splits;
+        if (n > 64) g = seg(i + lane);
+        SegCut sc = seg_cut(c, g, chunk, cut);
+        const int mine = sc.slots();
         const int end = base + wave_scan(mine);
         const uint64_t behind = __ballot(end > slot);
         if (behind) {
@@ -105,10 +150,23 @@ __device__ __forceinline__ PagedSlot paged_slot(const PagedKv& c, int M, float t
             r.seg.rows = __builtin_amdgcn_readlane(g.rows, k);
             r.seg.keys = __builtin_amdgcn_readlane(g.keys, k);
             r.seg.seq = __builtin_amdgcn_readlane(g.seq, k);
-            r.splits = __builtin_amdgcn_readlane(splits, k);
-            const int at = slot - __builtin_amdgcn_readlane(end - mine, k);
-            r.tile = at / r.splits;
-            r.split = at - r.tile * r.splits;
+            sc.tiles = __builtin_amdgcn_readlane(sc.tiles, k);
+            sc.whole = __builtin_amdgcn_readlane(sc.whole, k);
+            sc.most = __builtin_amdgcn_readlane(sc.most, k);
+            sc.behind = __builtin_amdgcn_readlane(sc.behind, k);
+            int at = slot - __builtin_amdgcn_readlane(end - mine, k);
+            // from the last tile down, those with the most chunks first
+            int parts = sc.most, top = sc.tiles;
+            for (;; --parts) {
+                const int low = parts > sc.whole ? sc.from(parts - 1) : 0;
+                const int slots = (top - low) * parts;
+                if (at < slots || low == 0) break;
+                at -= slots;
+                top = low;
+            }
+            const int back = at / parts;
+            r.tile = top - 1 - back;
+            r.split = at - back * parts;
             r.first_slot = slot - r.split;
             r.any = true;
             return r;
@@ -118,22 +176,14 @@ __device__ __forceinline__ PagedSlot paged_slot(const PagedKv& c, int M, float t
     return r;
 }
 
-// Where a tile's slots are noted for the joining of its chunks: distinct for the
-// tiles of a call, and to be had from a row without the other segments (a
-// sequence's rows before it fill at most first G / M tiles and one more each).
+// Where a tile's first slot is noted for the joining of its chunks: distinct for the tiles
+// of one kind, and to be had from a row without the other segments (those before it fill at
+// most first G / M tiles and one more each).
 __device__ __forceinline__ int tile_note(const PagedKv& c, const PagedSeg& g, int tile, int M) {
-    if (g.seq < c.B) return g.first * c.G / M + g.seq + tile;
-    return c.T * c.G / M + c.B + g.first * c.G / M + (g.seq - c.B) + tile;
+    return g.first * c.G / M + (g.seq < c.B ? g.seq : g.seq - c.B) + tile;
 }
 
-// Slots, and notes, that a call can have.
-struct PagedBounds {
-    int64_t slots, notes;
-};
-inline PagedBounds paged_bounds(const bz_paged_kv* d, int M, int target) {
-    const int64_t rows = (int64_t)d->T * (d->HQ / d->HKV) / M;
-    const int64_t tiles = rows + d->B + (d->groups > 0 ? rows + d->groups : 0);
-    return {tiles + target + 64, tiles};  // (the sum of the work is in fp32)
-}
+// Slots that a launch over so many tiles can have.
+inline int64_t paged_slots(int64_t tiles, int target) { return tiles + target + 8; }  // (the work is summed in fp32)
 
 }  // namespace bz

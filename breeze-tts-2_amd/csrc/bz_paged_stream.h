@@ -194,14 +194,13 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT < 256 || F8 || D == 
             pg_f32x4(&sv)[2] = score[rt];
             if (mask) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2; ++h) {
+                    // key 4 grp + r of the half step is attended and there
+                    const int bound = min(limit[rt] - at - 16 * h, there[h]) - 4 * grp;
+                    seen[rt] |= bound > 0;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int j = 16 * h + 4 * grp + r;
-                        const bool ok = at + j < limit[rt] && 4 * grp + r < there[h];
-                        sv[h][r] = ok ? sv[h][r] : -INFINITY;
-                        seen[rt] |= ok;
-                    }
+                    for (int r = 0; r < 4; ++r) sv[h][r] = r < bound ? sv[h][r] : -INFINITY;
+                }
             } else {
                 seen[rt] = true;
             }
@@ -287,7 +286,7 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT < 256 || F8 || D == 
     const bool whole = w.parts == 1 && c.groups == 0;  // no other slot has keys of these rows
     const PagedParts parts(a, c, slot, head, M, D);
     const float vs = F8 ? c.v_scale[head] : 1.0f;
-    if (!a.arrived && u.split == 0 && head == 0 && tid == 0) a.notes[tile_note(c, g, u.tile, M)] = make_int2(slot, u.chunk);
+    if (!a.arrived && u.split == 0 && head == 0 && tid == 0) note_tile(c, a, w, M, slot);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         if (16 * rt >= nrow) break;

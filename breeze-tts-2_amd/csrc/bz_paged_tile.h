@@ -1,25 +1,29 @@
 // Attention over a paged cache for many rows (prompts, a shared prefix's rows): one
-// workgroup of four waves per slot and key/value head, 64 keys at a time staged in
-// LDS for all waves.
+// workgroup per slot and key/value head, 64 keys at a time staged in LDS for all waves.
 //
-// Bound by the matrix cores, and by the softmax beside them.  WR waves have 32 rows each
-// (WR = 4: 128 rows, every wave takes all 64 keys; WR = 2: 64 rows, a wave takes
-// 32 of them, and the two parts of a row are merged at the end).
+// Bound by the matrix cores, and by the softmax beside them.  A wave has 32 rows.  With
+// D <= 128 it has them for itself; with D = 256 two waves share them (PAIR): each takes the
+// scores of 32 of the 64 keys, then each the products with half of the columns over
+// all 64, so that its accumulators leave room for two waves on a SIMD.
 //   scores  transposed, A = 32 keys from LDS, B = 32 rows in registers
 //           (v_mfma_f32_32x32x16_bf16): lane (row, half) gets keys 8 (r / 4) + 4 half + r % 4,
-//           so a row's maximum and sum are its own 16 or 32 numbers and one swap of the
-//           wave's halves
+//           so a row's maximum is over its own numbers, one swap of the wave's halves and
+//           (PAIR) what the other wave found
 //   p v     A = the values transposed, by transposing LDS reads
 //           (ds_read_b64_tr_b16: 4 keys of one column to a lane), in the order of keys in
-//           which the lane has its probabilities: these are the B operand as they
-//           are.  p is rounded to bf16 (2^-9 of it on average, as much as the output's own
-//           rounding; a second part would double these products); the sum l is over p
-//           before it is rounded
+//           which the lanes have their probabilities: these are the B operand as they
+//           are (PAIR: also the other wave's, through LDS).  p is rounded to bf16 (2^-9 of it on
+//           average, as much as the output's own rounding; a second part would double
+//           these products); the sum l is over p before it is rounded
 //   rescale only when a maximum grows by more than 2^8: until then p stays below
 //           2^8, which costs fp32 sums nothing
-//   LDS     two buffers, one barrier a tile; 16-byte pieces of a row are exchanged
-//           so that neither the row-wise reads of keys nor the transposing ones of values
-//           meet on a bank
+//   order   in one round: the softmax of a tile beside the scores of the next one, then
+//           its products; keys are fetched three tiles ahead, values one, and one
+//           barrier (PAIR: two, the probabilities have one buffer) ends a round's first half
+//   LDS     16-byte pieces of a row are exchanged so that neither the row-wise reads of
+//           keys nor the transposing ones of values meet on a bank.  Every buffer is a
+//           variable of its own and the rounds take them in turn by name: that tells the
+//           compiler that reads of one do not wait for loads under way into another
 #pragma once
 
 #include "bz_paged_attn.h"
@@ -48,32 +52,30 @@ __device__ __forceinline__ float other_half_sum(float v) {
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-// One 16-key piece of keys or values on its way to LDS.
-template <int D, bool F8>
+// A wave's RW rows of a tile's keys or values on their way to LDS.
+template <int D, bool F8, int RW>
 struct TileStage {
-    static constexpr int ROW = D * (F8 ? 1 : 2);   // bytes of a position
-    static constexpr int LR = ROW / 16;            // lanes of a row
-    static constexpr int N = 16 * ROW / 1024;      // loads of a wave
+    static constexpr int ROW = D * (F8 ? 1 : 2);  // bytes of a position
+    static constexpr int LR = ROW / 16;           // lanes of a row
+    static constexpr int ROWS = 64 / LR;          // rows of a load
+    static constexpr int N = RW * ROW / 1024;     // loads of a wave
+    static_assert(N > 0 && N * 1024 == RW * ROW, "whole loads of a wave");
     u32x4 w[N];
 
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t pos, int lane) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            w[i] = buffer_ld16(r, (uint32_t)(i * (64 / LR) + lane / LR) * pos + 16 * (lane % LR));
+            w[i] = buffer_ld16(r, (uint32_t)(i * ROWS + lane / LR) * pos + 16 * (lane % LR));
     }
-    // rows key0 .. key0 + 15 of a tile of bf16 rows, piece p of row key at p ^ swap(key)
+    // e4m3, widened, as the rows from `first` of a tile; piece p of row key at p ^ swap(key)
     template <typename X>
-    __device__ __forceinline__ void store(char* tile, int key0, int lane, X swap) const {
+    __device__ __forceinline__ void store(char* tile, int first, int lane, X swap) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int key = key0 + i * (64 / LR) + lane / LR, p = lane % LR;
+            const int key = first + i * ROWS + lane / LR, p = lane % LR;
             char* row = tile + key * (2 * D);
-            if constexpr (F8) {
-                *reinterpret_cast<u32x4*>(row + 16 * ((2 * p) ^ swap(key))) = f8_widen(w[i][0], w[i][1]);
-                *reinterpret_cast<u32x4*>(row + 16 * ((2 * p + 1) ^ swap(key))) = f8_widen(w[i][2], w[i][3]);
-            } else {
-                *reinterpret_cast<u32x4*>(row + 16 * (p ^ swap(key))) = w[i];
-            }
+            *reinterpret_cast<u32x4*>(row + 16 * ((2 * p) ^ swap(key))) = f8_widen(w[i][0], w[i][1]);
+            *reinterpret_cast<u32x4*>(row + 16 * ((2 * p + 1) ^ swap(key))) = f8_widen(w[i][2], w[i][3]);
         }
     }
     // bf16 straight into LDS, 16 bytes a lane one after the other: lane l writes piece
@@ -81,37 +83,50 @@ struct TileStage {
     // its scalar offset; a lane's offsets differ between loads only by the exchange of
     // pieces, which repeats.
     template <typename X>
-    __device__ __forceinline__ static void load_lds(__amdgpu_buffer_rsrc_t r, uint32_t pos, char* tile, int key0, int lane,
+    __device__ __forceinline__ static void load_lds(__amdgpu_buffer_rsrc_t r, uint32_t pos, char* tile, int first, int lane,
                                                     X swap) {
-        constexpr int rows = 64 / LR;
 #pragma unroll
         for (int i = 0; i < N; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                r, (__attribute__((address_space(3))) void*)(tile + (key0 + i * rows) * (2 * D)), 16,
-                (uint32_t)(lane / LR) * pos + 16 * ((lane % LR) ^ swap(i * rows + lane / LR)), i * rows * pos, 0, 0);
+                r, (__attribute__((address_space(3))) void*)(tile + (first + i * ROWS) * (2 * D)), 16,
+                (uint32_t)(lane / LR) * pos + 16 * ((lane % LR) ^ swap(first + i * ROWS + lane / LR)), i * ROWS * pos, 0, 0);
     }
     __device__ __forceinline__ bool odd() const {
         bool o = false;
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o |= F8 ? nan_f8x4(w[i][e]) : not_finite2(w[i][e]);
+            for (int e = 0; e < 4; ++e) o |= nan_f8x4(w[i][e]);
         return o;
     }
 };
 
-template <int D, bool F8, int WR>
-__global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) paged_attn_bf16_tile(PagedKv c, PagedAttn a) {
-    constexpr int WK = 4 / WR, M = 32 * WR, T = D / 16, ND = D / 32;
-    constexpr int KB = 2 / WK, GB = D == 256 ? 1 : KB;  // 32-key blocks of a wave, and at a time
-    constexpr int kTileBytes = kTileKeys * D * 2;
-    constexpr int kMerge = WK > 1 ? WR * 32 * (D + 4) * 4 : 0;
-    __shared__ __attribute__((aligned(16))) char lds[4 * kTileBytes > kMerge ? 4 * kTileBytes : kMerge];
-    __shared__ int odd[2][4];
-    __shared__ float st_m[WK][M], st_l[WK][M];
+// Order for the scheduler: N matrix products, each behind its R LDS reads, with the reads
+// of A products under way.
+template <int N, int R, int A>
+__device__ __forceinline__ void read_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, R * A, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i + A < N) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    }
+}
+
+template <int D, bool F8, int WAVES, bool PAIR>
+__global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c, PagedAttn a) {
+    constexpr int W = PAIR ? 2 : 1;  // waves of a row
+    constexpr int M = 32 * WAVES / W, RW = kTileKeys / WAVES, T = D / 16, ND = D / 32 / W, KB = 2 / W;
+    constexpr int kAhead = F8 ? 2 : 4;  // LDS reads under way, in products (e4m3 on its way takes registers)
+    constexpr int kTileBytes = kTileKeys * D * 2, kProbs = PAIR ? WAVES * 2048 : 16;
+    using Stage = TileStage<D, F8, RW>;
+    __shared__ __attribute__((aligned(16))) char k0[kTileBytes], k1[kTileBytes], v0[kTileBytes], v1[kTileBytes];
+    __shared__ __attribute__((aligned(16))) char probs[kProbs];
+    __shared__ float top0[PAIR ? WAVES : 1][32], top1[PAIR ? WAVES : 1][32];  // a tile's maxima
+    __shared__ int odd[2][WAVES];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wr = wave % WR, wk = wave / WR;
+    const int rg = wave / W, kp = wave % W;
     const int slot = blockIdx.x / c.HKV, head = blockIdx.x - slot * c.HKV;
 
     PagedWork w;
@@ -120,7 +135,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) paged_attn_bf16_tile(Pa
     const PagedSeg& g = u.seg;
 
     // the lane's row (behind the tile's rows, its last one again)
-    const int mine = u.tile * M + min(32 * wr + col, w.rows - 1);
+    const int mine = u.tile * M + min(32 * rg + col, w.rows - 1);
     const int row = mine / c.G, qh = head * c.G + (mine - row * c.G);
     const int limit = row_limit(g, w.kv_len, w.own, row);
     u32x4 q[T];
@@ -141,214 +156,263 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) paged_attn_bf16_tile(Pa
     float m = -INFINITY, l = 0.0f;
     bool seen = false, apart = false;
 
-    // pages of the next 16 tiles' pieces, one to a lane
-    int pages = -1, page_tile = -16;
-    auto refresh = [&](int tile) {
-        if (tile < page_tile + 16) return;
-        page_tile = tile;
-        const int at = w.begin + kTileKeys * tile + 16 * lane;
-        pages = at < w.end ? table[at >> c.shift] : -1;
-    };
-    auto page_of = [&](int tile, int piece) { return __builtin_amdgcn_readlane(pages, 4 * (tile - page_tile) + piece); };
+    // The next 16 tiles' pieces, one to a lane: where this wave's rows of its keys and values begin,
+    // and how many positions are there (of a tile's four, a byte each).  Worked out for 16 tiles at a time: with
+    // scalar instructions for each tile they were as many as all vector instructions.
+    uint64_t k_from = 0, v_from = 0;
+    uint32_t n_of = 0;
+    int from_tile = -16;
     const int tiles = (max(w.end - w.begin, 0) + kTileKeys - 1) / kTileKeys;
-    auto k_swap = [](int key) { return key & 7; };
-    auto v_swap = [](int key) { return 2 * (key & 3); };
-
-    TileStage<D, F8> sk, sv;  // (e4m3: on its way through registers, where it is widened)
-    uint32_t n_next = 0;      // positions there of a tile's four pieces, a byte each
-    auto fetch = [&](int tile, char* kt) {
-        refresh(tile);
-        const int at = w.begin + kTileKeys * tile;
-        n_next = 0;
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-            n_next |= (unsigned)page_of(tile, p) < (unsigned)c.num_pages
-                          ? (uint32_t)min(max(w.end - at - 16 * p, 0), 16) << (8 * p)
-                          : 0u;
-        const PagedPiece pc = paged_piece<TileStage<D, F8>::ROW>(c, kh, vh, page_of(tile, wave), at + 16 * wave, w.end);
-        if constexpr (F8) {
-            sk.load(pc.k, (uint32_t)c.k_pos, lane);
-            sv.load(pc.v, (uint32_t)c.v_pos, lane);
-        } else {
-            sk.load_lds(pc.k, (uint32_t)c.k_pos, kt, 16 * wave, lane, k_swap);
-            sv.load_lds(pc.v, (uint32_t)c.v_pos, kt + kTileBytes, 16 * wave, lane, v_swap);
-        }
-    };
-    if (tiles > 0) fetch(0, lds);
+    // (64 banks: a row of 256 bytes or more lies on all of them.  No conflicts; with 7 and 2 for all D
+    // 40% of the LDS cycles were conflicts)
+    auto k_swap = [](int key) { return key & (D == 64 ? 7 : 15); };
+    auto v_swap = [](int key) { return (D == 64 ? 2 : 4) * (key & 3); };
 
     // where this lane reads: its key's pieces 2 t + half (t of 0..3, then 8 pieces on), and its columns of keys
     // 4 half + 0..3 (of an even and an odd block of 32 columns, then 8 pieces on)
-    uint32_t k_at[4], v_at[2];
+    uint32_t k_at[T < 8 ? T : 8], v_at[ND];
     {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) k_at[t] = col * (2 * D) + 16 * ((2 * t + half) ^ k_swap(col));
+        for (int t = 0; t < 8 && t < T; ++t) k_at[t] = (32 * KB * kp + col) * (2 * D) + 16 * ((2 * t + half) ^ k_swap(col));
         const int i16 = lane & 15, key = 4 * half + (i16 >> 2), piece = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) v_at[t] = key * (2 * D) + 8 * (i16 & 1) + 16 * ((4 * t + piece) ^ v_swap(key));
+        for (int t = 0; t < ND; ++t)
+            v_at[t] = key * (2 * D) + 8 * (i16 & 1) + 16 * ((4 * (kp * ND + t) + piece) ^ v_swap(key));
     }
 
-    for (int tile = 0; tile < tiles; ++tile) {
+    struct Tile {
+        uint32_t n;            // positions there
+        uint32_t v_lo, v_hi;   // where this wave's rows of the values begin
+    };
+    Stage sk, sv;  // (e4m3: on its way through registers)
+    auto rows_at = [&](uint32_t lo, uint32_t hi, uint32_t n, uint32_t pos) {
+        const int there = (int)(n >> (8 * (RW * wave / 16)) & 0xFF) - RW * wave % 16;
+        return buffer_rsrc(reinterpret_cast<const char*>((uint64_t)hi << 32 | lo),
+                           there > 0 ? (uint32_t)(min(there, RW) - 1) * pos + Stage::ROW : 0u);
+    };
+    auto lane_of = [&](uint64_t x, int i, uint32_t& lo, uint32_t& hi) {
+        lo = __builtin_amdgcn_readlane((int)(uint32_t)x, i);
+        hi = __builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), i);
+    };
+    auto fetch_k = [&](int tile, char* to) {
+        if (tile >= from_tile + 16) {
+            from_tile = tile;
+            const int at = w.begin + kTileKeys * tile + 16 * lane;
+            const int page = at < w.end ? table[at >> c.shift] : -1;
+            const bool there = (unsigned)page < (unsigned)c.num_pages;
+            const int in_page = (at & ((1 << c.shift) - 1)) + RW * wave % 16;
+            k_from = (uint64_t)kh + (there ? page : 0) * c.k_page + in_page * c.k_pos;
+            v_from = (uint64_t)vh + (there ? page : 0) * c.v_page + in_page * c.v_pos;
+            uint32_t n = (there ? (uint32_t)min(w.end - at, 16) : 0u) << (8 * (lane & 3));
+            n |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)n, kDppXor1, 0xF, 0xF, false);
+            n_of = n | (uint32_t)__builtin_amdgcn_update_dpp(0, (int)n, kDppXor2, 0xF, 0xF, false);
+        }
+        const int first = 4 * (tile - from_tile), own = first + RW * wave / 16;
+        Tile x;
+        x.n = __builtin_amdgcn_readlane((int)n_of, first);
+        lane_of(v_from, own, x.v_lo, x.v_hi);
+        uint32_t lo, hi;
+        lane_of(k_from, own, lo, hi);
+        const __amdgpu_buffer_rsrc_t r = rows_at(lo, hi, x.n, (uint32_t)c.k_pos);
+        if constexpr (F8)
+            sk.load(r, (uint32_t)c.k_pos, lane);
+        else
+            Stage::load_lds(r, (uint32_t)c.k_pos, to, RW * wave, lane, k_swap);
+        return x;
+    };
+    auto fetch_v = [&](const Tile& x, char* to) {
+        const __amdgpu_buffer_rsrc_t r = rows_at(x.v_lo, x.v_hi, x.n, (uint32_t)c.v_pos);
+        if constexpr (F8)
+            sv.load(r, (uint32_t)c.v_pos, lane);
+        else
+            Stage::load_lds(r, (uint32_t)c.v_pos, to, RW * wave, lane, v_swap);
+    };
+    // scores of the wave's keys of a tile, masked, and their maximum (PAIR: to the other wave too)
+    pg_f32x16 s[KB];
+    auto scores = [&](int tile, const Tile& x, const char* kb, float (*top)[32]) {
+#pragma unroll
+        for (int b = 0; b < KB; ++b) s[b] = pg_f32x16{};
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+                s[b] = pg_mfma32(*reinterpret_cast<const u32x4*>(kb + k_at[t & 7] + 256 * (t >> 3) + 32 * b * (2 * D)), q[t], s[b]);
+        read_ahead<KB * T, 1, kAhead>();
         const int at = w.begin + kTileKeys * tile;
-        char* kt = lds + (tile & 1) * (2 * kTileBytes);
-        char* vt = kt + kTileBytes;
-        const uint32_t n_now = n_next;
-        const bool mask = at + kTileKeys > w.all || n_now != 0x10101010u;
+        if (at + kTileKeys > w.all || x.n != 0x10101010u) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    // key 8 (r / 4) + 4 half + r % 4 of the 32 is attended and there
+                    const int there = x.n >> (16 * (KB * kp + b) + 8 * p) & 0xFF;
+                    const int bound = min(limit - at - 32 * (KB * kp + b), 16 * p + there) - 4 * half;
+                    seen |= 16 * p < bound;
+#pragma unroll
+                    for (int r = 8 * p; r < 8 * p + 8; ++r) s[b][r] = 8 * (r / 4) + r % 4 < bound ? s[b][r] : -INFINITY;
+                }
+        } else {
+            seen = true;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+        mx = other_half_max(mx);
+        if constexpr (PAIR)
+            if (half == 0) top[wave][col] = mx;
+        return mx;
+    };
+    float mx = 0.0f;
+    Tile x0 = {}, x1 = {}, x2 = {};
+
+    // Tile `tile`: its softmax, the next one's scores, its products.  ke: where the keys two tiles on are
+    // under way to, ko: the next one's, and later those of three tiles on.
+    auto round = [&](int tile, char* ke, char* ko, char* vb, char* vn, float (*top)[32],
+                     float (*top_next)[32]) __attribute__((always_inline)) {
+        if constexpr (PAIR) mx = fmaxf(mx, top[wave ^ 1][col]);
+        mx *= sc;
+        const bool grow = mx > m + 8.0f;
+        if (__ballot(grow)) {
+            const float mn = grow ? mx : m;
+            const float f = mn == -INFINITY ? 1.0f : pg_exp2(m - mn);
+            l *= f;
+#pragma unroll
+            for (int t = 0; t < ND; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[t][r] *= f;
+            m = mn;
+        }
+#pragma unroll
+        for (int t = 0; t < ND; ++t) asm("" : "+v"(acc[t]));  // (in place: without it both sides of the branch were kept)
+        const float ms = m == -INFINITY ? 0.0f : m;
+        u32x4 p[KB][2];
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                const float e0 = pg_exp2(fmaf(s[b][r], sc, -ms)), e1 = pg_exp2(fmaf(s[b][r + 1], sc, -ms));
+                l += e0 + e1;
+                p[b][r / 8][r / 2 % 4] = pack_bf16x2(e0, e1);
+            }
+        if constexpr (PAIR) {
+            char* to = probs + 2048 * wave + 16 * lane;
+            *reinterpret_cast<u32x4*>(to) = p[0][0];
+            *reinterpret_cast<u32x4*>(to + 1024) = p[0][1];
+        }
+        mx = scores(tile + 1, x1, ko, top_next);  // (behind the last tile: -inf)
+
+        // this tile's values (and the keys two tiles on) are in LDS
+        const int at = w.begin + kTileKeys * tile;
+        const bool mask = at + kTileKeys > w.all || x0.n != 0x10101010u;
         const bool differ = mask && w.all < w.end;  // (behind all rows' limits there are zeros)
-        const int own_n = n_now >> (8 * wave) & 0xFF;
         if constexpr (F8) {
-            sk.store(kt, 16 * wave, lane, k_swap);
-            sv.store(vt, 16 * wave, lane, v_swap);
+            sk.store(ke, RW * wave, lane, k_swap);
+            sv.store(vb, RW * wave, lane, v_swap);
             if (differ) {
                 const bool o = __ballot(sv.odd()) != 0;
                 if (lane == 0) odd[tile & 1][wave] = o;
             }
         } else {
-            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's pieces are in LDS
+            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
             if (mask) {
                 // places that are not there, as zeros; the other values looked at
+                const int there = (int)(x0.n >> (8 * (RW * wave / 16)) & 0xFF) - RW * wave % 16;
                 bool o = false;
-                for (int i = lane; i < 16 * D / 8; i += 64) {
-                    u32x4* x = reinterpret_cast<u32x4*>(vt + 16 * wave * (2 * D)) + i;
-                    if (i / (D / 8) >= own_n) {
-                        *x = u32x4{0u, 0u, 0u, 0u};
+                for (int i = lane; i < RW * D / 8; i += 64) {
+                    u32x4* y = reinterpret_cast<u32x4*>(vb + RW * wave * (2 * D)) + i;
+                    if (i / (D / 8) >= there) {
+                        *y = u32x4{0u, 0u, 0u, 0u};
                     } else if (differ) {
-                        const u32x4 y = *x;
+                        const u32x4 z = *y;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o |= not_finite2(y[e]);
+                        for (int e = 0; e < 4; ++e) o |= not_finite2(z[e]);
                     }
                 }
                 o = __ballot(o) != 0;
                 if (lane == 0) odd[tile & 1][wave] = o;
             }
         }
-        if constexpr (F8)
-            if (tile + 1 < tiles) fetch(tile + 1, nullptr);
         __syncthreads();
         if (differ) {
-            apart = __builtin_amdgcn_readfirstlane(odd[tile & 1][0] | odd[tile & 1][1] | odd[tile & 1][2] | odd[tile & 1][3]);
-            if (apart) break;
+            int o = 0;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) o |= odd[tile & 1][i];
+            apart |= __builtin_amdgcn_readfirstlane(o) != 0;  // (what is summed from here on is not used)
         }
-        // (the other buffer: every wave is done with its last tile)
-        if constexpr (!F8)
-            if (tile + 1 < tiles) fetch(tile + 1, lds + (~tile & 1) * (2 * kTileBytes));
-
-#pragma unroll 1
-        for (int b0 = KB * wk; b0 < KB * (wk + 1); b0 += GB) {  // 32-key blocks
-            pg_f32x16 s[GB];
-#pragma unroll
-            for (int b = 0; b < GB; ++b) {
-                s[b] = pg_f32x16{};
-                const char* kr = kt + 32 * (b0 + b) * (2 * D);
-#pragma unroll
-                for (int t = 0; t < T; ++t)
-                    s[b] = pg_mfma32(*reinterpret_cast<const u32x4*>(kr + k_at[t & 3] + 128 * (t >> 2)), q[t], s[b]);
-            }
-            if (mask) {
-#pragma unroll
-                for (int b = 0; b < GB; ++b)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int in = 8 * (r / 4) + 4 * half + r % 4, p = 2 * (b0 + b) + r / 8;
-                        const bool ok = at + 32 * (b0 + b) + in < limit && (in & 15) < (int)(n_now >> (8 * p) & 0xFF);
-                        s[b][r] = ok ? s[b][r] : -INFINITY;
-                        seen |= ok;
-                    }
-            } else {
-                seen = true;
-            }
-            float mx = s[0][0];
-#pragma unroll
-            for (int b = 0; b < GB; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
-            mx = other_half_max(mx) * sc;
-            const bool grow = mx > m + 8.0f;
-            if (__ballot(grow)) {
-                const float mn = grow ? mx : m;
-                const float f = mn == -INFINITY ? 1.0f : pg_exp2(m - mn);
-                l *= f;
-#pragma unroll
-                for (int t = 0; t < ND; ++t)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[t][r] *= f;
-                m = mn;
-            }
-            const float ms = m == -INFINITY ? 0.0f : m;
-            uint32_t pb[GB][8];
-#pragma unroll
-            for (int b = 0; b < GB; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; r += 2) {
-                    const float p0 = pg_exp2(fmaf(s[b][r], sc, -ms)), p1 = pg_exp2(fmaf(s[b][r + 1], sc, -ms));
-                    l += p0 + p1;
-                    pb[b][r / 2] = pack_bf16x2(p0, p1);
-                }
-
-#pragma unroll
-            for (int b = 0; b < GB; ++b)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const u32x4 pj = {pb[b][4 * j], pb[b][4 * j + 1], pb[b][4 * j + 2], pb[b][4 * j + 3]};
-                    const char* vr = vt + (32 * (b0 + b) + 16 * j) * (2 * D);
-#pragma unroll
-                    for (int t = 0; t < ND; ++t) {
-                        const char* x = vr + v_at[t & 1] + 128 * (t >> 1);
-                        const uint2 lo = lds_column4(x), hi = lds_column4(x + 8 * (2 * D));
-                        acc[t] = pg_mfma32(u32x4{lo.x, lo.y, hi.x, hi.y}, pj, acc[t]);
-                    }
-                }
+        u32x4 o[2] = {};
+        if constexpr (PAIR) {
+            const char* from = probs + 2048 * (wave ^ 1) + 16 * lane;
+            o[0] = *reinterpret_cast<const u32x4*>(from);
+            o[1] = *reinterpret_cast<const u32x4*>(from + 1024);
+            __syncthreads();
         }
+        // (behind the last tile no page is there: nothing is read)
+        fetch_v(x1, vn);
+        const Tile x3 = fetch_k(tile + 3, ko);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {  // (PAIR: the wave's own 32 keys, the other's)
+            const char* vr = vb + 32 * (PAIR && b ? kp ^ 1 : PAIR ? kp : b) * (2 * D);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const u32x4 pj = PAIR && b ? o[j] : p[PAIR ? 0 : b][j];
+#pragma unroll
+                for (int t = 0; t < ND; ++t) {
+                    const char* y = vr + 16 * j * (2 * D) + v_at[t];
+                    const uint2 lo = lds_column4(y), hi = lds_column4(y + 8 * (2 * D));
+                    acc[t] = pg_mfma32(u32x4{lo.x, lo.y, hi.x, hi.y}, pj, acc[t]);
+                }
+            }
+        }
+        read_ahead<4 * ND, 2, kAhead>();
+        x0 = x1;
+        x1 = x2;
+        x2 = x3;
+    };
+    if (tiles > 0) {
+        x0 = fetch_k(0, k0);
+        if constexpr (F8) sk.store(k0, RW * wave, lane, k_swap);
+        x1 = fetch_k(1, k1);
+        if constexpr (F8) sk.store(k1, RW * wave, lane, k_swap);
+        fetch_v(x0, v0);
+        if constexpr (!F8) __builtin_amdgcn_s_waitcnt(0x0F70);
+        __syncthreads();
+        mx = scores(0, x0, k0, top0);
+        __syncthreads();
+        x2 = fetch_k(2, k0);
     }
-    if (u.split == 0 && head == 0 && tid == 0) a.notes[tile_note(c, g, u.tile, M)] = make_int2(slot, u.chunk);
+    // (no way out between two rounds: it made the accumulators live twice)
+    int tile = 0;
+    for (; tile + 1 < tiles; tile += 2) {
+        round(tile, k0, k1, v0, v1, top0, top1);
+        round(tile + 1, k1, k0, v1, v0, top1, top0);
+    }
+    if (tile < tiles) round(tile, k0, k1, v0, v1, top0, top1);
+    if (u.split == 0 && head == 0 && tid == 0) note_tile(c, a, w, M, slot);
     if (apart) {
-        paged_rows_apart<D, F8>(c, a, w, slot, head, M, wave, 4, lane);
+        paged_rows_apart<D, F8>(c, a, w, slot, head, M, wave, WAVES, lane);
         return;
     }
 
     l = other_half_sum(l);
     const bool any = __builtin_amdgcn_ballot_w64(seen) >> col & 0x100000001ull;
     if (m == -INFINITY) l = any ? 1.0f : 0.0f;
-    if constexpr (WK > 1) {
-        // the second wave's part of each row to the first
+    if constexpr (PAIR) {
+        __syncthreads();  // (the maxima have been read)
+        if (half == 0) top0[wave][col] = l;
         __syncthreads();
-        float* st = reinterpret_cast<float*>(lds) + (wr * 32 + col) * (D + 4) + 4 * half;
-        if (wk > 0) {
-            if (half == 0) {
-                st_m[0][32 * wr + col] = m;
-                st_l[0][32 * wr + col] = l;
-            }
-#pragma unroll
-            for (int t = 0; t < ND; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; r += 4)
-                    *reinterpret_cast<float4*>(st + 32 * t + 2 * r) =
-                        make_float4(acc[t][r], acc[t][r + 1], acc[t][r + 2], acc[t][r + 3]);
-        }
-        __syncthreads();
-        if (wk > 0) return;
-        const float m1 = st_m[0][32 * wr + col], l1 = st_l[0][32 * wr + col], mn = fmaxf(m, m1);
-        const float f0 = mn == -INFINITY ? 1.0f : pg_exp2(m - mn), f1 = mn == -INFINITY ? 1.0f : pg_exp2(m1 - mn);
-        m = mn;
-        l = l * f0 + l1 * f1;
-#pragma unroll
-        for (int t = 0; t < ND; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const float4 x = *reinterpret_cast<const float4*>(st + 32 * t + 2 * r);
-                acc[t][r] = acc[t][r] * f0 + x.x * f1;
-                acc[t][r + 1] = acc[t][r + 1] * f0 + x.y * f1;
-                acc[t][r + 2] = acc[t][r + 2] * f0 + x.z * f1;
-                acc[t][r + 3] = acc[t][r + 3] * f0 + x.w * f1;
-            }
+        l += top0[wave ^ 1][col];
     }
 
     const bool whole = w.parts == 1 && c.groups == 0;  // no other slot has keys of these rows
-    if (32 * wr + col >= w.rows) return;
+    const int rr = 32 * rg + col;
+    if (rr >= w.rows) return;
     const PagedParts parts(a, c, slot, head, M, D);
-    const int rr = 32 * wr + col;
     const float f = m == -INFINITY ? (l > 0.0f ? __builtin_nanf("") : 0.0f) : 1.0f / l * (F8 ? c.v_scale[head] : 1.0f);
-    uint16_t* o = a.out + (int64_t)(g.first + row) * a.ld_out + (int64_t)qh * D + 4 * half;
-    if (!whole && half == 0) parts.put_ml(rr, m, l);
+    const int first = 32 * ND * kp + 4 * half;
+    uint16_t* o = a.out + (int64_t)(g.first + row) * a.ld_out + (int64_t)qh * D + first;
+    if (!whole && half == 0 && kp == 0) parts.put_ml(rr, m, l);
 #pragma unroll
     for (int t = 0; t < ND; ++t)
 #pragma unroll
@@ -357,7 +421,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) paged_attn_bf16_tile(Pa
                 *reinterpret_cast<uint2*>(o + 32 * t + 2 * r) =
                     make_uint2(pack_bf16x2(acc[t][r] * f, acc[t][r + 1] * f), pack_bf16x2(acc[t][r + 2] * f, acc[t][r + 3] * f));
             else
-                parts.put4(rr * D + 4 * half + 32 * t + 2 * r, acc[t][r], acc[t][r + 1], acc[t][r + 2], acc[t][r + 3]);
+                parts.put4(rr * D + first + 32 * t + 2 * r, acc[t][r], acc[t][r + 1], acc[t][r + 2], acc[t][r + 3]);
         }
 }
 
