@@ -42,8 +42,8 @@ __device__ __forceinline__ float pg_exp2(float x) { return __builtin_amdgcn_exp2
 struct PagedPartsAt {
     float* part;          // [slots][HKV][M][D] accumulators
     float2* ml;           // [slots][HKV][M] (m, l)
-    int2* notes;          // (first slot, keys of a chunk) of a sequence's tile
-    int2* prefix_notes;   // and of a prefix's
+    uint64_t* notes;      // [..][HKV] first slot | keys of a chunk << 32, of a sequence's tile
+    uint64_t* prefix_notes;  // and of a prefix's
 };
 
 struct PagedAttn {
@@ -54,9 +54,11 @@ struct PagedAttn {
     int64_t ld_out;
     PagedCut cut;
     PagedPartsAt to;
-    // [notes][HKV] arrivals of a tile's parts, zero between calls; the last to arrive
-    // joins them.  NULL: a launch of its own does.
+    // [notes][HKV], then [prefix notes][HKV]: arrivals of the parts that are joined together, zero
+    // between calls; the last to arrive joins them.  NULL: a launch of its own does.
     unsigned* arrived;
+    int own_notes;
+    int slots;
 };
 
 // The position behind the last key that a row attends in its segment: row i of n of a
@@ -94,9 +96,10 @@ __device__ __forceinline__ bool paged_work(const PagedKv& c, const PagedAttn& a,
     w.all = row_limit(g, w.kv_len, w.own, first / c.G);
     return w.u.split < w.parts;
 }
-// The tile's first slot, noted by the workgroup that has it (of one head).
-__device__ __forceinline__ void note_tile(const PagedKv& c, const PagedAttn& a, const PagedWork& w, int M, int slot) {
-    (w.own ? a.to.notes : a.to.prefix_notes)[tile_note(c, w.u.seg, w.u.tile, M)] = make_int2(slot, w.u.chunk);
+// The tile's first slot, noted by the workgroup that has it.
+__device__ __forceinline__ void note_tile(const PagedKv& c, const PagedAttn& a, const PagedWork& w, int M, int slot, int head) {
+    uint64_t* to = (w.own ? a.to.notes : a.to.prefix_notes) + (int64_t)tile_note(c, w.u.seg, w.u.tile, M) * c.HKV + head;
+    __hip_atomic_store(to, (uint64_t)(unsigned)w.u.chunk << 32 | (unsigned)slot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // One 16-position piece of a segment's keys, none of whose rows is read beyond `n`.
@@ -243,38 +246,69 @@ struct PagedSum {
     }
 };
 
-// The last of a tile's workgroups (256 threads) joins the parts; all have been stored.
-// st: LDS of 256 rows of 8.
+// The last of the workgroups (256 threads) whose parts belong together joins them; all have
+// been stored.  These are a tile's parts, or, with prefixes (one row each, M a multiple of G),
+// those of a prefix's tile and of all the sequences whose rows are in it.  st: LDS of 256 rows of 8.
 template <int D, bool F8>
 __device__ __forceinline__ void paged_join_last(const PagedKv& c, const PagedAttn& a, const PagedWork& w, int head, int M,
-                                                int tid, float (*st)[8], int* last) {
+                                                int tid, int lane, float (*st)[8], int* last) {
     const PagedSeg& g = w.u.seg;
+    const int chunk = w.u.chunk;
+    int pre = -1, first = g.first, rows = w.rows, tile = w.u.tile, parts = w.parts, at = tile_note(c, g, tile, M);
+    if (c.groups > 0) {
+        pre = w.own ? prefix_of_seq(c, g.seq, lane) : g.seq - c.B;
+        if (pre >= 0) {
+            const PagedSeg p = paged_seg(c, c.B + pre);
+            const int per = M / c.G;
+            if (w.own) tile = (g.first - p.first) / per;
+            first = p.first + tile * per;
+            const int n = min(p.rows - tile * per, per);
+            const int own = lane < n ? parts_of(paged_seg(c, first + lane).keys, chunk) : 0;
+            rows = n * c.G;
+            parts = parts_of(p.keys, chunk);
+            at = a.own_notes + tile_note(c, p, tile, M);
+            const int all = parts + __builtin_amdgcn_readlane(wave_scan(own), 63);
+            if (tid == 0) *last = all;
+        }
+    }
+    if (pre < 0 && tid == 0) *last = parts;
     // every thread's stores have arrived before the workgroup counts itself in
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    unsigned* count = a.arrived + (int64_t)tile_note(c, g, w.u.tile, M) * c.HKV + head;
+    unsigned* count = a.arrived + (int64_t)at * c.HKV + head;
     if (tid == 0)
-        *last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)w.parts - 1u;
+        *last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)*last - 1u;
     __syncthreads();
     if (!*last) return;
     if (tid == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const float vs = F8 ? c.v_scale[head] : 1.0f;
-    const int64_t at0 = ((int64_t)w.u.first_slot * c.HKV + head) * M, step = (int64_t)c.HKV * M;
-    const int items = w.rows * (D / 4);
+    auto noted = [&](const uint64_t* notes, int i) {
+        const uint64_t n = __hip_atomic_load(notes + (int64_t)i * c.HKV + head, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return ((int64_t)(uint32_t)n * c.HKV + head) * M;
+    };
+    const int64_t step = (int64_t)c.HKV * M;
+    const int64_t at0 = pre < 0 ? ((int64_t)w.u.first_slot * c.HKV + head) * M
+                                : noted(a.to.prefix_notes, at - a.own_notes);
+    const int items = rows * (D / 4);
     // few items: several threads to each, taking parts in turn
     int P = 1;
-    while (2 * P * items <= 256 && P < w.parts) P *= 2;
+    while (2 * P * items <= 256 && P < parts) P *= 2;
     for (int i0 = 0; i0 < items; i0 += 256) {
         const int p = P > 1 ? tid / items : 0, i = i0 + tid - p * items;
         PagedSum sum;
         const bool on = P > 1 ? p < P : i < items;
         const int r = on ? i / (D / 4) : 0, d = 4 * (i % (D / 4));
-        if (on) sum.add_parts<true>(a.to, at0 + r, step, w.parts, p, P, D, d);
-        sum.across(st, tid, P, items, on && p == 0);
-        if (on && p == 0) {
-            const int k = w.u.tile * M + r, row = k / c.G, h = head * c.G + (k - row * c.G);
-            sum.store(a.out + (int64_t)(g.first + row) * a.ld_out + (int64_t)h * D + d, vs);
+        const int k = pre < 0 ? tile * M + r : r, row = k / c.G, h = head * c.G + (k - row * c.G);
+        if (on) {
+            if (pre >= 0) {
+                PagedSeg own = paged_seg(c, first + row);
+                sum.add_parts<true>(a.to, noted(a.to.notes, tile_note(c, own, 0, M)) + (k - row * c.G), step,
+                                    parts_of(own.keys, chunk), p, P, D, d);
+            }
+            sum.add_parts<true>(a.to, at0 + r, step, parts, p, P, D, d);
         }
+        sum.across(st, tid, P, items, on && p == 0);
+        if (on && p == 0) sum.store(a.out + (int64_t)(first + row) * a.ld_out + (int64_t)h * D + d, vs);
     }
 }
 

@@ -38,14 +38,15 @@ __global__ void __launch_bounds__(256) paged_attn_bf16_join(PagedKv c, PagedAttn
     for (int part = 0; part < 2; ++part) {
         if (!part && pre < 0) continue;
         const PagedSeg g = part ? own : paged_seg(c, c.B + pre);
-        const int k = (t - g.first) * c.G + (min(h, c.HQ - 1) - head * c.G), tile = k >> a.cut.log2_M;
-        const int2 note = (part ? a.to.notes : a.to.prefix_notes)[tile_note(c, g, tile, M)];
-        const int kv_len = part ? max(c.kv_lens[b], 0) : 0;
-        at[part] = ((int64_t)note.x * c.HKV + head) * M + (k - tile * M);
-        n[part] = parts_of(row_limit(g, kv_len, part, row), note.y);
+        const int k = max(t - g.first, 0) * c.G + (min(h, c.HQ - 1) - head * c.G), tile = k >> a.cut.log2_M;
+        const uint64_t note = (part ? a.to.notes : a.to.prefix_notes)[(int64_t)tile_note(c, g, tile, M) * c.HKV + head];
+        const int kv_len = part ? max(c.kv_lens[b], 0) : 0, chunk = (int)(note >> 32);
+        const int slot = (int)min((uint32_t)note, (uint32_t)a.slots - 1u);  // (anything, if starts decrease)
+        at[part] = ((int64_t)slot * c.HKV + head) * M + (k - tile * M);
+        n[part] = min(parts_of(row_limit(g, kv_len, part, row), chunk), a.slots - slot);
         if (c.groups == 0) {
             const int last = min(g.rows * c.G, (tile + 1) * M) - 1;
-            whole = parts_of(row_limit(g, kv_len, true, last / c.G), note.y) == 1;
+            whole = parts_of(row_limit(g, kv_len, true, last / c.G), chunk) == 1;
         }
     }
     PagedSum sum;
@@ -61,6 +62,7 @@ struct PagedPlan {
     int64_t slots;
     bool join;    // a tile may have several parts
     bool inside;  // which the last of its workgroups joins
+    int notes;    // tiles of sequences
     size_t part_at, ml_at, notes_at, prefix_notes_at;  // in the workspace, whose first bytes are the counters
     size_t bytes;
 };
@@ -94,7 +96,9 @@ static PagedPlan paged_plan(const bz_paged_kv* d) {
     // tiles that there can be, and with them notes
     const int64_t notes = (int64_t)d->T * G / M + d->B, prefix_notes = d->groups > 0 ? (int64_t)d->T * G / M + d->groups : 0;
     p.join = d->groups > 0 || (int64_t)d->table_width * d->page_size > p.cut.min_chunk;
-    p.inside = p.join && M <= 32 && d->groups == 0 && notes * d->HKV <= kPagedCounters && d->HKV <= 256;
+    p.inside = p.join && M <= 32 && (notes + prefix_notes) * d->HKV <= kPagedCounters &&
+               (d->groups == 0 || (!d->q_starts && M % G == 0));
+    p.notes = (int)notes;
     p.slots = p.join ? paged_slots(notes + prefix_notes, target) : notes;
     p.bytes = kPagedCounters * sizeof(unsigned);
     auto take = [&](size_t n) {
@@ -105,8 +109,8 @@ static PagedPlan paged_plan(const bz_paged_kv* d) {
     const size_t rows = p.join ? (size_t)p.slots * d->HKV * M : 0;
     p.part_at = take(rows * d->D * sizeof(float));
     p.ml_at = take(rows * sizeof(float2));
-    p.notes_at = take((size_t)notes * sizeof(int2));
-    p.prefix_notes_at = take((size_t)prefix_notes * sizeof(int2));
+    p.notes_at = take((size_t)notes * d->HKV * sizeof(uint64_t));
+    p.prefix_notes_at = take((size_t)prefix_notes * d->HKV * sizeof(uint64_t));
     return p;
 }
 
@@ -134,8 +138,10 @@ static void launch_tiles(const PagedKv& c, const PagedAttn& a, int64_t slots, hi
 template <int D>
 static void launch_attn(const PagedKv& c, PagedAttn a, const PagedPlan& p, char* ws, bool f8, hipStream_t st) {
     a.cut = p.cut;
+    a.own_notes = p.notes;
+    a.slots = (int)p.slots;
     a.to = {reinterpret_cast<float*>(ws + p.part_at), reinterpret_cast<float2*>(ws + p.ml_at),
-            reinterpret_cast<int2*>(ws + p.notes_at), reinterpret_cast<int2*>(ws + p.prefix_notes_at)};
+            reinterpret_cast<uint64_t*>(ws + p.notes_at), reinterpret_cast<uint64_t*>(ws + p.prefix_notes_at)};
     if (f8)
         launch_tiles<D, true>(c, a, p.slots, st);
     else

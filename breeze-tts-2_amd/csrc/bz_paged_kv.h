@@ -35,11 +35,12 @@ struct PagedKv {
 // Rows [first, end) of sequence b.
 struct RowRange {
     int first, end;
+    bool back;  // its starts decrease (it is then empty)
 };
 __device__ __forceinline__ RowRange seq_rows(const PagedKv& c, int b) {
-    if (!c.q_starts) return {b, b + 1};
-    const int s = min(max(c.q_starts[b], 0), c.T);
-    return {s, min(max(c.q_starts[b + 1], s), c.T)};
+    if (!c.q_starts) return {b, b + 1, false};
+    const int from = c.q_starts[b], to = c.q_starts[b + 1], s = min(max(from, 0), c.T);
+    return {s, min(max(to, s), c.T), to < from};
 }
 
 // The sequence of row t: the number of ends at or before it (B for a row of no

@@ -19,22 +19,26 @@ struct PagedSeg {
     int first, rows;  // rows of q and out
     int keys;
     int seq;    // the sequence, or B + the prefix
+    bool back;  // its starts decrease
 };
 
 // Segment B + p: prefix p.
 __device__ __forceinline__ PagedSeg paged_seg(const PagedKv& c, int s) {
-    PagedSeg g = {0, 0, 0, s};
+    PagedSeg g = {0, 0, 0, s, false};
     if (s < c.B) {
         const RowRange r = seq_rows(c, s);
         g.first = r.first;
         g.rows = r.end - r.first;
+        g.back = r.back;
         g.keys = min(max(c.kv_lens[s], 0), c.width << c.shift);
     } else {
         const int p = s - c.B;
         int lo = 0, hi = c.B;
         if (c.prefix_seqs) {
-            lo = min(max(c.prefix_seqs[p], 0), c.B);
-            hi = min(max(c.prefix_seqs[p + 1], lo), c.B);
+            const int from = c.prefix_seqs[p], to = c.prefix_seqs[p + 1];
+            lo = min(max(from, 0), c.B);
+            hi = min(max(to, lo), c.B);
+            g.back = to < from;
         }
         if (hi > lo) {
             g.first = seq_rows(c, lo).first;
@@ -113,18 +117,21 @@ __device__ __forceinline__ SegCut seg_cut(const PagedKv& c, const PagedSeg& g, i
 }
 
 // Slot `slot`: the prefixes' come first, and of a sequence its last tiles' (whose rows
-// attend most), so that long pieces start early.
+// attend most), so that long pieces start early.  Starts that decrease would put a row
+// into several segments, more slots than there is room for: of such a batch there are none.
 __device__ __forceinline__ PagedSlot paged_slot(const PagedKv& c, const PagedCut& cut, int slot, int lane) {
     const int n = c.groups + c.B;
     auto seg = [&](int i) {
-        PagedSeg g = {0, 0, 0, 0};
+        PagedSeg g = {};
         if (i < n) g = paged_seg(c, i < c.groups ? c.B + i : i - c.groups);
         return g;
     };
     float work = 0.0f;
+    bool back = false;
     PagedSeg g = {};
     for (int i = 0; i < n; i += 64) {
         g = seg(i + lane);
+        back |= g.back;
         float keys = (float)g.keys;
         if (g.seq < c.B && g.rows > 1) {  // of a tile on average, or more (a row attends half of the new ones)
             const float kv = (float)max(c.kv_lens[g.seq], 0);
@@ -137,6 +144,7 @@ __device__ __forceinline__ PagedSlot paged_slot(const PagedKv& c, const PagedCut
         max(cut.min_chunk, ((int)ceilf(fminf(work / cut.target, 1073741824.0f)) + 31) & ~31));
     PagedSlot r = {};
     r.chunk = chunk;
+    if (__ballot(back)) return r;
     int base = 0;
     for (int i = 0; i < n; i += 64) {
         if (n > 64) g = seg(i + lane);

@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT < 256 || F8 || D == 
     const bool whole = w.parts == 1 && c.groups == 0;  // no other slot has keys of these rows
     const PagedParts parts(a, c, slot, head, M, D);
     const float vs = F8 ? c.v_scale[head] : 1.0f;
-    if (!a.arrived && u.split == 0 && head == 0 && tid == 0) note_tile(c, a, w, M, slot);
+    if ((!a.arrived || c.groups > 0) && u.split == 0 && tid == 0) note_tile(c, a, w, M, slot, head);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         if (16 * rt >= nrow) break;
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT < 256 || F8 || D == 
     }
     if (!whole && a.arrived) {
         __syncthreads();  // (st_acc is used again)
-        paged_join_last<D, F8>(c, a, w, head, M, tid, reinterpret_cast<float(*)[8]>(&st_acc[0][0][0]), &st_apart[0]);
+        paged_join_last<D, F8>(c, a, w, head, M, tid, lane, reinterpret_cast<float(*)[8]>(&st_acc[0][0][0]), &st_apart[0]);
     }
 }
 

@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
         round(tile + 1, k1, k0, v1, v0, top1, top0);
     }
     if (tile < tiles) round(tile, k0, k1, v0, v1, top0, top1);
-    if (u.split == 0 && head == 0 && tid == 0) note_tile(c, a, w, M, slot);
+    if (u.split == 0 && tid == 0) note_tile(c, a, w, M, slot, head);
     if (apart) {
         paged_rows_apart<D, F8>(c, a, w, slot, head, M, wave, WAVES, lane);
         return;

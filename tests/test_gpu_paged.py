@@ -269,6 +269,37 @@ def test_prefix_many_sequences():
             prefix=([200, 60], [0, 70, 128]))
 
 
+@pytest.mark.parametrize("HQ,HKV,D", [(16, 8, 128), (16, 1, 64), (4, 4, 128), (9, 3, 128), (16, 4, 256)])
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+def test_prefix_many_groups(HQ, HKV, D, kv):
+    """One row each: prefixes of one sequence to 33, and of none, sequences before, between and behind them; more
+    segments than one wave counts at a time."""
+    rng = np.random.default_rng(16)
+    size = [1, 2, 0, 33, 1, 5, 8, 0, 3, 4, 9, 1, 1, 2]
+    starts = 2 + np.cumsum([0] + size)
+    B = int(starts[-1]) + 3
+    for _ in range(2):  # (the second time with the counters that the first has left)
+        _attend(17, HQ, HKV, D, list(rng.integers(0, 400, B)), kv=kv, prefix=(list(rng.integers(0, 700, len(size))),
+                                                                           [int(s) for s in starts]))
+
+
+def test_starts_that_decrease_leave_the_workspace_usable():
+    """What such rows hold is not said; the next call with good ones is right."""
+    rng = np.random.default_rng(18)
+    cache = Cache(rng, 64, 2, 16, 128)
+    table, ptable = cache.table(8, 4), cache.table(3, 4)
+    q = bf16(rng.standard_normal((8, 4, 128)))
+    lens = ints([50, 9, 64, 1, 0, 33, 20, 64])
+    good = (lambda: T.shared_prefix_attention(q, cache.k, cache.v, ptable, ints([60, 64, 7]), table, lens,
+                                              prefix_seqs=ints([0, 3, 3, 7])),
+            lambda: T.paged_attention(q, cache.k, cache.v, table, lens, ints([0, 2, 3, 3, 5, 6, 7, 8, 8])))
+    want = [f() for f in good]
+    T.shared_prefix_attention(q, cache.k, cache.v, ptable, ints([60, 64, 7]), table, lens, prefix_seqs=ints([0, 8, 0, 8]))
+    T.paged_attention(q, cache.k, cache.v, table, lens, ints([0, 8, 0, 8, 0, 8, 0, 8, 2]))
+    for f, w in zip(good, want):
+        assert torch.equal(f(), w)
+
+
 def _poison(cache, table, kv_lens):
     """NaN and infinities in every place of the pool that no position of these
     sequences has."""
