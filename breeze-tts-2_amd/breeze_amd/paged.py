@@ -23,6 +23,7 @@ kv_lens           int32 [B], the new rows included
 q_starts          int32 [B + 1]: sequence b has the rows q_starts[b] .. q_starts[b + 1] - 1,
                   its newest positions in order; None: one row each.  Rows of no sequence
                   are not touched: in a tensor that the call allocates they hold anything.
+                  Starts must not decrease; if they do, rows hold anything.
 
 Lengths, tables and starts are read on the device: no call synchronizes, and a
 captured graph follows them.  Calls may run on several streams at once, and graphs on
@@ -86,15 +87,6 @@ def _table(name: str, t: torch.Tensor, index: int) -> tuple:
     return rows, width, p, ld
 
 
-def _strides(t: torch.Tensor) -> tuple:
-    """Element strides of a pool; those of dimensions of size 1 are not used and count as D."""
-    a, b, c, d = t.stride()
-    if d != 1:
-        raise ValueError("a position's D elements must be contiguous")
-    pages, heads, _, D = t.shape
-    return a if pages > 1 else D, b if heads > 1 else D, c
-
-
 def _check_cache(k_pages, v_pages, index: int) -> None:
     """Raises what is wrong with the pools."""
     _gpu("k_pages", k_pages, index)
@@ -116,30 +108,43 @@ def _scale(name: str, t, HKV: int, index: int) -> int:
 
 def _cache(T: int, HQ: int, k_pages, v_pages, k_scale, v_scale, block_table, kv_lens, q_starts, index: int) -> tuple:
     """The fields of bz_paged_kv without the prefixes', checked."""
-    shape, dtype = k_pages.shape, k_pages.dtype
-    kind = _KV.get(dtype)
     # one expression for what is nearly always so; what it is not is found out afterwards
-    if not (kind is not None and k_pages.get_device() == index and v_pages.get_device() == index and index >= 0
-            and len(shape) == 4 and v_pages.shape == shape and v_pages.dtype == dtype):
+    shape, dtype, tshape = k_pages.shape, k_pages.dtype, block_table.shape
+    if not (dtype in _KV and k_pages.get_device() == index and v_pages.get_device() == index and index >= 0
+            and len(shape) == 4 and v_pages.shape == shape and v_pages.dtype is dtype):
         _check_cache(k_pages, v_pages, index)
     pages, HKV, ps, D = shape
-    if kind == KV_E4M3:
+    if dtype is not torch.bfloat16:
         ks, vs = _scale("k_scale", k_scale, HKV, index), _scale("v_scale", v_scale, HKV, index)
     elif k_scale is None and v_scale is None:
         ks = vs = 0
     else:
         raise ValueError("a bf16 cache has no scales")
-    B, width, table, ld = _table("block_table", block_table, index)
-    lens = _ints("kv_lens", kv_lens, (B,), index)
+    if (len(tshape) == 2 and kv_lens.dtype is block_table.dtype is torch.int32 and kv_lens.shape == tshape[:1]
+            and kv_lens.get_device() == block_table.get_device() == index and kv_lens.stride()[0] == 1
+            and (ts := block_table.stride())[1] == 1 and 1 <= tshape[1] <= ts[0]):
+        B, width = tshape
+        ld, table, lens = ts[0], block_table.data_ptr(), kv_lens.data_ptr()
+    else:
+        B, width, table, ld = _table("block_table", block_table, index)
+        lens = _ints("kv_lens", kv_lens, (B,), index)
     if q_starts is not None:
         starts = _ints("q_starts", q_starts, (B + 1,), index)
     elif T == B:
         starts = 0
     else:
         raise ValueError(f"{T} rows for {B} sequences: q_starts says which are whose")
-    return ((_lib.ABI_VERSION, T, B, HQ, HKV, D, kind, ps, pages, width),
-            (k_pages.data_ptr(), v_pages.data_ptr()) + _strides(k_pages) + _strides(v_pages)
-            + (ks, vs, table, ld, lens, starts))
+    k0, k1, k2, k3 = k_pages.stride()
+    v0, v1, v2, v3 = v_pages.stride()
+    if k3 != 1 or v3 != 1:
+        raise ValueError("a position's D elements must be contiguous")
+    # (strides of dimensions of size 1 are not used and count as D)
+    if pages == 1:
+        k0 = v0 = D
+    if HKV == 1:
+        k1 = v1 = D
+    return ((_lib.ABI_VERSION, T, B, HQ, HKV, D, _KV[dtype], ps, pages, width),
+            (k_pages.data_ptr(), v_pages.data_ptr(), k0, k1, k2, v0, v1, v2, ks, vs, table, ld, lens, starts))
 
 
 _NO_PREFIX = (0, 0), (0, 0, 0, 0)
@@ -209,13 +214,13 @@ def _norm(name: str, w: torch.Tensor, D: int, index: int) -> torch.Tensor:
     return w
 
 
-def _call(index: int, f, *args) -> None:
+def _call(index: int, stream: int, f, *args) -> None:
     """f(*args, stream) with the tensors' device current."""
     if torch._C._cuda_getDevice() == index:
-        rc = f(*args, torch._C._cuda_getCurrentRawStream(index))
+        rc = f(*args, stream)
     else:
         with torch.cuda.device(index):
-            rc = f(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = f(*args, stream)
     if rc:
         raise _lib.BzError(rc, f.__name__)
 
@@ -277,7 +282,7 @@ def paged_rope_cache(qkv, cos, sin, k_pages, v_pages, block_table, kv_lens, HQ: 
     q = qkv.new_empty((T, HQ, D)) if q_out is None else _result("q_out", q_out, (T, HQ, D), index, qkv)
     if T == 0 or sizes[2] == 0:
         return q
-    _call(index, _lib.lib().bz_paged_rope_cache, _lib.paged_kv(*sizes, 0, 0, *refs, 0, 0, 0, 0), qkv.data_ptr(),
+    _call(index, torch._C._cuda_getCurrentRawStream(index), _lib.lib().bz_paged_rope_cache, _lib.paged_kv(*sizes, 0, 0, *refs, 0, 0, 0, 0), qkv.data_ptr(),
           ld if T > 1 else width, None if qn is None else qn.data_ptr(), None if kn is None else kn.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), cs,
           ld_cs if shape[0] > 1 else D, shape[0], at, q.data_ptr(), q.stride()[0] if T > 1 else HQ * D)
     return q
@@ -303,8 +308,9 @@ def _attention(q, k_pages, v_pages, block_table, kv_lens, q_starts, prefix, scal
         return out
     sizes += psizes
     n = _workspace_bytes(sizes)
-    ws = _lib.stream_workspace(_WS, (index,), n, q.device, torch._C._cuda_getCurrentRawStream(index), _WS_RETIRED)
-    _call(index, _lib.lib().bz_paged_attn, _lib.paged_kv(*sizes, *refs, *prefs), q.data_ptr(),
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    ws = _lib.stream_workspace(_WS, (index,), n, q.device, stream, _WS_RETIRED)
+    _call(index, stream, _lib.lib().bz_paged_attn, _lib.paged_kv(*sizes, *refs, *prefs), q.data_ptr(),
           q.stride()[0] if T > 1 else width, D ** -0.5 if scale is None else scale, ws.data_ptr(), n, out.data_ptr(), ld)
     return out
 
