@@ -6,11 +6,14 @@
 
 namespace bz {
 
-// Workgroups that the keys are cut for: as many as run at once, so that none starts late.
+// Workgroups that the keys are cut for: for few rows as many as run at once, so that none
+// starts late.  For many rows two to a CU, less those that a tile's last, shorter chunk adds (24
+// sequences in three groups, e4m3, 16 / 4 heads of 256: 56 us with 512, 41 with 384, 43 with
+// 416; three chunks of prompts, bf16: 367 with 384, 349 with 416).
 static int paged_workgroups(int D, bool f8, int M) {
-    if (M > 32) return 384;
-    if (D == 256) return (f8 ? 512 : 256);
-    return (D == 64 ? (M == 16 ? 1024 : 768) : (M == 16 ? 768 : 512));
+    if (M > 32) return 416;
+    if (D == 256) return f8 ? 512 : 256;
+    return D == 64 ? (M == 16 ? 1024 : 768) : (M == 16 ? 768 : 512);
 }
 
 // The parts of a row joined in a launch of its own: its prefix's, then its own.
@@ -72,9 +75,9 @@ struct PagedPlan {
 constexpr int kPagedCounters = 16384;
 
 // Rows of a tile for segments of `rows` query rows.
-static int paged_tile_rows(int64_t rows, int D, bool f8) {
+static int paged_tile_rows(int64_t rows, int D) {
     if (rows <= 16) return 16;
-    if (D == 256) return rows <= 64 || f8 ? 64 : 128;  // (eight waves of e4m3 on its way do not fit the registers)
+    if (D == 256) return rows <= 64 ? 64 : 128;
     return rows <= 32 ? 32 : (rows <= 64 ? 64 : 128);
 }
 
@@ -84,7 +87,7 @@ static PagedPlan paged_plan(const bz_paged_kv* d) {
     const bool f8 = d->kv_dtype != BZ_DT_BF16;
     // by what a segment has on average, a prefix's or a sequence's
     const int64_t segs = d->groups > 0 ? std::min(d->B, d->groups) : d->B;
-    const int M = paged_tile_rows(((int64_t)d->T + segs - 1) / segs * G, d->D, f8);
+    const int M = paged_tile_rows(((int64_t)d->T + segs - 1) / segs * G, d->D);
     const int target = std::max(1, paged_workgroups(d->D, f8, M) / d->HKV);
     p.cut.M = M;
     p.cut.log2_M = __builtin_ctz(M);
@@ -128,9 +131,9 @@ static void launch_tiles(const PagedKv& c, const PagedAttn& a, int64_t slots, hi
             hipLaunchKernelGGL((paged_attn_bf16_tile<D, F8, 4, true>), grid, dim3(256), 0, st, c, a);
             break;
         default:
-            if constexpr (D == 256 && !F8)
+            if constexpr (D == 256)
                 hipLaunchKernelGGL((paged_attn_bf16_tile<D, F8, 8, true>), grid, dim3(512), 0, st, c, a);
-            else if constexpr (D < 256)
+            else
                 hipLaunchKernelGGL((paged_attn_bf16_tile<D, F8, 4, false>), grid, dim3(256), 0, st, c, a);
     }
 }

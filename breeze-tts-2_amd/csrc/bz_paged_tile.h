@@ -10,8 +10,8 @@
 //           so a row's maximum is over its own numbers, one swap of the wave's halves and
 //           (PAIR) what the other wave found
 //   p v     A = the values transposed, by transposing LDS reads
-//           (ds_read_b64_tr_b16: 4 keys of one column to a lane), in the order of keys in
-//           which the lanes have their probabilities: these are the B operand as they
+//           (ds_read_b64_tr_b16: 4 keys of one column to a lane, of e4m3 8 with
+//           ds_read_b64_tr_b8), in the order of keys in which the lanes have their probabilities: these are the B operand as they
 //           are (PAIR: also the other wave's, through LDS).  p is rounded to bf16 (2^-9 of it on
 //           average, as much as the output's own rounding; a second part would double
 //           these products); the sum l is over p before it is rounded
@@ -20,6 +20,8 @@
 //   order   in one round: the softmax of a tile beside the scores of the next one, then
 //           its products; keys are fetched three tiles ahead, values one, and one
 //           barrier (PAIR: two, the probabilities have one buffer) ends a round's first half
+//   e4m3    stays as it is in LDS, which leaves room for a second workgroup on a CU, and is widened
+//           by the wave that reads it (one instruction for two values)
 //   LDS     16-byte pieces of a row are exchanged so that neither the row-wise reads of
 //           keys nor the transposing ones of values meet on a bank.  Every buffer is a
 //           variable of its own and the rounds take them in turn by name: that tells the
@@ -52,7 +54,16 @@ __device__ __forceinline__ float other_half_sum(float v) {
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-// A wave's RW rows of a tile's keys or values on their way to LDS.
+// Eight keys of one column, e4m3: lane i of 16 points at key i / 2, columns 8 (i % 2) ..,
+// and gets column i of the eight keys.
+__device__ __forceinline__ u32x4 lds_column8(const char* p) {
+    typedef int s32x2 __attribute__((ext_vector_type(2)));
+    const auto v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+        (__attribute__((address_space(3))) s32x2*)(__attribute__((address_space(3))) void*)const_cast<char*>(p));
+    return f8_widen((uint32_t)v[0], (uint32_t)v[1]);
+}
+
+// A wave's RW rows of a tile's keys or values, straight into LDS.
 template <int D, bool F8, int RW>
 struct TileStage {
     static constexpr int ROW = D * (F8 ? 1 : 2);  // bytes of a position
@@ -60,55 +71,30 @@ struct TileStage {
     static constexpr int ROWS = 64 / LR;          // rows of a load
     static constexpr int N = RW * ROW / 1024;     // loads of a wave
     static_assert(N > 0 && N * 1024 == RW * ROW, "whole loads of a wave");
-    u32x4 w[N];
 
-    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t pos, int lane) {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            w[i] = buffer_ld16(r, (uint32_t)(i * ROWS + lane / LR) * pos + 16 * (lane % LR));
-    }
-    // e4m3, widened, as the rows from `first` of a tile; piece p of row key at p ^ swap(key)
-    template <typename X>
-    __device__ __forceinline__ void store(char* tile, int first, int lane, X swap) const {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int key = first + i * ROWS + lane / LR, p = lane % LR;
-            char* row = tile + key * (2 * D);
-            *reinterpret_cast<u32x4*>(row + 16 * ((2 * p) ^ swap(key))) = f8_widen(w[i][0], w[i][1]);
-            *reinterpret_cast<u32x4*>(row + 16 * ((2 * p + 1) ^ swap(key))) = f8_widen(w[i][2], w[i][3]);
-        }
-    }
-    // bf16 straight into LDS, 16 bytes a lane one after the other: lane l writes piece
-    // l % LR of its row, so it reads the piece that belongs there.  A load's rows are in
+    // 16 bytes a lane one after the other: lane l writes piece l % LR of its row, so it reads
+    // the piece that belongs there, piece p of row key at p ^ swap(key).  A load's rows are in
     // its scalar offset; a lane's offsets differ between loads only by the exchange of
     // pieces, which repeats.
     template <typename X>
-    __device__ __forceinline__ static void load_lds(__amdgpu_buffer_rsrc_t r, uint32_t pos, char* tile, int first, int lane,
-                                                    X swap) {
+    __device__ __forceinline__ static void load(__amdgpu_buffer_rsrc_t r, uint32_t pos, char* tile, int first, int lane,
+                                                X swap) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                r, (__attribute__((address_space(3))) void*)(tile + (first + i * ROWS) * (2 * D)), 16,
+                r, (__attribute__((address_space(3))) void*)(tile + (first + i * ROWS) * ROW), 16,
                 (uint32_t)(lane / LR) * pos + 16 * ((lane % LR) ^ swap(first + i * ROWS + lane / LR)), i * ROWS * pos, 0, 0);
-    }
-    __device__ __forceinline__ bool odd() const {
-        bool o = false;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o |= nan_f8x4(w[i][e]);
-        return o;
     }
 };
 
-// Order for the scheduler: N matrix products, each behind its R LDS reads, with the reads
-// of A products under way.
-template <int N, int R, int A>
+// Order for the scheduler: N steps of P matrix products, each behind its R LDS reads, with the
+// reads of A steps under way.
+template <int N, int P, int R, int A>
 __device__ __forceinline__ void read_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x100, R * A, 0);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, P, 0);
         if (i + A < N) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
     }
 }
@@ -117,9 +103,9 @@ template <int D, bool F8, int WAVES, bool PAIR>
 __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c, PagedAttn a) {
     constexpr int W = PAIR ? 2 : 1;  // waves of a row
     constexpr int M = 32 * WAVES / W, RW = kTileKeys / WAVES, T = D / 16, ND = D / 32 / W, KB = 2 / W;
-    constexpr int kAhead = F8 ? 2 : 4;  // LDS reads under way, in products (e4m3 on its way takes registers)
-    constexpr int kTileBytes = kTileKeys * D * 2, kProbs = PAIR ? WAVES * 2048 : 16;
+    constexpr int kAhead = 4;  // LDS reads under way, in steps
     using Stage = TileStage<D, F8, RW>;
+    constexpr int ROW = Stage::ROW, kTileBytes = kTileKeys * ROW, kProbs = PAIR ? WAVES * 2048 : 16;
     __shared__ __attribute__((aligned(16))) char k0[kTileBytes], k1[kTileBytes], v0[kTileBytes], v1[kTileBytes];
     __shared__ __attribute__((aligned(16))) char probs[kProbs];
     __shared__ float top0[PAIR ? WAVES : 1][32], top1[PAIR ? WAVES : 1][32];  // a tile's maxima
@@ -140,9 +126,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
     const int limit = row_limit(g, w.kv_len, w.own, row);
     u32x4 q[T];
     {
-        const uint16_t* p = a.q + (int64_t)(g.first + row) * a.ld_q + (int64_t)qh * D + 8 * half;
+        const uint16_t* p = a.q + (int64_t)(g.first + row) * a.ld_q + (int64_t)qh * D;
+        // (a lane's 16 bytes of e4m3 keys are those of two products)
 #pragma unroll
-        for (int t = 0; t < T; ++t) q[t] = ldg16(p + 16 * t);
+        for (int t = 0; t < T; ++t) q[t] = ldg16(p + (F8 ? 32 * (t / 2) + 16 * half + 8 * (t % 2) : 16 * t + 8 * half));
     }
     const int32_t* table = w.own ? c.table + (int64_t)g.seq * c.ld_table
                                  : c.prefix_table + (int64_t)(g.seq - c.B) * c.ld_prefix;
@@ -163,28 +150,36 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
     uint32_t n_of = 0;
     int from_tile = -16;
     const int tiles = (max(w.end - w.begin, 0) + kTileKeys - 1) / kTileKeys;
-    // (64 banks: a row of 256 bytes or more lies on all of them.  No conflicts; with 7 and 2 for all D
+    // (64 banks: the rows of ROW bytes begin on 256 / ROW places of them.  No conflicts; with 7 and 2 for all D
     // 40% of the LDS cycles were conflicts)
-    auto k_swap = [](int key) { return key & (D == 64 ? 7 : 15); };
-    auto v_swap = [](int key) { return (D == 64 ? 2 : 4) * (key & 3); };
+    auto k_swap = [](int key) { return F8 ? (ROW == 256 ? key & 15 : ROW == 128 ? key >> 1 & 7 : key >> 2 & 3) : key & (D == 64 ? 7 : 15); };
+    auto v_swap = [](int key) {
+        if (!F8) return (D == 64 ? 2 : 4) * (key & 3);
+        const int bit3 = key >> 3 & 1;
+        return 2 * (ROW == 256 ? (key & 3) + 4 * bit3 : ROW == 128 ? (key >> 1 & 1) + 2 * bit3 : bit3);
+    };
 
-    // where this lane reads: its key's pieces 2 t + half (t of 0..3, then 8 pieces on), and its columns of keys
-    // 4 half + 0..3 (of an even and an odd block of 32 columns, then 8 pieces on)
-    uint32_t k_at[T < 8 ? T : 8], v_at[ND];
+    // where this lane reads: its key's pieces 2 t + half (t of 0..7, then 16 pieces on), and its columns of keys
+    // 4 half + 0..3 (e4m3: and 8 on) of a block of 32 columns
+    constexpr int TK = F8 ? T / 2 : T;  // reads of a key
+    uint32_t k_at[TK < 8 ? TK : 8], v_at[ND];
     {
 #pragma unroll
-        for (int t = 0; t < 8 && t < T; ++t) k_at[t] = (32 * KB * kp + col) * (2 * D) + 16 * ((2 * t + half) ^ k_swap(col));
-        const int i16 = lane & 15, key = 4 * half + (i16 >> 2), piece = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
+        for (int t = 0; t < 8 && t < TK; ++t) k_at[t] = (32 * KB * kp + col) * ROW + 16 * ((2 * t + half) ^ k_swap(col));
+        const int i16 = lane & 15, r = F8 ? i16 >> 1 : i16 >> 2;
+        const int key = 4 * half + (r & 3) + 8 * (r >> 2);
 #pragma unroll
-        for (int t = 0; t < ND; ++t)
-            v_at[t] = key * (2 * D) + 8 * (i16 & 1) + 16 * ((4 * (kp * ND + t) + piece) ^ v_swap(key));
+        for (int t = 0; t < ND; ++t) {
+            const int block = kp * ND + t, hi = lane >> 4 & 1;
+            v_at[t] = F8 ? key * ROW + 8 * (i16 & 1) + 16 * ((2 * block + hi) ^ v_swap(key))
+                         : key * ROW + 8 * (i16 & 1) + 16 * ((4 * block + 2 * hi + (i16 >> 1 & 1)) ^ v_swap(key));
+        }
     }
 
     struct Tile {
         uint32_t n;            // positions there
         uint32_t v_lo, v_hi;   // where this wave's rows of the values begin
     };
-    Stage sk, sv;  // (e4m3: on its way through registers)
     auto rows_at = [&](uint32_t lo, uint32_t hi, uint32_t n, uint32_t pos) {
         const int there = (int)(n >> (8 * (RW * wave / 16)) & 0xFF) - RW * wave % 16;
         return buffer_rsrc(reinterpret_cast<const char*>((uint64_t)hi << 32 | lo),
@@ -214,18 +209,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
         uint32_t lo, hi;
         lane_of(k_from, own, lo, hi);
         const __amdgpu_buffer_rsrc_t r = rows_at(lo, hi, x.n, (uint32_t)c.k_pos);
-        if constexpr (F8)
-            sk.load(r, (uint32_t)c.k_pos, lane);
-        else
-            Stage::load_lds(r, (uint32_t)c.k_pos, to, RW * wave, lane, k_swap);
+        Stage::load(r, (uint32_t)c.k_pos, to, RW * wave, lane, k_swap);
         return x;
     };
     auto fetch_v = [&](const Tile& x, char* to) {
         const __amdgpu_buffer_rsrc_t r = rows_at(x.v_lo, x.v_hi, x.n, (uint32_t)c.v_pos);
-        if constexpr (F8)
-            sv.load(r, (uint32_t)c.v_pos, lane);
-        else
-            Stage::load_lds(r, (uint32_t)c.v_pos, to, RW * wave, lane, v_swap);
+        Stage::load(r, (uint32_t)c.v_pos, to, RW * wave, lane, v_swap);
     };
     // scores of the wave's keys of a tile, masked, and their maximum (PAIR: to the other wave too)
     pg_f32x16 s[KB];
@@ -233,11 +222,18 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
 #pragma unroll
         for (int b = 0; b < KB; ++b) s[b] = pg_f32x16{};
 #pragma unroll
-        for (int t = 0; t < T; ++t)
+        for (int t = 0; t < TK; ++t)
 #pragma unroll
-            for (int b = 0; b < KB; ++b)
-                s[b] = pg_mfma32(*reinterpret_cast<const u32x4*>(kb + k_at[t & 7] + 256 * (t >> 3) + 32 * b * (2 * D)), q[t], s[b]);
-        read_ahead<KB * T, 1, kAhead>();
+            for (int b = 0; b < KB; ++b) {
+                const u32x4 x = *reinterpret_cast<const u32x4*>(kb + k_at[t & 7] + 256 * (t >> 3) + 32 * b * ROW);
+                if constexpr (F8) {
+                    s[b] = pg_mfma32(f8_widen(x[0], x[1]), q[2 * t], s[b]);
+                    s[b] = pg_mfma32(f8_widen(x[2], x[3]), q[2 * t + 1], s[b]);
+                } else {
+                    s[b] = pg_mfma32(x, q[t], s[b]);
+                }
+            }
+        read_ahead<KB * TK, F8 ? 2 : 1, 1, kAhead>();
         const int at = w.begin + kTileKeys * tile;
         if (at + kTileKeys > w.all || x.n != 0x10101010u) {
 #pragma unroll
@@ -267,9 +263,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
     float mx = 0.0f;
     Tile x0 = {}, x1 = {}, x2 = {};
 
-    // Tile `tile`: its softmax, the next one's scores, its products.  ke: where the keys two tiles on are
-    // under way to, ko: the next one's, and later those of three tiles on.
-    auto round = [&](int tile, char* ke, char* ko, char* vb, char* vn, float (*top)[32],
+    // Tile `tile`: its softmax, the next one's scores, its products.  ko: the next one's keys, and later those of
+    // three tiles on.
+    auto round = [&](int tile, char* ko, char* vb, char* vn, float (*top)[32],
                      float (*top_next)[32]) __attribute__((always_inline)) {
         if constexpr (PAIR) mx = fmaxf(mx, top[wave ^ 1][col]);
         mx *= sc;
@@ -307,32 +303,23 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
         const int at = w.begin + kTileKeys * tile;
         const bool mask = at + kTileKeys > w.all || x0.n != 0x10101010u;
         const bool differ = mask && w.all < w.end;  // (behind all rows' limits there are zeros)
-        if constexpr (F8) {
-            sk.store(ke, RW * wave, lane, k_swap);
-            sv.store(vb, RW * wave, lane, v_swap);
-            if (differ) {
-                const bool o = __ballot(sv.odd()) != 0;
-                if (lane == 0) odd[tile & 1][wave] = o;
-            }
-        } else {
-            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-            if (mask) {
-                // places that are not there, as zeros; the other values looked at
-                const int there = (int)(x0.n >> (8 * (RW * wave / 16)) & 0xFF) - RW * wave % 16;
-                bool o = false;
-                for (int i = lane; i < RW * D / 8; i += 64) {
-                    u32x4* y = reinterpret_cast<u32x4*>(vb + RW * wave * (2 * D)) + i;
-                    if (i / (D / 8) >= there) {
-                        *y = u32x4{0u, 0u, 0u, 0u};
-                    } else if (differ) {
-                        const u32x4 z = *y;
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+        if (mask) {
+            // places that are not there, as zeros; the other values looked at
+            const int there = (int)(x0.n >> (8 * (RW * wave / 16)) & 0xFF) - RW * wave % 16;
+            bool o = false;
+            for (int i = lane; i < RW * Stage::LR; i += 64) {
+                u32x4* y = reinterpret_cast<u32x4*>(vb + RW * wave * ROW) + i;
+                if (i / Stage::LR >= there) {
+                    *y = u32x4{0u, 0u, 0u, 0u};
+                } else if (differ) {
+                    const u32x4 z = *y;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o |= not_finite2(z[e]);
-                    }
+                    for (int e = 0; e < 4; ++e) o |= F8 ? nan_f8x4(z[e]) : not_finite2(z[e]);
                 }
-                o = __ballot(o) != 0;
-                if (lane == 0) odd[tile & 1][wave] = o;
             }
+            o = __ballot(o) != 0;
+            if (lane == 0) odd[tile & 1][wave] = o;
         }
         __syncthreads();
         if (differ) {
@@ -353,30 +340,32 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
         const Tile x3 = fetch_k(tile + 3, ko);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {  // (PAIR: the wave's own 32 keys, the other's)
-            const char* vr = vb + 32 * (PAIR && b ? kp ^ 1 : PAIR ? kp : b) * (2 * D);
+            const char* vr = vb + 32 * (PAIR && b ? kp ^ 1 : PAIR ? kp : b) * ROW;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const u32x4 pj = PAIR && b ? o[j] : p[PAIR ? 0 : b][j];
 #pragma unroll
                 for (int t = 0; t < ND; ++t) {
-                    const char* y = vr + 16 * j * (2 * D) + v_at[t];
-                    const uint2 lo = lds_column4(y), hi = lds_column4(y + 8 * (2 * D));
-                    acc[t] = pg_mfma32(u32x4{lo.x, lo.y, hi.x, hi.y}, pj, acc[t]);
+                    const char* y = vr + 16 * j * ROW + v_at[t];
+                    if constexpr (F8) {
+                        acc[t] = pg_mfma32(lds_column8(y), pj, acc[t]);
+                    } else {
+                        const uint2 lo = lds_column4(y), hi = lds_column4(y + 8 * ROW);
+                        acc[t] = pg_mfma32(u32x4{lo.x, lo.y, hi.x, hi.y}, pj, acc[t]);
+                    }
                 }
             }
         }
-        read_ahead<4 * ND, 2, kAhead>();
+        read_ahead<4 * ND, 1, F8 ? 1 : 2, kAhead>();
         x0 = x1;
         x1 = x2;
         x2 = x3;
     };
     if (tiles > 0) {
         x0 = fetch_k(0, k0);
-        if constexpr (F8) sk.store(k0, RW * wave, lane, k_swap);
         x1 = fetch_k(1, k1);
-        if constexpr (F8) sk.store(k1, RW * wave, lane, k_swap);
         fetch_v(x0, v0);
-        if constexpr (!F8) __builtin_amdgcn_s_waitcnt(0x0F70);
+        __builtin_amdgcn_s_waitcnt(0x0F70);
         __syncthreads();
         mx = scores(0, x0, k0, top0);
         __syncthreads();
@@ -385,10 +374,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
     // (no way out between two rounds: it made the accumulators live twice)
     int tile = 0;
     for (; tile + 1 < tiles; tile += 2) {
-        round(tile, k0, k1, v0, v1, top0, top1);
-        round(tile + 1, k1, k0, v1, v0, top1, top0);
+        round(tile, k1, v0, v1, top0, top1);
+        round(tile + 1, k0, v1, v0, top1, top0);
     }
-    if (tile < tiles) round(tile, k0, k1, v0, v1, top0, top1);
+    if (tile < tiles) round(tile, k1, v0, v1, top0, top1);
     if (u.split == 0 && tid == 0) note_tile(c, a, w, M, slot, head);
     if (apart) {
         paged_rows_apart<D, F8>(c, a, w, slot, head, M, wave, WAVES, lane);
