@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
     const PagedSlot& u = w.u;
     const PagedSeg& g = u.seg;
 
+    const bool idle = 32 * rg >= w.rows;
     // the lane's row (behind the tile's rows, its last one again)
     const int mine = u.tile * M + min(32 * rg + col, w.rows - 1);
     const int row = mine / c.G, qh = head * c.G + (mine - row * c.G);
@@ -263,6 +264,44 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
     float mx = 0.0f;
     Tile x0 = {}, x1 = {}, x2 = {};
 
+    // Up to where all waves' values of the tile (and keys of the one two on) are in LDS.
+    auto arrive = [&](int tile, char* vb) __attribute__((always_inline)) {
+        const int at = w.begin + kTileKeys * tile;
+        const bool mask = at + kTileKeys > w.all || x0.n != 0x10101010u;
+        const bool differ = mask && w.all < w.end;  // (behind all rows' limits there are zeros)
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+        if (mask) {
+            // places that are not there, as zeros; the other values looked at
+            const int there = (int)(x0.n >> (8 * (RW * wave / 16)) & 0xFF) - RW * wave % 16;
+            bool o = false;
+            for (int i = lane; i < RW * Stage::LR; i += 64) {
+                u32x4* y = reinterpret_cast<u32x4*>(vb + RW * wave * ROW) + i;
+                if (i / Stage::LR >= there) {
+                    *y = u32x4{0u, 0u, 0u, 0u};
+                } else if (differ) {
+                    const u32x4 z = *y;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o |= F8 ? nan_f8x4(z[e]) : not_finite2(z[e]);
+                }
+            }
+            o = __ballot(o) != 0;
+            if (lane == 0) odd[tile & 1][wave] = o;
+        }
+        __syncthreads();
+        if (differ) {
+            int o = 0;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) o |= odd[tile & 1][i];
+            apart |= __builtin_amdgcn_readfirstlane(o) != 0;  // (what is summed from here on is not used)
+        }
+    };
+    auto fetch_next = [&](int tile, char* ko, char* vn) __attribute__((always_inline)) {
+        // (behind the last tile no page is there: nothing is read)
+        fetch_v(x1, vn);
+        const Tile x3 = fetch_k(tile + 3, ko);
+        return x3;
+    };
+
     // Tile `tile`: its softmax, the next one's scores, its products.  ko: the next one's keys, and later those of
     // three tiles on.
     auto round = [&](int tile, char* ko, char* vb, char* vn, float (*top)[32],
@@ -299,35 +338,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
         }
         mx = scores(tile + 1, x1, ko, top_next);  // (behind the last tile: -inf)
 
-        // this tile's values (and the keys two tiles on) are in LDS
-        const int at = w.begin + kTileKeys * tile;
-        const bool mask = at + kTileKeys > w.all || x0.n != 0x10101010u;
-        const bool differ = mask && w.all < w.end;  // (behind all rows' limits there are zeros)
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-        if (mask) {
-            // places that are not there, as zeros; the other values looked at
-            const int there = (int)(x0.n >> (8 * (RW * wave / 16)) & 0xFF) - RW * wave % 16;
-            bool o = false;
-            for (int i = lane; i < RW * Stage::LR; i += 64) {
-                u32x4* y = reinterpret_cast<u32x4*>(vb + RW * wave * ROW) + i;
-                if (i / Stage::LR >= there) {
-                    *y = u32x4{0u, 0u, 0u, 0u};
-                } else if (differ) {
-                    const u32x4 z = *y;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o |= F8 ? nan_f8x4(z[e]) : not_finite2(z[e]);
-                }
-            }
-            o = __ballot(o) != 0;
-            if (lane == 0) odd[tile & 1][wave] = o;
-        }
-        __syncthreads();
-        if (differ) {
-            int o = 0;
-#pragma unroll
-            for (int i = 0; i < WAVES; ++i) o |= odd[tile & 1][i];
-            apart |= __builtin_amdgcn_readfirstlane(o) != 0;  // (what is summed from here on is not used)
-        }
+        arrive(tile, vb);
         u32x4 o[2] = {};
         if constexpr (PAIR) {
             const char* from = probs + 2048 * (wave ^ 1) + 16 * lane;
@@ -335,9 +346,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
             o[1] = *reinterpret_cast<const u32x4*>(from + 1024);
             __syncthreads();
         }
-        // (behind the last tile no page is there: nothing is read)
-        fetch_v(x1, vn);
-        const Tile x3 = fetch_k(tile + 3, ko);
+        const Tile x3 = fetch_next(tile, ko, vn);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {  // (PAIR: the wave's own 32 keys, the other's)
             const char* vr = vb + 32 * (PAIR && b ? kp ^ 1 : PAIR ? kp : b) * ROW;
@@ -367,9 +376,33 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
         fetch_v(x0, v0);
         __builtin_amdgcn_s_waitcnt(0x0F70);
         __syncthreads();
-        mx = scores(0, x0, k0, top0);
+        if (!idle) mx = scores(0, x0, k0, top0);
         __syncthreads();
         x2 = fetch_k(2, k0);
+    }
+    // A wave without rows (a sequence's few beside a prefix's many) fetches alone, the same as the others.
+    if (idle) {
+        auto pass = [&](int tile, char* ko, char* vb, char* vn) {
+            arrive(tile, vb);
+            if constexpr (PAIR) __syncthreads();
+            const Tile x3 = fetch_next(tile, ko, vn);
+            x0 = x1;
+            x1 = x2;
+            x2 = x3;
+        };
+        int tile = 0;
+        for (; tile + 1 < tiles; tile += 2) {
+            pass(tile, k1, v0, v1);
+            pass(tile + 1, k0, v1, v0);
+        }
+        if (tile < tiles) pass(tile, k1, v0, v1);
+        if (apart) {
+            paged_rows_apart<D, F8>(c, a, w, slot, head, M, wave, WAVES, lane);
+        } else if constexpr (PAIR) {
+            __syncthreads();
+            __syncthreads();
+        }
+        return;
     }
     // (no way out between two rounds: it made the accumulators live twice)
     int tile = 0;
