@@ -133,10 +133,10 @@ __device__ __forceinline__ bool not_finite2(uint32_t w) {
 }
 // Whether one of four e4m3 codes is NaN (they have no infinities).
 __device__ __forceinline__ bool nan_f8x4(uint32_t w) { return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0; }
+
 // The parts that one workgroup leaves: [M][D] accumulators and [M] (m, l).  Where the
 // last workgroup of a tile joins them they are stored to the point at which all XCDs meet
-// (as agent-scope atomics are); for a launch of its own the end of this one does that
-// (those stores past the L2 took prompt tiles 8% longer).
+// (as agent-scope atomics are); for a launch of its own the end of this one does that.
 struct PagedParts {
     __amdgpu_buffer_rsrc_t acc, ml;
     bool agent;
@@ -158,6 +158,16 @@ struct PagedParts {
             __builtin_amdgcn_raw_buffer_store_b128(v, acc, i * 4, 0, kCpolAgent);
         else
             __builtin_amdgcn_raw_buffer_store_b128(v, acc, i * 4, 0, 0);
+    }
+    // (of another workgroup)
+    __device__ __forceinline__ u32x4 get4(int i) const {
+        return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(acc, i * 4, 0, kCpolAgent));
+    }
+    __device__ __forceinline__ float get_m(int r) const {
+        return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ml, r * 8, 0, kCpolAgent));
+    }
+    __device__ __forceinline__ float get_l(int r) const {
+        return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ml, r * 8 + 4, 0, kCpolAgent));
     }
     __device__ __forceinline__ void put_ml(int r, float m, float l) const {
         typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -316,9 +326,10 @@ __device__ __forceinline__ void paged_join_last(const PagedKv& c, const PagedAtt
 // tile in which a value that is not finite belongs to a key that only some of the rows
 // attend (0 times it is NaN, so a matrix product would carry it into the others).
 // Not fast; such a batch has a broken sequence in it.
-template <int D, bool F8>
+// part_at(row, column): where a part has it.
+template <int D, bool F8, typename X>
 __device__ __forceinline__ void paged_rows_apart(const PagedKv& c, const PagedAttn& a, const PagedWork& w, int slot,
-                                                 int head, int M, int wave, int waves, int lane) {
+                                                 int head, int M, int wave, int waves, int lane, X part_at) {
     constexpr int DL = D / 64;
     const PagedSeg& g = w.u.seg;
     const int32_t* table = w.own ? c.table + (int64_t)g.seq * c.ld_table
@@ -368,7 +379,7 @@ __device__ __forceinline__ void paged_rows_apart(const PagedKv& c, const PagedAt
             uint16_t* o = a.out + (int64_t)(g.first + row) * a.ld_out + (int64_t)h * D + DL * lane;
             for (int e = 0; e < DL; ++e) o[e] = f32_to_bf16(seen ? acc[e] / l * vs : 0.0f);
         } else {
-            for (int e = 0; e < DL; ++e) parts.put(rr * D + DL * lane + e, acc[e]);
+            for (int e = 0; e < DL; ++e) parts.put(part_at(rr, DL * lane + e), acc[e]);
             if (lane == 0) parts.put_ml(rr, m, m == -INFINITY ? (seen ? 1.0f : 0.0f) : l);
         }
     }

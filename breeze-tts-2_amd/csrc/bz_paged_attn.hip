@@ -99,8 +99,8 @@ static PagedPlan paged_plan(const bz_paged_kv* d) {
     // tiles that there can be, and with them notes
     const int64_t notes = (int64_t)d->T * G / M + d->B, prefix_notes = d->groups > 0 ? (int64_t)d->T * G / M + d->groups : 0;
     p.join = d->groups > 0 || (int64_t)d->table_width * d->page_size > p.cut.min_chunk;
-    p.inside = p.join && M <= 32 && (notes + prefix_notes) * d->HKV <= kPagedCounters &&
-               (d->groups == 0 || (!d->q_starts && M % G == 0));
+    p.inside = p.join && (notes + prefix_notes) * d->HKV <= kPagedCounters &&
+               (d->groups == 0 || (M <= 32 && !d->q_starts && M % G == 0));
     p.notes = (int)notes;
     p.slots = p.join ? paged_slots(notes + prefix_notes, target) : notes;
     p.bytes = kPagedCounters * sizeof(unsigned);

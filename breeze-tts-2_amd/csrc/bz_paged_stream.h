@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT < 256 || F8 || D == 
             for (int r = 0; r < 4; ++r) st_acc[wave][col][stream_col<D, F8>(t, 4 * grp + r)] = acc[rt][t][r];
         __syncthreads();
         if (rt == 0 && __builtin_amdgcn_readfirstlane(st_apart[0] | st_apart[1] | st_apart[2] | st_apart[3])) {
-            paged_rows_apart<D, F8>(c, a, w, slot, head, M, wave, kStreamWaves, lane);
+            paged_rows_apart<D, F8>(c, a, w, slot, head, M, wave, kStreamWaves, lane, [](int r, int d) { return r * D + d; });
             break;
         }
         for (int i = tid; i < 4 * D; i += 64 * kStreamWaves) {  // 16 rows of D / 4 pieces

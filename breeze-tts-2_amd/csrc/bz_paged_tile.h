@@ -264,6 +264,37 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
     float mx = 0.0f;
     Tile x0 = {}, x1 = {}, x2 = {};
 
+    const bool whole = w.parts == 1 && c.groups == 0;  // no other slot has keys of these rows
+    const bool inside = !whole && a.arrived;
+    // Where a part has column d of row r.  If this kernel joins it, as the lanes hold it: four columns of 64 lanes
+    // one after the other, whole lines past the L2 (row by row, as the joining launch reads them, 32 bytes at
+    // a time: a prompt of 2011 tokens, 16 / 8 heads of 128, 49.7 us, and 40.1 so).
+    auto part_at = [&](int r, int d) {
+        if (!inside) return r * D + d;
+        const int wv = r / 32 * W + d / (32 * ND), e = d % 32;
+        return (((wv * ND + d / 32 % ND) * 4 + e / 8) * 64 + e / 4 % 2 * 32 + r % 32) * 4 + e % 4;
+    };
+    // Whether this workgroup is the last of its tile's to come; if not, or not sure of it beforehand, its part is stored.
+    auto last_to_arrive = [&](auto store) {
+        int* last = &odd[0][0];
+        unsigned* count = a.arrived + (int64_t)tile_note(c, g, u.tile, M) * c.HKV + head;
+        const unsigned others = (unsigned)w.parts - 1u;
+        __syncthreads();
+        if (tid == 0)
+            *last = !apart && __hip_atomic_load(count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == others;
+        __syncthreads();
+        if (!__builtin_amdgcn_readfirstlane(*last)) {
+            store();
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (tid == 0) *last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == others;
+            __syncthreads();
+            if (!__builtin_amdgcn_readfirstlane(*last)) return false;
+        }
+        if (tid == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return true;
+    };
+
     // Up to where all waves' values of the tile (and keys of the one two on) are in LDS.
     auto arrive = [&](int tile, char* vb) __attribute__((always_inline)) {
         const int at = w.begin + kTileKeys * tile;
@@ -396,12 +427,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
             pass(tile + 1, k0, v1, v0);
         }
         if (tile < tiles) pass(tile, k1, v0, v1);
-        if (apart) {
-            paged_rows_apart<D, F8>(c, a, w, slot, head, M, wave, WAVES, lane);
-        } else if constexpr (PAIR) {
+        if constexpr (PAIR) {
             __syncthreads();
             __syncthreads();
         }
+        if (apart) paged_rows_apart<D, F8>(c, a, w, slot, head, M, wave, WAVES, lane, part_at);
+        if (inside) last_to_arrive([] {});
         return;
     }
     // (no way out between two rounds: it made the accumulators live twice)
@@ -412,10 +443,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
     }
     if (tile < tiles) round(tile, k1, v0, v1, top0, top1);
     if (u.split == 0 && tid == 0) note_tile(c, a, w, M, slot, head);
-    if (apart) {
-        paged_rows_apart<D, F8>(c, a, w, slot, head, M, wave, WAVES, lane);
-        return;
-    }
 
     l = other_half_sum(l);
     const bool any = __builtin_amdgcn_ballot_w64(seen) >> col & 0x100000001ull;
@@ -426,25 +453,79 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
         __syncthreads();
         l += top0[wave ^ 1][col];
     }
+    if (apart) paged_rows_apart<D, F8>(c, a, w, slot, head, M, wave, WAVES, lane, part_at);
 
-    const bool whole = w.parts == 1 && c.groups == 0;  // no other slot has keys of these rows
-    const int rr = 32 * rg + col;
-    if (rr >= w.rows) return;
+    const int rr = 32 * rg + col, first = 32 * ND * kp + 4 * half;
     const PagedParts parts(a, c, slot, head, M, D);
+    auto store_part = [&] {
+        if (apart || rr >= w.rows) return;
+        if (half == 0 && kp == 0) parts.put_ml(rr, m, l);
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4)
+                parts.put4(inside ? ((wave * ND + t) * 4 + r / 4) * 256 + 4 * lane : rr * D + first + 32 * t + 2 * r, acc[t][r], acc[t][r + 1], acc[t][r + 2], acc[t][r + 3]);
+    };
+    if (!whole && !inside) {
+        store_part();
+        return;
+    }
+    if (inside) {
+        if (!last_to_arrive(store_part)) return;
+        // all parts in their order, this workgroup's own from its registers: whichever is last, the sums are the same
+        float top = apart ? -INFINITY : m;
+        for (int i = 0; i < w.parts; i += 4) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                x[e] = PagedParts(a, c, u.first_slot + min(i + e, w.parts - 1), head, M, D).get_m(rr);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (apart || min(i + e, w.parts - 1) != u.split) top = fmaxf(top, x[e]);
+        }
+        pg_f32x16 sum[ND];
+#pragma unroll
+        for (int t = 0; t < ND; ++t) sum[t] = pg_f32x16{};
+        float ls = 0.0f;
+        for (int i = 0; i < w.parts; ++i) {
+            if (!apart && i == u.split) {
+                const float f = top == -INFINITY ? 1.0f : pg_exp2(m - top);
+                ls = fmaf(l, f, ls);
+#pragma unroll
+                for (int t = 0; t < ND; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sum[t][r] = fmaf(acc[t][r], f, sum[t][r]);
+            } else {
+                const PagedParts other(a, c, u.first_slot + i, head, M, D);
+                u32x4 x[ND][4];
+#pragma unroll
+                for (int t = 0; t < ND; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[t][r] = other.get4(((wave * ND + t) * 4 + r) * 256 + 4 * lane);
+                const float f = top == -INFINITY ? 1.0f : pg_exp2(other.get_m(rr) - top);
+                ls = fmaf(other.get_l(rr), f, ls);
+#pragma unroll
+                for (int t = 0; t < ND; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sum[t][r] = fmaf(__uint_as_float(x[t][r / 4][r % 4]), f, sum[t][r]);
+            }
+        }
+        m = top;
+        l = ls;
+#pragma unroll
+        for (int t = 0; t < ND; ++t) acc[t] = sum[t];
+    } else if (apart) {
+        return;  // (written there)
+    }
+    if (rr >= w.rows) return;
     const float f = m == -INFINITY ? (l > 0.0f ? __builtin_nanf("") : 0.0f) : 1.0f / l * (F8 ? c.v_scale[head] : 1.0f);
-    const int first = 32 * ND * kp + 4 * half;
     uint16_t* o = a.out + (int64_t)(g.first + row) * a.ld_out + (int64_t)qh * D + first;
-    if (!whole && half == 0 && kp == 0) parts.put_ml(rr, m, l);
 #pragma unroll
     for (int t = 0; t < ND; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            if (whole)
-                *reinterpret_cast<uint2*>(o + 32 * t + 2 * r) =
-                    make_uint2(pack_bf16x2(acc[t][r] * f, acc[t][r + 1] * f), pack_bf16x2(acc[t][r + 2] * f, acc[t][r + 3] * f));
-            else
-                parts.put4(rr * D + first + 32 * t + 2 * r, acc[t][r], acc[t][r + 1], acc[t][r + 2], acc[t][r + 3]);
-        }
+        for (int r = 0; r < 16; r += 4)
+            *reinterpret_cast<uint2*>(o + 32 * t + 2 * r) =
+                make_uint2(pack_bf16x2(acc[t][r] * f, acc[t][r + 1] * f), pack_bf16x2(acc[t][r + 2] * f, acc[t][r + 3] * f));
 }
 
 }  // namespace bz
