@@ -212,6 +212,29 @@ def test_attend_a_longer_prompt():
     _attend(6, 4, 2, 128, [700, 513], n=[700, 33], ps=64)
 
 
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("HQ,HKV,D", [(16, 1, 64), (4, 2, 128), (6, 2, 128), (8, 1, 256)])
+def test_attend_prompts_of_several_parts(HQ, HKV, D, kv):
+    """Chunks of prompts whose tiles' keys are cut, so that the last workgroup of a tile joins them; a sequence
+    with nothing before it, one row, fewer positions than rows, and none among them."""
+    _attend(26, HQ, HKV, D, [1500, 333, 1, 40, 0, 901], n=[200, 333, 1, 50, 3, 70], kv=kv, ps=32, before=1, behind=1)
+
+
+@pytest.mark.parametrize("HQ,HKV,D,n", [(8, 8, 64, [1] * 2200), (144, 9, 64, [3] * 1100)])
+def test_attend_more_tiles_than_counters(HQ, HKV, D, n):
+    """So many tiles that a launch of its own joins their parts.  The sequences share pages."""
+    rng = np.random.default_rng(27)
+    B, ps = len(n), 64
+    cache = Cache(rng, 48, HKV, ps, D)
+    table = ints(rng.integers(0, 48, (B, 6)))
+    lens = rng.integers(0, 20, B)
+    lens[::100] = rng.integers(300, 385, len(lens[::100]))
+    q = bf16(rng.standard_normal((sum(n), HQ, D)))
+    starts = starts_of(n)
+    got = T.paged_attention(q, cache.k, cache.v, table, ints(lens), ints(starts))
+    check_attention(got, q, cache, table, lens, starts)
+
+
 def test_attend_many_sequences():
     rng = np.random.default_rng(9)
     _attend(7, 2, 1, 64, list(rng.integers(0, 40, 150)), n=rng.integers(0, 4, 150), behind=1)
@@ -356,6 +379,29 @@ def test_later_rows_have_no_part(value, bad, rows):
         assert np.isnan(last).all()
 
 
+@pytest.mark.parametrize("HQ,HKV,D,kv", [(4, 2, 128, "bf16"), (16, 1, 64, "e4m3"), (8, 1, 256, "bf16"), (8, 1, 256, "e4m3")])
+def test_later_rows_have_no_part_in_parts(HQ, HKV, D, kv):
+    """The same where a tile's keys are cut, the bad token in the last chunk, and further rows behind it."""
+    rows, ps = 150, 32
+    rng = np.random.default_rng(29)
+    cache = Cache(rng, 60, HKV, ps, D, kv)
+    table = cache.table(1, 40)
+    q = bf16(rng.standard_normal((rows, HQ, D)))
+    length, j = 1200, 1150  # position j is row 100
+    bits = cache.v.view(torch.uint8) if kv == "e4m3" else cache.v.view(torch.int16)
+    bits[int(table[0, j // ps]), :, j % ps, ::3] = 0x7F if kv == "e4m3" else 0x7FC0
+    scales = {"k_scale": cache.k_scale, "v_scale": cache.v_scale}
+    out = T.paged_attention(q, cache.k, cache.v, table, ints([length]), ints([0, rows]), **scales)
+    ref, weight, size = P.attention(q[:100].float().cpu().numpy(), cache.values("k"), cache.values("v"),
+                                    table.cpu().numpy(), [j], [0, 100])
+    from tests._paged import attention_bound
+
+    got = out[:100].float().cpu().double().numpy().reshape(ref.shape)
+    assert (np.abs(got - ref) <= attention_bound(ref, weight, size, D)).all()
+    later = out[100:].float().cpu().numpy().reshape(50, HQ, D)
+    assert np.isnan(later[:, :, ::3]).all() and np.isfinite(np.delete(later, np.s_[::3], 2)).all()
+
+
 def test_keys_of_minus_infinity_scores():
     """A score of -inf weighs nothing next to a finite one; a row of nothing else has no
     softmax: NaN."""
@@ -492,6 +538,43 @@ def test_replayed_steps_follow_the_lengths():
                 assert torch.equal(a, b)
             now[:] = [n + 1 for n in now]
             assert lens.tolist() == now
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+def test_replayed_chunks_follow_the_lengths(kv):
+    """A captured call over chunks of prompts, and steps of other sizes that share its workspace."""
+    HQ, HKV, D, n = 8, 2, 256, [150, 1, 70]
+    rng = np.random.default_rng(28)
+    cache = Cache(rng, 200, HKV, 32, D, kv)
+    table, starts = cache.table(3, 50), ints(starts_of(n))
+    q, one = bf16(rng.standard_normal((221, HQ, D))), bf16(rng.standard_normal((3, HQ, D)))
+    scales = {"k_scale": cache.k_scale, "v_scale": cache.v_scale}
+
+    def both(lens):
+        return (T.paged_attention(one, cache.k, cache.v, table, lens, **scales),
+                T.paged_attention(q, cache.k, cache.v, table, lens, starts, **scales),
+                T.shared_prefix_attention(one, cache.k, cache.v, table[2], ints([700]), table[:, :9], lens, **scales)
+                if not torch.cuda.is_current_stream_capturing() else None)
+
+    lens = ints([900, 5, 1200])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both(lens)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both(lens)
+    for now in ([900, 5, 1200], [1600, 700, 71], [150, 0, 1], [1599, 1, 1000]):
+        lens.copy_(ints(now))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = both(ints(now))
+        for a, b in zip(got[:2], want):
+            assert torch.equal(a, b)
+        again = both(ints(now))
+        for a, b in zip(again, want):
+            assert torch.equal(a, b)
 
 
 def test_streams_at_once():
