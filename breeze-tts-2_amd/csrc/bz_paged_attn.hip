@@ -102,7 +102,12 @@ static PagedPlan paged_plan(const bz_paged_kv* d) {
     p.inside = p.join && (notes + prefix_notes) * d->HKV <= kPagedCounters &&
                (d->groups == 0 || (M <= 32 && !d->q_starts && M % G == 0));
     p.notes = (int)notes;
-    p.slots = p.join ? paged_slots(notes + prefix_notes, target) : notes;
+    // (and no tile has more chunks than its table has room for; workgroups without a slot cost no time that
+    // could be measured, 848 for 80 with one, but their room in the workspace)
+    auto chunks = [&](int64_t positions) { return (positions + p.cut.min_chunk - 1) / p.cut.min_chunk; };
+    const int64_t room = notes * chunks((int64_t)d->table_width * d->page_size) +
+                         prefix_notes * chunks((int64_t)d->prefix_width * d->page_size);
+    p.slots = p.join ? std::min(paged_slots(notes + prefix_notes, target), room) : notes;
     p.bytes = kPagedCounters * sizeof(unsigned);
     auto take = [&](size_t n) {
         const size_t at = p.bytes;

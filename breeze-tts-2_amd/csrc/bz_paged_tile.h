@@ -11,10 +11,11 @@
 //           (PAIR) what the other wave found
 //   p v     A = the values transposed, by transposing LDS reads
 //           (ds_read_b64_tr_b16: 4 keys of one column to a lane, of e4m3 8 with
-//           ds_read_b64_tr_b8), in the order of keys in which the lanes have their probabilities: these are the B operand as they
-//           are (PAIR: also the other wave's, through LDS).  p is rounded to bf16 (2^-9 of it on
-//           average, as much as the output's own rounding; a second part would double
-//           these products); the sum l is over p before it is rounded
+//           ds_read_b64_tr_b8), in the order of keys in which the lanes have their
+//           probabilities: these are the B operand as they are (PAIR: also the other wave's,
+//           through LDS).  p is rounded to bf16 (at most 2^-8 of it, as much as the output's
+//           own rounding; a second part would double these products); the sum l is over p
+//           before it is rounded
 //   rescale only when a maximum grows by more than 2^8: until then p stays below
 //           2^8, which costs fp32 sums nothing
 //   order   in one round: the softmax of a tile beside the scores of the next one, then
@@ -26,6 +27,12 @@
 //           keys nor the transposing ones of values meet on a bank.  Every buffer is a
 //           variable of its own and the rounds take them in turn by name: that tells the
 //           compiler that reads of one do not wait for loads under way into another
+//   parts   joined by the tile's last workgroup, or with prefixes by a launch
+// Measured: a prompt of 2011 tokens, 16 / 8 heads of 128, 40.2 us, of which 15 are start, first bytes and
+// parts and 10 rounds take 2.4 each; chunks of three prompts over up to 8000 positions, 16 / 4
+// heads of 256, 344 (680 TFLOP/s; without fetches 20% less, without the products 23%); 64 rows
+// of one prefix of 6007, 16 / 8 heads of 128, 35.6 with the sequences' own keys; 24 sequences of three
+// prefixes of up to 16383, e4m3, 16 / 4 heads of 256, 41.9.
 #pragma once
 
 #include "bz_paged_attn.h"
