@@ -256,6 +256,26 @@ def test_attend_pages_that_are_not_there():
     _attend(9, 4, 2, 128, [60, 16, 40, 130], edit=edit, width=9)
 
 
+@pytest.mark.parametrize("HQ,HKV,D,kv", [(4, 2, 64, "e4m3"), (16, 2, 128, "e4m3"), (8, 1, 256, "e4m3"), (8, 1, 256, "bf16")])
+def test_attend_chunks_with_pages_that_are_not_there(HQ, HKV, D, kv):
+    """In the middle of a tile of keys, a whole tile, the first and the last."""
+    def edit(cache, table):
+        table[0, 1:7] = -1
+        table[0, 30] = cache.pages
+        table[1, 0] = -2
+        table[1, 36] = 2 ** 31 - 1
+        table[2, :] = -5
+
+    _attend(30, HQ, HKV, D, [700, 599, 300], n=[140, 20, 40], kv=kv, edit=edit, width=44)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("layout", ["nhd", "pair"])
+def test_attend_chunks_of_other_layouts(kv, layout):
+    _attend(31, 8, 2, 128, [500, 260], n=[100, 260], kv=kv, layout=layout)
+    _attend(32, 8, 2, 64, [500, 260], n=[100, 20], kv=kv, layout=layout, ps=64)
+
+
 @pytest.mark.parametrize("spread,scale", [(12.0, None), (0.0, None), (1.0, 30.0), (3.0, 1e-4)])
 def test_attend_scales(spread, scale):
     """One key that takes all, keys that weigh alike, and other scales."""
@@ -637,6 +657,22 @@ def test_inputs_of_other_strides():
     cs[0, :, 1:D + 1], cs[1, :, 1:D + 1] = cos, sin
     got = T.paged_rope_cache(odd[:, 5:], cs[0, :, 1:D + 1], cs[1, :, 1:D + 1], cache.k, cache.v, table, lens, HQ)
     assert torch.equal(got, ref) and torch.equal(cache.k, keys)
+
+
+def test_chunks_between_other_columns():
+    """Queries and results that are columns of wider tensors; what lies beside them stays."""
+    rng = np.random.default_rng(33)
+    HQ, HKV, D, n = 8, 2, 128, [150, 3]
+    cache = Cache(rng, 60, HKV, 32, D)
+    table, lens, starts = cache.table(2, 30), [900, 77], starts_of(n)
+    wide = bf16(rng.standard_normal((153, 3 * HQ, D)))
+    big = bf16(rng.standard_normal((155, HQ * D + 64)))
+    old = big.clone()
+    q, out = wide[:, HQ:2 * HQ], big[1:154, 8:8 + HQ * D]
+    assert T.paged_attention(q, cache.k, cache.v, table, ints(lens), ints(starts), out=out) is out
+    check_attention(out, q, cache, table, lens, starts)
+    out.copy_(old[1:154, 8:8 + HQ * D])
+    assert torch.equal(big, old)
 
 
 def test_nothing_to_do():
