@@ -182,7 +182,7 @@ extern "C" int bz_paged_attn(const bz_paged_kv* kv, const void* q, int64_t ld_q,
     if (!aligned_to(q, 16) || !aligned_to(out, 16) || ld_q % 8 || ld_out % 8 || !aligned_to(workspace, 16))
         return BZ_ERR_ALIGNMENT;
     const PagedPlan p = paged_plan(kv);
-    if (p.slots * c.HKV > 0x7FFFFFFF) return BZ_ERR_UNSUPPORTED;
+    if (p.slots * c.HKV > 0x7FFFFF) return BZ_ERR_UNSUPPORTED;  // (a grid has less than 2^32 threads)
     if (!workspace || workspace_bytes < p.bytes) return BZ_ERR_INVALID_ARG;
     PagedAttn a = {};
     a.q = static_cast<const uint16_t*>(q);

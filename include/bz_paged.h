@@ -17,7 +17,7 @@
  * there: nothing is written to its positions and no row attends them.
  *
  * Rows: T rows of qkv, q and out.  Sequence b has the rows q_starts[b] ..
- * q_starts[b + 1] - 1 (non-decreasing, the ends clamped to [0, T]), one row b
+ * q_starts[b + 1] - 1 (non-decreasing, else the rows hold anything; the ends clamped to [0, T]), one row b
  * each when q_starts is NULL (then T = B).  They are its newest positions:
  * with n rows, row i of the sequence is position kv_lens[b] - n + i, so
  * kv_lens counts the new rows.  A row at a negative position is written nowhere
