@@ -282,9 +282,10 @@ def paged_rope_cache(qkv, cos, sin, k_pages, v_pages, block_table, kv_lens, HQ: 
     q = qkv.new_empty((T, HQ, D)) if q_out is None else _result("q_out", q_out, (T, HQ, D), index, qkv)
     if T == 0 or sizes[2] == 0:
         return q
-    _call(index, torch._C._cuda_getCurrentRawStream(index), _lib.lib().bz_paged_rope_cache, _lib.paged_kv(*sizes, 0, 0, *refs, 0, 0, 0, 0), qkv.data_ptr(),
-          ld if T > 1 else width, None if qn is None else qn.data_ptr(), None if kn is None else kn.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), cs,
-          ld_cs if shape[0] > 1 else D, shape[0], at, q.data_ptr(), q.stride()[0] if T > 1 else HQ * D)
+    _call(index, torch._C._cuda_getCurrentRawStream(index), _lib.lib().bz_paged_rope_cache,
+          _lib.paged_kv(*sizes, 0, 0, *refs, 0, 0, 0, 0), qkv.data_ptr(), ld if T > 1 else width,
+          None if qn is None else qn.data_ptr(), None if kn is None else kn.data_ptr(), eps, cos.data_ptr(),
+          sin.data_ptr(), cs, ld_cs if shape[0] > 1 else D, shape[0], at, q.data_ptr(), q.stride()[0] if T > 1 else HQ * D)
     return q
 
 

@@ -81,7 +81,8 @@ __device__ __forceinline__ int stream_col(int t, int i) {
 
 // RT row tiles of 16.
 template <int D, bool F8, int RT>
-__global__ void __launch_bounds__(64 * kStreamWaves, D * RT < 256 || F8 || D == 128 ? 2 : 1) paged_attn_bf16_stream(PagedKv c, PagedAttn a) {
+__global__ void __launch_bounds__(64 * kStreamWaves, D * RT < 256 || F8 || D == 128 ? 2 : 1)
+    paged_attn_bf16_stream(PagedKv c, PagedAttn a) {
     using S = StreamStep<D, F8>;
     constexpr int M = 16 * RT, T = D / 32, NT = D / 16;
     constexpr int kRow = D + 4;

@@ -160,7 +160,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
     const int tiles = (max(w.end - w.begin, 0) + kTileKeys - 1) / kTileKeys;
     // (64 banks: the rows of ROW bytes begin on 256 / ROW places of them.  No conflicts; with 7 and 2 for all D
     // 40% of the LDS cycles were conflicts)
-    auto k_swap = [](int key) { return F8 ? (ROW == 256 ? key & 15 : ROW == 128 ? key >> 1 & 7 : key >> 2 & 3) : key & (D == 64 ? 7 : 15); };
+    auto k_swap = [](int key) {
+        if (!F8) return key & (D == 64 ? 7 : 15);
+        return ROW == 256 ? key & 15 : ROW == 128 ? key >> 1 & 7 : key >> 2 & 3;
+    };
     auto v_swap = [](int key) {
         if (!F8) return (D == 64 ? 2 : 4) * (key & 3);
         const int bit3 = key >> 3 & 1;
@@ -434,6 +437,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
             pass(tile + 1, k0, v1, v0);
         }
         if (tile < tiles) pass(tile, k1, v0, v1);
+        __builtin_amdgcn_s_waitcnt(0x0F70);
         if constexpr (PAIR) {
             __syncthreads();
             __syncthreads();
@@ -449,6 +453,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
         round(tile + 1, k0, v1, v0, top1, top0);
     }
     if (tile < tiles) round(tile, k1, v0, v1, top0, top1);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // (no load into LDS, empty as the last ones are, outlives the workgroup)
     if (u.split == 0 && tid == 0) note_tile(c, a, w, M, slot, head);
 
     l = other_half_sum(l);
@@ -471,7 +476,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
         for (int t = 0; t < ND; ++t)
 #pragma unroll
             for (int r = 0; r < 16; r += 4)
-                parts.put4(inside ? ((wave * ND + t) * 4 + r / 4) * 256 + 4 * lane : rr * D + first + 32 * t + 2 * r, acc[t][r], acc[t][r + 1], acc[t][r + 2], acc[t][r + 3]);
+                parts.put4(inside ? ((wave * ND + t) * 4 + r / 4) * 256 + 4 * lane : rr * D + first + 32 * t + 2 * r,
+                           acc[t][r], acc[t][r + 1], acc[t][r + 2], acc[t][r + 3]);
     };
     if (!whole && !inside) {
         store_part();
