@@ -27,12 +27,14 @@ q_starts          int32 [B + 1]: sequence b has the rows q_starts[b] .. q_starts
 
 Lengths, tables and starts are read on the device: no call synchronizes, and a
 captured graph follows them.  Calls may run on several streams at once, and graphs on
-any: each stream and each capture has a workspace of its own.
+any: each stream and each capture has a workspace of its own.  They may come from
+several host threads: those on one stream go one after the other, each as a whole.
 """
 
 from __future__ import annotations
 
 import functools
+import threading
 from typing import Optional
 
 import torch
@@ -46,6 +48,11 @@ __all__ = ["paged_rope_cache", "paged_attention", "shared_prefix_attention"]
 # under way: the kernels leave its counters at zero.
 _WS: dict[tuple, torch.Tensor] = {}
 _WS_RETIRED: list = []
+
+# One lock for each device and stream.  A call can be two launches, the second of which reads what
+# the first left in the stream's workspace, and the library is called without the GIL: another
+# thread's first launch between the two would overwrite it.
+_LOCKS: dict[tuple, object] = {}
 
 _KV = {torch.bfloat16: DT_BF16, torch.float8_e4m3fn: KV_E4M3}
 _CS = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
@@ -310,9 +317,14 @@ def _attention(q, k_pages, v_pages, block_table, kv_lens, q_starts, prefix, scal
     sizes += psizes
     n = _workspace_bytes(sizes)
     stream = torch._C._cuda_getCurrentRawStream(index)
-    ws = _lib.stream_workspace(_WS, (index,), n, q.device, stream, _WS_RETIRED)
-    _call(index, stream, _lib.lib().bz_paged_attn, _lib.paged_kv(*sizes, *refs, *prefs), q.data_ptr(),
-          q.stride()[0] if T > 1 else width, D ** -0.5 if scale is None else scale, ws.data_ptr(), n, out.data_ptr(), ld)
+    kv = _lib.paged_kv(*sizes, *refs, *prefs)
+    lock = _LOCKS.get((index, stream))
+    if lock is None:
+        lock = _LOCKS.setdefault((index, stream), threading.RLock())
+    with lock:
+        ws = _lib.stream_workspace(_WS, (index,), n, q.device, stream, _WS_RETIRED)
+        _call(index, stream, _lib.lib().bz_paged_attn, kv, q.data_ptr(), q.stride()[0] if T > 1 else width,
+              D ** -0.5 if scale is None else scale, ws.data_ptr(), n, out.data_ptr(), ld)
     return out
 
 

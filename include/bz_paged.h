@@ -97,7 +97,9 @@ int bz_paged_rope_cache(const bz_paged_kv* kv, const void* qkv, int64_t ld_qkv,
  * values that a row does not attend have no part in it, whatever they hold.
  * scale > 0.  workspace: bz_paged_attn_workspace bytes, 16-byte aligned, zeroed
  * once before its first use (the kernels leave the counters at its front at zero
- * again, whatever the sizes of the calls); calls that share one must not overlap. */
+ * again, whatever the sizes of the calls); calls that share one must not overlap.
+ * A call can be two launches that hand over through the workspace: host threads that
+ * share one, on the same stream too, make their calls one after the other. */
 int bz_paged_attn(const bz_paged_kv* kv, const void* q, int64_t ld_q,
                   float scale, void* workspace, size_t workspace_bytes,
                   void* out, int64_t ld_out, void* stream);

@@ -8,6 +8,8 @@ below 2^-16 of its terms' magnitude."""
 
 from __future__ import annotations
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -686,3 +688,28 @@ def test_nothing_to_do():
     q = T.paged_rope_cache(torch.empty(0, 8 * 64, device=DEV, dtype=BF16), cos, sin, cache.k, cache.v, ints([[0]]),
                            ints([3]), 4, ints([0, 0]))
     assert q.shape == (0, 4, 64)
+
+
+def test_threads_on_one_stream():
+    """Calls of two launches each from several host threads on one stream: what each gives when it is alone."""
+    rng = np.random.default_rng(34)
+    HQ, HKV, D, B = 8, 2, 128, 40
+    cache = Cache(rng, 250, HKV, 32, D)
+    table, ptable, lens = cache.table(B, 4), cache.table(1, 40), ints(rng.integers(1, 128, B))
+    q = [bf16(rng.standard_normal((B, HQ, D))) for _ in range(3)]
+    plens = [ints([n]) for n in (1280, 900, 333)]
+
+    def call(i):
+        return T.shared_prefix_attention(q[i], cache.k, cache.v, ptable, plens[i], table, lens)
+
+    want = [call(i) for i in range(3)]
+    torch.cuda.synchronize()
+    got = [[] for _ in range(3)]
+    threads = [threading.Thread(target=lambda i=i: got[i].extend(call(i) for _ in range(40))) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(3):
+        assert len(got[i]) == 40 and all(torch.equal(g, want[i]) for g in got[i])

@@ -7,6 +7,8 @@ from __future__ import annotations
 import ctypes
 import shutil
 import subprocess
+import threading
+import time
 from pathlib import Path
 
 import numpy as np
@@ -317,3 +319,55 @@ def test_c_refuses_append(kw, status):
 def test_workspace_of_refused_sizes():
     assert _lib.lib().bz_paged_attn_workspace(_desc(D=96)) == 0
     assert _lib.lib().bz_paged_attn_workspace(None) == 0
+
+
+def _served_on(monkeypatch, call):
+    """The wrapper's way to the library on CPU tensors: `call` stands for the launches, the thread's name for its
+    stream; a workspace for each stream, as ever."""
+    monkeypatch.setattr(paged, "_gpu", lambda *a: None)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: int(threading.current_thread().name))
+    monkeypatch.setattr(_lib, "capture_of", lambda stream: None)
+    monkeypatch.setattr(paged, "_call", lambda index, stream, f, *args: call(stream, args))
+    monkeypatch.setattr(paged, "_WS", {})
+
+
+def _in_threads(streams, f):
+    errors = []
+
+    def work():
+        try:
+            f()
+        except BaseException as e:  # noqa: BLE001 - handed to the test
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, name=str(s)) for s in streams]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    if errors:
+        raise errors[0]
+
+
+def test_threads_of_one_stream_call_one_after_the_other(monkeypatch):
+    """A call can be two launches, the second of which reads what the first left in the stream's workspace: no
+    other call may come between them."""
+    inside, most = [], []
+
+    def call(stream, args):
+        inside.append(args[4])  # the workspace
+        most.append(max(inside.count(w) for w in inside))
+        time.sleep(0.005)
+        inside.remove(args[4])
+
+    _served_on(monkeypatch, call)
+    a = _args(prefix_table=torch.zeros(1, dtype=torch.int32), prefix_lens=torch.zeros(1, dtype=torch.int32))
+    _in_threads([1, 1, 1, 1], lambda: [paged.shared_prefix_attention(**a) for _ in range(5)])
+    assert len(most) == 20 and max(most) == 1
+
+
+def test_threads_of_two_streams_do_not_wait_for_each_other(monkeypatch):
+    together = threading.Barrier(2, timeout=20)
+    _served_on(monkeypatch, lambda stream, args: together.wait())
+    a = _args()
+    _in_threads([1, 2], lambda: paged.paged_attention(**a))
