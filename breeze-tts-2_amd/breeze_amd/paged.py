@@ -12,8 +12,8 @@ pages of one pool instead of a static [B, HKV, S, D] cache each:
 Common arguments:
 
 k_pages, v_pages  [pages, HKV, page_size, D] bf16, or float8_e4m3fn with k_scale /
-                  v_scale (fp32 [HKV]: a code stands for code * scale).  Any strides with
-                  contiguous D, so a [pages, page_size, HKV, D] pool is passed as its
+                  v_scale (fp32 [HKV]: a code stands for code * scale, whatever the scale's
+                  sign, 0 included).  Any strides with contiguous D, so a [pages, page_size, HKV, D] pool is passed as its
                   transpose(1, 2).  page_size a power of two, 16 .. 4096.
 block_table       int32 [B, W]: position j of sequence b lies in page
                   block_table[b, j // page_size].  Entries past a sequence's length are not
@@ -237,7 +237,8 @@ def paged_rope_cache(qkv, cos, sin, k_pages, v_pages, block_table, kv_lens, HQ: 
                      q_out=None) -> torch.Tensor:
     """Per-head q/k RMSNorm and rotate-half RoPE of the rows' qkv (bf16
     [T, (HQ + 2 HKV) D], q heads, k heads, v heads); their keys and values into
-    the pages (e4m3: rounded once, saturated); q as bf16 [T, HQ, D] (returned).
+    the pages (e4m3: value / scale, rounded once, saturated; by a scale of 0 that is
+    NaN for a value of 0); q as bf16 [T, HQ, D] (returned).
     What qkv_rope_cache does for a static cache, for any number of rows of
     each sequence.
 

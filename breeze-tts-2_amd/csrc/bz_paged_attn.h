@@ -102,6 +102,29 @@ __device__ __forceinline__ void note_tile(const PagedKv& c, const PagedAttn& a, 
     __hip_atomic_store(to, (uint64_t)(unsigned)w.u.chunk << 32 | (unsigned)slot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// The factor of a head's scores, in exponents of 2, where they come from matrix products.  A masked
+// score is -inf before it is multiplied and the maximum is taken of the products, so the factor is positive:
+// an e4m3 head's scale gives its sign to the queries (exact), and a scale of 0, or a product that
+// underflows, becomes the smallest number there is (2^-149: scores below 2^128 stay below 2^-21, and
+// e^0 within that).  A scale that is NaN makes the queries NaN, so that masked scores stay -inf.
+struct ScoreFactor {
+    float f;
+    uint32_t keep, flip;  // of two queries' bits
+    __device__ __forceinline__ bool plain() const { return keep == ~0u && flip == 0u; }
+    __device__ __forceinline__ u32x4 query(u32x4 q) const { return (q & keep) ^ flip; }
+};
+template <bool F8>
+__device__ __forceinline__ ScoreFactor score_factor(const PagedKv& c, const PagedAttn& a, int head) {
+    ScoreFactor s = {a.scale * kPagedLog2e, ~0u, 0u};
+    if constexpr (F8) {
+        const float ks = c.k_scale[head], f = s.f * fabsf(ks);
+        s.f = f > 0.0f ? f : 0x1p-149f;
+        if (ks < 0.0f) s.flip = 0x80008000u;
+        if (ks != ks) s.keep = 0u, s.flip = 0x7FC07FC0u;
+    }
+    return s;
+}
+
 // One 16-position piece of a segment's keys, none of whose rows is read beyond `n`.
 struct PagedPiece {
     __amdgpu_buffer_rsrc_t k, v;

@@ -117,7 +117,13 @@ __global__ void __launch_bounds__(64 * kStreamWaves, D * RT < 256 || F8 || D == 
     const int32_t* table = own ? c.table + (int64_t)g.seq * c.ld_table : c.prefix_table + (int64_t)(g.seq - c.B) * c.ld_prefix;
     const char* kh = c.k + head * c.k_head;
     const char* vh = c.v + head * c.v_head;
-    const float sc = a.scale * kPagedLog2e * (F8 ? c.k_scale[head] : 1.0f);
+    const ScoreFactor factor = score_factor<F8>(c, a, head);
+    const float sc = factor.f;
+    if (F8 && !factor.plain())
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int t = 0; t < T; ++t) q[rt][t] = factor.query(q[rt][t]);
 
     pg_f32x4 acc[RT][NT];
     float m[RT], l[RT];

@@ -143,7 +143,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attn_bf16_tile(PagedKv c,
                                  : c.prefix_table + (int64_t)(g.seq - c.B) * c.ld_prefix;
     const char* kh = c.k + head * c.k_head;
     const char* vh = c.v + head * c.v_head;
-    const float sc = a.scale * kPagedLog2e * (F8 ? c.k_scale[head] : 1.0f);
+    const ScoreFactor factor = score_factor<F8>(c, a, head);
+    const float sc = factor.f;
+    if (F8 && !factor.plain())
+#pragma unroll
+        for (int t = 0; t < T; ++t) q[t] = factor.query(q[t]);
 
     pg_f32x16 acc[ND];
 #pragma unroll

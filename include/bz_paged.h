@@ -57,7 +57,7 @@ typedef struct bz_paged_kv {
     void* v_pages;
     int64_t k_page, k_head, k_pos; /* elements from a page / kv head / position to the next */
     int64_t v_page, v_head, v_pos;
-    const float* k_scale; /* [HKV], BZ_KV_E4M3 only: a code stands for code * scale */
+    const float* k_scale; /* [HKV], BZ_KV_E4M3 only: a code stands for code * scale (of any sign, or 0) */
     const float* v_scale;
     const int32_t* block_table; /* [B][ld_table] */
     int64_t ld_table;
@@ -74,7 +74,7 @@ typedef struct bz_paged_kv {
 
 /* New tokens into the cache: per-head q/k RMSNorm (q_norm / k_norm bf16 [D],
  * both or neither) and rotate-half RoPE in fp32, k and v of every row into its
- * position's page (bf16, or e4m3 of value / scale, saturated at 448), the
+ * position's page (bf16, or e4m3 of value / scale, saturated at 448, NaN for 0 / 0), the
  * rotated q to q_out (bf16 [T][ld_q], head h at columns h D ..; must not overlap
  * qkv).  qkv bf16 [T][ld_qkv], columns [q heads | k heads | v heads] x D.
  * cos / sin [cs_rows][ld_cs], bf16 or fp32: row t uses row positions[t] (int64

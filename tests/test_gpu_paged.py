@@ -713,3 +713,38 @@ def test_threads_on_one_stream():
     torch.cuda.synchronize()
     for i in range(3):
         assert len(got[i]) == 40 and all(torch.equal(g, want[i]) for g in got[i])
+
+
+def _scales(cache, table):
+    """Heads whose codes stand for their negatives, for nothing, and for next to nothing."""
+    for scale in (cache.k_scale, cache.v_scale):
+        scale[0] = 0.0
+        scale[1] *= -1
+        scale[2] = 1e-42
+    cache.v_scale.copy_(cache.v_scale.roll(1))
+
+
+@pytest.mark.parametrize("scale", [None, 3.0])
+@pytest.mark.parametrize("HQ,HKV,D,n", [(16, 4, 128, None), (8, 4, 64, [5, 9, 3, 2, 7]), (4, 4, 128, [150, 9, 60, 40, 3]),
+                                        (16, 4, 64, [80, 9, 40, 5, 0]), (8, 4, 256, [70, 30, 5, 40, 1]),
+                                        (16, 4, 256, None)])
+def test_attend_any_scale_of_a_head(HQ, HKV, D, n, scale):
+    """A head's scale may be negative, zero or tiny: its scores are what codes times scale give."""
+    lens = [40, 3, 700, 900, 0]
+    _attend(35, HQ, HKV, D, lens, n=n, kv="e4m3", ps=32, edit=_scales, scale=scale)
+    _attend(36, HQ, HKV, D, lens, n=n, kv="e4m3", ps=32, edit=_scales, scale=scale, prefix=([300, 33], [0, 3, 4]))
+
+
+@pytest.mark.parametrize("D,rows", [(128, 3), (64, 100), (256, 100)])
+def test_attend_a_scale_that_is_no_number(D, rows):
+    """What such a head's rows attend is NaN, a row that attends nothing zero, the other head as without it."""
+    cache = Cache(np.random.default_rng(37), 10, 2, 32, D, "e4m3")
+    table, q = cache.table(2, 4), bf16(np.random.default_rng(38).standard_normal((2 * rows, 4, D)))
+    lens, starts = ints([rows - 2, 0]), ints([0, rows, 2 * rows])
+    f = lambda: T.paged_attention(q, cache.k, cache.v, table, lens, starts, k_scale=cache.k_scale,  # noqa: E731
+                                  v_scale=cache.v_scale).view(2 * rows, 2, 2 * D)
+    want = f()
+    cache.k_scale[0] = float("nan")
+    got = f()
+    assert torch.isnan(got[2:rows, 0]).all() and not got[:2].any() and not got[rows:].any()
+    assert torch.equal(got[:, 1], want[:, 1])
