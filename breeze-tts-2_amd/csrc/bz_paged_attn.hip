@@ -122,6 +122,12 @@ static PagedPlan paged_plan(const bz_paged_kv* d) {
     return p;
 }
 
+// Whether the launches' grids can be: one of less than 2^32 threads in each dimension, 256 or 512
+// to a workgroup.
+static bool paged_plan_fits(const bz_paged_kv* d, const PagedPlan& p) {
+    return p.slots * d->HKV <= 0x7FFFFF && (!p.join || p.inside || d->T < kPagedMaxGrid);
+}
+
 template <int D, bool F8>
 static void launch_tiles(const PagedKv& c, const PagedAttn& a, int64_t slots, hipStream_t st) {
     const dim3 grid((unsigned)(slots * c.HKV));
@@ -168,7 +174,9 @@ static void launch_attn(const PagedKv& c, PagedAttn a, const PagedPlan& p, char*
 using namespace bz;
 
 extern "C" size_t bz_paged_attn_workspace(const bz_paged_kv* kv) {
-    return paged_check_sizes(kv) == BZ_OK ? paged_plan(kv).bytes : 0;
+    if (paged_check_sizes(kv) != BZ_OK) return 0;
+    const PagedPlan p = paged_plan(kv);
+    return paged_plan_fits(kv, p) ? p.bytes : 0;
 }
 
 extern "C" int bz_paged_attn(const bz_paged_kv* kv, const void* q, int64_t ld_q, float scale, void* workspace,
@@ -182,7 +190,7 @@ extern "C" int bz_paged_attn(const bz_paged_kv* kv, const void* q, int64_t ld_q,
     if (!aligned_to(q, 16) || !aligned_to(out, 16) || ld_q % 8 || ld_out % 8 || !aligned_to(workspace, 16))
         return BZ_ERR_ALIGNMENT;
     const PagedPlan p = paged_plan(kv);
-    if (p.slots * c.HKV > 0x7FFFFF) return BZ_ERR_UNSUPPORTED;  // (a grid has less than 2^32 threads)
+    if (!paged_plan_fits(kv, p)) return BZ_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < p.bytes) return BZ_ERR_INVALID_ARG;
     PagedAttn a = {};
     a.q = static_cast<const uint16_t*>(q);

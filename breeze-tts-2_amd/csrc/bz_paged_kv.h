@@ -9,6 +9,7 @@
 namespace bz {
 
 constexpr int kPagedMaxG = 16;  // query heads of one key/value head
+constexpr int kPagedMaxGrid = 1 << 24;  // workgroups of 256 threads: less than this
 
 // What a kernel needs of the cache; strides in bytes.
 struct PagedKv {

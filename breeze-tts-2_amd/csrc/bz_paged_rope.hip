@@ -177,6 +177,7 @@ extern "C" int bz_paged_rope_cache(const bz_paged_kv* kv, const void* qkv, int64
     PagedKv c = {};
     const int rc = paged_setup(kv, c);
     if (rc != BZ_OK) return rc;
+    if (kv->T >= kPagedMaxGrid) return BZ_ERR_UNSUPPORTED;
     if (!qkv || !cos || !sin || !q_out || (q_norm == nullptr) != (k_norm == nullptr)) return BZ_ERR_INVALID_ARG;
     if (cs_dtype != BZ_DT_BF16 && cs_dtype != BZ_DT_F32) return BZ_ERR_INVALID_ARG;
     const int D = kv->D;

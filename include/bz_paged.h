@@ -44,7 +44,7 @@ extern "C" {
 
 typedef struct bz_paged_kv {
     int32_t abi_version; /* BZ_ABI_VERSION */
-    int32_t T;           /* rows */
+    int32_t T;           /* rows; append, and attention that takes two launches, refuse 2^24 or more */
     int32_t B;           /* sequences */
     int32_t HQ, HKV, D;  /* HQ % HKV == 0, HQ / HKV <= 16; D 64, 128 or 256 */
     int32_t kv_dtype;

@@ -371,3 +371,36 @@ def test_threads_of_two_streams_do_not_wait_for_each_other(monkeypatch):
     _served_on(monkeypatch, lambda stream, args: together.wait())
     a = _args()
     _in_threads([1, 2], lambda: paged.paged_attention(**a))
+
+
+# A grid's dimension has less than 2^32 threads, 256 or 512 to a workgroup.
+TOO_MANY = [
+    # a workgroup for each row of the joining launch
+    {"T": 1 << 24, "q_starts": FAKE},
+    {"T": (1 << 24) + 5, "HQ": 2, "HKV": 1, "q_starts": FAKE, "groups": 1, "prefix_width": 1, "ld_prefix": 1,
+     "prefix_table": FAKE, "prefix_lens": FAKE, "table_width": 1},
+    # a workgroup for each tile and key/value head
+    {"T": 1 << 23, "B": 1 << 23, "table_width": 1, "ld_table": 1, "HQ": 4, "HKV": 4},
+]
+
+
+@pytest.mark.parametrize("kw", TOO_MANY)
+def test_c_refuses_more_workgroups_than_a_grid_has(kw):
+    d, L = _desc(**({"table_width": 64, "ld_table": 64} | kw)), _lib.lib()
+    width = d.HQ * d.D
+    assert L.bz_paged_attn(d, FAKE, width, 0.1, None, 0, FAKE, width, None) == _lib.ERR_UNSUPPORTED
+    assert L.bz_paged_attn_workspace(d) == 0
+
+
+def test_workspace_of_as_many_rows_as_there_can_be():
+    L = _lib.lib()
+    assert L.bz_paged_attn_workspace(_desc(T=(1 << 24) - 1, q_starts=FAKE, table_width=64, ld_table=64)) > 0
+    # positions for one chunk: no parts to be joined
+    assert L.bz_paged_attn_workspace(_desc(T=1 << 24, B=1 << 20, HQ=1, HKV=1, q_starts=FAKE, table_width=8)) > 0
+
+
+@pytest.mark.parametrize("T", [1 << 24, (1 << 24) + 1])
+def test_c_refuses_append_of_more_rows_than_a_grid_has(T):
+    d = _desc(T=T, q_starts=FAKE)
+    assert _lib.lib().bz_paged_rope_cache(d, FAKE, 512, None, None, 1e-6, FAKE, FAKE, _lib.DT_F32, 64, 5, None, FAKE, 256,
+                                          None) == _lib.ERR_UNSUPPORTED
