@@ -16,6 +16,7 @@ import torch
 
 from oracle import bz_paged_oracle as P
 from tests._paged import BF16, Cache, bf16, check_attention, ints, starts_of
+from tests._paged_parts import KEYS, check_parts, midway
 
 from breeze_amd import paged as T
 
@@ -748,3 +749,41 @@ def test_attend_a_scale_that_is_no_number(D, rows):
     got = f()
     assert torch.isnan(got[2:rows, 0]).all() and not got[:2].any() and not got[rows:].any()
     assert torch.equal(got[:, 1], want[:, 1])
+
+
+FEW = [(16, 8, 128, None), (16, 1, 128, None), (6, 2, 64, None), (16, 4, 256, None), (8, 2, 128, [5, 5, 5, 5]),
+       (4, 2, 64, [9, 2, 12, 1]), (8, 2, 256, [4, 4, 3, 4])]
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("HQ,HKV,D,n", FEW)
+def test_few_rows_keep_their_probabilities(HQ, HKV, D, n, kv):
+    """Two bf16 parts of each, in chunks that are joined and with a prefix too."""
+    rng = np.random.default_rng(39)
+    cache, lens = Cache(rng, 120, HKV, 32, D, kv), [290, 40, 17, 500]
+    table, ptable, plens = cache.table(4, 16), cache.table(1, 10), [277]
+    starts = None if n is None else starts_of(n)
+    q = bf16(rng.standard_normal((4 if n is None else sum(n), HQ, D)) * 1.5)
+    args = (table, ints(lens), None if n is None else ints(starts))
+    scales = {"k_scale": cache.k_scale, "v_scale": cache.v_scale}
+    check_parts(T.paged_attention(q, cache.k, cache.v, *args, **scales), q, cache, table, lens, starts)
+    if sum(n or [1] * 4) * HQ // HKV <= (16 if D == 256 else 32):  # (all rows are the prefix's)
+        got = T.shared_prefix_attention(q, cache.k, cache.v, ptable, ints(plens), *args, **scales)
+        check_parts(got, q, cache, table, lens, starts, None, (ptable.cpu().numpy(), plens, None))
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("HQ,HKV,D,rows", [(4, 2, 64, 1), (16, 1, 128, 2), (16, 4, 256, 1), (4, 2, 128, 9)])
+def test_few_rows_do_not_round_their_probabilities_to_bf16(HQ, HKV, D, rows, kv):
+    """Probabilities midway between two bf16 numbers; the earlier rows of several attend fewer of them."""
+    cache = Cache(np.random.default_rng(40), 8, HKV, 16, D, kv)
+    table = cache.table(1, 7)
+    for scale in (cache.k_scale, cache.v_scale):
+        if scale is not None:
+            scale.fill_(1.0)
+    scale = midway(cache, table)
+    q = torch.zeros(rows, HQ, D, device=DEV, dtype=BF16)
+    q[:, :, 0] = 1.0
+    got = T.paged_attention(q, cache.k, cache.v, table, ints([KEYS]), ints([0, rows]), scale=scale, k_scale=cache.k_scale,
+                            v_scale=cache.v_scale)
+    check_parts(got, q, cache, table, [KEYS], [0, rows], scale)

@@ -17,6 +17,7 @@ import torch
 
 from oracle import bz_paged_oracle as P
 from tests._paged import BF16, E4M3, Cache, ints, starts_of
+from tests._paged_parts import KEYS, PROB, VALUE, half_step, parts_bound
 
 from breeze_amd import _lib, paged
 
@@ -404,3 +405,16 @@ def test_c_refuses_append_of_more_rows_than_a_grid_has(T):
     d = _desc(T=T, q_starts=FAKE)
     assert _lib.lib().bz_paged_rope_cache(d, FAKE, 512, None, None, 1e-6, FAKE, FAKE, _lib.DT_F32, 64, 5, None, FAKE, 256,
                                           None) == _lib.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("one_part", [0.5, 0.50390625])
+def test_bound_of_two_parts_tells_them_from_one(one_part):
+    """One bf16 part of the probabilities of tests/_paged_parts.midway, rounded down (or cut) or up."""
+    ref = np.full((1, 1, 64), VALUE)
+    total = 1 + (KEYS - 1) * PROB
+    bound = parts_bound(ref, ref, np.full((1, 1), -np.log(PROB)), 64, KEYS)
+    wrong = torch.tensor(VALUE * (1 + (KEYS - 1) * one_part) / total).to(BF16).double().item()
+    assert (abs(wrong - ref) > bound).all()
+    first, rest = 0.5, PROB - 0.5  # (both bf16 numbers)
+    assert (abs(VALUE * (1 + (KEYS - 1) * (first + rest)) / total - ref) <= bound).all()
+    assert half_step(1.75) == half_step(1.0) == 2.0 ** -8 and half_step(2.0) == 2.0 ** -7 and half_step(0.9) == 2.0 ** -9
