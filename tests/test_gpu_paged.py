@@ -787,3 +787,34 @@ def test_few_rows_do_not_round_their_probabilities_to_bf16(HQ, HKV, D, rows, kv)
     got = T.paged_attention(q, cache.k, cache.v, table, ints([KEYS]), ints([0, rows]), scale=scale, k_scale=cache.k_scale,
                             v_scale=cache.v_scale)
     check_parts(got, q, cache, table, [KEYS], [0, rows], scale)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("HQ,HKV,D", [(8, 2, 256), (4, 4, 256), (8, 2, 128), (16, 1, 64), (6, 2, 64)])
+def test_prefix_prompts(HQ, HKV, D, kv):
+    """Prompts and chunks behind prefixes, their own keys cut too: tiles of 64 and 128 rows with a launch that joins
+    their parts; sequences of no prefix, of no rows, of no own positions for some rows."""
+    _attend(41, HQ, HKV, D, [150, 1, 0, 700, 5, 40], n=[150, 1, 0, 70, 5, 44], kv=kv, ps=32,
+            prefix=([600, 33], [0, 4, 5]), before=1, behind=2)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("HQ,HKV,D", [(16, 4, 256), (8, 2, 128), (4, 4, 64)])
+def test_prefix_drafted_tokens_of_many(HQ, HKV, D, kv):
+    """A few rows for each of many sequences: a prefix's tiles hold rows of several sequences."""
+    rng = np.random.default_rng(42)
+    _attend(42, HQ, HKV, D, list(rng.integers(2, 300, 20)), n=rng.integers(0, 6, 20), kv=kv, ps=32,
+            prefix=([900, 100, 257], [0, 9, 9, 18]))
+
+
+def test_append_by_a_scale_of_zero():
+    """value / 0: the largest code of either sign, NaN for a value of 0."""
+    cache = Cache(np.random.default_rng(43), 2, 1, 16, 64, "e4m3")
+    cache.v_scale.zero_()
+    x = torch.zeros(1, 3 * 64, device=DEV, dtype=BF16)
+    x[0, 128:130] = torch.tensor([1e-3, -2.0])
+    one, zero = torch.ones(1, 64, device=DEV), torch.zeros(1, 64, device=DEV)
+    T.paged_rope_cache(x, one, zero, cache.k, cache.v, ints([[1]]), ints([1]), 1, k_scale=cache.k_scale,
+                       v_scale=cache.v_scale)
+    v = cache.v.float()[1, 0, 0]
+    assert v[:2].tolist() == [448.0, -448.0] and torch.isnan(v[2:]).all()
