@@ -7,14 +7,15 @@ pages of one pool instead of a static [B, HKV, S, D] cache each:
                              values into the pages, rotated queries out
 ``paged_attention``          attention of each sequence's newest rows over its pages
 ``shared_prefix_attention``  the same where sequences begin with a shared prompt (a
-                             voice), whose pages are stored and read once
+                             voice), whose pages are stored once and read once for many rows
 
 Common arguments:
 
 k_pages, v_pages  [pages, HKV, page_size, D] bf16, or float8_e4m3fn with k_scale /
                   v_scale (fp32 [HKV]: a code stands for code * scale, whatever the scale's
-                  sign, 0 included).  Any strides with contiguous D, so a [pages, page_size, HKV, D] pool is passed as its
-                  transpose(1, 2).  page_size a power of two, 16 .. 4096.
+                  sign, 0 included).  Any strides with contiguous D, so a
+                  [pages, page_size, HKV, D] pool is passed as its transpose(1, 2).
+                  page_size a power of two, 16 .. 4096.
 block_table       int32 [B, W]: position j of sequence b lies in page
                   block_table[b, j // page_size].  Entries past a sequence's length are not
                   read; one outside [0, pages) is a page that is not there (not written,
@@ -27,8 +28,15 @@ q_starts          int32 [B + 1]: sequence b has the rows q_starts[b] .. q_starts
 
 Lengths, tables and starts are read on the device: no call synchronizes, and a
 captured graph follows them.  Calls may run on several streams at once, and graphs on
-any: each stream and each capture has a workspace of its own.  They may come from
-several host threads: those on one stream go one after the other, each as a whole.
+any: each stream and each capture has a workspace of its own, for the life of the
+process (1 MB for the steps of a few requests, 100 MB for 8191 rows of 16 heads of 128;
+a graph clears its own once a replay).  Calls may come from several host threads: those
+on one stream go one after the other, each as a whole.
+
+Sums and softmax are in fp32.  Probabilities go into their products with the values as
+two bf16 parts where the sequences (or prefixes) of a call have 32 query rows of a
+key/value head or fewer on average (16 for D = 256), else rounded to one: a token's
+result depends in its last bits on the company it has.
 """
 
 from __future__ import annotations
@@ -350,6 +358,7 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_lens, bloc
     prefix: of all).  Every row attends its whole prefix, then its sequence's own
     positions as in paged_attention; kv_lens and block_table are about the own
     positions alone, and kv_lens may leave a row none of them.  The prefix's keys and
-    values are read once for all rows of its sequences."""
+    values are read once for every 16 to 128 of its sequences' query rows of a key/value
+    head, not once for each sequence."""
     return _attention(q, k_pages, v_pages, block_table, kv_lens, q_starts, (prefix_table, prefix_lens, prefix_seqs),
                       scale, k_scale, v_scale, out)

@@ -7,9 +7,12 @@
 namespace bz {
 
 // Workgroups that the keys are cut for: for few rows as many as run at once, so that none
-// starts late.  For many rows two to a CU, less those that a tile's last, shorter chunk adds (24
-// sequences in three groups, e4m3, 16 / 4 heads of 256: 56 us with 512, 41 with 384, 43 with
-// 416; three chunks of prompts, bf16: 367 with 384, 349 with 416).
+// starts late.  For many rows two to a CU, less those that a tile's last, shorter chunk adds.
+// us with 384 / 416 / 448 / 512, calls in a graph: a prompt of 2011 tokens, bf16, 16 / 8 heads of 128
+// 39 / 38 / 38 / 51, of 64 27 / 27 / 27 / 38, 16 / 4 of 256 75 / 74 / 81 / 90; chunks of three prompts, 16 / 4
+// of 256 298 / 281 / 282 / 311 (e4m3 302 / 288 / 283 / 321), 16 / 8 of 128 144 / 177 / 148 / 157 (e4m3 160 / 197 /
+// 155 / 162), 6 / 2 of 64 49 / 46 / 46 / 58; 24 sequences in three groups, e4m3, 16 / 4 of 256 42 / 44 / 43 / 54.
+// Not the best for every batch: how a batch's chunks fall into whole rounds of workgroups differs.
 static int paged_workgroups(int D, bool f8, int M) {
     if (M > 32) return 416;
     if (D == 256) return f8 ? 512 : 256;
@@ -74,7 +77,16 @@ struct PagedPlan {
 // zero between calls of different sizes.
 constexpr int kPagedCounters = 16384;
 
-// Rows of a tile for segments of `rows` query rows.
+// Rows of a tile for segments of `rows` query rows: the fewest of the sizes that hold a segment, so that
+// its keys are read once; 128 for longer ones.  Both sides of the borders, us of a call in a graph, 16
+// sequences of 97 .. 2043 positions before their rows, bf16:
+//   8 / 2 heads of 128   20 rows in tiles of 16 / 32 19.9 / 16.6, 40 in 32 / 64 26.4 / 22.2, 80 in 64 / 128 27.3 / 27.8
+//   16 / 8 of 128        18 in 16 / 32 29.7 / 31.9, 40 in 32 / 64 42.1 / 29.4, 80 in 64 / 128 29.2 / 32.4
+//   16 / 1 of 64         32 in 16 / 32 11.8 / 13.1, 64 in 32 / 64 13.4 / 15.9, 128 in 64 / 128 17.3 / 20.4
+//   16 / 4 of 256        20 in 16 / 64 43.4 / 42.0, 80 in 64 / 128 57.8 / 48.6 (e4m3 34.7 / 27.1 and 39.7 / 48.0)
+// and in tiles of 64 / 128: a prompt of 2011 tokens, 16 / 8 of 128, 50.3 / 38.8; chunks of three prompts, 16 / 4 of 256, 536 /
+// 281.  One rule for all heads and types: beside its borders another size can be up to a third faster (tiles
+// of 64 for 18 .. 32 rows of 16 / 8 heads of 128, 26.4, and for 80 .. 128 rows in e4m3 of 256; of 32 for 64 .. 128 of 16 / 1 of 64).
 static int paged_tile_rows(int64_t rows, int D) {
     if (rows <= 16) return 16;
     if (D == 256) return rows <= 64 ? 64 : 128;
@@ -162,6 +174,9 @@ static void launch_attn(const PagedKv& c, PagedAttn a, const PagedPlan& p, char*
         launch_tiles<D, false>(c, a, p.slots, st);
     if (!p.join || p.inside) return;
     const int items = c.HQ * (D / 4);
+    // few items leave CUs idle, so several threads share one's parts.  us of a call in a graph with P and 1 threads:
+    // rows behind one prefix of 6007, 16 / 8 heads of 128, 32768 items 40.3 and 40.4, 65536 61.0 and 57.5, 131072 117 and 109;
+    // 16 / 4 of 256, 49152 39.7 and 41.0, 131072 76.2 and 73.2; 8 / 2 of 64, 16384 22.8 and 24.6, 65536 52.3 and 48.7
     constexpr int P = 1024 / D > 8 ? 8 : 1024 / D;
     if ((int64_t)c.T * items <= 65536)
         hipLaunchKernelGGL((paged_attn_bf16_join<D, P>), dim3(c.T, (items * P + 255) / 256), dim3(256), 0, st, c, a, f8);

@@ -13,8 +13,8 @@
 // of each half of a head: the rotary partner is its own, every access is 16
 // bytes (8 into an e4m3 cache), and a head's sum of squares is 2 to 4 DPP steps over
 // the D / 16 threads of the head.  Measured: seven prompts of 33 .. 611 tokens, bf16, 16 / 4 heads
-// of 256, 14.6 us (4.6 TB/s), a chunk of 8191 tokens into e4m3, 16 / 8 heads of 128, 27.0 (4.7 TB/s;
-// 5.2 is what a large copy reaches), two rows 2.7.
+// of 256, 14.6 us (4.6 TB/s), a chunk of 8191 tokens into e4m3, 16 / 8 heads of 128, 27.1 (4.7 TB/s;
+// 5.2 is what a large copy reaches), two rows 2.9.
 #include "bz_paged_kv.h"
 
 namespace bz {

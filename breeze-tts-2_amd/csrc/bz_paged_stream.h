@@ -14,9 +14,9 @@
 //   waves   merged through LDS at the end, in wave order
 //   parts   joined by the last workgroup of those that have them
 // Measured, heads of 128 unless said: one token for each of 48 sequences of 40 .. 4095 positions,
-// 16 / 8 heads, 83.5 us (4.9 TB/s, 94% of a large copy's rate); four of 30 .. 65 thousand, e4m3, 16 / 4
-// heads of 256, 99.5 (4.5 TB/s); five tokens for 16 of 97 .. 2043, 8 / 2 heads, 17.9; one for
-// two of 610, 16 / 8 heads, 9.8: the chain of launch, lengths, table, keys, values, store, count
+// 16 / 8 heads, 85.0 us (4.8 TB/s, 93% of a large copy's rate); four of 30 .. 65 thousand, e4m3, 16 / 4
+// heads of 256, 100.7 (4.4 TB/s); five tokens for 16 of 97 .. 2043, 8 / 2 heads, 17.5; one for
+// two of 610, 16 / 8 heads, 9.9: the chain of launch, lengths, table, keys, values, store, count
 // and join.
 #pragma once
 
