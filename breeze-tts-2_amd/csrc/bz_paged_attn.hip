@@ -6,8 +6,12 @@
 
 namespace bz {
 
-// Workgroups that the keys are cut for: for few rows as many as run at once, so that none
-// starts late.  For many rows two to a CU, less those that a tile's last, shorter chunk adds.
+// Workgroups that the keys are cut for: for few rows about as many as run at once, so that none
+// starts late.  us with the number here, and fewer and more, calls in a graph: 48 sequences of up to 4095 positions, 16 / 8
+// heads of 128, 768 82 (512 87, 1024 85), of 64 1024 41 (768 44, 1280 39.5); four of 30 .. 65 thousand, 16 / 8 of 64 1024 88
+// (768 85, 1280 91), of 128 768 165 (512 189, 1024 172), 16 / 4 of 256, e4m3, 512 101 (256 123, 768 106), bf16 256 225 (384
+// 171, 512 183); five tokens for 16 of up to 2043, 8 / 2 of 128, 512 16.6 (256 .. 1024 the same), of up to 16000 45 (384 42, 768 53).
+// For many rows two to a CU, less those that a tile's last, shorter chunk adds.
 // us with 384 / 416 / 448 / 512, calls in a graph: a prompt of 2011 tokens, bf16, 16 / 8 heads of 128
 // 39 / 38 / 38 / 51, of 64 27 / 27 / 27 / 38, 16 / 4 of 256 75 / 74 / 81 / 90; chunks of three prompts, 16 / 4
 // of 256 298 / 281 / 282 / 311 (e4m3 302 / 288 / 283 / 321), 16 / 8 of 128 144 / 177 / 148 / 157 (e4m3 160 / 197 /

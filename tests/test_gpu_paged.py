@@ -818,3 +818,18 @@ def test_append_by_a_scale_of_zero():
                        v_scale=cache.v_scale)
     v = cache.v.float()[1, 0, 0]
     assert v[:2].tolist() == [448.0, -448.0] and torch.isnan(v[2:]).all()
+
+
+@pytest.mark.parametrize("HQ,HKV,D,rows", [(4, 4, 128, 5), (4, 4, 128, 150), (8, 4, 64, 60), (8, 4, 256, 70)])
+def test_later_rows_have_no_part_whatever_the_scales(HQ, HKV, D, rows):
+    """A value that is NaN in the last token, with scales of any sign and zero: the rows before it are as without it."""
+    rng = np.random.default_rng(44)
+    cache = Cache(rng, 20, HKV, 32, D, "e4m3")
+    table = cache.table(1, 16)
+    _scales(cache, table)
+    q, j = bf16(rng.standard_normal((rows, HQ, D))), rows + 330
+    cache.v.view(torch.uint8)[int(table[0, j // 32]), :, j % 32, ::3] = 0x7F
+    out = T.paged_attention(q, cache.k, cache.v, table, ints([j + 1]), ints([0, rows]), k_scale=cache.k_scale,
+                            v_scale=cache.v_scale)
+    check_attention(out[:-1], q[:-1], cache, table, [j], [0, rows - 1])
+    assert torch.isnan(out[-1].view(HQ, D)[:, ::3]).all()
