@@ -25,10 +25,14 @@ ERR_INVALID_ARG, ERR_SHAPE, ERR_ALIGNMENT, ERR_UNSUPPORTED, ERR_LAUNCH, ERR_ABI,
 GEMV_SCRATCH_BYTES = 8 << 20  # BZ_GEMV_SCRATCH_BYTES
 W_INT4_ZP, W_INT4_MIN, W_FP8, W_BF16 = 0, 1, 2, 3
 W_INT4_TILED, W_INT4_TILED_PAIRED, W_FP8_TILED, W_FP8_TILED_PAIRED = 4, 5, 6, 7
+W_MXFP4, W_MXFP4_TILED, W_MXFP4_TILED_PAIRED = 8, 10, 11
 EPI_NONE, EPI_SILU_GATE, EPI_RESIDUAL = 0, 1, 2
 DT_BF16, DT_F32 = 0, 1
 MASK_BOOL = 2  # include/bz_attn.h
 KV_E4M3 = 3  # include/bz_paged.h
+MX_E2M1, MX_E4M3 = 0, 1  # include/bz_mx.h
+MX_F16 = 2
+MX_ROWS, MX_TILED = 0, 1
 STEP_INV_BF16 = 256  # added to bz_step_tables' dtype
 
 EXPORTS = (
@@ -58,6 +62,10 @@ EXPORTS = (
     "bz_paged_rope_cache",
     "bz_paged_attn",
     "bz_paged_attn_workspace",
+    "bz_mx_rows_bytes",
+    "bz_mx_quantize",
+    "bz_mx_dequantize",
+    "bz_mx_gemm",
     "bz_sample_cfg",
     "bz_sample_next",
     "bz_stream_read",
@@ -217,6 +225,14 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.bz_paged_attn.argtypes = [ctypes.POINTER(PagedKv), vp, i64, f32, vp, ctypes.c_size_t, vp, i64, vp]
     lib.bz_paged_attn_workspace.restype = ctypes.c_size_t
     lib.bz_paged_attn_workspace.argtypes = [ctypes.POINTER(PagedKv)]
+    lib.bz_mx_rows_bytes.restype = ctypes.c_size_t
+    lib.bz_mx_rows_bytes.argtypes = [i32, i32, i32]
+    lib.bz_mx_quantize.restype = ctypes.c_int
+    lib.bz_mx_quantize.argtypes = [vp, i32, i64, i32, i32, i32, i32, vp, vp, vp]
+    lib.bz_mx_dequantize.restype = ctypes.c_int
+    lib.bz_mx_dequantize.argtypes = [vp, vp, i32, i32, i32, vp, i32, i64, vp]
+    lib.bz_mx_gemm.restype = ctypes.c_int
+    lib.bz_mx_gemm.argtypes = [i32, vp, i32, vp, i32, i32, vp, i32, i64, vp, i32, i64, vp]
     lib.bz_stream_read.restype = ctypes.c_int
     lib.bz_stream_read.argtypes = [vp, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_uint32, vp, vp]
     lib.bz_shared_read.restype = ctypes.c_int

@@ -38,6 +38,8 @@ from ..gemv import (
     W_INT4_TILED,
     W_INT4_TILED_PAIRED,
     W_INT4_ZP,
+    W_MXFP4_TILED,
+    W_MXFP4_TILED_PAIRED,
     gemv_traceable,
     pack_tiled,
     quantize_fp8_device,
@@ -81,10 +83,11 @@ def pack_fp8(weight: torch.Tensor):
 _TILED_FMT = {
     (8, False): W_FP8_TILED, (8, True): W_FP8_TILED_PAIRED,
     (4, False): W_INT4_TILED, (4, True): W_INT4_TILED_PAIRED,
+    ("mx4", False): W_MXFP4_TILED, ("mx4", True): W_MXFP4_TILED_PAIRED,
 }
 
 
-def _tile_rows(bits: int, paired: bool, parts, N: int, K: int):
+def _tile_rows(bits, paired: bool, parts, N: int, K: int):
     """Pack row-major or tiled parts (each (src_wfmt, bytes, scales, rows))
     into one tiled weight of N logical rows, the parts stacked along N in
     order.  Returns None when the shape cannot be tiled."""
@@ -121,7 +124,8 @@ class FusedWeight:
       "row"          bits 8, e4m3 (N, K) with the per-row scale s;
       "tiled"        bits 4 or 8, the tiled format, scales inside w (s None);
       "tiled-paired" the same with gate|up rows interleaved per 16-row block
-                     for the SiLU-gate epilogue.
+                     for the SiLU-gate epilogue;
+      "mx-tiled", "mx-tiled-paired"  bits 4, the same two of MXFP4 (from_mxfp4).
     ``paired`` asks for the paired layout: the weight is [gate | up] along N."""
 
     def __init__(self, weight: torch.Tensor, bits: int = 16, paired: bool = False):
@@ -206,7 +210,21 @@ class FusedWeight:
         s = torch.cat([m.scales_zeros for m in mods], 1).contiguous()
         return cls._assemble(4, group, N, K, "zp", w, s)
 
+    @classmethod
+    def from_mxfp4(cls, *mods, paired: bool = False) -> "FusedWeight":
+        """Adopt Mxfp4Linear buffers, re-tiled into one weight stacked along N
+        (paired for gate|up).  A decode step reads its activations in bf16,
+        whatever the modules' act_bits, as the modules themselves do."""
+        N, K = _stack_shape(mods, paired)
+        if K % 128 or any(m.out_features % 16 for m in mods):
+            raise ValueError("mxfp4 modules stored with padding cannot be fused")
+        parts = [(W_MXFP4_TILED, m.weight_mxfp4, None, m.out_features) for m in mods]
+        return cls._assemble(4, GROUP, N, K, "mx-tiled-paired" if paired else "mx-tiled",
+                             _tile_rows("mx4", paired, parts, N, K))
+
     def gemv_args(self) -> dict:
+        if self.layout.startswith("mx-"):
+            return {"wfmt": _TILED_FMT[("mx4", self.layout == "mx-tiled-paired")], "w": self.w}
         if self.layout.startswith("tiled"):
             return {"wfmt": _TILED_FMT[(self.bits, self.layout == "tiled-paired")], "w": self.w,
                     "group": self.group}
@@ -240,9 +258,9 @@ def rms_gemv(x, fw: FusedWeight, norm_weight=None, eps: float = 1e-6, epilogue: 
     N = fw.N
     n_out = N // 2 if epilogue == EPI_SILU_GATE else N
     out_dtype = torch.bfloat16 if residual is None else residual.dtype
-    if fw.layout == "tiled-paired" and epilogue != EPI_SILU_GATE:
+    if fw.layout.endswith("tiled-paired") and epilogue != EPI_SILU_GATE:
         raise ValueError("a paired gate|up weight is only read with the SiLU-gate epilogue")
-    if fw.layout == "tiled" and epilogue == EPI_SILU_GATE:
+    if fw.layout.endswith("tiled") and epilogue == EPI_SILU_GATE:
         gu = rms_gemv(x, fw, norm_weight, eps)
         y = _silu_mul(gu[:, : N // 2], gu[:, N // 2:])
         if out is not None:

@@ -19,7 +19,8 @@ Differences from the reference, on purpose:
     from_int4); the reference keeps tinygemm there and needs rmsnorm, two
     matmuls, silu_mul and an add (models/fused/layer.py:51-53, 92-95);
   * Fp8Linear / Int4Linear attention projections are adopted as well (the
-    reference reads q_proj.weight and so needs bf16 projections);
+    reference reads q_proj.weight and so needs bf16 projections), and
+    Mxfp4Linear ones anywhere;
   * with transformers >= 5, whose StaticLayer writes at its own fill counter
     (cumulative_length) and whose models pass no cache_position, the step
     position comes from that counter and the counter is advanced by the
@@ -46,15 +47,17 @@ def _kind(mod) -> str:
 
 def _adopt(mods, bits: int, paired: bool = False) -> FusedWeight:
     """One FusedWeight over the modules' outputs stacked along N: the
-    quantized buffers of Int4Linear / Fp8Linear (re-tiled where the shape
-    allows), otherwise the float weights quantized to ``bits`` (16 = bf16).
+    quantized buffers of Int4Linear / Fp8Linear / Mxfp4Linear (re-tiled where the
+    shape allows), otherwise the float weights quantized to ``bits`` (16 = bf16).
     ``paired``: the two modules are gate and up of a SiLU-gate MLP."""
     kinds = {_kind(m) for m in mods}
     if kinds == {"Int4Linear"}:
         return FusedWeight.from_int4(*mods, paired=paired)
     if kinds == {"Fp8Linear"}:
         return FusedWeight.from_fp8(*mods, paired=paired)
-    if kinds & {"Int4Linear", "Fp8Linear"}:
+    if kinds == {"Mxfp4Linear"}:
+        return FusedWeight.from_mxfp4(*mods, paired=paired)
+    if kinds & {"Int4Linear", "Fp8Linear", "Mxfp4Linear"}:
         raise TypeError(f"cannot fuse a mix of {sorted(kinds)}")
     return FusedWeight(torch.cat([m.weight for m in mods], 0).detach(), bits, paired=paired)
 

@@ -36,6 +36,9 @@ from ._lib import (
     W_INT4_TILED,
     W_INT4_TILED_PAIRED,
     W_INT4_ZP,
+    W_MXFP4,
+    W_MXFP4_TILED,
+    W_MXFP4_TILED_PAIRED,
 )
 
 __all__ = [
@@ -60,9 +63,13 @@ __all__ = [
     "W_INT4_TILED_PAIRED",
     "W_FP8_TILED",
     "W_FP8_TILED_PAIRED",
+    "W_MXFP4",
+    "W_MXFP4_TILED",
+    "W_MXFP4_TILED_PAIRED",
 ]
 
-TILED_FORMATS = (W_INT4_TILED, W_INT4_TILED_PAIRED, W_FP8_TILED, W_FP8_TILED_PAIRED)
+TILED_FORMATS = (W_INT4_TILED, W_INT4_TILED_PAIRED, W_FP8_TILED, W_FP8_TILED_PAIRED, W_MXFP4_TILED,
+                 W_MXFP4_TILED_PAIRED)
 
 _DT = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
 _NO_CFG = (0, 0, 0, 0, 0)
@@ -207,6 +214,8 @@ def _weight_spec(wfmt: int, n: int, k: int, group: int):
         return n * k, (torch.float32, n), None
     if wfmt == W_BF16:
         return 2 * n * k, None, None
+    if wfmt == W_MXFP4:
+        return n * k // 2, (torch.uint8, n * (k // 32)), None
     if wfmt in TILED_FORMATS:
         return tiled_bytes(wfmt, n, k), None, None
     return None
@@ -250,18 +259,19 @@ def pack_tiled(src_wfmt: int, w: torch.Tensor, k: int, dst_wfmt: int, *, sc0: Op
                n_total: Optional[int] = None, row0: int = 0, out: Optional[torch.Tensor] = None,
                group: int = 128) -> torch.Tensor:
     """Tile the rows of ``w`` (row-major BZ_W_INT4_ZP with scales_zeros
-    ``sc0``, BZ_W_FP8 with row scales ``sc0``, or an unpaired tiled weight)
+    ``sc0``, BZ_W_FP8 with row scales ``sc0``, BZ_W_MXFP4 with scale codes
+    ``sc0`` (mx.quantize_mx), or an unpaired tiled weight)
     into logical rows [row0, row0 + n) of a ``dst_wfmt`` weight of
     ``n_total`` rows (default n).  ``out`` (uint8, tiled_bytes bytes) is
     allocated zero-filled when omitted.  Returns ``out``."""
     _require_gpu("w", w, w.device)
-    if src_wfmt in (W_INT4_ZP, W_FP8):
-        row_bytes = k // 2 if src_wfmt == W_INT4_ZP else k
+    if src_wfmt in (W_INT4_ZP, W_FP8, W_MXFP4):
+        row_bytes = k if src_wfmt == W_FP8 else k // 2
         n = (w.numel() * w.element_size()) // row_bytes
         if sc0 is None:
             raise ValueError("a row-major source needs its scales (sc0)")
         _check_weight(w, src_wfmt, n, k, group, sc0, None)
-    elif src_wfmt in (W_INT4_TILED, W_FP8_TILED):
+    elif src_wfmt in (W_INT4_TILED, W_FP8_TILED, W_MXFP4_TILED):
         per16 = tiled_bytes(src_wfmt, 16, k)
         if not per16 or (w.numel() * w.element_size()) % per16:
             raise ValueError("source is not a whole number of tiled row blocks")
@@ -488,12 +498,12 @@ def dequant(wfmt: int, w: torch.Tensor, n: int, k: int, *, sc0=None, sc1=None, g
 def dequant_matmul(x: torch.Tensor, w: torch.Tensor, wfmt: int, n: int, k: int,
                    chunk_bytes: int = 16 << 20) -> torch.Tensor:
     """x [M, k] @ w_eff^T -> bf16 [M, n] for prefill-sized M, over an unpaired
-    tiled weight (BZ_W_INT4_TILED, group 128, or BZ_W_FP8_TILED): one GEMM
-    (bz_gemm_tiled) that decodes the weight in registers, so no decoded copy
+    tiled weight (BZ_W_INT4_TILED, group 128, BZ_W_FP8_TILED or
+    BZ_W_MXFP4_TILED): one GEMM (bz_gemm_tiled) that decodes the weight in registers, so no decoded copy
     exists; where it slices K, the slices' fp32 sums are held for the call.
     An x that autograd follows goes through torch's linear over the decoded
     weight instead (at most ``chunk_bytes`` of fp32 weight at a time)."""
-    if wfmt not in (W_INT4_TILED, W_FP8_TILED):
+    if wfmt not in (W_INT4_TILED, W_FP8_TILED, W_MXFP4_TILED):
         raise ValueError(f"dequant_matmul reads the unpaired tiled formats, not format {wfmt}")
     _require_gpu("x", x, x.device)
     _require_gpu("w", w, x.device)

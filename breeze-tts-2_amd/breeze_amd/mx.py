@@ -1,0 +1,239 @@
+"""Operators over microscaled blocks (include/bz_mx.h).
+
+A microscaled tensor keeps, for each 32 consecutive values of a row, elements
+of a narrow floating-point type and one power of two:
+
+``quantize_mx``    rows to elements and scale codes, the layout checkpoints hold
+``dequantize_mx``  the values they stand for
+``mx_rows``        rows to the operand order of the matrix cores, for several
+                   ``mx_linear`` over the same rows
+``mx_linear``      rows, quantised to blocks, times a 4-bit weight on the matrix
+                   cores' block-scaled arithmetic
+
+Element types ("elem"): "e2m1" (4 bits, 0 0.5 1 1.5 2 3 4 6) and "e4m3" (OCP
+FP8, up to 448).  A block with largest magnitude a has the scale
+2^max(floor(log2 a) - emax, -126), emax 2 or 8, stored as the exponent plus 127
+in a byte; each element is its value over the scale, rounded to the nearest
+(ties to the even code), magnitudes above the type's largest to the largest.
+A block that holds a NaN or an infinity has the code 255 and reads back as NaN.
+
+Weights are e2m1: ``quantize_mx`` of an [N, K] weight, laid out for the kernels
+by ``gemv.pack_tiled(W_MXFP4, codes, K, W_MXFP4_TILED, sc0=scales)``.  bf16 rows
+times such a weight, with nothing quantised on the way, are ``gemv.gemv`` and
+``gemv.dequant_matmul``; ``mxfp4_linear.Mxfp4Linear`` is the module.
+
+Calls follow torch's current stream of the tensors' device, do not synchronise,
+and may be captured into graphs and made from several streams at once.  None of
+them has a gradient.
+"""
+
+from __future__ import annotations
+
+import functools
+from typing import Optional, Union
+
+import torch
+
+from . import _lib
+from ._lib import DT_BF16, DT_F32, MX_E2M1, MX_E4M3, MX_F16, MX_ROWS, MX_TILED, W_MXFP4_TILED
+
+__all__ = ["BLOCK", "MxRows", "quantize_mx", "dequantize_mx", "mx_rows", "mx_linear"]
+
+BLOCK = 32
+
+_ELEM = {"e2m1": MX_E2M1, "e4m3": MX_E4M3}
+_X = {torch.bfloat16: DT_BF16, torch.float32: DT_F32, torch.float16: MX_F16}
+_OUT = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
+
+
+def _elem(elem: str) -> int:
+    code = _ELEM.get(elem)
+    if code is None:
+        raise ValueError(f"elem must be 'e2m1' or 'e4m3', got {elem!r}")
+    return code
+
+
+def _gpu(name: str, t: torch.Tensor, index: int) -> None:
+    at = t.get_device()  # -1 on the CPU
+    if at < 0:
+        raise RuntimeError(f"{name} must be a GPU tensor (got {t.device}); the HIP path has no CPU fallback")
+    if at != index:
+        raise RuntimeError(f"{name} is on {t.device}, expected cuda:{index}")
+
+
+def _no_grad(x: torch.Tensor, what: str) -> None:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on x.detach()")
+
+
+def _call(index: int, f, *args) -> None:
+    """f(*args, stream) on the device's current stream, with the device current."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = f(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = f(*args, stream)
+    if rc:
+        raise _lib.BzError(rc, f.__name__)
+
+
+def _rows(x: torch.Tensor, unit: int) -> tuple:
+    """(x with rows the kernels can read, M, K, row stride)."""
+    if x.dim() != 2:
+        raise ValueError(f"x must be [rows, columns], got {list(x.shape)}")
+    if x.dtype not in _X:
+        raise TypeError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
+    M, K = x.shape
+    if K < 1 or K % unit:
+        raise ValueError(f"{K} columns are not a positive multiple of {unit}")
+    ld, inner = x.stride()
+    if M > 1 and ld < K or inner != 1 and K > 1:  # an expanded row, a transposed matrix
+        x, ld = x.contiguous(), K
+    return x, M, K, ld if M > 1 else K
+
+
+def quantize_mx(x: torch.Tensor, elem: str = "e2m1") -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of x [M, K] (bf16, fp16 or fp32; K a multiple of 32):
+    codes uint8 [M, K/2] with the even column in the low half (e2m1) or
+    float8_e4m3fn [M, K]; scales uint8 [M, K/32]."""
+    code = _elem(elem)
+    index = x.get_device()
+    _gpu("x", x, index)
+    x, M, K, ld = _rows(x, BLOCK)
+    codes = torch.empty(M, K // 2 if code == MX_E2M1 else K, device=x.device,
+                        dtype=torch.uint8 if code == MX_E2M1 else torch.float8_e4m3fn)
+    scales = torch.empty(M, K // BLOCK, device=x.device, dtype=torch.uint8)
+    if M:
+        _call(index, _lib.lib().bz_mx_quantize, x.data_ptr(), _X[x.dtype], ld, M, K, code, MX_ROWS, codes.data_ptr(),
+              scales.data_ptr())
+    return codes, scales
+
+
+def dequantize_mx(codes: torch.Tensor, scales: torch.Tensor, elem: str = "e2m1",
+                  dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values [M, K] (bf16 or fp32) that quantize_mx's codes and scales stand
+    for: exact, in bf16 down to 2^-126."""
+    code = _elem(elem)
+    index = codes.get_device()
+    _gpu("codes", codes, index)
+    _gpu("scales", scales, index)
+    if dtype not in _OUT:
+        raise TypeError(f"values are bfloat16 or float32, not {dtype}")
+    if codes.dim() != 2 or codes.element_size() != 1 or scales.dtype != torch.uint8:
+        raise ValueError("codes must be a 2-D tensor of bytes and scales uint8")
+    M, K = codes.shape
+    K *= 2 if code == MX_E2M1 else 1
+    if K < 1 or K % BLOCK or scales.shape != (M, K // BLOCK):
+        raise ValueError(f"codes {list(codes.shape)} and scales {list(scales.shape)} are not those of {elem} rows")
+    codes, scales = codes.contiguous(), scales.contiguous()
+    if codes.data_ptr() % 4:
+        codes = codes.clone()
+    out = torch.empty(M, K, device=codes.device, dtype=dtype)
+    if M:
+        _call(index, _lib.lib().bz_mx_dequantize, codes.data_ptr(), scales.data_ptr(), code, M, K, out.data_ptr(),
+              _OUT[dtype], K)
+    return out
+
+
+class MxRows:
+    """Quantised rows in the operand order of the matrix cores (mx_rows)."""
+
+    __slots__ = ("data", "shape", "elem")
+
+    def __init__(self, data: torch.Tensor, shape: tuple[int, int], elem: str):
+        self.data, self.shape, self.elem = data, shape, elem
+
+
+@functools.lru_cache(maxsize=4096)
+def _rows_bytes(elem: int, M: int, K: int) -> int:
+    return int(_lib.lib().bz_mx_rows_bytes(elem, M, K))
+
+
+def mx_rows(x: torch.Tensor, elem: str = "e2m1") -> MxRows:
+    """x [M, K] (bf16, fp16 or fp32; K a multiple of 128) quantised to blocks,
+    for mx_linear: once for all products that read the same rows."""
+    code = _elem(elem)
+    index = x.get_device()
+    _gpu("x", x, index)
+    _no_grad(x, "mx_rows")
+    x, M, K, ld = _rows(x, 128)
+    data = torch.empty(_rows_bytes(code, M, K), device=x.device, dtype=torch.uint8)
+    if M:
+        _call(index, _lib.lib().bz_mx_quantize, x.data_ptr(), _X[x.dtype], ld, M, K, code, MX_TILED, data.data_ptr(),
+              None)
+    return MxRows(data, (M, K), elem)
+
+
+@functools.lru_cache(maxsize=1024)
+def _weight_bytes(n: int, k: int) -> int:
+    return int(_lib.lib().bz_tiled_bytes(W_MXFP4_TILED, n, k))
+
+
+def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: str = "e2m1",
+              residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+              out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """q(x) @ w_eff^T (+ residual) -> [M, n]: x [M, K] (bf16, fp16 or fp32), quantised to
+    blocks of ``elem`` on the way, or the MxRows of it; w a W_MXFP4_TILED weight of n
+    rows and K columns.  Products are exact, sums fp32; the result is rounded once,
+    to out's dtype (bf16 or fp32).  residual: [M, n] bf16 or fp32, may be out itself;
+    out: [M, n] with unit column stride, apart from x and w."""
+    rows = isinstance(x, MxRows)
+    if rows:
+        src, (M, K), code, index = x.data, x.shape, _elem(x.elem), x.data.get_device()
+    else:
+        code, index = _elem(elem), x.get_device()
+        _gpu("x", x, index)
+        _no_grad(x, "mx_linear")
+        src, M, K, ld = _rows(x, 128)
+    if w.get_device() != index:
+        _gpu("w", w, index)
+    if w.numel() * w.element_size() != (_weight_bytes(n, K) or -1) or not w.is_contiguous() or w.data_ptr() % 16:
+        raise ValueError(f"w must be a contiguous W_MXFP4_TILED weight of {n} x {K} (rows a multiple of 16), "
+                         f"{_weight_bytes(n, K)} bytes; got {w.numel() * w.element_size()}")
+    if out is None:
+        if out_dtype not in _OUT:
+            raise TypeError(f"out is bfloat16 or float32, not {out_dtype}")
+        out = torch.empty(M, n, device=w.device, dtype=out_dtype)
+    else:
+        _gpu("out", out, index)
+        if out.dtype not in _OUT or out.shape != (M, n) or (out.stride(1) != 1 and n > 1) \
+                or (M > 1 and out.stride(0) < n):
+            raise ValueError(f"out must be a bf16 or fp32 [{M}, {n}] tensor whose rows are contiguous")
+        for name, t in (("x", src), ("w", w)):
+            if _overlap(out, t):
+                raise ValueError(f"out must not overlap {name}")
+    res = rdt = ldr = 0
+    if residual is not None:
+        _gpu("residual", residual, index)
+        if residual.dtype not in _OUT or residual.shape != (M, n):
+            raise ValueError(f"residual must be a bf16 or fp32 [{M}, {n}] tensor")
+        if (residual.stride(1) != 1 and n > 1) or (M > 1 and residual.stride(0) < n) \
+                or (_overlap(out, residual) and not _same(out, residual)):
+            residual = residual.clone(memory_format=torch.contiguous_format)
+        res, rdt, ldr = residual.data_ptr(), _OUT[residual.dtype], residual.stride(0) if M > 1 else n
+    if M == 0:
+        return out
+    if not rows:
+        data = torch.empty(_rows_bytes(code, M, K), device=w.device, dtype=torch.uint8)
+        _call(index, _lib.lib().bz_mx_quantize, src.data_ptr(), _X[src.dtype], ld, M, K, code, MX_TILED,
+              data.data_ptr(), None)
+        src = data
+    _call(index, _lib.lib().bz_mx_gemm, code, src.data_ptr(), M, w.data_ptr(), n, K, res, rdt, ldr, out.data_ptr(),
+          _OUT[out.dtype], out.stride(0) if M > 1 else n)
+    return out
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    size = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + size * t.element_size()
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether each element of b lies where that of a does."""
+    return a.data_ptr() == b.data_ptr() and a.dtype == b.dtype and a.stride() == b.stride()

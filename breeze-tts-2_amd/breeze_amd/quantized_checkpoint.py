@@ -27,6 +27,8 @@ This build's additions to the manifest and the loader:
   [N, K] codes).  An fp8 entry without a tag is the reference's row-major
   buffer and is read as such; a row-major module of a tileable shape is
   re-tiled on its GPU after loading;
+* Mxfp4Linear modules are recorded as kind "mxfp4", with their act_bits and
+  ``"layout"`` mxfp4_linear.LAYOUT_TILED ("bz-mxfp4-tiled16-v1");
 * ``convert_logical_int4`` turns the logical nibbles the reference's
   quantizer builds before its repack (odd k in the low nibble,
   models/int4_linear.py:57-58) into this build's row-major buffer.
@@ -48,8 +50,10 @@ from safetensors.torch import save_file
 from torch import nn
 
 from . import fp8_linear as _f8
+from . import mxfp4_linear as _m4
 from .fp8_linear import FP8_DTYPE, Fp8Linear
 from .int4_linear import LAYOUT_ROWMAJOR, LAYOUT_TILED, Int4Linear, layout_of, retile, tileable, tiled_shape
+from .mxfp4_linear import Mxfp4Linear
 
 INT4_LAYOUT = LAYOUT_TILED
 FORMAT_VERSION = 1
@@ -120,11 +124,21 @@ def _fp8_shapes(spec: dict) -> dict:
     return {"weight_fp8": codes, "weight_scale": [1, n]}
 
 
+def _mxfp4_shapes(spec: dict) -> dict:
+    if spec.get("layout") != _m4.LAYOUT_TILED:
+        raise ValueError(f"mxfp4 module stored in layout {spec.get('layout')!r}; this build reads {_m4.LAYOUT_TILED!r}")
+    if spec.get("act_bits") not in (4, 8, 16):
+        raise ValueError(f"act_bits {spec.get('act_bits')} is not 4, 8 or 16")
+    return {"weight_mxfp4": list(_m4.tiled_shape(spec["out_features"], spec["in_features"]))}
+
+
 _KINDS = (
     _Kind("int4", Int4Linear, {"weight_int4": torch.int32, "scales_zeros": torch.bfloat16},
           ("in_features", "out_features", "group_size"), _int4_shapes),
     _Kind("fp8", Fp8Linear, {"weight_fp8": FP8_DTYPE, "weight_scale": torch.float32},
           ("in_features", "out_features"), _fp8_shapes),
+    _Kind("mxfp4", Mxfp4Linear, {"weight_mxfp4": torch.uint8}, ("in_features", "out_features", "act_bits"),
+          _mxfp4_shapes),
 )
 _BY_NAME = {k.name: k for k in _KINDS}
 
@@ -145,6 +159,8 @@ def describe(model: nn.Module) -> dict[str, dict]:
             entry["layout"] = layout_of(module.weight_int4, module.out_features, module.in_features)
         elif kind.name == "fp8":
             entry["layout"] = _f8.layout_of(module.weight_fp8, module.out_features, module.in_features)
+        elif kind.name == "mxfp4":
+            entry["layout"] = _m4.LAYOUT_TILED
         entry.update({a: int(getattr(module, a)) for a in kind.attrs})
         entry["shapes"] = {b: list(getattr(module, b).shape) for b in kind.buffers}
         entries[path] = entry

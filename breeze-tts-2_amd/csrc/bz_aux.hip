@@ -15,6 +15,7 @@
 // torch formulas they restate.
 #include "bz_device.h"
 #include "bz_gemv.h"
+#include "bz_mx.h"
 
 namespace bz {
 
@@ -325,6 +326,10 @@ extern "C" int bz_dequant(int32_t wfmt, const void* w, const void* sc0, const vo
     if (!w || !out || N < 1 || K < 1) return BZ_ERR_INVALID_ARG;
     if (is_tiled(wfmt))
         return dequant_tiled(wfmt, w, N, K, group, static_cast<float*>(out), static_cast<hipStream_t>(stream));
+    if (wfmt == BZ_W_MXFP4) {
+        if (!sc0) return BZ_ERR_INVALID_ARG;
+        return bz_mx_dequantize(w, sc0, BZ_MX_E2M1, N, K, out, BZ_DT_F32, K, stream);
+    }
     if (wfmt < BZ_W_INT4_ZP || wfmt > BZ_W_BF16) return BZ_ERR_INVALID_ARG;
     const bool i4 = (wfmt == BZ_W_INT4_ZP || wfmt == BZ_W_INT4_MIN);
     if ((i4 || wfmt == BZ_W_FP8) && !sc0) return BZ_ERR_INVALID_ARG;

@@ -47,6 +47,8 @@
 //   * int4: w = bf16((q - 8) s + z), the effective weight rounded to bf16 as
 //     bz_dequant's float would be.  The lane's dword d holds k = 32 g + 8 d + 0..7:
 //     one MFMA operand, met by piece 4 g + d of the x row's half.
+//   * MXFP4: the exact bf16 value, scale in it, from the scaled conversion;
+//     operands as for int4.
 //   * fp8: the exact bf16 value of each code; the row scale multiplies the
 //     finished sum.  Codes 8 e..8 e+7 of lane row g in tile h of the half meet
 //     piece 8 h + 2 g + e.
@@ -101,8 +103,8 @@ __device__ __forceinline__ u32x4 int4_weights(uint32_t v, float s, float zp) {
 template <int WF, int MT, int NT>
 __global__ void __launch_bounds__(kGemmThreads, 2) gemm_tiled(GemmParams p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    constexpr bool I4 = tiled_i4(WF);
-    constexpr int TPU = I4 ? 1 : 2;                // tiles per block and 128 k
+    constexpr bool I4 = tiled_i4(WF), MX = tiled_mx(WF), F8 = !I4 && !MX;
+    constexpr int TPU = F8 ? 2 : 1;                // tiles per block and 128 k
     constexpr int PX = MT <= 4 || MT * NT <= 12 ? 2 : 1, PW = 2;  // steps ahead: x, weights
     constexpr int kBuf = MT * 16 * kGemmStepK * 2;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -149,10 +151,10 @@ __global__ void __launch_bounds__(kGemmThreads, 2) gemm_tiled(GemmParams p) {
     for (int t = 0; t < NT; ++t) {
         const bool live = blk0 + t < p.nblk;
         const uint8_t* c = p.w + (int64_t)(live ? blk0 + t : 0) * p.chunk;
-        wrs[t] = buffer_rsrc(c, live ? (uint32_t)p.NU * (I4 ? 1088u : 1024u) : 0u);
+        wrs[t] = buffer_rsrc(c, live ? (uint32_t)p.NU * (I4 ? 1088u : 1024u) + (MX ? (uint32_t)mx_scale_bytes(p.NU) : 0u) : 0u);
     }
     const int ue = min(p.NU, s_end * kGemmKGroups * TPU);
-    const uint32_t wl = j * 64 + kq * 16;
+    const uint32_t wl = tiled_lane_byte(WF, lane);
     u32x4 wv[PW][NT][TPU];
     uint32_t sz[PW][NT];
     auto w_load = [&](int set, int s) {
@@ -165,13 +167,17 @@ __global__ void __launch_bounds__(kGemmThreads, 2) gemm_tiled(GemmParams p) {
             if (I4)
                 sz[set][t] =
                     buffer_ld4(wrs[t], u0 < ue ? (uint32_t)p.NU * 1024u + (uint32_t)u0 * 64u + j * 4 : kBufferOob);
+            if (MX)
+                sz[set][t] = buffer_ld4(wrs[t], u0 < ue ? (uint32_t)p.NU * 1024u + mx_scale_offset(u0, lane) : kBufferOob);
         }
     };
     // operand d (32 k) of the wave's unit
-    auto decode = [&](u32x4 (&o)[NT], int set, int d) {
+    auto decode = [&](u32x4 (&o)[NT], int set, int s, int d) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            if (I4) {
+            if (MX) {
+                o[t] = mx4_weights(wv[set][t][0][d], mx_scale(sz[set][t], s * kGemmKGroups + kg));
+            } else if (I4) {
                 const float sc = bf16_lo(sz[set][t]);
                 o[t] = int4_weights(wv[set][t][0][d], sc, fmaf(-8.0f, sc, bf16_hi(sz[set][t])));
             } else {
@@ -193,11 +199,11 @@ __global__ void __launch_bounds__(kGemmThreads, 2) gemm_tiled(GemmParams p) {
     auto step = [&](int set, int s, int buf) {
         const uint8_t* xb = smem + buf * kBuf + j * 512 + kg * 256;
         u32x4 wd[2][NT];
-        decode(wd[0], set, 0);
+        decode(wd[0], set, s, 0);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-            const int piece = I4 ? 4 * kq + d : 8 * (d >> 1) + 2 * kq + (d & 1);
-            if (d < 3) decode(wd[(d + 1) & 1], set, d + 1);
+            const int piece = !F8 ? 4 * kq + d : 8 * (d >> 1) + 2 * kq + (d & 1);
+            if (d < 3) decode(wd[(d + 1) & 1], set, s, d + 1);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 const u32x4 xf = *reinterpret_cast<const u32x4*>(xb + i * 8192 + ((piece ^ j) << 4));
@@ -255,13 +261,13 @@ __global__ void __launch_bounds__(kGemmThreads, 2) gemm_tiled(GemmParams p) {
             for (int t = 0; t < NT; ++t) {
                 if (blk0 + t >= p.nblk) continue;
                 f32x4_t sc = {1.0f, 1.0f, 1.0f, 1.0f};
-                if (!I4)
+                if (F8)
                     sc = *reinterpret_cast<const f32x4_t*>(p.w + (int64_t)(blk0 + t) * p.chunk + (int64_t)p.NU * 1024 +
                                                            kq * 16);
 #pragma unroll
                 for (int i = P; i < MT; i += 2) {
                     const int m = m0 + i * 16 + j;
-                    if (m < p.M) store(m, (blk0 + t) * 16 + 4 * kq, I4 ? acc[i][t] : acc[i][t] * sc);
+                    if (m < p.M) store(m, (blk0 + t) * 16 + 4 * kq, F8 ? acc[i][t] * sc : acc[i][t]);
                 }
             }
         };
@@ -331,5 +337,6 @@ int launch_gemm_wf(const GemmParams& p, const GemmLaunch& l, hipStream_t st) {
 // One instantiation set per unpaired tiled format (bz_gemm_<fmt>.hip).
 int launch_gemm_i4t(const GemmParams& p, const GemmLaunch& l, hipStream_t st);
 int launch_gemm_f8t(const GemmParams& p, const GemmLaunch& l, hipStream_t st);
+int launch_gemm_mx4t(const GemmParams& p, const GemmLaunch& l, hipStream_t st);
 
 }  // namespace bz

@@ -49,13 +49,13 @@ constexpr GemmCost kGemmCostI4 = {-0.245f, 0.144f, 0.374f, 0.0156f, -0.457f, 0.1
 constexpr GemmCost kGemmCostF8 = {-0.206f, 0.108f, 0.217f, 0.0215f, 0.365f, 0.210f, 0.547f, 1.60f, 1.57f, 0.0172f};
 
 static float gemm_cost(int wf, int M, int N, int K, int mt, int nt, const GemmPlan& pl) {
-    const GemmCost& c = tiled_i4(wf) ? kGemmCostI4 : kGemmCostF8;
+    const GemmCost& c = tiled_4bit(wf) ? kGemmCostI4 : kGemmCostF8;
     const float mn = (float)(mt * nt);
     const float one = c.wg0 + c.wg_mn * mn +
                       (float)(pl.sps + (pl.sps & 1)) * (c.step0 + c.step_m * mt + c.step_n * nt + c.step_mn * mn);
     const float full = (float)pl.l.grid / 256.0f;
     const float rounds = mn > 8.0f ? (float)((pl.l.grid + 255) / 256) : full <= 1.0f ? 1.0f : full + c.overlap;
-    const float w_mb = (float)N * (float)K * (tiled_i4(wf) ? 0.53e-6f : 1e-6f), x_mb = (float)M * (float)K * 2e-6f;
+    const float w_mb = (float)N * (float)K * (tiled_4bit(wf) ? 0.53e-6f : 1e-6f), x_mb = (float)M * (float)K * 2e-6f;
     const float sums = pl.nsl > 1 ? c.sum0 + c.sum_mb * (float)pl.nsl * (float)M * (float)N * 1e-6f : 0.0f;
     return one * rounds + sums + c.traffic_mb * ((float)pl.mtiles * w_mb + (float)pl.ntiles * x_mb);
 }
@@ -108,7 +108,7 @@ static int gemm_plan(int wf, int M, int N, int K, int cfg_mt, int cfg_nt, int cf
 
 static int gemm_check(int wf, int M, int N, int K) {
     if (M < 1 || N < 1 || K < 1) return BZ_ERR_INVALID_ARG;
-    if (wf != BZ_W_INT4_TILED && wf != BZ_W_FP8_TILED) return BZ_ERR_INVALID_ARG;
+    if (wf != BZ_W_INT4_TILED && wf != BZ_W_FP8_TILED && wf != BZ_W_MXFP4_TILED) return BZ_ERR_INVALID_ARG;
     if (N % 16 || !tiled_units(wf, K)) return BZ_ERR_SHAPE;
     return BZ_OK;
 }
@@ -156,7 +156,9 @@ extern "C" int bz_gemm_tiled(int32_t wfmt, const void* x, int64_t ldx, int32_t M
     p.sps = pl.sps;
     p.out_f32 = out_dtype == BZ_DT_F32;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const int lrc = wfmt == BZ_W_INT4_TILED ? launch_gemm_i4t(p, pl.l, st) : launch_gemm_f8t(p, pl.l, st);
+    const int lrc = wfmt == BZ_W_INT4_TILED    ? launch_gemm_i4t(p, pl.l, st)
+                    : wfmt == BZ_W_MXFP4_TILED ? launch_gemm_mx4t(p, pl.l, st)
+                                               : launch_gemm_f8t(p, pl.l, st);
     if (lrc != BZ_OK || pl.nsl == 1) return lrc;
     const int64_t items = (int64_t)M * (N / 4);
     hipLaunchKernelGGL(gemm_sum_slices, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, p.part, pl.nsl, M, N,

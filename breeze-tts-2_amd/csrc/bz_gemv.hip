@@ -56,7 +56,7 @@ static int check_desc(const bz_gemv_desc* d, DescInfo& di) {
     if (d->abi_version != BZ_ABI_VERSION) return BZ_ERR_ABI;
     const int M = d->M, N = d->N, K = d->K, wf = d->wfmt, epi = d->epilogue;
     if (M < 1 || N < 1 || K < 1) return BZ_ERR_INVALID_ARG;
-    if (wf < BZ_W_INT4_ZP || wf > BZ_W_FP8_TILED_PAIRED) return BZ_ERR_INVALID_ARG;
+    if ((wf < BZ_W_INT4_ZP || wf > BZ_W_FP8_TILED_PAIRED) && !is_tiled(wf)) return BZ_ERR_INVALID_ARG;
     if (epi < BZ_EPI_NONE || epi > BZ_EPI_RESIDUAL) return BZ_ERR_INVALID_ARG;
     if (d->out_dtype != BZ_DT_BF16 && d->out_dtype != BZ_DT_F32) return BZ_ERR_INVALID_ARG;
     if (!d->x || !d->w || !d->out) return BZ_ERR_INVALID_ARG;
@@ -75,6 +75,7 @@ static int check_desc(const bz_gemv_desc* d, DescInfo& di) {
         // store (the panel kernel also without RMSNorm)
         if (d->cfg_path == PATH_TILE || d->cfg_path == PATH_PANEL) {
             if (tiled_paired(wf) || d->n_out2) return BZ_ERR_UNSUPPORTED;
+            if (d->cfg_path == PATH_TILE && tiled_mx(wf)) return BZ_ERR_UNSUPPORTED;
             if (d->cfg_path == PATH_PANEL && d->gamma) return BZ_ERR_UNSUPPORTED;
         } else if (d->cfg_path && d->cfg_path != PATH_STREAM) {
             return BZ_ERR_UNSUPPORTED;
@@ -91,7 +92,7 @@ static int check_desc(const bz_gemv_desc* d, DescInfo& di) {
         if (d->n_out2 && !aligned(d->out2, d->out_dtype == BZ_DT_F32 ? 4 : 2)) return BZ_ERR_ALIGNMENT;
         di.n_out = n_out;
         di.glog2 = 7;
-        di.row_bytes = tiled_i4(wf) ? K / 2 : K;
+        di.row_bytes = tiled_4bit(wf) ? K / 2 : K;
         di.i4 = tiled_i4(wf);
         return BZ_OK;
     }
@@ -206,8 +207,8 @@ constexpr int kTileMinRows = 5;
 static bool panel_auto(const bz_gemv_desc* d);
 static bool stream_rows_auto(const bz_gemv_desc* d);
 static bool tile_auto(const bz_gemv_desc* d) {
-    return d->cfg_path == 0 && d->M >= kTileMinRows && !d->n_out2 && !tiled_paired(d->wfmt) && !panel_auto(d) &&
-           !stream_rows_auto(d);
+    return d->cfg_path == 0 && d->M >= kTileMinRows && !d->n_out2 && !tiled_paired(d->wfmt) && !tiled_mx(d->wfmt) &&
+           !panel_auto(d) && !stream_rows_auto(d);
 }
 
 static int launch_tile(int wf, const TileParams& tp, const TileLaunch& l, hipStream_t st) {
@@ -238,8 +239,8 @@ static int stream_plan(const bz_gemv_desc* d, int rows, StreamLaunch& l) {
     int nw = d->cfg_waves;
     if (nw < 0 || nw > kStreamMaxWaves) return BZ_ERR_INVALID_ARG;
     const bool few_blocks = d->N / 16 <= 256;
-    const int per_wave = few_blocks ? (NU <= 32 ? 2 : (NU >= 64 ? (tiled_i4(wf) ? 5 : 8) : 4))
-                                    : (NU >= 64 ? 8 : (tiled_i4(wf) ? 4 : 6));
+    const int per_wave = few_blocks ? (NU <= 32 ? 2 : (NU >= 64 ? (tiled_4bit(wf) ? 5 : 8) : 4))
+                                    : (NU >= 64 ? 8 : (tiled_4bit(wf) ? 4 : 6));
     if (!nw) nw = std::min(kStreamMaxWaves, (NU + per_wave - 1) / per_wave);
     const int need = (NU + nw - 1) / nw;
     int upw = 0;
@@ -266,6 +267,8 @@ static int launch_stream(int wf, const StreamParams& p, const StreamLaunch& l, h
         case WF_I4TP: return launch_stream_i4tp(p, l, st);
         case WF_F8T: return launch_stream_f8t(p, l, st);
         case WF_F8TP: return launch_stream_f8tp(p, l, st);
+        case WF_MX4T: return launch_stream_mx4t(p, l, st);
+        case WF_MX4TP: return launch_stream_mx4tp(p, l, st);
         default: return BZ_ERR_INVALID_ARG;
     }
 }
@@ -276,6 +279,8 @@ static int launch_wide(int wf, const StreamParams& p, const WideLaunch& l, int n
         case WF_I4TP: return launch_wide_i4tp(p, l, nblk, st);
         case WF_F8T: return launch_wide_f8t(p, l, nblk, st);
         case WF_F8TP: return launch_wide_f8tp(p, l, nblk, st);
+        case WF_MX4T: return launch_wide_mx4t(p, l, nblk, st);
+        case WF_MX4TP: return launch_wide_mx4tp(p, l, nblk, st);
         default: return BZ_ERR_INVALID_ARG;
     }
 }
@@ -299,7 +304,7 @@ static int wide_plan(const bz_gemv_desc* d, int rows, int T, WideLaunch& l) {
     // units per wave: int4 2, or 4 over more than 20 units with more than 2
     // rows (int4 K4096 N2560 M = 5: 8 waves x 4 units 4.51 us, 16 x 2 4.74+);
     // fp8 5 over several blocks, 8 over one
-    const int per_wave = tiled_i4(wf) ? (mm > 2 && NU > 20 ? 4 : 2) : T > 1 ? 5 : 8;
+    const int per_wave = tiled_4bit(wf) ? (mm > 2 && NU > 20 ? 4 : 2) : T > 1 ? 5 : 8;
     if (!nw) nw = std::min(kStreamMaxWaves, (NU + per_wave - 1) / per_wave);
     const int need = (NU + nw - 1) / nw;
     int upw = 0;
@@ -345,7 +350,7 @@ constexpr int kWideShortK = 8192;
 static int wide_rule(const bz_gemv_desc* d, int rows) {
     const int nblk = d->N / 16, NU = tiled_units(d->wfmt, d->K);
     if (nblk > 256) return std::min(kWideMaxBlocks, (nblk + 255) / 256);
-    if (!tiled_i4(d->wfmt) && NU >= 64) return 1;
+    if (!tiled_4bit(d->wfmt) && NU >= 64) return 1;
     if (rows >= 3 && d->K <= kWideShortK && !tiled_paired(d->wfmt) && !d->gamma) {
         WideLaunch w{};
         if (wide_plan(d, rows, 1, w) == BZ_OK) return 1;
@@ -542,7 +547,7 @@ static int panel_plan(const bz_gemv_desc* d, int rows, PanelLaunch& l, int slice
     if (d->cfg_slices < 0) return BZ_ERR_INVALID_ARG;
     int nsl = slices ? slices : d->cfg_slices;
     const int slice_blocks =
-        std::max(1, std::min(tiled_i4(wf) ? kPanelSliceBlocksI4 : kPanelSliceBlocksF8, nblk / kPanelSliceBlockRows));
+        std::max(1, std::min(tiled_4bit(wf) ? kPanelSliceBlocksI4 : kPanelSliceBlocksF8, nblk / kPanelSliceBlockRows));
     const int slice_groups = (nblk + slice_blocks - 1) / slice_blocks;
     const bool rule_slices = !nsl && d->K >= kPanelSliceMinK &&
                              ((int64_t)rows * d->K * 2 > kPanelSliceX || nblk < kPanelSliceFewBlocks) &&
@@ -634,7 +639,9 @@ static int gemv_panel_rows(const bz_gemv_desc* d, hipStream_t st) {
         p.x = static_cast<const uint16_t*>(d->x) + (int64_t)m0 * d->ldx;
         p.out = static_cast<uint8_t*>(d->out) + (int64_t)m0 * d->ldo * osz;
         p.res = d->residual ? static_cast<const uint8_t*>(d->residual) + (int64_t)m0 * d->ldr * rsz : nullptr;
-        const int lrc = d->wfmt == WF_I4T ? launch_panel_i4t(p, q, st) : launch_panel_f8t(p, q, st);
+        const int lrc = d->wfmt == WF_I4T    ? launch_panel_i4t(p, q, st)
+                        : d->wfmt == WF_MX4T ? launch_panel_mx4t(p, q, st)
+                                             : launch_panel_f8t(p, q, st);
         if (lrc != BZ_OK) return lrc;
     }
     return BZ_OK;

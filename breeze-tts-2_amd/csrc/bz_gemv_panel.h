@@ -51,6 +51,8 @@
 //       sum_k x_k w_k = s_n D + (z_n - 136 s_n) X,   D = sum_k x_k (128 + q_k),
 //     with X = sum of x over the unit's 128 k, from an MFMA with A = ones
 //     (the same D placement: every element of a lane holds its row's X).
+//   * MXFP4: gfx950's scaled conversion of the lane's dword d gives MFMA d its
+//     exact bf16 weights, the block's scale in them (bz_gemv_stream.h).
 //   * fp8: gfx950's exact OCP e4m3 -> bf16 conversion of codes 0-7 and 8-15
 //     gives the A operands of two MFMAs; the accumulator runs over all units
 //     and the row scale multiplies the finished sum.
@@ -142,9 +144,9 @@ __global__ void __launch_bounds__(T == 1 ? 1024 : 512) gemv_panel(const uint8_t*
     p.nblk = hnblk;
     p.nsl = hnsl;
     p.ups = hups;
-    constexpr bool I4 = tiled_i4(WF);
-    constexpr int D = panel_depth(I4, MT, T, UPW);
-    constexpr int NX = I4 ? 4 : 2;     // x pieces (16 bytes) per unit and row half
+    constexpr bool I4 = tiled_i4(WF), MX = tiled_mx(WF), F8 = !I4 && !MX;
+    constexpr int D = panel_depth(!F8, MT, T, UPW);
+    constexpr int NX = F8 ? 2 : 4;     // x pieces (16 bytes) per unit and row half
     constexpr int UK = tiled_unit_k(WF);
     const int nthr = blockDim.x, NW = nthr >> 6;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -174,8 +176,9 @@ __global__ void __launch_bounds__(T == 1 ? 1024 : 512) gemv_panel(const uint8_t*
     // (int4 K2560 N20480 M = 32 14.5 -> 14.2 us; with one row half, M = 8 /
     // 16, about 1 us slower, where each quad reads four 16-byte pieces over
     // two lines of its row instead of one 64-byte run).
-    constexpr bool XT = I4 && MT == 2;
-    const int kx = I4 ? (XT ? 32 * qb : 8 * qb) : 16 * (qb & 1) + 8 * (qb >> 1);
+    // MXFP4 always does: the scale belongs to the lane's own block of 32 k.
+    constexpr bool XT = MX || (I4 && MT == 2);
+    const int kx = !F8 ? (XT ? 32 * qb : 8 * qb) : 16 * (qb & 1) + 8 * (qb >> 1);
     constexpr uint32_t kXStep = XT ? 16u : 64u;  // bytes between a lane's pieces d
     const uint32_t xbytes = (uint32_t)(((int64_t)(M - 1) * p.ldx + p.K) * 2);
     constexpr uint32_t kXOob = 0x80000000u;
@@ -197,13 +200,15 @@ __global__ void __launch_bounds__(T == 1 ? 1024 : 512) gemv_panel(const uint8_t*
         const bool live = blk0 + t < p.nblk;
         const uint8_t* chunk = p.w + (int64_t)(live ? blk0 + t : 0) * p.chunk;
         wrs[t] = buffer_rsrc(chunk, live ? (uint32_t)ue * 1024u : 0u);
-        srs[t] = buffer_rsrc(chunk + (int64_t)NU * 1024, live && I4 ? (uint32_t)ue * 64u : 0u);
+        srs[t] = buffer_rsrc(chunk + (int64_t)NU * 1024,
+                             live && I4 ? (uint32_t)ue * 64u : live && MX ? (uint32_t)mx_scale_bytes(ue) : 0u);
     }
-    const uint32_t wlane = j * 64 + kq * 16, slane = kq * 16;
+    const uint32_t wlane = tiled_lane_byte(WF, lane), slane = kq * 16;
 
     u32x4 xv[UPW][MT][NX];
     u32x4 wv[UPW][T];
-    u32x4 sv[UPW][T];
+    u32x4 sv[UPW][T];      // int4
+    uint32_t mv[UPW][T];   // MXFP4
     auto issue = [&](int q) {
         const int u = u0 + q;
         const uint32_t ux = (uint32_t)u * UK * 2;
@@ -218,6 +223,10 @@ __global__ void __launch_bounds__(T == 1 ? 1024 : 512) gemv_panel(const uint8_t*
         if (I4) {
 #pragma unroll
             for (int t = 0; t < T; ++t) sv[q][t] = buffer_ld16(srs[t], (uint32_t)u * 64u + slane);
+        }
+        if (MX) {
+#pragma unroll
+            for (int t = 0; t < T; ++t) mv[q][t] = buffer_ld4(srs[t], mx_scale_offset(u, lane));
         }
     };
 #pragma unroll
@@ -284,6 +293,31 @@ __global__ void __launch_bounds__(T == 1 ? 1024 : 512) gemv_panel(const uint8_t*
                         acc[t][mt][r] = fmaf(sc, dv[r], fmaf(zp, xs[mt][r], acc[t][mt][r]));
                     }
                 }
+            }
+        } else if (MX) {
+            u32x4 xp[MT][4], wr[T];
+            float s[T];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) xp[mt][d] = xmove(xv[q][mt][d]);
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                wr[t] = wv[q][t];
+                s[t] = mx_scale(mv[q][t], u0 + q);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // as for int4
+            if (next) issue(q + D);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                u32x4 bq[4];
+#pragma unroll
+                for (int d = 0; d < 4; ++d) bq[d] = mx4_weights(wr[t][d], s[t]);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) acc[t][mt] = mfma_bf16(bq[d], xp[mt][d], acc[t][mt]);
             }
         } else {
             u32x4 b0[T], b1[T];
@@ -363,7 +397,7 @@ __global__ void __launch_bounds__(T == 1 ? 1024 : 512) gemv_panel(const uint8_t*
                                    : bf16_to_f32(reinterpret_cast<const uint16_t*>(p.res)[ri + q]);
         }
         e.sc = f32x4_t{1.0f, 1.0f, 1.0f, 1.0f};
-        if (!I4)
+        if (F8)
             e.sc = *reinterpret_cast<const f32x4_t*>(p.w + (int64_t)(blk0 + t) * p.chunk + (int64_t)NU * 1024 + n * 4);
         return e;
     };
@@ -372,7 +406,7 @@ __global__ void __launch_bounds__(T == 1 ? 1024 : 512) gemv_panel(const uint8_t*
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             float v = a[q];
-            if (!I4) v *= e.sc[q];
+            if (F8) v *= e.sc[q];
             if (p.epi == BZ_EPI_RESIDUAL) v += e.r[q];
             if (p.out_f32)
                 reinterpret_cast<float*>(p.out)[oi + q] = v;
@@ -499,5 +533,6 @@ int launch_panel_wf(const PanelParams& p, const PanelLaunch& l, hipStream_t st) 
 // One instantiation set per unpaired tiled format (bz_gemv_panel_<fmt>.hip).
 int launch_panel_i4t(const PanelParams& p, const PanelLaunch& l, hipStream_t st);
 int launch_panel_f8t(const PanelParams& p, const PanelLaunch& l, hipStream_t st);
+int launch_panel_mx4t(const PanelParams& p, const PanelLaunch& l, hipStream_t st);
 
 }  // namespace bz

@@ -59,11 +59,17 @@
 //   * fp8: gfx950's OCP e4m3 -> bf16 conversion (exact) of codes 0-7 and 8-15
 //     gives the B operands of two MFMAs; x is staged in natural order.  The
 //     accumulator runs over all units; the row scale is applied at the end.
+//   * MXFP4: tiles lie in lane order (piece g of row r at byte 16 (16 g + r));
+//     a piece is one block of 32 k with its own scale 2^e.  The conversion
+//     v_cvt_scalef32_pk_bf16_fp4 multiplies by the scale, so dword d gives the
+//     bf16 weights (exact) of MFMA d in natural order and nothing is left for
+//     the sums.  Four consecutive units' scale codes of a lane are one dword.
 //   * RMSNorm is folded as in the row-major paths: LDS holds u = bf16(gamma x)
 //     and the per-row 1/rms multiplies the finished dot products.
 #pragma once
 
 #include "bz_gemv_i8.h"
+#include "bz_mx_device.h"
 
 namespace bz {
 
@@ -71,17 +77,28 @@ enum {
     WF_I4T = BZ_W_INT4_TILED,
     WF_I4TP = BZ_W_INT4_TILED_PAIRED,
     WF_F8T = BZ_W_FP8_TILED,
-    WF_F8TP = BZ_W_FP8_TILED_PAIRED
+    WF_F8TP = BZ_W_FP8_TILED_PAIRED,
+    WF_MX4T = BZ_W_MXFP4_TILED,
+    WF_MX4TP = BZ_W_MXFP4_TILED_PAIRED
 };
 
 __host__ __device__ constexpr bool tiled_i4(int wf) { return wf == WF_I4T || wf == WF_I4TP; }
-__host__ __device__ constexpr bool tiled_paired(int wf) { return wf == WF_I4TP || wf == WF_F8TP; }
+__host__ __device__ constexpr bool tiled_mx(int wf) { return wf == WF_MX4T || wf == WF_MX4TP; }
+__host__ __device__ constexpr bool tiled_4bit(int wf) { return tiled_i4(wf) || tiled_mx(wf); }
+__host__ __device__ constexpr bool tiled_paired(int wf) { return wf == WF_I4TP || wf == WF_F8TP || wf == WF_MX4TP; }
 
 // k per 64-byte unit, and bytes of one row block's chunk.
-__host__ __device__ constexpr int tiled_unit_k(int wf) { return tiled_i4(wf) ? 128 : 64; }
+__host__ __device__ constexpr int tiled_unit_k(int wf) { return tiled_4bit(wf) ? 128 : 64; }
 __host__ __device__ inline int64_t tiled_chunk_bytes(int wf, int NU) {
+    if (tiled_mx(wf)) return mx4_chunk_bytes(NU);
     const int64_t raw = (int64_t)NU * 1024 + (tiled_i4(wf) ? (int64_t)NU * 64 : 64);
     return (raw + 127) / 128 * 128;
+}
+
+// Byte of a tile that a lane's 16 bytes start at: row j = lane % 16, piece
+// kq = lane / 16.
+__host__ __device__ constexpr uint32_t tiled_lane_byte(int wf, int lane) {
+    return tiled_mx(wf) ? lane * 16 : (lane & 15) * 64 + (lane >> 4) * 16;
 }
 
 struct StreamParams {
@@ -166,7 +183,7 @@ __global__ void __launch_bounds__(1024) gemv_stream(const uint8_t* hw, const uin
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     stream_hot(p, hw, hx, hg, hchunk, hldx, hK, hNU, hM, hnorm);
     p.x_lead = hlead;
-    constexpr bool I4 = tiled_i4(WF);
+    constexpr bool I4 = tiled_i4(WF), MX = tiled_mx(WF), F8 = !I4 && !MX;
     constexpr bool PAIR = tiled_paired(WF);
     constexpr int D = stream_depth(UPW);
     constexpr int BPU = tiled_unit_k(WF) / 8;   // blocks of 8 x values per unit
@@ -228,7 +245,7 @@ __global__ void __launch_bounds__(1024) gemv_stream(const uint8_t* hw, const uin
     if (p.epi == BZ_EPI_RESIDUAL && g0 < ngrp && gw == 0) resv = load_res(g0);
     const float* rsc = reinterpret_cast<const float*>(chunk + (int64_t)NU * 1024);  // fp8 row scales
     float rs0 = 1.0f, rs1 = 1.0f;
-    if (!I4 && g0 < ngrp) {
+    if (F8 && g0 < ngrp) {
         const int c = g0 % ocols;
         rs0 = rsc[c];
         if (PAIR) rs1 = rsc[c + 8];
@@ -245,8 +262,14 @@ __global__ void __launch_bounds__(1024) gemv_stream(const uint8_t* hw, const uin
 #pragma unroll
         for (int q = 0; q < UPW; ++q) sc[q] = buffer_ld4(srs, (uint32_t)(u0 + q) * 64u + j * 4);
     }
+    if (MX) {  // four units' scale codes of this lane's row and block of 32 k
+        const __amdgpu_buffer_rsrc_t srs = buffer_rsrc(chunk + (int64_t)NU * 1024, (uint32_t)mx_scale_bytes(NU));
+#pragma unroll
+        for (int q = 0; q < UPW; ++q) sc[q] = buffer_ld4(srs, mx_scale_offset(u0 + q, lane));
+    }
     u32x4 wv[UPW];
-    auto issue = [&](int q) { wv[q] = buffer_ld16_nt(wrs, (uint32_t)(u0 + q) * 1024u + j * 64 + kq * 16); };
+    const uint32_t wlane = tiled_lane_byte(WF, lane);
+    auto issue = [&](int q) { wv[q] = buffer_ld16_nt(wrs, (uint32_t)(u0 + q) * 1024u + wlane); };
     // Long rows (80 units or more) over at most 256 row blocks (at most one
     // workgroup per CU): the x loads get about 270 ns before the first tiles
     // go out, so they do not queue behind the tiles of every wave of the CU.
@@ -366,6 +389,15 @@ __global__ void __launch_bounds__(1024) gemv_stream(const uint8_t* hw, const uin
                     y[r] = fmaf(s, dv[r], fmaf(zp, X, y[r]));
                 }
             }
+        } else if (MX) {
+            const float s = mx_scale(sc[q], u0 + q);
+            u32x4 bq[4];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) bq[d] = mx4_weights(wv[q][d], s);
+            if (next) issue(q + D);
+            const uint8_t* xu = xa + (u * 128 + kq * 32) * 2;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) facc = mfma_bf16(*reinterpret_cast<const u32x4*>(xu + d * 16), bq[d], facc);
         } else {
             u32x4 b0, b1;
             b0[0] = fp8x2_bf16<false>(wv[q][0]);
@@ -418,10 +450,10 @@ __global__ void __launch_bounds__(1024) gemv_stream(const uint8_t* hw, const uin
         if (p.norm) s2 = sum16_dpp(s2);
         if (gw == 0) {
             const float inv = p.norm ? rsqrtf(s2 / (float)K + p.eps) : 1.0f;
-            const float s0 = I4 ? 1.0f : (first ? rs0 : rsc[c]);
+            const float s0 = !F8 ? 1.0f : (first ? rs0 : rsc[c]);
             float o;
             if (PAIR) {
-                const float s1 = I4 ? 1.0f : (first ? rs1 : rsc[c + 8]);
+                const float s1 = !F8 ? 1.0f : (first ? rs1 : rsc[c + 8]);
                 o = silu(a * inv * s0) * (a2 * inv * s1);
             } else {
                 o = a * inv * s0;
@@ -503,5 +535,7 @@ int launch_stream_i4t(const StreamParams& p, const StreamLaunch& l, hipStream_t 
 int launch_stream_i4tp(const StreamParams& p, const StreamLaunch& l, hipStream_t st);
 int launch_stream_f8t(const StreamParams& p, const StreamLaunch& l, hipStream_t st);
 int launch_stream_f8tp(const StreamParams& p, const StreamLaunch& l, hipStream_t st);
+int launch_stream_mx4t(const StreamParams& p, const StreamLaunch& l, hipStream_t st);
+int launch_stream_mx4tp(const StreamParams& p, const StreamLaunch& l, hipStream_t st);
 
 }  // namespace bz

@@ -54,12 +54,12 @@ __host__ __device__ inline WideLds wide_lds(int wf, int M, int K, int T) {
     return L;
 }
 
-// Units per wave the wide kernel is instantiated for (int4 up to 5 over one
+// Units per wave the wide kernel is instantiated for (4 bits up to 5 over one
 // or two rows of x and up to 4 over more: beyond that the two tile sets and
 // the accumulators do not fit the 128 registers of a 16-wave workgroup
 // without spilling), and the most row blocks of one workgroup.
 constexpr int kWideUpw[] = {2, 3, 4, 5, 6, 8, 10};
-__host__ __device__ constexpr int wide_max_upw(int wf, int mm) { return tiled_i4(wf) ? (mm <= 2 ? 5 : 4) : 10; }
+__host__ __device__ constexpr int wide_max_upw(int wf, int mm) { return tiled_4bit(wf) ? (mm <= 2 ? 5 : 4) : 10; }
 constexpr int kWideMaxBlocks = 8;
 
 // TC > 0: the row blocks per workgroup fixed at compile time (every
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(1024) gemv_wide(const uint8_t* hw, const uint1
                                                   StreamParams p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     stream_hot(p, hw, hx, hg, hchunk, hldx, hK, hNU, hM, hnorm);  // the preloaded arguments (bz_gemv_stream.h)
-    constexpr bool I4 = tiled_i4(WF);
+    constexpr bool I4 = tiled_i4(WF), MX = tiled_mx(WF), F8 = !I4 && !MX;
     constexpr bool PAIR = tiled_paired(WF);
     constexpr int BPU = tiled_unit_k(WF) / 8;   // blocks of 8 x values per unit
     constexpr int RK = (UPW * BPU + 63) / 64;   // rounds of blocks per lane over a wave's slice
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(1024) gemv_wide(const uint8_t* hw, const uint1
     if (g0 < nout) {
         int jb, m, c;
         out_coords(g0, jb, m, c);
-        if (!I4) {
+        if (F8) {
             rs0 = row_scale(jb, c)[0];
             if (PAIR) rs1 = row_scale(jb, c)[8];
         }
@@ -151,12 +151,14 @@ __global__ void __launch_bounds__(1024) gemv_wide(const uint8_t* hw, const uint1
     // two register sets with fixed roles (a: even blocks, b: odd blocks), so
     // no tile register is carried around the block loop (a carried one made
     // the compiler wait for every load in flight at each block)
+    const uint32_t wlane = tiled_lane_byte(WF, lane);
     u32x4 wa[UPW], wb[UPW];
     uint32_t sa[UPW], sb[UPW];
     auto issue = [&](int jb, int q, u32x4* wv, uint32_t* sc) {  // unit q of block jb into slot q
         const bool ok = jb < nb && u0 + q < NU;
         const uint32_t base = (uint32_t)(jb * p.chunk);
-        wv[q] = buffer_ld16_nt(wrs, ok ? base + (uint32_t)(u0 + q) * 1024u + j * 64 + kq * 16 : kBufferOob);
+        wv[q] = buffer_ld16_nt(wrs, ok ? base + (uint32_t)(u0 + q) * 1024u + wlane : kBufferOob);
+        if (MX) sc[q] = buffer_ld4(wrs, ok ? base + (uint32_t)NU * 1024u + mx_scale_offset(u0 + q, lane) : kBufferOob);
         if (I4) sc[q] = buffer_ld4(wrs, ok ? base + (uint32_t)NU * 1024u + (uint32_t)(u0 + q) * 64u + j * 4 : kBufferOob);
     };
     __builtin_amdgcn_sched_barrier(0);
@@ -269,6 +271,15 @@ __global__ void __launch_bounds__(1024) gemv_wide(const uint8_t* hw, const uint1
                         y[r] = fmaf(s, dv[r], fmaf(zp, X, y[r]));
                     }
                 }
+            } else if (MX) {
+                const float s = mx_scale(cs[q], u0 + q);
+                u32x4 bq[4];
+#pragma unroll
+                for (int d = 0; d < 4; ++d) bq[d] = mx4_weights(cw[q][d], s);
+                issue(jb + 1, q, nw2, ns2);
+                const uint8_t* xu = xa + (u * 128 + kq * 32) * 2;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) facc = mfma_bf16(*reinterpret_cast<const u32x4*>(xu + d * 16), bq[d], facc);
             } else {
                 u32x4 c0, c1;
                 c0[0] = fp8x2_bf16<false>(cw[q][0]);
@@ -334,11 +345,11 @@ __global__ void __launch_bounds__(1024) gemv_wide(const uint8_t* hw, const uint1
         const float* rg = red + ((jb * M + m) * 16 + c) * 16;
         const float a = wave_sum(rg);
         const float inv = p.norm ? rsqrtf(wave_sum(sq + m * 16) / (float)K + p.eps) : 1.0f;
-        const float s0 = I4 ? 1.0f : (first ? rs0 : row_scale(jb, c)[0]);
+        const float s0 = !F8 ? 1.0f : (first ? rs0 : row_scale(jb, c)[0]);
         float o;
         if (PAIR) {
             const float a2 = wave_sum(rg + 8 * 16);
-            const float s1 = I4 ? 1.0f : (first ? rs1 : row_scale(jb, c)[8]);
+            const float s1 = !F8 ? 1.0f : (first ? rs1 : row_scale(jb, c)[8]);
             o = silu(a * inv * s0) * (a2 * inv * s1);
         } else {
             o = a * inv * s0;
@@ -383,10 +394,10 @@ int launch_wide_kernel(const StreamParams& p, const WideLaunch& l, int nblk, hip
 
 template <int WF, int MM>
 int launch_wide_upw(const StreamParams& p, const WideLaunch& l, int nblk, hipStream_t st) {
-    // the int4 decode shapes with the block count fixed at compile time: 2
+    // the 4-bit decode shapes with the block count fixed at compile time: 2
     // units per wave over 5 blocks (gate|up N20480), and over 2 blocks (qkv
     // N6144) at 2 rows (at one row measured 0.02-0.03 us slower)
-    if constexpr (MM <= 2 && tiled_i4(WF)) {
+    if constexpr (MM <= 2 && tiled_4bit(WF)) {
         if (l.upw == 2 && l.T == 5 && nblk % 5 == 0) return launch_wide_kernel<WF, MM, 2, 5>(p, l, nblk, st);
         if constexpr (MM == 2)
             if (l.upw == 2 && l.T == 2 && nblk % 2 == 0) return launch_wide_kernel<WF, MM, 2, 2>(p, l, nblk, st);
@@ -427,5 +438,7 @@ int launch_wide_i4t(const StreamParams& p, const WideLaunch& l, int nblk, hipStr
 int launch_wide_i4tp(const StreamParams& p, const WideLaunch& l, int nblk, hipStream_t st);
 int launch_wide_f8t(const StreamParams& p, const WideLaunch& l, int nblk, hipStream_t st);
 int launch_wide_f8tp(const StreamParams& p, const WideLaunch& l, int nblk, hipStream_t st);
+int launch_wide_mx4t(const StreamParams& p, const WideLaunch& l, int nblk, hipStream_t st);
+int launch_wide_mx4tp(const StreamParams& p, const WideLaunch& l, int nblk, hipStream_t st);
 
 }  // namespace bz

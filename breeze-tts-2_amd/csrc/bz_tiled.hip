@@ -14,7 +14,9 @@
 
 namespace bz {
 
-bool is_tiled(int wf) { return wf == WF_I4T || wf == WF_I4TP || wf == WF_F8T || wf == WF_F8TP; }
+bool is_tiled(int wf) {
+    return wf == WF_I4T || wf == WF_I4TP || wf == WF_F8T || wf == WF_F8TP || wf == WF_MX4T || wf == WF_MX4TP;
+}
 
 // Units per row of a tiled weight, or 0 when K cannot be tiled.
 int tiled_units(int wf, int K) {
@@ -68,6 +70,31 @@ __global__ void pack_tiled_kernel(int src_wf, const uint8_t* src, const void* sc
     }
 }
 
+// The same for MXFP4: 16-byte pieces are one block of 32 k each, in lane
+// order; codes and scales row-major (BZ_W_MXFP4) or an unpaired tiled weight.
+__global__ void pack_mx4_kernel(bool src_tiled, const uint8_t* src, const uint8_t* sc0, int n, int K, bool paired,
+                                uint8_t* dst, int N, int row0, int NU) {
+    const int64_t chunk = mx4_chunk_bytes(NU);
+    const int64_t total = (int64_t)n * NU;
+    for (int64_t idx = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; idx < total;
+         idx += (int64_t)gridDim.x * blockDim.x) {
+        const int rs = (int)(idx / NU), u = (int)(idx % NU);
+        int blk, tr;
+        tiled_row_pos(paired, N, row0 + rs, blk, tr);
+        const uint8_t* sb = src + (rs >> 4) * chunk;
+        uint8_t* cb = dst + blk * chunk;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int ls = 16 * q + (rs & 15), ld = 16 * q + tr;
+            *reinterpret_cast<u32x4*>(cb + (int64_t)u * 1024 + ld * 16) =
+                ldg16(src_tiled ? sb + (int64_t)u * 1024 + ls * 16 : src + (int64_t)rs * (K / 2) + u * 64 + q * 16);
+            cb[(int64_t)NU * 1024 + mx_scale_offset(u, ld) + (u & 3)] =
+                src_tiled ? sb[(int64_t)NU * 1024 + mx_scale_offset(u, ls) + (u & 3)]
+                          : sc0[(int64_t)rs * (K / 32) + u * 4 + q];
+        }
+    }
+}
+
 // One thread per (logical row, unit, 16-byte piece of the unit).
 __global__ void dequant_tiled_kernel(int wf, const uint8_t* w, int N, int K, int NU, int64_t chunk, float* out) {
     const bool i4 = tiled_i4(wf), paired = tiled_paired(wf);
@@ -79,9 +106,21 @@ __global__ void dequant_tiled_kernel(int wf, const uint8_t* w, int N, int K, int
     int blk, tr;
     tiled_row_pos(paired, N, r, blk, tr);
     const uint8_t* cb = w + blk * chunk;
-    const u32x4 q = ldg16(cb + (int64_t)u * 1024 + tr * 64 + kq * 16);
+    const u32x4 q = ldg16(cb + (int64_t)u * 1024 + tiled_lane_byte(wf, 16 * kq + tr));
     float* o = out + (int64_t)r * K;
-    if (i4) {
+    if (tiled_mx(wf)) {
+        const uint32_t sc = *reinterpret_cast<const uint32_t*>(cb + (int64_t)NU * 1024 + mx_scale_offset(u, 16 * kq + tr));
+        o += u * 128 + kq * 32;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const u32x4 b = mx4_weights(q[d], mx_scale(sc, u));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                o[8 * d + 2 * e] = bf16_lo(b[e]);
+                o[8 * d + 2 * e + 1] = bf16_hi(b[e]);
+            }
+        }
+    } else if (i4) {
         const int k0 = u * 128 + kq * 32;
         const uint32_t sz = *reinterpret_cast<const uint32_t*>(cb + (int64_t)NU * 1024 + u * 64 + tr * 4);
         const float s = bf16_lo(sz), zp = bf16_hi(sz);
@@ -134,18 +173,24 @@ extern "C" int bz_pack_tiled(int32_t src_wfmt, const void* src_w, const void* sr
                              int32_t group, int32_t dst_wfmt, void* dst, int32_t N, int32_t row0, void* stream) {
     if (!src_w || !dst || n < 1 || K < 1 || N < 1 || row0 < 0) return BZ_ERR_INVALID_ARG;
     if (!is_tiled(dst_wfmt)) return BZ_ERR_INVALID_ARG;
-    const bool i4 = tiled_i4(dst_wfmt);
-    const bool src_tiled = src_wfmt == (i4 ? BZ_W_INT4_TILED : BZ_W_FP8_TILED);
-    if (src_wfmt != (i4 ? BZ_W_INT4_ZP : BZ_W_FP8) && !src_tiled) return BZ_ERR_INVALID_ARG;
+    const bool i4 = tiled_i4(dst_wfmt), mx = tiled_mx(dst_wfmt);
+    const bool src_tiled = src_wfmt == (i4 ? BZ_W_INT4_TILED : mx ? BZ_W_MXFP4_TILED : BZ_W_FP8_TILED);
+    if (src_wfmt != (i4 ? BZ_W_INT4_ZP : mx ? BZ_W_MXFP4 : BZ_W_FP8) && !src_tiled) return BZ_ERR_INVALID_ARG;
     if (!src_tiled && !src_sc0) return BZ_ERR_INVALID_ARG;
     if ((int64_t)row0 + n > N) return BZ_ERR_INVALID_ARG;
     const int NU = tiled_units(dst_wfmt, K);
     if (!NU || N % 16 || (src_tiled && n % 16) || (i4 && group != 128)) return BZ_ERR_SHAPE;
     if ((reinterpret_cast<uintptr_t>(src_w) & 15) || (reinterpret_cast<uintptr_t>(dst) & 15) ||
-        (!src_tiled && (reinterpret_cast<uintptr_t>(src_sc0) & 3)))
+        (!src_tiled && !mx && (reinterpret_cast<uintptr_t>(src_sc0) & 3)))
         return BZ_ERR_ALIGNMENT;
     const int64_t total = (int64_t)n * NU;
     const unsigned grid = (unsigned)std::min<int64_t>((total + 255) / 256, 65535);
+    if (mx) {
+        hipLaunchKernelGGL(pack_mx4_kernel, dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream), src_tiled,
+                           static_cast<const uint8_t*>(src_w), static_cast<const uint8_t*>(src_sc0), n, K,
+                           tiled_paired(dst_wfmt), static_cast<uint8_t*>(dst), N, row0, NU);
+        return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
+    }
     hipLaunchKernelGGL(pack_tiled_kernel, dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream), src_wfmt,
                        static_cast<const uint8_t*>(src_w), src_sc0, n, K, dst_wfmt, static_cast<uint8_t*>(dst), N,
                        row0, NU, tiled_chunk_bytes(dst_wfmt, NU), tiled_chunk_bytes(src_wfmt, NU));

@@ -76,10 +76,19 @@ typedef enum bz_status {
  *   8b .. 8b+7 then up rows 8b .. 8b+7 (logical rows 8b+r and N/2+8b+r), so a
  *   block finishes 8 outputs silu(g) * u.  Only valid with BZ_EPI_SILU_GATE;
  *   the unpaired tiled formats do not take that epilogue.
+ * BZ_W_MXFP4    : microscaled 4-bit floating point (bz_mx.h): w uint8
+ *                [N][K/2] e2m1 codes, even k in the low nibble; sc0 = uint8
+ *                [N][K/32] scale codes, w_eff = element * 2^(code - 127).
+ * BZ_W_MXFP4_TILED, _PAIRED: the same blocks of 16 rows, units of 128 k; a
+ *   tile of 1024 bytes holds the four 32-k blocks of its 16 rows block by
+ *   block (block g of row r at byte 256 g + 16 r), and the scales follow the
+ *   tiles, per four units 256 bytes (unit u, block g, row r at byte 64 g +
+ *   4 r + u % 4).  Runs on paths 5 and 6; w_eff is exact in bf16, so the
+ *   products equal those of the bf16 weight.
  * The tiled formats run on GEMV path 5, the streaming kernel (M <= 8 rows
  * per launch; more rows run as several launches), and the unpaired ones also
- * on the several-row paths 4 and 6 (see below).  They need K % 128 == 0
- * (int4) or K % 64 == 0 (fp8); int4 group must be 128.
+ * on the several-row paths 4 (int4, fp8) and 6 (see below).  They need K %
+ * 128 == 0 (int4, MXFP4) or K % 64 == 0 (fp8); int4 group must be 128.
  */
 typedef enum bz_wfmt {
     BZ_W_INT4_ZP = 0,
@@ -89,7 +98,10 @@ typedef enum bz_wfmt {
     BZ_W_INT4_TILED = 4,
     BZ_W_INT4_TILED_PAIRED = 5,
     BZ_W_FP8_TILED = 6,
-    BZ_W_FP8_TILED_PAIRED = 7
+    BZ_W_FP8_TILED_PAIRED = 7,
+    BZ_W_MXFP4 = 8,              /* source of bz_pack_tiled and bz_dequant only */
+    BZ_W_MXFP4_TILED = 10,       /* (9 is no format) */
+    BZ_W_MXFP4_TILED_PAIRED = 11
 } bz_wfmt;
 
 /* Epilogues of models/fused/kernels.py:8-13 (EPI 0/1/2). */
@@ -149,7 +161,7 @@ typedef enum bz_dtype {
  *
  * Several rows over the tiled formats (path 6, the panel kernel).  Up to 32
  * rows of x per launch against an unpaired tiled int4 or fp8 weight
- * (BZ_W_INT4_TILED, BZ_W_FP8_TILED), no RMSNorm, epilogue NONE or RESIDUAL,
+ * (BZ_W_INT4_TILED, BZ_W_FP8_TILED, BZ_W_MXFP4_TILED), no RMSNorm, epilogue NONE or RESIDUAL,
  * no second store: each workgroup of cfg_waves waves (0: about 5 units per
  * wave; at most 16, or 8 with several blocks) covers cfg_tiles consecutive
  * 16-row blocks (1..5; 0: enough to keep about 256 workgroups, or with K
@@ -225,7 +237,8 @@ size_t bz_gemv_workspace(const bz_gemv_desc* d);
 int bz_gemv(const bz_gemv_desc* d, void* stream);
 
 /* Prefill GEMM: out[M][N] = x[M][K] @ w_eff^T for prompt-sized M over an
- * unpaired tiled weight (BZ_W_INT4_TILED, group 128, or BZ_W_FP8_TILED); x
+ * unpaired tiled weight (BZ_W_INT4_TILED, group 128, BZ_W_FP8_TILED or
+ * BZ_W_MXFP4_TILED); x
  * bf16 with 16-byte aligned rows (ldx >= K), out bf16 or fp32 (ldo >= N),
  * fp32 accumulation.  Replaces torch._weight_int4pack_mm and
  * torch._scaled_mm (weight-only form) for the rows of a prompt
@@ -312,7 +325,7 @@ int bz_quantize_fp8(const void* w, int32_t w_dtype, int32_t N, int32_t K,
 
 /* Bytes of a tiled weight (wfmt one of the BZ_W_*_TILED formats) of N rows
  * and K columns; 0 when the shape cannot be tiled (N % 16, or K not a
- * multiple of the unit's 128 (int4) / 64 (fp8) values). */
+ * multiple of the unit's 128 (int4, MXFP4) / 64 (fp8) values). */
 size_t bz_tiled_bytes(int32_t wfmt, int32_t N, int32_t K);
 
 /* Write logical rows [row0, row0 + n) of a tiled weight of N rows (dst,
@@ -320,7 +333,8 @@ size_t bz_tiled_bytes(int32_t wfmt, int32_t N, int32_t K);
  * rows: row-major BZ_W_INT4_ZP (group 128; src_sc0 = scales_zeros bf16
  * [K/128][n][2]) or BZ_W_INT4_TILED (n % 16 == 0, src_sc0 unused) for the
  * int4 tiled formats; BZ_W_FP8 (src_sc0 = float [n] row scales) or
- * BZ_W_FP8_TILED for the fp8 ones.  For the paired formats logical row r < N/2 is
+ * BZ_W_FP8_TILED for the fp8 ones; BZ_W_MXFP4 (src_sc0 = uint8 [n][K/32]) or
+ * BZ_W_MXFP4_TILED for the MXFP4 ones.  For the paired formats logical row r < N/2 is
  * gate row r and r >= N/2 up row r - N/2, so [gate; up] is packed by one call
  * over all N rows or by one call per half (row0 = 0, row0 = N/2).  Load-time
  * work with no counterpart in the reference: it replaces the repack step of

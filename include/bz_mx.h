@@ -1,0 +1,75 @@
+/*
+ * bz_mx.h -- C ABI of the operators over microscaled (MX) blocks: quantising
+ * rows to them, reading them back, and products of rows quantised that way
+ * with a 4-bit microscaled weight.  The products of bf16 rows with such a
+ * weight are bz_gemv and bz_gemm_tiled (bz_gemv.h, BZ_W_MXFP4_TILED).  No
+ * counterpart in the reference, whose weights are int4 or fp8
+ * (models/int4_linear.py, models/fp8_linear.py).
+ *
+ * A block is 32 consecutive columns of a row: elements of a narrow
+ * floating-point type and one scale code c (a byte) that stands for
+ * 2^(c - 127).  With a the largest magnitude of the block,
+ *   c = max(floor(log2 a) - emax, -126) + 127   (a = 0: 1),
+ *   element = value / 2^(c - 127) rounded to the nearest (ties to the even
+ *   code), magnitudes above the type's largest to the largest.
+ * A block with a NaN or an infinity gets c = 255 and reads back as NaN; its
+ * elements mean nothing.
+ *   BZ_MX_E2M1  4 bits, emax 2, largest 6; two to a byte, the even column in
+ *               the low half;
+ *   BZ_MX_E4M3  8 bits (OCP FP8 E4M3), emax 8, largest 448.
+ *
+ * Conventions as in bz_gemv.h: device pointers, nothing is allocated or
+ * synchronised, errors are returned before any launch.
+ */
+#ifndef BZ_MX_H
+#define BZ_MX_H
+
+#include "bz_gemv.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+typedef enum bz_mx_elem { BZ_MX_E2M1 = 0, BZ_MX_E4M3 = 1 } bz_mx_elem;
+
+/* x types of bz_mx_quantize beside BZ_DT_BF16 and BZ_DT_F32. */
+#define BZ_MX_F16 2
+
+/* Layouts of quantised rows.
+ * BZ_MX_ROWS : codes uint8 [M][K/2] (e2m1) or [M][K] (e4m3), scales uint8
+ *              [M][K/32]; K % 32 == 0.  With e2m1 this is the weight format
+ *              BZ_W_MXFP4.
+ * BZ_MX_TILED: the operand order of the matrix cores (bz_mx_device.h), in one
+ *              buffer of bz_mx_rows_bytes bytes with the rows rounded up to 16
+ *              (the added rows hold zeros); K % 128 == 0.  With e2m1 it is
+ *              the weight format BZ_W_MXFP4_TILED.  scales is NULL. */
+typedef enum bz_mx_layout { BZ_MX_ROWS = 0, BZ_MX_TILED = 1 } bz_mx_layout;
+
+/* Bytes of BZ_MX_TILED rows, 0 when K % 128 or a size is not positive. */
+size_t bz_mx_rows_bytes(int32_t elem, int32_t M, int32_t K);
+
+/* Quantise x [M][ldx] (bf16, fp32 or fp16; K columns, ldx >= K; any ldx and
+ * any alignment of the type's own size).  codes is 16-byte aligned for
+ * BZ_MX_TILED, 4-byte aligned for BZ_MX_ROWS. */
+int bz_mx_quantize(const void* x, int32_t x_dtype, int64_t ldx, int32_t M, int32_t K, int32_t elem, int32_t layout,
+                   void* codes, void* scales, void* stream);
+
+/* Read BZ_MX_ROWS back: out [M][ldo] bf16 or fp32 (exact but where a bf16
+ * cannot hold a value below 2^-126 or above its range).  codes 4-byte
+ * aligned; any alignment of out. */
+int bz_mx_dequantize(const void* codes, const void* scales, int32_t elem, int32_t M, int32_t K, void* out,
+                     int32_t out_dtype, int64_t ldo, void* stream);
+
+/* out[M][N] = q(x) @ w_eff^T (+ residual): x already quantised, BZ_MX_TILED
+ * rows of `elem`; w a BZ_W_MXFP4_TILED weight of N rows; products and sums on
+ * the block-scaled matrix instructions, fp32 accumulation.  residual (bf16
+ * or fp32, [M][ldr], may alias out) is added when not NULL.  out is bf16 or
+ * fp32 [M][ldo]. */
+int bz_mx_gemm(int32_t elem, const void* xq, int32_t M, const void* w, int32_t N, int32_t K, const void* residual,
+               int32_t residual_dtype, int64_t ldr, void* out, int32_t out_dtype, int64_t ldo, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* BZ_MX_H */

@@ -1,0 +1,558 @@
+"""Operators over microscaled blocks on the GPU, against the oracle in 64 bits."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+from torch import nn
+
+from oracle import bz_mx_oracle as O
+from tests._util import bf16_tensor
+
+from breeze_amd import _lib as L
+from breeze_amd import gemv as G
+from breeze_amd import mx
+from breeze_amd import mxfp4_linear as M4
+from breeze_amd import quantized_checkpoint as Q
+from breeze_amd.fused import kernels as FK
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+ELEMS = [O.E2M1, O.E4M3]
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _rows(m, k, seed=0, dtype=BF16, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g) * torch.exp(spread * torch.randn(k, generator=g))
+    return x.to(dtype).cuda()
+
+
+def _codes(codes, elem):
+    """The GPU's codes as one element code a byte."""
+    c = codes.view(torch.uint8).cpu().numpy()
+    return np.stack([c & 15, c >> 4], -1).reshape(c.shape[0], -1) if elem == O.E2M1 else c
+
+
+class Weight:
+    """A random e2m1 weight: oracle codes, values and the GPU's buffers."""
+
+    def __init__(self, n, k, seed=0, paired=False):
+        rng = np.random.default_rng(seed + n + k)
+        w = rng.standard_normal((n, k)) * k ** -0.5 * np.exp(rng.standard_normal((n, 1)))
+        self.n, self.k = n, k
+        self.codes, self.scales = O.quantize(w, O.E2M1)
+        self.values = O.values(self.codes, self.scales, O.E2M1)
+        self.rows = torch.from_numpy(O.pack_nibbles(self.codes)).cuda()
+        self.sc = torch.from_numpy(self.scales).cuda()
+        self.fmt = G.W_MXFP4_TILED_PAIRED if paired else G.W_MXFP4_TILED
+        self.tiled = torch.from_numpy(O.tile(self.codes, self.scales, O.E2M1, paired)).cuda()
+
+
+def _bound(x, w, ref, k, out_dtype=BF16, before=0.0, extra=0.0):
+    """Rounding of the output, and of K fp32 additions (2^-24 of the sum of
+    magnitudes each); before: relative error of the product before the
+    epilogue, extra: absolute."""
+    total = np.abs(x) @ np.abs(w).T
+    return torch.finfo(out_dtype).eps / 2 * (np.abs(ref) + extra) + (k * 2.0 ** -24 + before) * total + extra
+
+
+def _close(out, ref, bound):
+    err = np.abs(_np(out) - ref)
+    assert (err <= bound).all(), (err / np.maximum(bound, 1e-300)).max()
+
+
+# ---- quantising and reading back ---------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("m,k", [(1, 32), (3, 96), (17, 160), (2, 2560), (301, 672)])
+def test_quantize(elem, dtype, m, k):
+    x = _rows(m, k, 1, dtype, 2.0)
+    codes, scales = mx.quantize_mx(x, elem)
+    want, want_s = O.quantize(_np(x), elem)
+    assert (_codes(codes, elem) == want).all() and (scales.cpu().numpy() == want_s).all()
+    for dt in (BF16, F32):
+        got = mx.dequantize_mx(codes, scales, elem, dt)
+        assert got.dtype == dt and (_np(got) == O.values(want, want_s, elem)).all()
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_quantize_strides_and_alignment(elem, dtype):
+    base = _rows(9, 700, 2, dtype)
+    views = [base[:, 1:577], base[:, 8:584], base[::2, 3:35], base.t()[:96, :5].t(), base[4:5].expand(6, 700)[:, :32],
+             base.view(-1)[1:1 + 640].view(5, 128)]
+    for x in views:
+        codes, scales = mx.quantize_mx(x, elem)
+        want, want_s = O.quantize(_np(x), elem)
+        assert (_codes(codes, elem) == want).all() and (scales.cpu().numpy() == want_s).all()
+    x = views[1][:, :512]
+    got, (c, s) = mx.mx_rows(x, elem), O.quantize(_np(x), elem)
+    assert (got.data.cpu().numpy() == O.tile(c, s, elem)).all()
+    x = views[0][:, :512]  # rows at odd addresses
+    got, (c, s) = mx.mx_rows(x, elem), O.quantize(_np(x), elem)
+    assert (got.data.cpu().numpy() == O.tile(c, s, elem)).all()
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+def test_every_bf16_value_rounds_to_nearest_even(elem):
+    """Each magnitude in a block of its own beside the block's largest."""
+    bits = np.arange(0x7F80, dtype=np.uint16)
+    for top in (0x4000, 0x3F80, 0x0080, 0x0001, 0x7F7F, 0x3FC0):
+        x = np.zeros((bits.size, 32), np.uint16)
+        x[:, 0], x[:, 1], x[:, 2] = top, bits, bits | 0x8000
+        x = bf16_tensor(x)
+        codes, scales = mx.quantize_mx(x, elem)
+        want, want_s = O.quantize(_np(x), elem)
+        assert (_codes(codes, elem) == want).all() and (scales.cpu().numpy() == want_s).all()
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_blocks_with_nan_infinity_zero_and_the_extremes(elem, dtype):
+    fi = torch.finfo(dtype)
+    x = torch.zeros(8, 256, dtype=dtype)
+    x[0, 5], x[1, 37], x[2, 64], x[3, 255] = float("nan"), float("inf"), -float("inf"), -float("nan")
+    x[4] = -0.0
+    x[5, :64], x[5, 64:] = fi.max, -fi.max
+    x[6, ::3], x[6, 1::3] = fi.tiny, -fi.tiny / 4
+    x[7] = torch.randn(256).to(dtype)
+    x[0, 64:], x[1, :32] = 1.5, 2.5
+    x = x.cuda()
+    codes, scales = mx.quantize_mx(x, elem)
+    want, want_s = O.quantize(_np(x), elem)
+    assert (scales.cpu().numpy() == want_s).all()
+    keep = np.repeat(want_s != 255, 32, -1)
+    assert (_codes(codes, elem) == want)[keep].all()
+    assert [(want_s[i] == 255).sum() for i in range(8)] == [1, 1, 1, 1, 0, 0, 0, 0]
+    for dt in (BF16, F32):
+        got = _np(mx.dequantize_mx(codes, scales, elem, dt))
+        assert (np.isnan(got) == ~keep).all() and (got == O.values(want, want_s, elem))[keep].all()
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+def test_read_back_every_code_and_scale(elem):
+    n = 16 if elem == O.E2M1 else 256
+    codes = np.tile(np.arange(n, dtype=np.uint8), (256, 256 // n))
+    scales = np.repeat(np.arange(256, dtype=np.uint8)[:, None], 8, 1)
+    want = O.values(codes, scales, elem)
+    if elem == O.E4M3:
+        want[:, [127, 255]] = np.nan  # the type's own NaN
+    dev = torch.from_numpy(O.pack_nibbles(codes) if elem == O.E2M1 else codes).cuda()
+    got = mx.dequantize_mx(dev, torch.from_numpy(scales).cuda(), elem, F32)
+    with np.errstate(over="ignore"):
+        assert np.array_equal(_np(got), want.astype(np.float32).astype(np.float64), equal_nan=True)
+    got = mx.dequantize_mx(dev, torch.from_numpy(scales).cuda(), elem)
+    fits = torch.from_numpy(want).to(BF16)  # exact but below 2^-126 and above the range
+    assert torch.equal(torch.nan_to_num(got.cpu().float(), nan=7e37), torch.nan_to_num(fits.float(), nan=7e37))
+
+
+def test_read_back_of_other_layouts():
+    x = _rows(6, 128, 3)
+    codes, scales = mx.quantize_mx(x)
+    want = mx.dequantize_mx(codes, scales)
+    buf = torch.zeros(6 * 64 + 1, dtype=torch.uint8, device="cuda")
+    buf[1:].view(6, 64).copy_(codes)
+    assert torch.equal(mx.dequantize_mx(buf[1:].view(6, 64), scales.t().contiguous().t()), want)
+    assert torch.equal(mx.dequantize_mx(codes[::2], scales[::2]), want[::2])
+    with pytest.raises(ValueError, match="not those of"):
+        mx.dequantize_mx(codes, scales[:, :3])
+    with pytest.raises(ValueError, match="not those of"):
+        mx.dequantize_mx(codes, scales, "e4m3")
+    with pytest.raises(TypeError, match="bfloat16 or float32"):
+        mx.dequantize_mx(codes, scales, dtype=F16)
+
+
+def test_quantize_refusals_and_no_rows():
+    x = _rows(4, 128)
+    for bad, err in ((x[:, :40], ValueError), (x[:, :0], ValueError), (x[0], ValueError), (x.double(), TypeError)):
+        with pytest.raises(err):
+            mx.quantize_mx(bad)
+    with pytest.raises(ValueError, match="multiple of 128"):
+        mx.mx_rows(x[:, :96])
+    with pytest.raises(RuntimeError, match="no gradient"):
+        mx.mx_rows(x.float().requires_grad_())
+    c, s = mx.quantize_mx(x[:0])
+    assert c.shape == (0, 64) and s.shape == (0, 4) and mx.dequantize_mx(c, s).shape == (0, 128)
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("m,k", [(1, 128), (16, 384), (17, 512), (33, 640), (130, 1280)])
+def test_tiled_rows(elem, m, k):
+    for dtype in (BF16, F16, F32):
+        x = _rows(m, k, 4, dtype)
+        got = mx.mx_rows(x, elem)
+        assert got.shape == (m, k) and (got.data.cpu().numpy() == O.tile(*O.quantize(_np(x), elem), elem)).all()
+
+
+# ---- the weight's layouts ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n,k", [(16, 128), (48, 640), (160, 1280)])
+@pytest.mark.parametrize("paired", [False, True])
+def test_packing(n, k, paired):
+    w = Weight(n, k, paired=paired)
+    got = G.pack_tiled(G.W_MXFP4, w.rows, k, w.fmt, sc0=w.sc)
+    assert torch.equal(got, w.tiled)
+    assert (_np(G.dequant(w.fmt, got, n, k)) == w.values).all()
+    assert (_np(G.dequant(G.W_MXFP4, w.rows, n, k, sc0=w.sc)) == w.values).all()
+    plain = torch.from_numpy(O.tile(w.codes, w.scales, O.E2M1)).cuda()
+    assert torch.equal(G.pack_tiled(G.W_MXFP4_TILED, plain, k, w.fmt), w.tiled)
+    if n % 32 == 0 and n > 32:  # by halves: gate, then up
+        out = None
+        for i, r in enumerate(torch.split(w.rows, n // 2)):
+            out = G.pack_tiled(G.W_MXFP4, r.contiguous(), k, w.fmt, sc0=w.sc[i * n // 2:(i + 1) * n // 2].contiguous(),
+                               n_total=n, row0=i * n // 2, out=out)
+        assert torch.equal(out, w.tiled)
+
+
+# ---- bf16 rows times the weight --------------------------------------------------------------------------
+
+
+def _gemv_reference(x, w, epi, gamma, eps, res, out_dtype):
+    xd, extra, before = _np(x), 0.0, 0.0
+    if gamma is not None:
+        xd, scale = _np((x.float() * gamma.float()).to(BF16)), O.rmsnorm_scale(xd, eps)
+        before = 2.0 ** -20 + x.shape[1] * 2.0 ** -24  # of 1 / rms: K sums, the mean, the root
+    else:
+        scale = np.ones((x.shape[0], 1))
+    y = xd @ w.values.T * scale
+    if epi == G.EPI_SILU_GATE:
+        h = w.n // 2
+        g, u = y[:, :h], y[:, h:]
+        ref = O.silu(g) * u
+        # d silu <= 1.1 dg; the exponential and the division are within 2^-20 of it
+        eg, eu = (_bound(np.abs(xd) * scale, p, 0.0, w.k, before=before) for p in (w.values[:h], w.values[h:]))
+        bound = torch.finfo(out_dtype).eps / 2 * np.abs(ref) + (1.1 * eg * np.abs(u) + (np.abs(O.silu(g)) + 1.1 * eg) * eu
+                                                                + 2.0 ** -20 * np.abs(ref)) * 1.01
+        return ref, bound
+    ref = y
+    if epi == G.EPI_RESIDUAL:
+        ref = y + _np(res)
+        extra = 2.0 ** -24 * np.abs(ref)
+    return ref, _bound(np.abs(xd) * scale, w.values, ref, w.k, out_dtype, before, extra)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 5, 8, 9, 16, 17, 33])
+@pytest.mark.parametrize("n,k", [(16, 128), (272, 640), (64, 2048), (4112, 512), (2560, 1280)])
+@pytest.mark.parametrize("epi,norm", [(G.EPI_NONE, False), (G.EPI_RESIDUAL, False), (G.EPI_SILU_GATE, True),
+                                      (G.EPI_NONE, True), (G.EPI_SILU_GATE, False)])
+def test_gemv(m, n, k, epi, norm):
+    w = Weight(n, k, paired=epi == G.EPI_SILU_GATE)
+    x = _rows(m, k, 5)
+    gamma = (1 + 0.2 * torch.randn(k)).to(BF16).cuda() if norm else None
+    n_out = n // 2 if epi == G.EPI_SILU_GATE else n
+    res = torch.randn(m, n_out).to(BF16).cuda() if epi == G.EPI_RESIDUAL else None
+    out = G.gemv(x, w.tiled, w.fmt, n, gamma=gamma, epilogue=epi, residual=res)
+    _close(out, *_gemv_reference(x, w, epi, gamma, 1e-6, res, BF16))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 2560, 10240), (2, 1024, 10240), (7, 1024, 8192), (13, 1024, 8192), (32, 2560, 10240),
+                                   (4, 20480, 2560)])
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+def test_gemv_long_rows(m, n, k, out_dtype):
+    w, x = Weight(n, k), _rows(m, k, 6)
+    res = torch.randn(m, n).to(out_dtype).cuda()
+    out = G.gemv(x, w.tiled, w.fmt, n, epilogue=G.EPI_RESIDUAL, residual=res, out_dtype=out_dtype)
+    _close(out, *_gemv_reference(x, w, G.EPI_RESIDUAL, None, 0.0, res, out_dtype))
+
+
+def test_gemv_second_store_strides_and_forced_shapes():
+    w = Weight(96, 640)
+    wide = torch.randn(5, 700).to(BF16).cuda()
+    x = wide[:, 8:648]  # rows at 16-byte steps of 1400 bytes: copied by the wrapper or read in place
+    out, out2 = torch.zeros(5, 128, device="cuda", dtype=BF16), torch.zeros(5, 32, device="cuda", dtype=BF16)
+    G.gemv(x, w.tiled, w.fmt, 96, out=out[:, 16:112], out2=out2)
+    ref, bound = _gemv_reference(x, w, G.EPI_NONE, None, 0.0, None, BF16)
+    _close(out[:, 16:112], ref, bound)
+    assert torch.equal(out2, out[:, 16:48]) and not out[:, :16].any() and not out[:, 112:].any()
+    for cfg in ((0, 0, 0, 5), (0, 3, 0, 5), (0, 0, 1, 5), (0, 2, 3, 5), (0, 1, 8, 5), (0, 0, 0, 6), (0, 2, 4, 6),
+                (0, 0, 2, 6, 2)):
+        _close(G.gemv(x, w.tiled, w.fmt, 96, cfg=cfg), ref, bound)
+
+
+@pytest.mark.parametrize("m", [33, 64, 203, 300])
+@pytest.mark.parametrize("n,k", [(48, 128), (272, 640), (2560, 1280), (80, 4992)])
+def test_prompt(m, n, k):
+    w, x = Weight(n, k), _rows(m, k, 7)
+    out = G.dequant_matmul(x, w.tiled, w.fmt, n, k)
+    _close(out, *_gemv_reference(x, w, G.EPI_NONE, None, 0.0, None, BF16))
+
+
+def test_prompt_follows_autograd():
+    w, x = Weight(48, 256), _rows(40, 256, 8, F32)
+    x.requires_grad_()
+    g = torch.randn(40, 48).to(BF16).cuda()
+    G.dequant_matmul(x, w.tiled, w.fmt, 48, 256).backward(g)
+    ref = _np(g) @ w.values
+    # the gradient of a bf16 product, rounded once to bf16
+    _close(x.grad, ref, 2.0 ** -8 * np.abs(ref) + 48 * 2.0 ** -24 * (np.abs(_np(g)) @ np.abs(w.values)))
+
+
+# ---- quantised rows times the weight ---------------------------------------------------------------------
+
+
+def _eights(codes, scales, elem, least):
+    """Largest magnitude of each eight consecutive columns, at least ``least``
+    times the block's scale."""
+    v = np.abs(O.values(codes, scales, elem)).reshape(codes.shape[0], -1, 8).max(-1)
+    return np.maximum(v, least * np.repeat(np.ldexp(1.0, scales.astype(np.int64) - 127), 4, -1))
+
+
+def _mx_reference(x, w, elem, res, out_dtype):
+    """With 8-bit elements the matrix core adds eight products (those of eight
+    consecutive columns) on a grid: each is cut toward zero at 2^(E - 13), E
+    the largest sum of the two factors' exponents among the eight
+    (test_the_grid_of_eight_products).  An exponent is that of the magnitude,
+    but at least -6 for e4m3 and 0 for e2m1, the types' subnormal ones; so
+    2^E <= max(|a|, 2^-6 s_a) max(|b|, s_b) over the eight, with the blocks'
+    scales s.  Seven products can lose less than a grid step each (the one
+    that sets E spans 4 + 2 bits and loses nothing).  4-bit products lie
+    within 2^-6 of one another and lose nothing."""
+    codes, scales = O.quantize(_np(x), elem)
+    xq = O.values(codes, scales, elem)
+    ref, extra = xq @ w.values.T, 0.0
+    if elem == O.E4M3:
+        extra = 7 * 2.0 ** -13 * (_eights(codes, scales, elem, 2.0 ** -6) @ _eights(w.codes, w.scales, O.E2M1, 1.0).T)
+    if res is not None:
+        ref = ref + _np(res)
+        extra = extra + 2.0 ** -24 * np.abs(ref)
+    return ref, _bound(xq, w.values, ref, w.k, out_dtype, extra=extra)
+
+
+def test_the_grid_of_eight_products():
+    """2^10 - 2^10 + 2^e: what the tolerance of 8-bit products rests on."""
+    w = Weight(16, 128)
+    w.codes[:], w.scales[:] = 0, 127
+    for small, lost in ((2, True), (7, True), (8, False), (40, False), (100, False)):
+        w.codes[:] = 0
+        w.codes[:, 0], w.codes[:, 1], w.codes[:, small] = 6, 14, 2  # 4, -4, 1
+        tiled = torch.from_numpy(O.tile(w.codes, w.scales, O.E2M1)).cuda()
+        e = np.arange(-9, 9)
+        x = np.zeros((e.size, 128))
+        x[:, 0] = x[:, 1] = 256
+        x[:, 32::32] = 256  # every block's scale is 1; these columns meet zeros
+        x[:, small] = 2.0 ** e
+        out = mx.mx_linear(mx.mx_rows(torch.from_numpy(x).float().cuda(), O.E4M3), tiled, 16, out_dtype=F32)
+        want = np.where(lost & (e < -3), 0.0, 2.0 ** e)
+        assert (_np(out) == want[:, None]).all()
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("m", [1, 2, 5, 16, 17, 32, 33, 48, 65, 129, 257, 300])
+@pytest.mark.parametrize("n,k", [(16, 128), (48, 384), (272, 640), (528, 1280), (1040, 2176)])
+def test_mx_linear(elem, m, n, k):
+    w, x = Weight(n, k), _rows(m, k, 9)
+    res = torch.randn(m, n).to(BF16).cuda() if (m + n) % 3 else None
+    out = mx.mx_linear(x, w.tiled, n, elem=elem, residual=res)
+    _close(out, *_mx_reference(x, w, elem, res, BF16))
+    assert torch.equal(mx.mx_linear(mx.mx_rows(x, elem), w.tiled, n, residual=res), out) or m <= 32
+    again = mx.mx_linear(mx.mx_rows(x, elem), w.tiled, n, residual=res)
+    _close(again, *_mx_reference(x, w, elem, res, BF16))
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("m,n,k", [(1, 2560, 10240), (5, 1024, 8192), (40, 2560, 10240), (513, 2560, 2560), (1030, 4096, 1024)])
+def test_mx_linear_of_layers(elem, m, n, k):
+    w, x = Weight(n, k), _rows(m, k, 10)
+    res = torch.randn(m, n).to(F32).cuda()
+    out = mx.mx_linear(x, w.tiled, n, elem=elem, residual=res, out_dtype=F32)
+    _close(out, *_mx_reference(x, w, elem, res, F32))
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("m", [3, 40, 260])
+def test_mx_linear_types_strides_and_aliases(elem, m):
+    n, k = 144, 512
+    w = Weight(n, k)
+    for dtype in (F16, F32):
+        x = _rows(m, k, 11, dtype)
+        _close(mx.mx_linear(x, w.tiled, n, elem=elem), *_mx_reference(x, w, elem, None, BF16))
+    wide = _rows(m, 600, 12)
+    for x in (wide[:, 8:520], wide[:, 1:513], wide[:1, 3:515].expand(m, k), wide.t()[7:519].t()):
+        _close(mx.mx_linear(x, w.tiled, n, elem=elem), *_mx_reference(x, w, elem, None, BF16))
+    # rows of wider tensors, the residual in the output's place, the rest untouched
+    x = wide[:, 8:520]
+    big = torch.randn(m + 2, n + 40).to(BF16).cuda()
+    before, out = big.clone(), big[1:m + 1, 17:17 + n]
+    ref, bound = _mx_reference(x, w, elem, out.clone(), BF16)
+    assert mx.mx_linear(x, w.tiled, n, elem=elem, residual=out, out=out) is out
+    _close(out, ref, bound)
+    before[1:m + 1, 17:17 + n] = big[1:m + 1, 17:17 + n]
+    assert torch.equal(before, big)
+    # a residual that lies partly in the output
+    flat = torch.randn(2 * m * n).to(BF16).cuda()
+    out, res = flat[:m * n].view(m, n), flat[5:5 + m * n].view(m, n)
+    ref, bound = _mx_reference(x, w, elem, res.clone(), BF16)
+    _close(mx.mx_linear(x, w.tiled, n, elem=elem, residual=res, out=out), ref, bound)
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("m", [4, 70])
+def test_mx_linear_rows_with_nan_and_infinity(elem, m):
+    """Rows are independent: those with a block that cannot be quantised are NaN, the others as ever."""
+    n, k = 48, 640
+    w, x = Weight(n, k), _rows(m, k, 13)
+    clean = mx.mx_linear(x, w.tiled, n, elem=elem)
+    x[1, 300], x[3, 0] = float("nan"), float("inf")
+    out = mx.mx_linear(x, w.tiled, n, elem=elem)
+    bad = torch.zeros(m, dtype=torch.bool)
+    bad[1] = bad[3] = True
+    assert out[bad.cuda()].isnan().all() and torch.equal(out[~bad.cuda()], clean[~bad.cuda()])
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+def test_mx_linear_large_and_small_scales(elem):
+    """Blocks from 2^-60 to 2^60 in one row: each scale stays its own."""
+    n, k, m = 32, 512, 40
+    w = Weight(n, k)
+    x = (_rows(m, k, 14, F32) * 2.0 ** torch.linspace(-60, 60, 16).round().repeat_interleave(32).cuda()).to(BF16)
+    _close(mx.mx_linear(x, w.tiled, n, elem=elem, out_dtype=F32), *_mx_reference(x, w, elem, None, F32))
+
+
+def test_mx_linear_refusals():
+    w, x = Weight(32, 256), _rows(4, 256)
+    for kw, err in (({"elem": "int4"}, ValueError), ({"residual": x}, ValueError), ({"out_dtype": F16}, TypeError),
+                    ({"out": torch.empty(4, 32, device="cuda", dtype=F16)}, ValueError),
+                    ({"out": torch.empty(32, 4, device="cuda", dtype=BF16).t()}, ValueError),
+                    ({"out": torch.empty(1, 32, device="cuda", dtype=BF16).expand(4, 32)}, ValueError),
+                    ({"out": x[:, :32]}, ValueError), ({"residual": torch.zeros(4, 32)}, RuntimeError)):
+        with pytest.raises(err):
+            mx.mx_linear(x, w.tiled, 32, **kw)
+    for bad in (w.tiled[:-16], w.tiled.view(2, -1).t(), torch.cat([w.tiled, w.tiled])):
+        with pytest.raises(ValueError, match="W_MXFP4_TILED"):
+            mx.mx_linear(x, bad, 32)
+    with pytest.raises(ValueError, match="W_MXFP4_TILED"):
+        mx.mx_linear(x, w.tiled, 24)
+    with pytest.raises(ValueError, match="multiple of 128"):
+        mx.mx_linear(x[:, :192], w.tiled, 32)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        mx.mx_linear(x.float().requires_grad_(), w.tiled, 32)
+    assert mx.mx_linear(x[:0], w.tiled, 32).shape == (0, 32)
+    assert mx.mx_linear(mx.mx_rows(x[:0]), w.tiled, 32).shape == (0, 32)
+
+
+@pytest.mark.parametrize("m", [2, 20, 150])
+def test_runs_in_a_graph_and_on_another_stream(m):
+    """Several operators in a row, captured, replayed beside eager work on new inputs."""
+    n, k = 96, 640
+    w, w2 = Weight(n, k), Weight(k, 128 * 3, seed=1)
+    x, g = _rows(m, k, 15), (1 + 0.1 * torch.randn(k)).to(BF16).cuda()
+    src = _rows(m, 384, 16)
+
+    def run():
+        h = mx.mx_linear(src, w2.tiled, k, elem="e4m3", residual=x)
+        codes, scales = mx.quantize_mx(h, "e2m1")
+        q = mx.mx_rows(h, "e2m1")
+        a = mx.mx_linear(q, w.tiled, n)
+        b = G.gemv(h, w.tiled, w.fmt, n, gamma=g)
+        return mx.dequantize_mx(codes, scales), a, b, mx.mx_linear(h, w.tiled, n, elem="e4m3", residual=a)
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run()
+    for i in range(4):
+        x.copy_(_rows(m, k, 20 + i))
+        src.copy_(_rows(m, 384, 30 + i))
+        graph.replay()
+        eager = run()
+        torch.cuda.synchronize()
+        for a, b in zip(held, eager):
+            assert torch.equal(a, b)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = run()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(other, eager):
+        assert torch.equal(a, b)
+
+
+# ---- the module --------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n,k", [(64, 256), (50, 200)])
+@pytest.mark.parametrize("act_bits", [16, 8, 4])
+def test_module(n, k, act_bits):
+    lin = nn.Linear(k, n, bias=False).cuda()
+    mod = M4.Mxfp4Linear(lin, act_bits=act_bits)
+    wq = O.rounded(np.pad(_np(lin.weight), ((0, 0), (0, -k % 32))), O.E2M1)[:, :k]
+    for shape in ((3, k), (1, k), (2, 30, k), (4, 5, 9, k)):
+        x = torch.randn(*shape).to(BF16).cuda()
+        xd = _np(x).reshape(-1, k)
+        if xd.shape[0] > M4.PREFILL_ROWS and act_bits != 16:
+            xd = O.rounded(np.pad(xd, ((0, 0), (0, -k % 32))), {8: O.E4M3, 4: O.E2M1}[act_bits])[:, :k]
+        with torch.no_grad():
+            out = mod(x)
+        assert out.shape == (*shape[:-1], n) and out.dtype == BF16
+        ref = xd @ wq.T
+        _close(out.reshape(-1, n), ref, _bound(xd, wq, ref, k))
+    assert mod(torch.randn(3, k).cuda()).dtype == F32
+    assert mod(torch.zeros(0, k, device="cuda", dtype=BF16)).shape == (0, n)
+    cpu = M4.Mxfp4Linear(nn.Linear(k, n, bias=False), device="cuda")
+    assert cpu.weight_mxfp4.is_cuda
+
+
+def test_module_gradient_of_a_prompt():
+    lin = nn.Linear(256, 48, bias=False).cuda()
+    x = torch.randn(40, 256, device="cuda", requires_grad=True)
+    M4.Mxfp4Linear(lin)(x).sum().backward()
+    ref = np.ones((40, 48)) @ O.rounded(_np(lin.weight), O.E2M1)
+    _close(x.grad, ref, 2.0 ** -8 * np.abs(ref) + 48 * 2.0 ** -24 * 48 * np.abs(O.rounded(_np(lin.weight), O.E2M1)).max())
+    with pytest.raises(RuntimeError, match="no gradient"):
+        M4.Mxfp4Linear(lin, act_bits=8)(x)
+
+
+def test_module_swap_checkpoint_and_compile(tmp_path):
+    class Mlp(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.gate_proj, self.up_proj = (nn.Linear(256, 512, bias=False) for _ in range(2))
+            self.down_proj = nn.Linear(512, 256, bias=False)
+
+        def forward(self, x):
+            return self.down_proj(torch.nn.functional.silu(self.gate_proj(x)) * self.up_proj(x))
+
+    mlp = Mlp().cuda().to(BF16)
+    stats = M4.quantize_module_mxfp4(mlp, min_bytes=0, act_bits=8)
+    assert stats == {"converted": 3, "skipped_below_threshold": 0, "weight_bytes_saved": 3 * 262144 * 47 // 64}
+    x = torch.randn(5, 256).to(BF16).cuda()
+    with torch.no_grad():
+        want = mlp(x)
+        Q.save_quantized(mlp, tmp_path, {}, source="synthetic")
+        fresh = Mlp()
+        Q.install_shells(fresh, Q.read_manifest(tmp_path), "cuda")
+        Q.load_quantized_state(fresh, tmp_path, "cuda")
+        assert torch.equal(fresh(x), want) and fresh.up_proj.act_bits == 8
+        assert torch.equal(torch.compile(mlp.up_proj, fullgraph=True, backend="eager")(x), mlp.up_proj(x))
+
+
+def test_fused_weight_of_modules():
+    """gate|up of a SiLU-gate MLP as one launch, behind the norm."""
+    gate, up, down = (M4.Mxfp4Linear(nn.Linear(a, b, bias=False).cuda()) for a, b in ((256, 512), (256, 512), (512, 256)))
+    x, g = _rows(2, 256, 17), (1 + 0.1 * torch.randn(256)).to(BF16).cuda()
+    wgu, wd = FK.FusedWeight.from_mxfp4(gate, up, paired=True), FK.FusedWeight.from_mxfp4(down)
+    assert (wgu.N, wgu.K, wgu.layout, wd.layout) == (1024, 256, "mx-tiled-paired", "mx-tiled")
+    act = FK.rms_gemv(x, wgu, g, epilogue=G.EPI_SILU_GATE)
+    out = FK.rms_gemv(act, wd, None, epilogue=G.EPI_RESIDUAL, residual=x)
+    w = Weight.__new__(Weight)
+    w.n, w.k = 1024, 256
+    w.values = np.concatenate([_np(G.dequant(G.W_MXFP4_TILED, m.weight_mxfp4, 512, 256)) for m in (gate, up)])
+    _close(act, *_gemv_reference(x, w, G.EPI_SILU_GATE, g, 1e-6, None, BF16))
+    w.n, w.k, w.values = 256, 512, _np(G.dequant(G.W_MXFP4_TILED, down.weight_mxfp4, 256, 512))
+    _close(out, *_gemv_reference(act, w, G.EPI_RESIDUAL, None, 0.0, x, BF16))
+    assert torch.equal(FK.rms_gemv(act, wd.clone(), None), FK.rms_gemv(act, wd, None))
+    with pytest.raises(ValueError, match="paired"):
+        FK.rms_gemv(x, wgu, g)
+    unpaired = FK.FusedWeight.from_mxfp4(gate, up)
+    gu = FK.rms_gemv(x, unpaired, g)
+    two = FK.rms_gemv(x, unpaired, g, epilogue=G.EPI_SILU_GATE)
+    assert torch.equal(two, FK.silu_mul(gu[:, :512], gu[:, 512:]))
