@@ -65,7 +65,10 @@ EXPORTS = (
     "bz_mx_rows_bytes",
     "bz_mx_quantize",
     "bz_mx_dequantize",
+    "bz_mx_gemm_workspace",
     "bz_mx_gemm",
+    "bz_mx_gemv_workspace",
+    "bz_mx_gemv",
     "bz_sample_cfg",
     "bz_sample_next",
     "bz_stream_read",
@@ -232,7 +235,13 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.bz_mx_dequantize.restype = ctypes.c_int
     lib.bz_mx_dequantize.argtypes = [vp, vp, i32, i32, i32, vp, i32, i64, vp]
     lib.bz_mx_gemm.restype = ctypes.c_int
-    lib.bz_mx_gemm.argtypes = [i32, vp, i32, vp, i32, i32, vp, i32, i64, vp, i32, i64, vp]
+    lib.bz_mx_gemm.argtypes = [i32, vp, i32, vp, i32, i32, vp, i32, i64, vp, i32, i64, vp, ctypes.c_size_t, i32, vp]
+    lib.bz_mx_gemm_workspace.restype = ctypes.c_size_t
+    lib.bz_mx_gemm_workspace.argtypes = [i32, i32, i32, i32, i32]
+    lib.bz_mx_gemv.restype = ctypes.c_int
+    lib.bz_mx_gemv.argtypes = [i32, vp, i64] + lib.bz_mx_gemm.argtypes[2:]
+    lib.bz_mx_gemv_workspace.restype = ctypes.c_size_t
+    lib.bz_mx_gemv_workspace.argtypes = [i32, i32, i32, i32, i32]
     lib.bz_stream_read.restype = ctypes.c_int
     lib.bz_stream_read.argtypes = [vp, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_uint32, vp, vp]
     lib.bz_shared_read.restype = ctypes.c_int

@@ -41,6 +41,9 @@ __all__ = ["BLOCK", "MxRows", "quantize_mx", "dequantize_mx", "mx_rows", "mx_lin
 
 BLOCK = 32
 
+# Up to this many rows mx_linear is one launch over the rows themselves.
+FEW_ROWS = 32
+
 _ELEM = {"e2m1": MX_E2M1, "e4m3": MX_E4M3}
 _X = {torch.bfloat16: DT_BF16, torch.float32: DT_F32, torch.float16: MX_F16}
 _OUT = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
@@ -165,6 +168,19 @@ def mx_rows(x: torch.Tensor, elem: str = "e2m1") -> MxRows:
     return MxRows(data, (M, K), elem)
 
 
+# Workspaces of products that slice K: one for each device and stream, and for
+# each graph capture under way.
+_NO_WAY = (1 << 64) - 1  # what bz_mx_gemv_workspace gives for a shape it does not take
+_WS: dict = {}
+_WS_RETIRED: list = []
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(few: bool, elem: int, M: int, n: int, k: int, cfg: int) -> int:
+    f = _lib.lib().bz_mx_gemv_workspace if few else _lib.lib().bz_mx_gemm_workspace
+    return int(f(elem, M, n, k, cfg))
+
+
 @functools.lru_cache(maxsize=1024)
 def _weight_bytes(n: int, k: int) -> int:
     return int(_lib.lib().bz_tiled_bytes(W_MXFP4_TILED, n, k))
@@ -172,12 +188,13 @@ def _weight_bytes(n: int, k: int) -> int:
 
 def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: str = "e2m1",
               residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
-              out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+              out_dtype: torch.dtype = torch.bfloat16, cfg: int = 0) -> torch.Tensor:
     """q(x) @ w_eff^T (+ residual) -> [M, n]: x [M, K] (bf16, fp16 or fp32), quantised to
     blocks of ``elem`` on the way, or the MxRows of it; w a W_MXFP4_TILED weight of n
     rows and K columns.  Products are exact, sums fp32; the result is rounded once,
     to out's dtype (bf16 or fp32).  residual: [M, n] bf16 or fp32, may be out itself;
-    out: [M, n] with unit column stride, apart from x and w."""
+    out: [M, n] with unit column stride, apart from x and w.  cfg: a launch shape
+    (bz_mx.h) instead of the built-in rule's."""
     rows = isinstance(x, MxRows)
     if rows:
         src, (M, K), code, index = x.data, x.shape, _elem(x.elem), x.data.get_device()
@@ -214,13 +231,22 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
         res, rdt, ldr = residual.data_ptr(), _OUT[residual.dtype], residual.stride(0) if M > 1 else n
     if M == 0:
         return out
-    if not rows:
+    lib, tail = _lib.lib(), (res, rdt, ldr, out.data_ptr(), _OUT[out.dtype], out.stride(0) if M > 1 else n)
+    # up to 32 rows that a launch can read as they are: quantised inside it
+    few = not rows and M <= FEW_ROWS and src.dtype == torch.bfloat16 and src.data_ptr() % 16 == 0 and ld % 8 == 0 \
+        and M * ld < 1 << 30 and _workspace_bytes(True, code, M, n, K, cfg) != _NO_WAY
+    if not few and not rows:
         data = torch.empty(_rows_bytes(code, M, K), device=w.device, dtype=torch.uint8)
-        _call(index, _lib.lib().bz_mx_quantize, src.data_ptr(), _X[src.dtype], ld, M, K, code, MX_TILED,
-              data.data_ptr(), None)
+        _call(index, lib.bz_mx_quantize, src.data_ptr(), _X[src.dtype], ld, M, K, code, MX_TILED, data.data_ptr(), None)
         src = data
-    _call(index, _lib.lib().bz_mx_gemm, code, src.data_ptr(), M, w.data_ptr(), n, K, res, rdt, ldr, out.data_ptr(),
-          _OUT[out.dtype], out.stride(0) if M > 1 else n)
+    need, ws = _workspace_bytes(few, code, M, n, K, cfg), None
+    if need:
+        ws = _lib.stream_workspace(_WS, (index,), need, w.device, torch._C._cuda_getCurrentRawStream(index), _WS_RETIRED)
+        ws = ws.data_ptr()
+    if few:
+        _call(index, lib.bz_mx_gemv, code, src.data_ptr(), ld, M, w.data_ptr(), n, K, *tail, ws, need, cfg)
+    else:
+        _call(index, lib.bz_mx_gemm, code, src.data_ptr(), M, w.data_ptr(), n, K, *tail, ws, need, cfg)
     return out
 
 

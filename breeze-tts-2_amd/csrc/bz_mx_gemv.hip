@@ -1,0 +1,142 @@
+// Host side of the few-row products of rows quantised on the way (C ABI
+// entries bz_mx_gemv and bz_mx_gemv_workspace).
+#include <algorithm>
+
+#include "bz_gemv_kernel.h"
+#include "bz_mx_gemv.h"
+
+namespace bz {
+
+struct MxGemvPlan {
+    MxGemvLaunch l;
+    int T, nsl, ups;
+    size_t ws;
+};
+
+// Built-in rule (sweeps of blocks, units per wave and slices on MI355X, M = 1
+// .. 32, us): one slice and about one workgroup per CU while a row has up to
+// 32 units, 2 units per wave (e2m1 N20480 K2560 M = 5: 5 blocks x 2 units
+// 7.97, x 4 units 8.22, 3 blocks x 2 8.41); longer rows, whose x every
+// workgroup would read whole, in slices of about 20 units (N2560 K10240 M =
+// 5: 4 slices of 3 blocks 8.01, one slice 9.10); more than 16 rows in slices
+// of about 13, a unit per wave (N2560 K10240 M = 32: 6 slices of 4 blocks 11.2,
+// 4 of 3 12.2; e4m3 N10240 K2560: 2 slices of 5 11.0, one of 3 11.6).  8-bit
+// elements prefer a unit per wave over slices (N1024 K8192 M = 8: 7.12, 7.19).
+static int mx_gemv_plan(int elem, int M, int N, int K, int cfg, MxGemvPlan& pl) {
+    const int NU = K / 128, nblk = N / 16, mt = M > 16 ? 2 : 1;
+    const int cT = cfg & 255, cu = (cfg >> 8) & 255, cs = cfg >> 16;
+    if (cT > kMxGemvBlocks || cs > 64) return BZ_ERR_INVALID_ARG;
+    auto blocks = [&](int slices) { return cT ? cT : (int)(((int64_t)nblk * slices + 255) / 256); };
+    int nsl = cs ? cs : mt == 2 ? std::max(1, (NU + 6) / 13) : NU <= 32 ? 1 : (NU + 19) / 20;
+    if (!cs && blocks(nsl) > kMxGemvBlocks) nsl = 1;
+    nsl = std::min(nsl, NU);
+    const int T = std::min(kMxGemvBlocks, blocks(nsl));
+    const int groups = (nblk + T - 1) / T;
+    int upw = 0;
+    for (;; ++nsl) {  // more slices where the waves do not hold the row
+        if (nsl > 64 || (nsl > 1 && (groups > kMxCounters || (int64_t)nsl * M * N * 4 >= (int64_t)1 << 31)))
+            return BZ_ERR_UNSUPPORTED;
+        pl.ups = (NU + nsl - 1) / nsl;
+        for (int u : kMxGemvUpw)
+            if (!upw && mx_gemv_built(mt, u) && (cu ? u == cu : u >= 2 || pl.ups == 1 || (nsl > 1 && (mt == 2 || elem == BZ_MX_E4M3))) &&
+                mx_gemv_waves(elem, mt, u) * u >= pl.ups)
+                upw = u;
+        if (upw) break;
+        if (cu || cs) return BZ_ERR_INVALID_ARG;
+    }
+    pl.nsl = (NU + pl.ups - 1) / pl.ups;
+    pl.l.upw = upw;
+    pl.l.nw = (pl.ups + upw - 1) / upw;
+    pl.T = T;
+    pl.l.mt = mt;
+    pl.l.grid = (unsigned)(groups * pl.nsl);
+    pl.l.lds = (size_t)mx_gemv_lds(pl.l.nw, T, mt);
+    if (pl.l.lds > 160 * 1024) return BZ_ERR_UNSUPPORTED;
+    pl.ws = pl.nsl > 1 ? kMxPartOffset + (size_t)pl.nsl * M * N * 4 : 0;
+    return BZ_OK;
+}
+
+template <int ELEM, int MT, int UPW>
+static int launch_kernel(const MxGemvParams& p, const MxGemvLaunch& l, hipStream_t st) {
+    if constexpr (mx_gemv_built(MT, UPW)) {
+        auto kern = mx_gemv<ELEM, MT, UPW>;
+        if (l.lds > 65536 && raise_lds_limit(reinterpret_cast<const void*>(kern)) != BZ_OK) return BZ_ERR_LAUNCH;
+        hipLaunchKernelGGL(kern, dim3(l.grid), dim3(64 * l.nw), l.lds, st, p);
+        return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
+    } else {
+        return BZ_ERR_INVALID_ARG;
+    }
+}
+template <int ELEM, int MT>
+static int launch_t(const MxGemvParams& p, const MxGemvLaunch& l, hipStream_t st) {
+    switch (l.upw) {
+        case 1: return launch_kernel<ELEM, MT, 1>(p, l, st);
+        case 2: return launch_kernel<ELEM, MT, 2>(p, l, st);
+        case 3: return launch_kernel<ELEM, MT, 3>(p, l, st);
+        case 4: return launch_kernel<ELEM, MT, 4>(p, l, st);
+        case 5: return launch_kernel<ELEM, MT, 5>(p, l, st);
+        case 6: return launch_kernel<ELEM, MT, 6>(p, l, st);
+        default: return launch_kernel<ELEM, MT, 8>(p, l, st);
+    }
+}
+template <int ELEM>
+static int launch_mt(const MxGemvParams& p, const MxGemvLaunch& l, hipStream_t st) {
+    return l.mt == 1 ? launch_t<ELEM, 1>(p, l, st) : launch_t<ELEM, 2>(p, l, st);
+}
+
+static int mx_gemv_check(int elem, int M, int N, int K) {
+    if (M < 1 || N < 1 || K < 1 || (elem != BZ_MX_E2M1 && elem != BZ_MX_E4M3)) return BZ_ERR_INVALID_ARG;
+    if (N % 16 || K % 128) return BZ_ERR_SHAPE;
+    return M > kMxGemvRows || K > (1 << 22) ? BZ_ERR_UNSUPPORTED : BZ_OK;
+}
+
+}  // namespace bz
+
+using namespace bz;
+
+extern "C" size_t bz_mx_gemv_workspace(int32_t elem, int32_t M, int32_t N, int32_t K, int32_t cfg) {
+    MxGemvPlan pl;
+    if (cfg < 0 || mx_gemv_check(elem, M, N, K) != BZ_OK) return (size_t)-1;
+    return mx_gemv_plan(elem, M, N, K, cfg, pl) == BZ_OK ? pl.ws : (size_t)-1;
+}
+
+extern "C" int bz_mx_gemv(int32_t elem, const void* x, int64_t ldx, int32_t M, const void* w, int32_t N, int32_t K,
+                          const void* residual, int32_t residual_dtype, int64_t ldr, void* out, int32_t out_dtype,
+                          int64_t ldo, void* workspace, size_t workspace_bytes, int32_t cfg, void* stream) {
+    if (!x || !w || !out || cfg < 0) return BZ_ERR_INVALID_ARG;
+    if (out_dtype != BZ_DT_BF16 && out_dtype != BZ_DT_F32) return BZ_ERR_INVALID_ARG;
+    if (residual && residual_dtype != BZ_DT_BF16 && residual_dtype != BZ_DT_F32) return BZ_ERR_INVALID_ARG;
+    const int rc = mx_gemv_check(elem, M, N, K);
+    if (rc != BZ_OK) return rc;
+    if (ldx < K || ldo < N || (residual && ldr < N)) return BZ_ERR_INVALID_ARG;
+    auto off = [](const void* q, uintptr_t a) { return (reinterpret_cast<uintptr_t>(q) & (a - 1)) != 0; };
+    if (off(x, 16) || ldx % 8 || off(w, 16) || off(out, out_dtype == BZ_DT_F32 ? 4 : 2) ||
+        (residual && off(residual, residual_dtype == BZ_DT_F32 ? 4 : 2)))
+        return BZ_ERR_ALIGNMENT;
+    if (((int64_t)(M - 1) * ldx + K) * 2 >= (int64_t)1 << 31) return BZ_ERR_UNSUPPORTED;  // 32-bit offsets
+    MxGemvPlan pl;
+    const int prc = mx_gemv_plan(elem, M, N, K, cfg, pl);
+    if (prc != BZ_OK) return prc;
+    if (pl.ws && (!workspace || off(workspace, 16) || workspace_bytes < pl.ws)) return BZ_ERR_INVALID_ARG;
+    MxGemvParams p{};
+    p.x = static_cast<const uint16_t*>(x);
+    p.ldx = ldx;
+    p.w = static_cast<const uint8_t*>(w);
+    p.res = residual;
+    p.ldr = ldr;
+    p.out = out;
+    p.ldo = ldo;
+    p.cnt = static_cast<uint32_t*>(workspace);
+    p.part = pl.ws ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kMxPartOffset) : nullptr;
+    p.M = M;
+    p.K = K;
+    p.NU = K / 128;
+    p.nblk = N / 16;
+    p.T = pl.T;
+    p.nsl = pl.nsl;
+    p.ups = pl.ups;
+    p.res_f32 = residual_dtype == BZ_DT_F32;
+    p.out_f32 = out_dtype == BZ_DT_F32;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return elem == BZ_MX_E2M1 ? launch_mt<BZ_MX_E2M1>(p, pl.l, st) : launch_mt<BZ_MX_E4M3>(p, pl.l, st);
+}
