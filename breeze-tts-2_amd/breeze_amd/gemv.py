@@ -157,7 +157,7 @@ def gemv(
             residual = residual.contiguous()
         res_dt = _DT[residual.dtype]
     if out is None:
-        out = torch.empty(M, n_out, device=dev, dtype=out_dtype)
+        out = torch.empty((M, n_out), dtype=out_dtype, device=dev)
     else:
         _require_gpu("out", out, dev)
         if out.dtype not in _DT or out.shape != (M, n_out) or out.stride(1) != 1:
@@ -167,9 +167,10 @@ def gemv(
         if out2.dim() != 2 or out2.dtype != out.dtype or out2.shape[0] != M or out2.stride(1) != 1 \
                 or not 0 < out2.shape[1] <= n_out:
             raise ValueError(f"out2 must be a row-major [M, <= {n_out}] tensor of out's dtype")
-    for name, t in (("sc0", sc0), ("sc1", sc1)):
-        if t is not None:
-            _require_gpu(name, t, dev)
+    if sc0 is not None:
+        _require_gpu("sc0", sc0, dev)
+    if sc1 is not None:
+        _require_gpu("sc1", sc1, dev)
     _check_weight(w, wfmt, n, K, group, sc0, sc1)
     if M == 0:  # no rows: the empty result, nothing launched (the library rejects M = 0)
         return out
@@ -181,13 +182,14 @@ def gemv(
             cfg = _NO_CFG
     if len(cfg) != 5:
         cfg = (tuple(cfg) + _NO_CFG)[:5]
-    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     has_res = epilogue == EPI_RESIDUAL
     d = _lib.gemv_desc(
         _lib.ABI_VERSION, M, n, K, group, wfmt, epilogue, _DT[out.dtype], res_dt, *cfg, eps, x.data_ptr(), x.stride(0),
-        w.data_ptr(), ptr(sc0), ptr(sc1), ptr(gamma), residual.data_ptr() if has_res else 0,
-        residual.stride(0) if has_res else 0, out.data_ptr(), out.stride(0), 0, 0, ptr(out2),
-        0 if out2 is None else out2.stride(0), 0 if out2 is None else out2.shape[1], 0)
+        w.data_ptr(), 0 if sc0 is None else sc0.data_ptr(), 0 if sc1 is None else sc1.data_ptr(),
+        0 if gamma is None else gamma.data_ptr(), residual.data_ptr() if has_res else 0,
+        residual.stride(0) if has_res else 0, out.data_ptr(), out.stride(0), 0, 0,
+        0 if out2 is None else out2.data_ptr(), 0 if out2 is None else out2.stride(0),
+        0 if out2 is None else out2.shape[1], 0)
     stream = _lib.stream_of(x)
     lib = _lib.lib()
     if M >= _TILE_MIN_ROWS or cfg[3] in (_PATH_TILE, _PATH_PANEL):
@@ -239,6 +241,8 @@ def _check_weight(w, wfmt, n, k, group, sc0, sc1) -> None:
     if w.numel() * w.element_size() != wbytes:
         raise ValueError(f"weight buffer holds {w.numel() * w.element_size()} bytes, format {wfmt} with "
                          f"N={n}, K={k} needs {wbytes}")
+    if s0 is None and s1 is None:
+        return
     for name, t, want in (("sc0", sc0, s0), ("sc1", sc1, s1)):
         if want is None:
             continue

@@ -47,6 +47,7 @@ FEW_ROWS = 32
 _ELEM = {"e2m1": MX_E2M1, "e4m3": MX_E4M3}
 _X = {torch.bfloat16: DT_BF16, torch.float32: DT_F32, torch.float16: MX_F16}
 _OUT = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
+_BYTES = (torch.uint8, torch.float8_e4m3fn, torch.int8)
 
 
 def _elem(elem: str) -> int:
@@ -82,18 +83,24 @@ def _call(index: int, f, *args) -> None:
 
 
 def _rows(x: torch.Tensor, unit: int) -> tuple:
-    """(x with rows the kernels can read, M, K, row stride)."""
-    if x.dim() != 2:
-        raise ValueError(f"x must be [rows, columns], got {list(x.shape)}")
-    if x.dtype not in _X:
+    """(x with rows the kernels can read, M, K, row stride, type code, device
+    index)."""
+    index, shape, dt = x.get_device(), x.shape, _X.get(x.dtype)
+    if index < 0:
+        _gpu("x", x, index)
+    if len(shape) != 2:
+        raise ValueError(f"x must be [rows, columns], got {list(shape)}")
+    if dt is None:
         raise TypeError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
-    M, K = x.shape
+    M, K = shape
     if K < 1 or K % unit:
         raise ValueError(f"{K} columns are not a positive multiple of {unit}")
     ld, inner = x.stride()
-    if M > 1 and ld < K or inner != 1 and K > 1:  # an expanded row, a transposed matrix
+    if M <= 1:
+        ld = K
+    if inner != 1 or ld < K:  # a transposed matrix, an expanded row
         x, ld = x.contiguous(), K
-    return x, M, K, ld if M > 1 else K
+    return x, M, K, ld, dt, index
 
 
 def quantize_mx(x: torch.Tensor, elem: str = "e2m1") -> tuple[torch.Tensor, torch.Tensor]:
@@ -101,14 +108,14 @@ def quantize_mx(x: torch.Tensor, elem: str = "e2m1") -> tuple[torch.Tensor, torc
     codes uint8 [M, K/2] with the even column in the low half (e2m1) or
     float8_e4m3fn [M, K]; scales uint8 [M, K/32]."""
     code = _elem(elem)
-    index = x.get_device()
-    _gpu("x", x, index)
-    x, M, K, ld = _rows(x, BLOCK)
-    codes = torch.empty(M, K // 2 if code == MX_E2M1 else K, device=x.device,
-                        dtype=torch.uint8 if code == MX_E2M1 else torch.float8_e4m3fn)
-    scales = torch.empty(M, K // BLOCK, device=x.device, dtype=torch.uint8)
+    x, M, K, ld, dt, index = _rows(x, BLOCK)
+    if code == MX_E2M1:
+        codes = torch.empty((M, K // 2), dtype=torch.uint8, device=x.device)
+    else:
+        codes = torch.empty((M, K), dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((M, K // BLOCK), dtype=torch.uint8, device=x.device)
     if M:
-        _call(index, _lib.lib().bz_mx_quantize, x.data_ptr(), _X[x.dtype], ld, M, K, code, MX_ROWS, codes.data_ptr(),
+        _call(index, _lib.lib().bz_mx_quantize, x.data_ptr(), dt, ld, M, K, code, MX_ROWS, codes.data_ptr(),
               scales.data_ptr())
     return codes, scales
 
@@ -117,25 +124,27 @@ def dequantize_mx(codes: torch.Tensor, scales: torch.Tensor, elem: str = "e2m1",
                   dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values [M, K] (bf16 or fp32) that quantize_mx's codes and scales stand
     for: exact, in bf16 down to 2^-126."""
-    code = _elem(elem)
-    index = codes.get_device()
-    _gpu("codes", codes, index)
-    _gpu("scales", scales, index)
-    if dtype not in _OUT:
+    code, index, shape = _elem(elem), codes.get_device(), codes.shape
+    if index < 0 or scales.get_device() != index:
+        _gpu("codes", codes, index)
+        _gpu("scales", scales, index)
+    dt = _OUT.get(dtype)
+    if dt is None:
         raise TypeError(f"values are bfloat16 or float32, not {dtype}")
-    if codes.dim() != 2 or codes.element_size() != 1 or scales.dtype != torch.uint8:
+    if len(shape) != 2 or codes.dtype not in _BYTES or scales.dtype is not torch.uint8:
         raise ValueError("codes must be a 2-D tensor of bytes and scales uint8")
-    M, K = codes.shape
-    K *= 2 if code == MX_E2M1 else 1
+    M, K = shape
+    if code == MX_E2M1:
+        K *= 2
     if K < 1 or K % BLOCK or scales.shape != (M, K // BLOCK):
-        raise ValueError(f"codes {list(codes.shape)} and scales {list(scales.shape)} are not those of {elem} rows")
-    codes, scales = codes.contiguous(), scales.contiguous()
-    if codes.data_ptr() % 4:
-        codes = codes.clone()
-    out = torch.empty(M, K, device=codes.device, dtype=dtype)
+        raise ValueError(f"codes {list(shape)} and scales {list(scales.shape)} are not those of {elem} rows")
+    if not codes.is_contiguous() or codes.data_ptr() % 4:
+        codes = codes.clone(memory_format=torch.contiguous_format)
+    if not scales.is_contiguous():
+        scales = scales.contiguous()
+    out = torch.empty((M, K), dtype=dtype, device=codes.device)
     if M:
-        _call(index, _lib.lib().bz_mx_dequantize, codes.data_ptr(), scales.data_ptr(), code, M, K, out.data_ptr(),
-              _OUT[dtype], K)
+        _call(index, _lib.lib().bz_mx_dequantize, codes.data_ptr(), scales.data_ptr(), code, M, K, out.data_ptr(), dt, K)
     return out
 
 
@@ -157,33 +166,36 @@ def mx_rows(x: torch.Tensor, elem: str = "e2m1") -> MxRows:
     """x [M, K] (bf16, fp16 or fp32; K a multiple of 128) quantised to blocks,
     for mx_linear: once for all products that read the same rows."""
     code = _elem(elem)
-    index = x.get_device()
-    _gpu("x", x, index)
+    x, M, K, ld, dt, index = _rows(x, 128)
     _no_grad(x, "mx_rows")
-    x, M, K, ld = _rows(x, 128)
+    return MxRows(_tiled_rows(x, M, K, ld, dt, code, index), (M, K), elem)
+
+
+def _tiled_rows(x, M: int, K: int, ld: int, dt: int, code: int, index: int) -> torch.Tensor:
     data = torch.empty(_rows_bytes(code, M, K), device=x.device, dtype=torch.uint8)
     if M:
-        _call(index, _lib.lib().bz_mx_quantize, x.data_ptr(), _X[x.dtype], ld, M, K, code, MX_TILED, data.data_ptr(),
-              None)
-    return MxRows(data, (M, K), elem)
+        _call(index, _lib.lib().bz_mx_quantize, x.data_ptr(), dt, ld, M, K, code, MX_TILED, data.data_ptr(), None)
+    return data
 
 
 # Workspaces of products that slice K: one for each device and stream, and for
 # each graph capture under way.
-_NO_WAY = (1 << 64) - 1  # what bz_mx_gemv_workspace gives for a shape it does not take
 _WS: dict = {}
 _WS_RETIRED: list = []
+_NO_WAY = (1 << 64) - 1  # what bz_mx_gemv_workspace gives for a shape it does not take
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(few: bool, elem: int, M: int, n: int, k: int, cfg: int) -> int:
-    f = _lib.lib().bz_mx_gemv_workspace if few else _lib.lib().bz_mx_gemm_workspace
-    return int(f(elem, M, n, k, cfg))
-
-
-@functools.lru_cache(maxsize=1024)
-def _weight_bytes(n: int, k: int) -> int:
-    return int(_lib.lib().bz_tiled_bytes(W_MXFP4_TILED, n, k))
+def _plan(elem: int, M: int, n: int, k: int, cfg: int, rows: bool) -> tuple[int, bool, int]:
+    """(bytes of the weight, whether one launch over bf16 rows takes the shape,
+    workspace bytes)."""
+    lib = _lib.lib()
+    weight = int(lib.bz_tiled_bytes(W_MXFP4_TILED, n, k)) or -1
+    if rows and 0 < M <= FEW_ROWS:
+        need = int(lib.bz_mx_gemv_workspace(elem, M, n, k, cfg))
+        if need != _NO_WAY:
+            return weight, True, need
+    return weight, False, int(lib.bz_mx_gemm_workspace(elem, M, n, k, cfg))
 
 
 def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: str = "e2m1",
@@ -191,62 +203,69 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
               out_dtype: torch.dtype = torch.bfloat16, cfg: int = 0) -> torch.Tensor:
     """q(x) @ w_eff^T (+ residual) -> [M, n]: x [M, K] (bf16, fp16 or fp32), quantised to
     blocks of ``elem`` on the way, or the MxRows of it; w a W_MXFP4_TILED weight of n
-    rows and K columns.  Products are exact, sums fp32; the result is rounded once,
-    to out's dtype (bf16 or fp32).  residual: [M, n] bf16 or fp32, may be out itself;
-    out: [M, n] with unit column stride, apart from x and w.  cfg: a launch shape
-    (bz_mx.h) instead of the built-in rule's."""
+    rows and K columns.  Products are exact, sums fp32 (with e4m3 after a first sum
+    of eight products on the matrix core's grid, include/bz_mx.h); the result is
+    rounded once, to out's dtype (bf16 or fp32).  residual: [M, n] bf16 or fp32, may
+    be out itself; out: [M, n] with unit column stride, apart from x and w.  cfg: a
+    launch shape (include/bz_mx.h) instead of the built-in rule's."""
     rows = isinstance(x, MxRows)
     if rows:
-        src, (M, K), code, index = x.data, x.shape, _elem(x.elem), x.data.get_device()
+        src, (M, K), code = x.data, x.shape, _elem(x.elem)
+        index, few = src.get_device(), False
     else:
-        code, index = _elem(elem), x.get_device()
-        _gpu("x", x, index)
+        code = _elem(elem)
+        src, M, K, ld, dt, index = _rows(x, 128)
         _no_grad(x, "mx_linear")
-        src, M, K, ld = _rows(x, 128)
-    if w.get_device() != index:
+        # up to 32 rows that a launch can read as they are: quantised inside it
+        few = dt == DT_BF16 and M <= FEW_ROWS and not (ld & 7 or src.data_ptr() & 15) and M * ld < 1 << 30
+    weight, few, need = _plan(code, M, n, K, cfg, few)
+    if w.get_device() != index or w.numel() * w.element_size() != weight or not w.is_contiguous() or w.data_ptr() & 15:
         _gpu("w", w, index)
-    if w.numel() * w.element_size() != (_weight_bytes(n, K) or -1) or not w.is_contiguous() or w.data_ptr() % 16:
         raise ValueError(f"w must be a contiguous W_MXFP4_TILED weight of {n} x {K} (rows a multiple of 16), "
-                         f"{_weight_bytes(n, K)} bytes; got {w.numel() * w.element_size()}")
+                         f"{max(weight, 0)} bytes; got {w.numel() * w.element_size()}")
     if out is None:
-        if out_dtype not in _OUT:
+        odt = _OUT.get(out_dtype)
+        if odt is None:
             raise TypeError(f"out is bfloat16 or float32, not {out_dtype}")
-        out = torch.empty(M, n, device=w.device, dtype=out_dtype)
+        out, ldo = torch.empty((M, n), dtype=out_dtype, device=w.device), n
+        fresh = True
     else:
         _gpu("out", out, index)
-        if out.dtype not in _OUT or out.shape != (M, n) or (out.stride(1) != 1 and n > 1) \
-                or (M > 1 and out.stride(0) < n):
+        odt, fresh = _OUT.get(out.dtype), False
+        if odt is None or out.shape != (M, n) or (out.stride(1) != 1 and n > 1) or (M > 1 and out.stride(0) < n):
             raise ValueError(f"out must be a bf16 or fp32 [{M}, {n}] tensor whose rows are contiguous")
         for name, t in (("x", src), ("w", w)):
             if _overlap(out, t):
                 raise ValueError(f"out must not overlap {name}")
+        ldo = out.stride(0) if M > 1 else n
     res = rdt = ldr = 0
     if residual is not None:
-        _gpu("residual", residual, index)
-        if residual.dtype not in _OUT or residual.shape != (M, n):
+        rdt = _OUT.get(residual.dtype)
+        if residual.get_device() != index or rdt is None or residual.shape != (M, n):
+            _gpu("residual", residual, index)
             raise ValueError(f"residual must be a bf16 or fp32 [{M}, {n}] tensor")
-        if (residual.stride(1) != 1 and n > 1) or (M > 1 and residual.stride(0) < n) \
-                or (_overlap(out, residual) and not _same(out, residual)):
+        ldr, inner = residual.stride()
+        if (inner != 1 and n > 1) or (M > 1 and ldr < n) \
+                or not (fresh or _same(out, residual) or not _overlap(out, residual)):
             residual = residual.clone(memory_format=torch.contiguous_format)
-        res, rdt, ldr = residual.data_ptr(), _OUT[residual.dtype], residual.stride(0) if M > 1 else n
+            ldr = n
+        res = residual.data_ptr()
+        if M <= 1:
+            ldr = n
     if M == 0:
         return out
-    lib, tail = _lib.lib(), (res, rdt, ldr, out.data_ptr(), _OUT[out.dtype], out.stride(0) if M > 1 else n)
-    # up to 32 rows that a launch can read as they are: quantised inside it
-    few = not rows and M <= FEW_ROWS and src.dtype == torch.bfloat16 and src.data_ptr() % 16 == 0 and ld % 8 == 0 \
-        and M * ld < 1 << 30 and _workspace_bytes(True, code, M, n, K, cfg) != _NO_WAY
-    if not few and not rows:
-        data = torch.empty(_rows_bytes(code, M, K), device=w.device, dtype=torch.uint8)
-        _call(index, lib.bz_mx_quantize, src.data_ptr(), _X[src.dtype], ld, M, K, code, MX_TILED, data.data_ptr(), None)
-        src = data
-    need, ws = _workspace_bytes(few, code, M, n, K, cfg), None
+    lib, ws = _lib.lib(), 0
+    if not (few or rows):
+        src = _tiled_rows(src, M, K, ld, dt, code, index)
     if need:
-        ws = _lib.stream_workspace(_WS, (index,), need, w.device, torch._C._cuda_getCurrentRawStream(index), _WS_RETIRED)
-        ws = ws.data_ptr()
+        ws = _lib.stream_workspace(_WS, (index,), need, w.device, torch._C._cuda_getCurrentRawStream(index),
+                                   _WS_RETIRED).data_ptr()
     if few:
-        _call(index, lib.bz_mx_gemv, code, src.data_ptr(), ld, M, w.data_ptr(), n, K, *tail, ws, need, cfg)
+        _call(index, lib.bz_mx_gemv, code, src.data_ptr(), ld, M, w.data_ptr(), n, K, res, rdt, ldr, out.data_ptr(),
+              odt, ldo, ws, need, cfg)
     else:
-        _call(index, lib.bz_mx_gemm, code, src.data_ptr(), M, w.data_ptr(), n, K, *tail, ws, need, cfg)
+        _call(index, lib.bz_mx_gemm, code, src.data_ptr(), M, w.data_ptr(), n, K, res, rdt, ldr, out.data_ptr(),
+              odt, ldo, ws, need, cfg)
     return out
 
 

@@ -45,11 +45,11 @@ def arch_of(device: torch.device) -> str:
     return a
 
 
+_BUCKETS = (1, 1, 2, 4, 4) + (8,) * 4 + (16,) * 8  # of 0 .. 16 rows
+
+
 def m_bucket(M: int) -> int:
-    for b in (1, 2, 4, 8, 16):
-        if M <= b:
-            return b
-    return 32
+    return _BUCKETS[M] if 0 <= M <= 16 else 32 if M > 16 else 1
 
 
 def table_key(arch: str, N: int, K: int, wfmt: int, epilogue: int, norm: bool, M: int) -> str:

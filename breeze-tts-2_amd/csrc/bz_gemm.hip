@@ -42,14 +42,18 @@ struct GemmPlan {
 // launch and its traffic where K is sliced.  Over those shapes the shape it
 // picks takes 2% (int4) / 3% (fp8) longer than the best of the sweep on
 // average, at worst 24% / 42% (fp8 K2048 N6144 M = 256: 23.9 us for 16.8).
+// MXFP4's were chosen for the shapes they pick: over 130 (M, N, K), 6630
+// timings, 0.7% longer than the best on average, at worst 16% (int4's: 5.7%
+// and 35%).
 struct GemmCost {
     float step0, step_m, step_n, step_mn, wg0, wg_mn, overlap, sum0, sum_mb, traffic_mb;
 };
 constexpr GemmCost kGemmCostI4 = {-0.245f, 0.144f, 0.374f, 0.0156f, -0.457f, 0.154f, 0.546f, 1.90f, 1.89f, 0.0106f};
+constexpr GemmCost kGemmCostMx = {-0.208f, 0.187f, 0.187f, 0.0164f, -0.326f, 0.183f, 0.817f, 1.83f, 1.88f, 0.00711f};
 constexpr GemmCost kGemmCostF8 = {-0.206f, 0.108f, 0.217f, 0.0215f, 0.365f, 0.210f, 0.547f, 1.60f, 1.57f, 0.0172f};
 
 static float gemm_cost(int wf, int M, int N, int K, int mt, int nt, const GemmPlan& pl) {
-    const GemmCost& c = tiled_4bit(wf) ? kGemmCostI4 : kGemmCostF8;
+    const GemmCost& c = tiled_i4(wf) ? kGemmCostI4 : tiled_mx(wf) ? kGemmCostMx : kGemmCostF8;
     const float mn = (float)(mt * nt);
     const float one = c.wg0 + c.wg_mn * mn +
                       (float)(pl.sps + (pl.sps & 1)) * (c.step0 + c.step_m * mt + c.step_n * nt + c.step_mn * mn);

@@ -23,6 +23,9 @@ struct MxBf16 {
     __device__ __forceinline__ void zero() { v = u32x4{0u, 0u, 0u, 0u}; }
     __device__ __forceinline__ float at(int i) const { return (i & 1) ? bf16_hi(v[i >> 1]) : bf16_lo(v[i >> 1]); }
     __device__ __forceinline__ uint32_t pack4(float s) const { return mx4_pack_bf16(v, s); }
+    __device__ __forceinline__ void pack8(uint32_t code, float s, uint32_t& lo, uint32_t& hi) const {
+        mx8_pack_bf16(v, code, s, lo, hi);
+    }
 };
 struct MxF32 {
     static constexpr int kBytes = 4;
@@ -45,6 +48,10 @@ struct MxF32 {
     }
     __device__ __forceinline__ float at(int i) const { return v[i]; }
     __device__ __forceinline__ uint32_t pack4(float s) const { return mx4_pack_f32(v, s); }
+    __device__ __forceinline__ void pack8(uint32_t, float s, uint32_t& lo, uint32_t& hi) const {
+        lo = mx8_pack_f32(v[0], v[1], v[2], v[3], s);
+        hi = mx8_pack_f32(v[4], v[5], v[6], v[7], s);
+    }
 };
 struct MxF16 : MxF32 {  // (widened: exact)
     static constexpr int kBytes = 2;
@@ -73,13 +80,16 @@ template <int ELEM>
 constexpr int kMxEmax = ELEM == BZ_MX_E2M1 ? 2 : 8;
 
 template <int ELEM, class X>
-__device__ __forceinline__ void mx_store8(uint8_t* at, const X& x, float s) {
+__device__ __forceinline__ void mx_store8(uint8_t* at, const X& x, uint32_t code) {
+    const float s = __uint_as_float(code << 23);
     if (ELEM == BZ_MX_E2M1) {
         *reinterpret_cast<uint32_t*>(at) = x.pack4(s);
     } else {
+        uint2 q;
+        x.pack8(code, s, q.x, q.y);
         uint32_t* o = reinterpret_cast<uint32_t*>(at);
-        o[0] = mx8_pack_f32(x.at(0), x.at(1), x.at(2), x.at(3), s);
-        o[1] = mx8_pack_f32(x.at(4), x.at(5), x.at(6), x.at(7), s);
+        o[0] = q.x;
+        o[1] = q.y;
     }
 }
 
@@ -101,7 +111,7 @@ __global__ void __launch_bounds__(256) mx_quantize_rows(const uint8_t* x, int64_
     a = max(a, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, kDppXor1, 0xF, 0xF, false));
     a = max(a, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, kDppXor2, 0xF, 0xF, false));
     const uint32_t code = mx_code<kMxEmax<ELEM>>(a >> 23);
-    mx_store8<ELEM>(codes + (int64_t)it * (ELEM == BZ_MX_E2M1 ? 4 : 8), v, __uint_as_float(code << 23));
+    mx_store8<ELEM>(codes + (int64_t)it * (ELEM == BZ_MX_E2M1 ? 4 : 8), v, code);
     if ((it & 3) == 0) scales[it >> 2] = (uint8_t)code;
 }
 
@@ -145,12 +155,8 @@ __global__ void __launch_bounds__(256) mx_quantize_tiled(const uint8_t* x, int64
             for (int h = 0; h < 2; ++h) {
                 const int c = 2 * g + h;
                 uint32_t q[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const X& e = v[2 * h + (i >> 1)];
-                    const int b = 4 * (i & 1);
-                    q[i] = mx8_pack_f32(e.at(b), e.at(b + 1), e.at(b + 2), e.at(b + 3), s);
-                }
+                v[2 * h].pack8(code, s, q[0], q[1]);
+                v[2 * h + 1].pack8(code, s, q[2], q[3]);
                 *reinterpret_cast<u32x4*>(t + (c >> 2) * 1024 + (16 * (c & 3) + r) * 16) = u32x4{q[0], q[1], q[2], q[3]};
             }
         }

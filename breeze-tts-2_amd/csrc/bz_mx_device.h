@@ -88,4 +88,24 @@ __device__ __forceinline__ uint32_t mx8_pack_f32(float a, float b, float c, floa
     return __builtin_bit_cast(uint32_t, r);
 }
 
+// The same of eight bf16 values (two dwords) without widening them: 448 times
+// a scale code's power of two is a bf16, and magnitudes compare as integers.
+typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void mx8_pack_bf16(u32x4 v, uint32_t code, float s, uint32_t& lo, uint32_t& hi) {
+    typedef short short2_t __attribute__((ext_vector_type(2)));
+    const unsigned short t = (unsigned short)((code + 8u) << 7 | 0x60u);
+    const us2_t top = {t, t};
+    auto clamp = [&](uint32_t x) {
+        const uint32_t m = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(us2_t, x & 0x7FFF7FFFu), top));
+        return as_bf16x2(m | (x & 0x80008000u));
+    };
+    short2_t a = {0, 0}, b = {0, 0};
+    a = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(a, clamp(v[0]), s, false);
+    a = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(a, clamp(v[1]), s, true);
+    b = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(b, clamp(v[2]), s, false);
+    b = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(b, clamp(v[3]), s, true);
+    lo = __builtin_bit_cast(uint32_t, a);
+    hi = __builtin_bit_cast(uint32_t, b);
+}
+
 }  // namespace bz

@@ -62,12 +62,11 @@ constexpr bool mx_gemv_built(int mt, int upw) { return mt == 1 || upw <= 5; }
 // four dwords; e4m3: eight).
 template <int ELEM>
 __device__ __forceinline__ uint32_t mx_quantize_block(const u32x4 (&v)[4], u32x4& lo, u32x4& hi) {
-    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
-    us2 m = {0, 0};  // magnitudes of bf16 compare as integers, NaN on top
+    us2_t m = {0, 0};  // magnitudes of bf16 compare as integers, NaN on top
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, v[i][e] & 0x7FFF7FFFu));
+        for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2_t, v[i][e] & 0x7FFF7FFFu));
     const uint32_t a = max((uint32_t)m[0], (uint32_t)m[1]);
     const uint32_t code = mx_code<ELEM == BZ_MX_E2M1 ? 2 : 8>(a >> 7);
     const float s = __uint_as_float(code << 23);
@@ -75,16 +74,14 @@ __device__ __forceinline__ uint32_t mx_quantize_block(const u32x4 (&v)[4], u32x4
         lo = u32x4{mx4_pack_bf16(v[0], s), mx4_pack_bf16(v[1], s), mx4_pack_bf16(v[2], s), mx4_pack_bf16(v[3], s)};
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t p = v[i][2 * h], q = v[i][2 * h + 1];
-                const uint32_t c = mx8_pack_f32(bf16_lo(p), bf16_hi(p), bf16_lo(q), bf16_hi(q), s);
-                if (i < 2)
-                    lo[2 * i + h] = c;
-                else
-                    hi[2 * (i - 2) + h] = c;
-            }
+        for (int i = 0; i < 4; ++i) {
+            uint32_t a, b;
+            mx8_pack_bf16(v[i], code, s, a, b);
+            if (i < 2)
+                lo[2 * i] = a, lo[2 * i + 1] = b;
+            else
+                hi[2 * i - 4] = a, hi[2 * i - 3] = b;
+        }
     }
     return code;
 }
