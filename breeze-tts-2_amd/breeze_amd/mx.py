@@ -47,7 +47,6 @@ FEW_ROWS = 32
 _ELEM = {"e2m1": MX_E2M1, "e4m3": MX_E4M3}
 _X = {torch.bfloat16: DT_BF16, torch.float32: DT_F32, torch.float16: MX_F16}
 _OUT = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
-_BYTES = (torch.uint8, torch.float8_e4m3fn, torch.int8)
 
 
 def _elem(elem: str) -> int:
@@ -131,8 +130,9 @@ def dequantize_mx(codes: torch.Tensor, scales: torch.Tensor, elem: str = "e2m1",
     dt = _OUT.get(dtype)
     if dt is None:
         raise TypeError(f"values are bfloat16 or float32, not {dtype}")
-    if len(shape) != 2 or codes.dtype not in _BYTES or scales.dtype is not torch.uint8:
-        raise ValueError("codes must be a 2-D tensor of bytes and scales uint8")
+    if len(shape) != 2 or scales.dtype is not torch.uint8 or not (
+            codes.dtype is torch.uint8 or code == MX_E4M3 and codes.dtype is torch.float8_e4m3fn):
+        raise ValueError("codes must be 2-D, uint8 (or float8_e4m3fn for e4m3), and scales uint8")
     M, K = shape
     if code == MX_E2M1:
         K *= 2
@@ -193,8 +193,8 @@ def _plan(elem: int, M: int, n: int, k: int, cfg: int, rows: bool) -> tuple[int,
     weight = int(lib.bz_tiled_bytes(W_MXFP4_TILED, n, k)) or -1
     if rows and 0 < M <= FEW_ROWS:
         need = int(lib.bz_mx_gemv_workspace(elem, M, n, k, cfg))
-        if need != _NO_WAY:
-            return weight, True, need
+        if need != _NO_WAY or cfg:  # (a forced shape it does not take is refused by the call)
+            return weight, True, 0 if need == _NO_WAY else need
     return weight, False, int(lib.bz_mx_gemm_workspace(elem, M, n, k, cfg))
 
 
@@ -222,7 +222,7 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
     if w.get_device() != index or w.numel() * w.element_size() != weight or not w.is_contiguous() or w.data_ptr() & 15:
         _gpu("w", w, index)
         raise ValueError(f"w must be a contiguous W_MXFP4_TILED weight of {n} x {K} (rows a multiple of 16), "
-                         f"{max(weight, 0)} bytes; got {w.numel() * w.element_size()}")
+                         f"{max(weight, 0)} bytes, at a multiple of 16; got {w.numel() * w.element_size()}")
     if out is None:
         odt = _OUT.get(out_dtype)
         if odt is None:

@@ -16,7 +16,7 @@ and Fp8Linear do: a decode step is bound by the weight's bytes.  Longer ones
 (a prompt) are bound by the matrix cores, and ``act_bits`` says what they
 multiply: 16, the bf16 activations; 8 or 4, activations quantised to
 microscaled blocks (e4m3 or e2m1) on the way, at the matrix cores' 8- or 4-bit
-rate.
+rate, and without a gradient.
 """
 
 from __future__ import annotations
@@ -90,8 +90,10 @@ class Mxfp4Linear(nn.Module):
             flat = flat.to(torch.bfloat16)
         if k_pad != k:
             flat = torch.nn.functional.pad(flat, (0, k_pad - k))
-        # (a traced call is a GEMV of any row count, as for the other modules)
-        if flat.shape[0] <= PREFILL_ROWS or torch.compiler.is_compiling():
+        # a traced call is a GEMV of any row count, as for the other modules; one
+        # that autograd follows goes the way of the prompts, which it can follow
+        grad = flat.requires_grad and torch.is_grad_enabled()
+        if torch.compiler.is_compiling() or (flat.shape[0] <= PREFILL_ROWS and not grad):
             out = gemv_traceable(flat, w, W_MXFP4_TILED, n_pad)
         elif self.act_bits == 16:
             out = dequant_matmul(flat, w, W_MXFP4_TILED, n_pad, k_pad)

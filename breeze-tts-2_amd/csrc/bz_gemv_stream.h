@@ -268,8 +268,9 @@ __global__ void __launch_bounds__(1024) gemv_stream(const uint8_t* hw, const uin
         for (int q = 0; q < UPW; ++q) sc[q] = buffer_ld4(srs, mx_scale_offset(u0 + q, lane));
     }
     u32x4 wv[UPW];
-    const uint32_t wlane = tiled_lane_byte(WF, lane);
-    auto issue = [&](int q) { wv[q] = buffer_ld16_nt(wrs, (uint32_t)(u0 + q) * 1024u + wlane); };
+    auto issue = [&](int q) {
+        wv[q] = buffer_ld16_nt(wrs, (uint32_t)(u0 + q) * 1024u + (MX ? lane * 16 : j * 64 + kq * 16));
+    };
     // Long rows (80 units or more) over at most 256 row blocks (at most one
     // workgroup per CU): the x loads get about 270 ns before the first tiles
     // go out, so they do not queue behind the tiles of every wave of the CU.

@@ -151,13 +151,12 @@ __global__ void __launch_bounds__(1024) gemv_wide(const uint8_t* hw, const uint1
     // two register sets with fixed roles (a: even blocks, b: odd blocks), so
     // no tile register is carried around the block loop (a carried one made
     // the compiler wait for every load in flight at each block)
-    const uint32_t wlane = tiled_lane_byte(WF, lane);
     u32x4 wa[UPW], wb[UPW];
     uint32_t sa[UPW], sb[UPW];
     auto issue = [&](int jb, int q, u32x4* wv, uint32_t* sc) {  // unit q of block jb into slot q
         const bool ok = jb < nb && u0 + q < NU;
         const uint32_t base = (uint32_t)(jb * p.chunk);
-        wv[q] = buffer_ld16_nt(wrs, ok ? base + (uint32_t)(u0 + q) * 1024u + wlane : kBufferOob);
+        wv[q] = buffer_ld16_nt(wrs, ok ? base + (uint32_t)(u0 + q) * 1024u + (MX ? lane * 16 : j * 64 + kq * 16) : kBufferOob);
         if (MX) sc[q] = buffer_ld4(wrs, ok ? base + (uint32_t)NU * 1024u + mx_scale_offset(u0 + q, lane) : kBufferOob);
         if (I4) sc[q] = buffer_ld4(wrs, ok ? base + (uint32_t)NU * 1024u + (uint32_t)(u0 + q) * 64u + j * 4 : kBufferOob);
     };

@@ -91,6 +91,9 @@ __global__ void pack_mx4_kernel(bool src_tiled, const uint8_t* src, const uint8_
             cb[(int64_t)NU * 1024 + mx_scale_offset(u, ld) + (u & 3)] =
                 src_tiled ? sb[(int64_t)NU * 1024 + mx_scale_offset(u, ls) + (u & 3)]
                           : sc0[(int64_t)rs * (K / 32) + u * 4 + q];
+            // the codes of units past the row: the kernels multiply their zeros too
+            if (u == NU - 1)
+                for (int v = NU; v & 3; ++v) cb[(int64_t)NU * 1024 + mx_scale_offset(v, ld) + (v & 3)] = 0;
         }
     }
 }

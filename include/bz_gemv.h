@@ -83,7 +83,7 @@ typedef enum bz_status {
  *   tile of 1024 bytes holds the four 32-k blocks of its 16 rows block by
  *   block (block g of row r at byte 256 g + 16 r), and the scales follow the
  *   tiles, per four units 256 bytes (unit u, block g, row r at byte 64 g +
- *   4 r + u % 4).  Runs on paths 5 and 6; w_eff is exact in bf16, so the
+ *   4 r + u % 4; the bytes of units past the last are zero).  Runs on paths 5 and 6; w_eff is exact in bf16, so the
  *   products equal those of the bf16 weight.
  * The tiled formats run on GEMV path 5, the streaming kernel (M <= 8 rows
  * per launch; more rows run as several launches), and the unpaired ones also
@@ -340,7 +340,8 @@ size_t bz_tiled_bytes(int32_t wfmt, int32_t N, int32_t K);
  * work with no counterpart in the reference: it replaces the repack step of
  * torch._convert_weight_to_int4pack (models/int4_linear.py:59) by this
  * build's own layout.  Bytes a call does not cover (chunk padding, rows of
- * other calls) are left as they are. */
+ * other calls) are left as they are, but for the MXFP4 scale codes past a
+ * row's last unit, which are written as zeros. */
 int bz_pack_tiled(int32_t src_wfmt, const void* src_w, const void* src_sc0, int32_t n, int32_t K, int32_t group,
                   int32_t dst_wfmt, void* dst, int32_t N, int32_t row0, void* stream);
 

@@ -556,3 +556,166 @@ def test_fused_weight_of_modules():
     gu = FK.rms_gemv(x, unpaired, g)
     two = FK.rms_gemv(x, unpaired, g, epilogue=G.EPI_SILU_GATE)
     assert torch.equal(two, FK.silu_mul(gu[:, :512], gu[:, 512:]))
+
+
+def test_fused_layer_of_modules():
+    """A decoder layer whose seven projections are Mxfp4Linear, step by step
+    against the float32 layer with the dequantised weights (the bar of
+    tests/test_gpu_layer.py)."""
+    import copy
+
+    from breeze_amd.fused.layer import FusedDecoderLayer
+    from tests.test_gpu_layer import TOL, _cfg, _layer, _run_steps
+
+    cfg = _cfg()
+    layer = _layer(cfg)
+    ref, own = copy.deepcopy(layer), copy.deepcopy(layer).to("cuda", BF16)
+    names = ("gate_proj", "up_proj", "down_proj", "q_proj", "k_proj", "v_proj", "o_proj")
+    assert M4.quantize_module_mxfp4(own, target_names=names, min_bytes=0, act_bits=8)["converted"] == 7
+    for name, lin in ref.named_modules():
+        if name.rpartition(".")[2] in names:
+            with torch.no_grad():
+                lin.weight.copy_(torch.from_numpy(O.rounded(lin.weight.double().numpy(), O.E2M1)).float())
+    errs, c_ref, c_own = _run_steps(cfg, ref, FusedDecoderLayer(own, 0), B=2, S=64, steps=8)
+    assert max(errs) <= TOL, errs
+
+
+# ---- calls beside each other, and what earlier calls leave behind -------------------------------------------
+
+
+@pytest.mark.parametrize("m", [1, 9, 33])
+@pytest.mark.parametrize("k", [128, 384, 640])
+def test_packing_into_a_used_buffer(m, k):
+    """Rows whose last units do not fill a dword of scale codes: what the buffer held is not read."""
+    w, x = Weight(48, k), _rows(m, k, 18)
+    used = torch.full_like(w.tiled, 255)
+    G.pack_tiled(G.W_MXFP4, w.rows, k, w.fmt, sc0=w.sc, out=used)
+    assert torch.equal(used, w.tiled)
+    again = torch.full_like(used, 255)
+    G.pack_tiled(G.W_MXFP4_TILED, used, k, w.fmt, out=again)
+    assert torch.equal(again, w.tiled)
+    _close((G.gemv if m <= 32 else lambda x, w, f, n: G.dequant_matmul(x, w, f, n, k))(x, used, w.fmt, 48),
+           *_gemv_reference(x, w, G.EPI_NONE, None, 0.0, None, BF16))
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("m", [40, 300])
+def test_short_rows_after_rows_of_nan(elem, m):
+    """LDS holds codes of NaN from the call before; units past a short row are zeros all the same."""
+    bad = torch.full((m, 1024), float("nan"), device="cuda", dtype=BF16)
+    wide = Weight(1024, 1024)
+    for k in (128, 256, 384, 640):
+        w, x = Weight(1024, k), _rows(m, k, 19)
+        assert mx.mx_linear(bad, wide.tiled, 1024, elem=elem).isnan().all()
+        _close(mx.mx_linear(x, w.tiled, 1024, elem=elem), *_mx_reference(x, w, elem, None, BF16))
+
+
+def test_forced_shapes():
+    """Every launch shape that is built, and refusals of those that are not."""
+    n, k = 272, 1664
+    w = Weight(n, k)
+    for elem in ELEMS:
+        for m in (5, 32):
+            x = _rows(m, k, 21)
+            ref, bound = _mx_reference(x, w, elem, None, BF16)
+            for t in (1, 2, 3, 8):
+                for upw, nsl in ((0, 0), (0, 3), (1, 2), (2, 1), (3, 1), (4, 2), (5, 1), (5, 13)):
+                    _close(mx.mx_linear(x, w.tiled, n, elem=elem, cfg=t | upw << 8 | nsl << 16), ref, bound)
+        x = _rows(150, k, 22)
+        ref, bound = _mx_reference(x, w, elem, None, BF16)
+        for a, b in ((1, 2), (2, 2), (4, 2), (6, 2), (4, 4), (8, 4) if elem == O.E2M1 else (6, 4)):
+            for nsl in (0, 1, 2, 4):
+                _close(mx.mx_linear(x, w.tiled, n, elem=elem, cfg=a | b << 8 | nsl << 16), ref, bound)
+        for m, cfg in ((5, 9), (5, 7 << 8), (5, 65 << 16), (150, 3), (150, 1 | 4 << 8), (150, 65 << 16)):
+            with pytest.raises(L.BzError):
+                mx.mx_linear(_rows(m, k, 23), w.tiled, n, elem=elem, cfg=cfg)
+
+
+def test_threads_and_streams_at_once():
+    """Products that slice K from host threads, on one stream and on their own."""
+    import threading
+
+    n, k = 1024, 8192
+    w = Weight(n, k)
+    xs = [_rows(m, k, 24 + m) for m in (5, 20, 40, 64)]
+    want = [mx.mx_linear(x, w.tiled, n, elem="e4m3") for x in xs]
+    torch.cuda.synchronize()
+    for own_stream in (False, True):
+        wrong = []
+
+        def work(i):
+            stream = torch.cuda.Stream() if own_stream else torch.cuda.current_stream()
+            with torch.cuda.stream(stream):
+                for _ in range(40):
+                    got = mx.mx_linear(xs[i], w.tiled, n, elem="e4m3")
+                    stream.synchronize()
+                    if not torch.equal(got, want[i]):
+                        wrong.append(i)
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(len(xs))]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not wrong
+
+
+def test_two_graphs_at_once():
+    """Two captured products that slice K, replayed on two streams."""
+    n, k = 1024, 8192
+    w = Weight(n, k)
+    xs = [_rows(5, k, 30), _rows(48, k, 31)]
+    want = [mx.mx_linear(x, w.tiled, n) for x in xs]
+    graphs, outs = [], []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(mx.mx_linear(x, w.tiled, n))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, e in zip(outs, want):
+            assert torch.equal(o, e)
+            o.zero_()
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_module_gradient_of_any_call(rows):
+    lin = nn.Linear(256, 48, bias=False).cuda()
+    mod, x = M4.Mxfp4Linear(lin), torch.randn(rows, 256, device="cuda", requires_grad=True)
+    g = torch.randn(rows, 48, device="cuda").to(BF16)
+    mod(x).backward(g.float())
+    wq = O.rounded(_np(lin.weight), O.E2M1)
+    ref = _np(g) @ wq
+    _close(x.grad, ref, 2.0 ** -8 * np.abs(ref) + 48 * 2.0 ** -24 * (np.abs(_np(g)) @ np.abs(wq)))
+    with torch.no_grad():
+        assert torch.equal(mod(x), mod(x.detach()))
+
+
+def test_large_row_offsets():
+    """Rows whose codes and outputs lie past 2^31 bytes of one another."""
+    m, k, n = 70_000, 16_384, 32
+    x = torch.zeros(m, k, device="cuda", dtype=BF16)  # 2.3 GB
+    tail = _rows(300, k, 32)
+    x[-300:] = tail
+    w = Weight(n, k)
+    ref = mx.mx_linear(tail, w.tiled, n, elem="e4m3")
+    out = mx.mx_linear(x, w.tiled, n, elem="e4m3")
+    assert not out[:-300].any() and torch.equal(out[-300:], ref)
+    codes, scales = mx.quantize_mx(x, "e4m3")
+    assert torch.equal(mx.dequantize_mx(codes[-300:], scales[-300:], "e4m3"),
+                       mx.dequantize_mx(*mx.quantize_mx(tail, "e4m3"), "e4m3"))
+    del x, codes, scales
+    wide = torch.empty(400, 6_000_000, device="cuda", dtype=BF16)  # rows 12 MB apart
+    view = wide[:, 1024:1024 + k]
+    view[:300] = tail
+    assert torch.equal(mx.mx_linear(view[:300], w.tiled, n, elem="e4m3"), ref)
+    few = mx.mx_linear(tail[:20], w.tiled, n, elem="e4m3")
+    _close(mx.mx_linear(view[:20], w.tiled, n, elem="e4m3"), *_mx_reference(tail[:20], w, "e4m3", None, BF16))
+    assert few.shape == (20, n)
