@@ -65,6 +65,12 @@ def _table(arch: str) -> dict:
     return t
 
 
+def plans(index: int) -> dict:
+    """What callers derive from the table of this device's architecture, under
+    keys of their own: forgotten with the table."""
+    return _table(_ARCH.get(index) or arch_of(torch.device("cuda", index)))
+
+
 def lookup(device: torch.device, N: int, K: int, wfmt: int, epilogue: int, norm: bool, M: int) -> Optional[tuple]:
     """The table's launch shape for this GEMV, or None for the built-in rule."""
     arch = arch_of(device)
