@@ -212,6 +212,9 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
     if rows:
         src, (M, K), code = x.data, x.shape, _elem(x.elem)
         index, few = src.get_device(), False
+        if index < 0 or src.numel() * src.element_size() != _rows_bytes(code, M, K) or not src.is_contiguous():
+            _gpu("x", src, index)
+            raise ValueError(f"these are not the MxRows of {M} x {K} {x.elem} rows")
     else:
         code = _elem(elem)
         src, M, K, ld, dt, index = _rows(x, 128)

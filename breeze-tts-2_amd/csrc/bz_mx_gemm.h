@@ -50,15 +50,15 @@ __device__ __forceinline__ void mx_load_lds(__amdgpu_buffer_rsrc_t r, char* p, u
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)p, 16, lane_off, off, 0, 0);
 }
 
-constexpr int kMxWavesM = 2;  // waves along the rows of x; WN along the weight's
+constexpr int kMxWaves = 8;   // WM along the rows of x, the rest along the weight's
 constexpr int kMxStages = 4;
 constexpr int kMxCounters = 4096;
 constexpr size_t kMxPartOffset = kMxCounters * 4;
 
-template <int ELEM, int MT, int NT, int WN>
+template <int ELEM, int MT, int NT, int WM>
 struct MxShape {
     static constexpr int XP = ELEM == BZ_MX_E2M1 ? 1 : 2;  // KiB of an x tile
-    static constexpr int TM = MT * kMxWavesM, TN = NT * WN, kWaves = kMxWavesM * WN;
+    static constexpr int kWaves = kMxWaves, TM = MT * WM, TN = NT * (kWaves / WM);
     static constexpr int kPieces = TM * XP + TN;           // KiB of a stage
     // of each wave; few x tiles are loaded by several waves, to the same place
     static constexpr int kXLoads = (TM * XP + kWaves - 1) / kWaves, kLoads = kXLoads + TN / kWaves;
@@ -70,16 +70,16 @@ struct MxShape {
 // s_waitcnt for all LDS operations and all but n vector memory ones (6 bits, split).
 constexpr int mx_wait(int n) { return (n & 15) | (n >> 4) << 14 | 0x0070; }
 
-template <int ELEM, int MT, int NT, int WN>
-__global__ void __launch_bounds__(64 * kMxWavesM * WN, 2) mx_gemm(MxGemmParams p) {
-    using S = MxShape<ELEM, MT, NT, WN>;
+template <int ELEM, int MT, int NT, int WM>
+__global__ void __launch_bounds__(64 * kMxWaves, 2) mx_gemm(MxGemmParams p) {
+    using S = MxShape<ELEM, MT, NT, WM>;
     constexpr int W = S::kWaves, XP = S::XP, TM = S::TM, TN = S::TN, L = S::kLoads, LX = S::kXLoads, SC = MT + NT;
     // one array a stage: the compiler then knows which loads into LDS a read waits for
     __shared__ __attribute__((aligned(16))) char s0[S::kPieces * 1024], s1[S::kPieces * 1024], s2[S::kPieces * 1024],
         s3[S::kPieces * 1024];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave & 1, wn = wave >> 1;
+    const int wm = wave % WM, wn = wave / WM;
 
     // this workgroup's tile: XCD c = bid % 8 takes a run of consecutive ids,
     // which go down `band` row tiles, then to the next column tile
@@ -305,44 +305,46 @@ __global__ void __launch_bounds__(64 * kMxWavesM * WN, 2) mx_gemm(MxGemmParams p
 }
 
 struct MxGemmLaunch {
-    int mt, nt;
+    int tm, tn;  // 32 rows of x and 64 of the weight in a tile
     unsigned grid;
 };
 
-constexpr int kMxWn = 4;
-// The shapes that are built: 16-row groups of x and row blocks of the weight
-// of each wave (32 mt rows of x and 64 nt of the weight in a tile).
-constexpr bool mx_shape_ok(int elem, int mt, int nt) {
-    return nt == 2 ? mt == 1 || mt == 2 || mt == 4 || mt == 6
-                   : nt == 4 && (mt == 4 || mt == (elem == BZ_MX_E2M1 ? 8 : 6));
+// The tiles that are built, in 32 rows of x and 64 of the weight.
+constexpr bool mx_shape_ok(int elem, int tm, int tn) {
+    return tn == 2 ? tm == 1 || tm == 2 || tm == 4 || tm == 6
+                   : tn == 4 && (tm == 4 || tm == (elem == BZ_MX_E2M1 ? 8 : 6));
 }
+// Waves along the rows of x.  A wave reads its rows of x and of the weight from
+// LDS, MT * XP + NT KiB for MT * NT products.
+constexpr int mx_waves_m(int tm, int tn) { return tn == 2 && tm >= 4 ? 4 : 2; }
 
-template <int ELEM, int MT, int NT>
+template <int ELEM, int TM, int TN>
 int launch_mx_gemm_kernel(const MxGemmParams& p, const MxGemmLaunch& l, hipStream_t st) {
-    if constexpr (mx_shape_ok(ELEM, MT, NT)) {
-        static_assert(MxShape<ELEM, MT, NT, kMxWn>::ok);
-        hipLaunchKernelGGL((mx_gemm<ELEM, MT, NT, kMxWn>), dim3(l.grid), dim3(64 * kMxWavesM * kMxWn), 0, st, p);
+    if constexpr (mx_shape_ok(ELEM, TM, TN)) {
+        constexpr int WM = mx_waves_m(TM, TN), MT = 2 * TM / WM, NT = TN * 4 * WM / kMxWaves;
+        static_assert(MxShape<ELEM, MT, NT, WM>::ok && MT * WM == 2 * TM);
+        hipLaunchKernelGGL((mx_gemm<ELEM, MT, NT, WM>), dim3(l.grid), dim3(64 * kMxWaves), 0, st, p);
         return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
     } else {
         return BZ_ERR_INVALID_ARG;
     }
 }
-template <int ELEM, int NT>
-int launch_mx_gemm_nt(const MxGemmParams& p, const MxGemmLaunch& l, hipStream_t st) {
-    switch (l.mt) {
-        case 1: return launch_mx_gemm_kernel<ELEM, 1, NT>(p, l, st);
-        case 2: return launch_mx_gemm_kernel<ELEM, 2, NT>(p, l, st);
-        case 4: return launch_mx_gemm_kernel<ELEM, 4, NT>(p, l, st);
-        case 6: return launch_mx_gemm_kernel<ELEM, 6, NT>(p, l, st);
-        case 8: return launch_mx_gemm_kernel<ELEM, 8, NT>(p, l, st);
+template <int ELEM, int TN>
+int launch_mx_gemm_tn(const MxGemmParams& p, const MxGemmLaunch& l, hipStream_t st) {
+    switch (l.tm) {
+        case 1: return launch_mx_gemm_kernel<ELEM, 1, TN>(p, l, st);
+        case 2: return launch_mx_gemm_kernel<ELEM, 2, TN>(p, l, st);
+        case 4: return launch_mx_gemm_kernel<ELEM, 4, TN>(p, l, st);
+        case 6: return launch_mx_gemm_kernel<ELEM, 6, TN>(p, l, st);
+        case 8: return launch_mx_gemm_kernel<ELEM, 8, TN>(p, l, st);
         default: return BZ_ERR_INVALID_ARG;
     }
 }
 template <int ELEM>
 int launch_mx_gemm_elem(const MxGemmParams& p, const MxGemmLaunch& l, hipStream_t st) {
-    switch (l.nt) {
-        case 2: return launch_mx_gemm_nt<ELEM, 2>(p, l, st);
-        case 4: return launch_mx_gemm_nt<ELEM, 4>(p, l, st);
+    switch (l.tn) {
+        case 2: return launch_mx_gemm_tn<ELEM, 2>(p, l, st);
+        case 4: return launch_mx_gemm_tn<ELEM, 4>(p, l, st);
         default: return BZ_ERR_INVALID_ARG;
     }
 }

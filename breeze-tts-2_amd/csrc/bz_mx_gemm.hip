@@ -12,11 +12,11 @@ struct MxGemmPlan {
     size_t ws;
 };
 
-static int mx_gemm_shape(int M, int N, int K, int mt, int nt, int nsl, MxGemmPlan& pl) {
+static int mx_gemm_shape(int M, int N, int K, int tm32, int tn64, int nsl, MxGemmPlan& pl) {
     const int mblk = (M + 15) / 16, nblk = N / 16, groups = (K / 128 + 3) / 4;
-    const int tm = mt * kMxWavesM, tn = nt * kMxWn;
-    pl.l.mt = mt;
-    pl.l.nt = nt;
+    const int tm = 2 * tm32, tn = 4 * tn64;
+    pl.l.tm = tm32;
+    pl.l.tn = tn64;
     pl.mtiles = (mblk + tm - 1) / tm;
     pl.ntiles = (nblk + tn - 1) / tn;
     const int64_t tiles = (int64_t)pl.mtiles * pl.ntiles;
@@ -31,49 +31,50 @@ static int mx_gemm_shape(int M, int N, int K, int mt, int nt, int nsl, MxGemmPla
 }
 
 // Microseconds a launch shape is expected to take, from which the rule picks
-// the smallest: a workgroup's start and end (wg0) and its units; with room for
-// several workgroups on a CU a unit takes the longer of one workgroup's time
-// and of the CU's for all it holds (full); the workspace's traffic where K is
-// sliced; and reading x and the weight for every tile.  Fitted to graph
-// replays over 13 (N, K) (the model's layers, 1024 squared, 656 x 384 and 7408
-// x 3968), M = 33 .. 2048 and 1 .. 8 slices on MI355X, 7211 timings.  Over
-// those the shape it picks takes 2.2% (e2m1) / 1.8% (e4m3) longer than the
-// best one of the sweep, which had 19 shapes, on average; at worst 19% (M =
-// 100, N 20480, K 2560: 11.4 us for 9.6) / 39% (M = 400, N 2560, K 10240: 28.6
-// for 20.6).
+// the smallest: a workgroup's start and end (wg0) and its units, which take the
+// longer of one workgroup's time (unit) and, where several fit a CU, of the
+// CU's for all it holds (full each); the workspace's traffic where K is sliced;
+// and reading x and the weight for every tile.  Workgroups come in whole rounds
+// over the 256 CUs; where one fills a CU, the last round's are spread a little
+// (0.2 of it counts by its share).  Fitted to graph replays over 15 (N, K) (the
+// model's layers, 1024 squared, 656 x 384, 4800 x 640 and 7408 x 3968), M = 33
+// .. 2048 and 1 .. 8 slices on MI355X, 6169 timings.  Over those the shape it
+// picks takes 1.0% (e2m1) / 0.3% (e4m3) longer than the best one on average, at
+// worst 20% (M = 400, N 2560, K 10240: 22.3 us for 18.6) / 7%.
 struct MxGemmCost {
-    int mt, nt;
+    int tm, tn;
     float wg0, unit, full, sum0, sum_mb, traffic_mb;
 };
 constexpr MxGemmCost kMxCostE2m1[] = {
-    {1, 2, 3.435f, 0.1493f, 0.1647f, 2.297f, 0.3003f, 0.01155f},
-    {2, 2, 3.695f, 0.1696f, 0.1919f, 2.457f, 0.2701f, 0.01151f},
-    {4, 2, 4.149f, 0.2301f, 0.2958f, 2.936f, 0.2929f, 0.01471f},
-    {6, 2, 4.86f, 0.313f, 0.4354f, 4.551f, 0.2658f, 0.02368f},
-    {4, 4, 5.208f, 0.3543f, 0.03681f, 6.453f, 0.1808f, 0.01889f},
-    {8, 4, 8.477f, 0.5144f, 0.1102f, 10.3f, 0.1231f, 0.0387f},
+    {1, 2, 3.492f, 0.1442f, 0.1346f, 2.414f, 0.2298f, 0.01163f},
+    {2, 2, 3.798f, 0.1564f, 0.1414f, 2.791f, 0.2351f, 0.01697f},
+    {4, 2, 4.336f, 0.2222f, 0.2074f, 2.97f, 0.269f, 0.01945f},
+    {6, 2, 5.324f, 0.2988f, 0.294f, 3.458f, 0.2343f, 0.02057f},
+    {4, 4, 5.804f, 0.3463f, 0.0f, 5.006f, 0.2019f, 0.01741f},
+    {8, 4, 8.683f, 0.5218f, 0.0f, 9.015f, 0.1578f, 0.03885f},
 };
 constexpr MxGemmCost kMxCostE4m3[] = {
-    {1, 2, 3.481f, 0.1694f, 0.1605f, 2.288f, 0.3089f, 0.01263f},
-    {2, 2, 3.702f, 0.1891f, 0.2153f, 2.427f, 0.3021f, 0.01287f},
-    {4, 2, 4.202f, 0.3289f, 0.3259f, 3.312f, 0.2267f, 0.01016f},
-    {6, 2, 5.035f, 0.4422f, 0.1915f, 5.155f, 0.2229f, 0.01297f},
-    {4, 4, 5.432f, 0.4727f, 0.253f, 7.898f, 0.1254f, 0.02434f},
-    {6, 4, 6.983f, 0.706f, 0.2364f, 8.631f, 0.1302f, 0.03006f},
+    {1, 2, 3.503f, 0.1696f, 0.14f, 2.381f, 0.2329f, 0.01058f},
+    {2, 2, 3.774f, 0.1825f, 0.1605f, 2.503f, 0.295f, 0.01348f},
+    {4, 2, 4.103f, 0.3225f, 0.0f, 3.248f, 0.2535f, 0.009315f},
+    {6, 2, 4.817f, 0.4247f, 0.0f, 3.577f, 0.236f, 0.01382f},
+    {4, 4, 5.961f, 0.4698f, 0.0f, 5.354f, 0.1974f, 0.02202f},
+    {6, 4, 7.125f, 0.7275f, 0.0f, 7.692f, 0.1409f, 0.02822f},
 };
 
 static float mx_gemm_cost(int elem, int M, int N, int K, const MxGemmCost& c, const MxGemmPlan& pl) {
     const int xp = elem == BZ_MX_E2M1 ? 1 : 2;
-    const int lds = (kMxWavesM * c.mt * xp + kMxWn * c.nt) * kMxStages;  // KiB
-    const float units = 4.0f * pl.gps, full = (float)pl.l.grid / 256.0f, room = (float)(160 / lds);
+    const int lds = (2 * c.tm * xp + 4 * c.tn) * kMxStages;  // KiB
+    const int room = 160 / lds;                              // workgroups on a CU
+    const float units = 4.0f * pl.gps, rounds = (float)((pl.l.grid + 255) / 256);
     float t;
-    if (room < 2.0f)
-        t = (c.wg0 + units * c.unit) * (float)((pl.l.grid + 255) / 256);
-    else if (full <= room)
-        t = c.wg0 + units * std::max(c.unit, c.full * full);
+    if (room < 2)
+        t = (c.wg0 + units * c.unit) * (0.8f * rounds + 0.2f * std::max(1.0f, (float)pl.l.grid / 256.0f));
+    else if (rounds <= (float)room)
+        t = c.wg0 + units * std::max(c.unit, c.full * rounds);
     else
-        t = (c.wg0 + units * c.full * room) * full / room;
-    const float tile_mb = (float)(kMxWavesM * c.mt * kMxWn * c.nt) * 1024e-6f;
+        t = (c.wg0 + units * c.full * (float)room) * rounds / (float)room;
+    const float tile_mb = (float)(8 * c.tm * c.tn) * 1024e-6f;
     if (pl.nsl > 1) t += c.sum0 + c.sum_mb * (float)pl.l.grid * tile_mb;
     const float w_mb = (float)N * (float)K * 0.53e-6f, x_mb = (float)M * (float)K * 0.53e-6f * xp;
     return t + c.traffic_mb * ((float)pl.mtiles * w_mb + (float)pl.ntiles * x_mb);
@@ -83,16 +84,19 @@ constexpr int kMxSlices[] = {1, 2, 3, 4, 6, 8};
 constexpr unsigned kMxSlicedGrid = 600;  // more workgroups than this never won with slices
 
 static int mx_gemm_plan(int elem, int M, int N, int K, int cfg, MxGemmPlan& pl) {
-    const int cmt = cfg & 255, cnt = (cfg >> 8) & 255, csl = cfg >> 16;
+    const int ctm = cfg & 255, ctn = (cfg >> 8) & 255, csl = cfg >> 16;
     if (csl > 64) return BZ_ERR_INVALID_ARG;
     float best = 0.0f;
     bool found = false;
-    auto look = [&](const MxGemmCost& c) -> int {
-        if ((cmt && cmt != c.mt) || (cnt && cnt != c.nt)) return BZ_OK;
+    int rc = BZ_ERR_INVALID_ARG;
+    auto look = [&](const MxGemmCost& c) {
+        if ((ctm && ctm != c.tm) || (ctn && ctn != c.tn)) return;
         for (int nsl : kMxSlices) {
             MxGemmPlan q;
-            const int rc = mx_gemm_shape(M, N, K, c.mt, c.nt, csl ? csl : nsl, q);
-            if (rc != BZ_OK) return rc;
+            if (mx_gemm_shape(M, N, K, c.tm, c.tn, csl ? csl : nsl, q) != BZ_OK) {
+                rc = BZ_ERR_UNSUPPORTED;  // (too many workgroups: a larger tile may do)
+                continue;
+            }
             if (!csl && nsl > 1 && (q.l.grid > kMxSlicedGrid || q.nsl != nsl)) continue;
             const float t = mx_gemm_cost(elem, M, N, K, c, q);
             if (!found || t < best) {
@@ -102,17 +106,12 @@ static int mx_gemm_plan(int elem, int M, int N, int K, int cfg, MxGemmPlan& pl) 
             }
             if (csl) break;
         }
-        return BZ_OK;
     };
-    int rc = BZ_ERR_INVALID_ARG;
-    if (elem == BZ_MX_E2M1) {
-        for (const MxGemmCost& c : kMxCostE2m1)
-            if ((rc = look(c)) != BZ_OK) return rc;
-    } else {
-        for (const MxGemmCost& c : kMxCostE4m3)
-            if ((rc = look(c)) != BZ_OK) return rc;
-    }
-    return found ? BZ_OK : BZ_ERR_INVALID_ARG;
+    if (elem == BZ_MX_E2M1)
+        for (const MxGemmCost& c : kMxCostE2m1) look(c);
+    else
+        for (const MxGemmCost& c : kMxCostE4m3) look(c);
+    return found ? BZ_OK : rc;
 }
 
 static int mx_gemm_check(int elem, int M, int N, int K) {

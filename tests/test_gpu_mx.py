@@ -719,3 +719,25 @@ def test_large_row_offsets():
     few = mx.mx_linear(tail[:20], w.tiled, n, elem="e4m3")
     _close(mx.mx_linear(view[:20], w.tiled, n, elem="e4m3"), *_mx_reference(tail[:20], w, "e4m3", None, BF16))
     assert few.shape == (20, n)
+
+
+def test_more_small_tiles_than_a_launch_holds():
+    """The launch shapes with the smallest tiles are passed over, not the call refused."""
+    m, n, k = 270_000, 131_072, 128
+    x, w = _rows(400, k, 33), Weight(n, k)
+    big = torch.zeros(m, k, device="cuda", dtype=BF16)
+    big[:200], big[-200:] = x[:200], x[200:]
+    out = mx.mx_linear(big, w.tiled, n)  # 71 GB
+    few = mx.mx_linear(x, w.tiled, n)
+    assert torch.equal(out[:200], few[:200]) and torch.equal(out[-200:], few[200:]) and not out[m // 2].any()
+
+
+def test_rows_that_are_not_of_their_shape():
+    w, q = Weight(32, 256), mx.mx_rows(_rows(40, 256))
+    for data, shape in ((q.data[:-16], q.shape), (q.data, (64, 256)), (q.data, (40, 128))):
+        with pytest.raises(ValueError):
+            mx.mx_linear(mx.MxRows(data, shape, q.elem), w.tiled, 32)
+    with pytest.raises(ValueError, match="MxRows"):
+        mx.mx_linear(mx.MxRows(q.data, q.shape, O.E4M3), w.tiled, 32)
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        mx.mx_linear(mx.MxRows(q.data.cpu(), q.shape, q.elem), w.tiled.cpu(), 32)
