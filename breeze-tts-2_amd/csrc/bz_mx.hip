@@ -1,6 +1,11 @@
 // Microscaled blocks (bz_mx_device.h): quantising rows and reading them back.
 //
-// Both are one pass over memory and bound by it.
+// Both are one pass over memory and bound by it; a few rows by the launch.
+// Measured on MI355X (kernel trace; a copy of 1 GiB reaches 5.2 TB/s, and what
+// the last-level cache still holds comes faster): 10240 x 2560 fp32 to e2m1
+// 17.1 us (6.9 TB/s), 2011 x 10240 bf16 to e4m3 11.1 us (5.7) and back 9.6 us
+// (6.5), 2 x 2560 1.3 us either way; tiled, 2011 x 10240 to e4m3 11.9 us (5.3),
+// 8192 x 2560 to e2m1 11.3 us (4.7).
 #include <algorithm>
 
 #include "bz_mx.h"
@@ -94,7 +99,9 @@ __device__ __forceinline__ void mx_store8(uint8_t* at, const X& x, uint32_t code
 }
 
 // Row-major: eight values per lane, a block per quad of lanes, so loads and
-// stores of a wave are contiguous.
+// stores of a wave are contiguous and the largest magnitude of a block takes
+// two exchanges within the quad.  One item a lane: there is nothing to keep
+// from one to the next, and the grid's waves hide the loads.
 template <int ELEM, class X>
 __global__ void __launch_bounds__(256) mx_quantize_rows(const uint8_t* x, int64_t ldx, uint32_t items, int K8, bool vec,
                                                         uint8_t* codes, uint8_t* scales) {
@@ -117,7 +124,9 @@ __global__ void __launch_bounds__(256) mx_quantize_rows(const uint8_t* x, int64_
 
 // Tiled: a workgroup takes four units of a row block, a wave one of them, a
 // lane a block (lane 16 g + r: block g of row r), so a tile is stored in one
-// instruction.  Rows past M are zeros.
+// instruction and the four units' scale codes leave as one dword a lane, by way
+// of LDS.  A lane's loads are 64 contiguous bytes, four of them a line of a
+// row.  Rows past M are zeros.
 template <int ELEM, class X>
 __global__ void __launch_bounds__(256) mx_quantize_tiled(const uint8_t* x, int64_t ldx, int M, int NU, bool vec,
                                                          uint8_t* out, int64_t chunk, int groups) {

@@ -3,7 +3,40 @@
 //
 // Arithmetic: v_mfma_scale_f32_16x16x128_f8f6f4, A = 16 weight rows, B = 16
 // rows of x, each lane with one block of 32 k and its scale code; D[n][m]
-// lands in lane m + 16 (n / 4), element n % 4.
+// lands in lane m + 16 (n / 4), element n % 4.  Sums stay in fp32 until the
+// result's one rounding.
+//
+// Work decomposition
+//   * A workgroup of eight waves owns a tile of 32 TM rows of x and 64 TN of
+//     the weight, a unit (128 k) at a time.  Both operands are 1 KiB pieces
+//     (2 KiB of 8-bit x) in the order of the instruction's lanes, so they go
+//     from memory straight into LDS (16 bytes a lane) and from there to
+//     registers without conversion, swizzle or bank conflict.
+//   * Four stages of LDS: the loads of unit u + 3 go out in unit u, x operands
+//     are read one unit ahead and weight operands one block ahead, so a unit
+//     waits for nothing but its barrier.  Scale codes are a dword a lane for
+//     four units, loaded a group ahead.
+//   * A wave reads its own rows of x and of the weight from LDS, MT * XP + NT
+//     KiB for MT * NT products, 128 bytes a cycle for the CU: that is what
+//     bounds a unit of the narrower tiles.  Eight waves of half the
+//     registers ran where four with 64 accumulator tiles each spilled their
+//     operands to accumulator registers and back.
+//   * Workgroups of one XCD go down `band` (at most 6) row tiles, then to the
+//     next column tile: the XCD's L2 then holds x of 6 tiles and two or three
+//     column tiles' weights (8192 x 20480 x 2560, e2m1: 226 us, whole
+//     columns 257, single rows 244; e4m3 334, 376, 354).
+//   * K slices where the tiles would leave CUs idle: fp32 sums to the
+//     workspace, added in slice order by the last workgroup to arrive.
+//
+// Bound by the LDS reads in the narrower tiles, by power in large products: the
+// card lowers its clock to 1.75 .. 1.9 GHz under the block-scaled instructions
+// (over zeros the same kernel keeps 2.38 GHz: e2m1 8192 cubed 184 us, 242 over
+// random values).  Two workgroups a CU of smaller tiles, wave priorities, waves
+// half a unit apart and deeper stages changed nothing there.
+// Measured on MI355X (graph replays): e2m1 8192 cubed 242 us (4550 TFLOP/s),
+// 8192 x 20480 x 2560 226 us (3800), 611 x 10240 x 2560 15.5 us (2070); e4m3 8192
+// cubed 369 us (2980), 2011 x 2560 x 10240 45.1 us (2340).  The card's large
+// bf16 matmul reaches 1269.
 #pragma once
 
 #include <type_traits>
@@ -314,8 +347,11 @@ constexpr bool mx_shape_ok(int elem, int tm, int tn) {
     return tn == 2 ? tm == 1 || tm == 2 || tm == 4 || tm == 6
                    : tn == 4 && (tm == 4 || tm == (elem == BZ_MX_E2M1 ? 8 : 6));
 }
-// Waves along the rows of x.  A wave reads its rows of x and of the weight from
-// LDS, MT * XP + NT KiB for MT * NT products.
+// Waves along the rows of x: four over the narrow tiles, where two would read
+// more of LDS for the same products (e4m3 6 x 2: 14 KiB a wave for 12, with four
+// 10; 2011 x 2560 x 10240 48.9 -> 46.7 us) and, for e2m1 6 x 2, need 128
+// registers and more, so that a CU held one workgroup (2011 x 20480 x 2560 81.5
+// -> 66.9 us).  4 x 4: 94.3 us with two, 95.3 with four.
 constexpr int mx_waves_m(int tm, int tn) { return tn == 2 && tm >= 4 ? 4 : 2; }
 
 template <int ELEM, int TM, int TN>

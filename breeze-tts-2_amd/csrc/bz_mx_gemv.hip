@@ -21,7 +21,9 @@ struct MxGemvPlan {
 // 5: 4 slices of 3 blocks 8.01, one slice 9.10); more than 16 rows in slices
 // of about 13, a unit per wave (N2560 K10240 M = 32: 6 slices of 4 blocks 11.2,
 // 4 of 3 12.2; e4m3 N10240 K2560: 2 slices of 5 11.0, one of 3 11.6).  8-bit
-// elements prefer a unit per wave over slices (N1024 K8192 M = 8: 7.12, 7.19).
+// elements take a unit per wave over slices, whose longer conversion then runs in
+// more waves (N1024 K8192 M = 1: 6.48 us, 2 units 6.65; M = 5: 6.80, 6.90; 4-bit
+// 6.77, 6.27).
 static int mx_gemv_plan(int elem, int M, int N, int K, int cfg, MxGemvPlan& pl) {
     const int NU = K / 128, nblk = N / 16, mt = M > 16 ? 2 : 1;
     const int cT = cfg & 255, cu = (cfg >> 8) & 255, cs = cfg >> 16;

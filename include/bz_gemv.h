@@ -83,8 +83,9 @@ typedef enum bz_status {
  *   tile of 1024 bytes holds the four 32-k blocks of its 16 rows block by
  *   block (block g of row r at byte 256 g + 16 r), and the scales follow the
  *   tiles, per four units 256 bytes (unit u, block g, row r at byte 64 g +
- *   4 r + u % 4; the bytes of units past the last are zero).  Runs on paths 5 and 6; w_eff is exact in bf16, so the
- *   products equal those of the bf16 weight.
+ *   4 r + u % 4; the bytes of units past the last are zero).  Runs on
+ *   paths 5 and 6; w_eff is exact in bf16, so the products equal those of the
+ *   bf16 weight.
  * The tiled formats run on GEMV path 5, the streaming kernel (M <= 8 rows
  * per launch; more rows run as several launches), and the unpaired ones also
  * on the several-row paths 4 (int4, fp8) and 6 (see below).  They need K %
@@ -160,9 +161,9 @@ typedef enum bz_dtype {
  * needed), else it keeps the row-sliced paths.
  *
  * Several rows over the tiled formats (path 6, the panel kernel).  Up to 32
- * rows of x per launch against an unpaired tiled int4 or fp8 weight
- * (BZ_W_INT4_TILED, BZ_W_FP8_TILED, BZ_W_MXFP4_TILED), no RMSNorm, epilogue NONE or RESIDUAL,
- * no second store: each workgroup of cfg_waves waves (0: about 5 units per
+ * rows of x per launch against an unpaired tiled weight (BZ_W_INT4_TILED,
+ * BZ_W_FP8_TILED, BZ_W_MXFP4_TILED), no RMSNorm, epilogue NONE or RESIDUAL, no
+ * second store: each workgroup of cfg_waves waves (0: about 5 units per
  * wave; at most 16, or 8 with several blocks) covers cfg_tiles consecutive
  * 16-row blocks (1..5; 0: enough to keep about 256 workgroups, or with K
  * slices 2 (int4) / 3 (fp8), one per 48 blocks for fewer) over the whole K
@@ -238,8 +239,7 @@ int bz_gemv(const bz_gemv_desc* d, void* stream);
 
 /* Prefill GEMM: out[M][N] = x[M][K] @ w_eff^T for prompt-sized M over an
  * unpaired tiled weight (BZ_W_INT4_TILED, group 128, BZ_W_FP8_TILED or
- * BZ_W_MXFP4_TILED); x
- * bf16 with 16-byte aligned rows (ldx >= K), out bf16 or fp32 (ldo >= N),
+ * BZ_W_MXFP4_TILED); x bf16 with 16-byte aligned rows (ldx >= K), out bf16 or fp32 (ldo >= N),
  * fp32 accumulation.  Replaces torch._weight_int4pack_mm and
  * torch._scaled_mm (weight-only form) for the rows of a prompt
  * (models/int4_linear.py:103-108, models/fp8_linear.py:76-82).

@@ -71,10 +71,10 @@ int bz_mx_dequantize(const void* codes, const void* scales, int32_t elem, int32_
  * bz_mx_gemm_workspace gives the bytes of workspace the call needs (16-byte
  * aligned, zero-filled before its first use; every call leaves its counters
  * zero; calls that share it must not overlap), 0 where K is not sliced.  cfg =
- * 0 takes the built-in launch shape, else 16-row groups of x per wave | row
- * blocks per wave << 8 | K slices << 16 (a part left 0 keeps the rule's
- * choice; groups and blocks 1, 2, 4 or 6 and 2, 4 and 4, or 8 (e2m1) or 6
- * (e4m3) and 4). */
+ * 0 takes the built-in launch shape, else the tile of a workgroup, 32 rows of x
+ * | 64 of the weight << 8 | K slices << 16 (a part left 0 keeps the rule's
+ * choice; tiles of 1, 2, 4 or 6 and 2, 4 and 4, or 8 (e2m1) or 6 (e4m3) and
+ * 4).  K up to 2^22. */
 size_t bz_mx_gemm_workspace(int32_t elem, int32_t M, int32_t N, int32_t K, int32_t cfg);
 int bz_mx_gemm(int32_t elem, const void* xq, int32_t M, const void* w, int32_t N, int32_t K, const void* residual,
                int32_t residual_dtype, int64_t ldr, void* out, int32_t out_dtype, int64_t ldo, void* workspace,
@@ -84,7 +84,7 @@ int bz_mx_gemm(int32_t elem, const void* xq, int32_t M, const void* w, int32_t N
  * x [M][ldx] bf16, 16-byte aligned rows (ldx % 8 == 0).  The result is that of
  * bz_mx_quantize and bz_mx_gemm up to the order of its fp32 sums.  Workspace
  * as for bz_mx_gemm; bz_mx_gemv_workspace is (size_t)-1 where the call is
- * refused (rows too long for 64 K slices).  cfg = 0 takes the built-in launch
+ * refused (K above 2^22 or too long for 64 K slices).  cfg = 0 takes the built-in launch
  * shape, else row blocks per workgroup (1 .. 8) | units of 128 columns per
  * wave (1 .. 6, 8) << 8 | K slices << 16 (a part left 0 keeps the rule's
  * choice). */
