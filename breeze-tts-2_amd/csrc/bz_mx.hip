@@ -1,11 +1,10 @@
 // Microscaled blocks (bz_mx_device.h): quantising rows and reading them back.
 //
 // Both are one pass over memory and bound by it; a few rows by the launch.
-// Measured on MI355X (kernel trace; a copy of 1 GiB reaches 5.2 TB/s, and what
-// the last-level cache still holds comes faster): 10240 x 2560 fp32 to e2m1
-// 17.1 us (6.9 TB/s), 2011 x 10240 bf16 to e4m3 11.1 us (5.7) and back 9.6 us
-// (6.5), 2 x 2560 1.3 us either way; tiled, 2011 x 10240 to e4m3 11.9 us (5.3),
-// 8192 x 2560 to e2m1 11.3 us (4.7).
+// Measured on MI355X (kernel trace, three tensors in turn; a copy of 1 GiB
+// reaches 5.2 TB/s): 10240 x 2560 fp32 to e2m1 21.3 us (5.6 TB/s), 2011 x 10240
+// bf16 to e4m3 11.8 us (5.3) and back 11.2 us (5.6), tiled 12.3 us (5.1); 2 x
+// 2560 1.5 us and back 1.6 us.
 #include <algorithm>
 
 #include "bz_mx.h"
