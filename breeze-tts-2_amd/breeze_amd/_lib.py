@@ -10,6 +10,7 @@ in it.  There is no fallback: if the library is missing the import fails.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import struct
 import os
 from pathlib import Path
@@ -268,6 +269,26 @@ def lib() -> ctypes.CDLL:
             raise RuntimeError(f"{LIB_PATH} has ABI {version}, this binding expects {ABI_VERSION}")
         _lib = handle
     return _lib
+
+
+BINDING_PATH = Path(__file__).resolve().parent / "_bztorch.so"
+_binding = None
+
+
+def binding():
+    """The torch binding (csrc/bz_torch.cpp) over the loaded library; raises if
+    it has not been built."""
+    global _binding
+    if _binding is None:
+        if not BINDING_PATH.exists():
+            raise RuntimeError(f"{BINDING_PATH} is missing: build it with `python -m breeze_amd.build`")
+        spec = importlib.util.spec_from_file_location("_bztorch", BINDING_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(*(ctypes.cast(getattr(lib(), f), ctypes.c_void_p).value
+                      for f in ("bz_gemv", "bz_mx_gemv", "bz_mx_quantize", "bz_mx_dequantize")))
+        _binding = module
+    return _binding
 
 
 def strerror(status: int) -> str:

@@ -1,4 +1,5 @@
-"""Compile libbzgemv.so (the gfx950 kernels + C ABI) in-tree.
+"""Compile libbzgemv.so (the gfx950 kernels + C ABI) and _bztorch.so (the torch
+binding of its hottest calls) in-tree.
 
     python -m breeze_amd.build          (from breeze-tts-2_amd/)
 
@@ -22,6 +23,7 @@ SRC_DIR = PKG_DIR.parent / "csrc"
 INCLUDE_DIR = PKG_DIR.parents[1] / "include"
 LIB_NAME = "libbzgemv.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+BINDING_PATH = PKG_DIR / "_bztorch.so"
 ARCH = "gfx950"
 
 # Packed-fp32 instructions stay disabled: hipcc would otherwise emit
@@ -93,9 +95,32 @@ def sources() -> list[Path]:
     return sorted(SRC_DIR.glob("*.hip"))
 
 
+def build_binding(verbose: bool = False) -> Path:
+    """Compile and link BINDING_PATH: host code over torch's C++ headers."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    cmd = [_hipcc(), "-x", "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1",
+           "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE_DIR}",
+           "-isystem", str(root / "include"), "-isystem", str(root / "include/torch/csrc/api/include"),
+           "-isystem", str(Path(_hipcc()).resolve().parents[1] / "include"), "-isystem", sysconfig.get_paths()["include"],
+           str(SRC_DIR / "bz_torch.cpp"), "-o", str(tmp),
+           f"-L{root / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"building the torch binding failed:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
+
+
 def build(verbose: bool = False) -> Path:
-    """Compile every HIP source for gfx950 and link LIB_PATH.  Always
-    recompiles (this is the build check)."""
+    """Compile every HIP source for gfx950 and link LIB_PATH, and build
+    BINDING_PATH.  Always recompiles (this is the build check)."""
     hipcc = _hipcc()
     obj_dir = PKG_DIR / "_build"
     obj_dir.mkdir(exist_ok=True)
@@ -114,7 +139,9 @@ def build(verbose: bool = False) -> Path:
         return obj, kernel_resources(res.stderr)
 
     with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as pool:
+        binding = pool.submit(build_binding, verbose)
         done = list(pool.map(compile_one, srcs))
+        binding.result()
     objs = [o for o, _ in done]
     kernels = sorted({k for _, ks in done for k in ks})
     (obj_dir / "kernel_resources.txt").write_text(

@@ -130,8 +130,10 @@ def gemv(
     with ``n`` rows, optional RMSNorm gamma [K], epilogue NONE / SILU_GATE
     (N_out = n/2) / RESIDUAL (residual [M, N_out]).  Returns ``out``.
     """
-    if cfg is _NO_CFG and out is None and out2 is None and sc0 is None and sc1 is None:
-        y = _gemv_tiled(x, w, wfmt, n, gamma, eps, epilogue, residual, out_dtype)
+    plain = cfg is _NO_CFG and out is None and out2 is None and wfmt in TILED_FORMATS and x.is_cuda
+    if plain:  # a decode step's call: nothing to convert, checked and made in C++
+        y = (_lib._binding or _lib.binding()).gemv(_tuning._TABLES, _tuning._ARCH, _raw_workspace, x, w, wfmt, n,
+                                                   gamma, eps, epilogue, residual, out_dtype)
         if y is not None:
             return y
     if x.dim() != 2:
@@ -186,6 +188,8 @@ def gemv(
             cfg = _NO_CFG
     if len(cfg) != 5:
         cfg = (tuple(cfg) + _NO_CFG)[:5]
+    if plain and M <= 32:
+        _plan_tiled(dev, wfmt, n, K, epilogue, gamma is not None, M, cfg)
     has_res = epilogue == EPI_RESIDUAL
     d = _lib.gemv_desc(
         _lib.ABI_VERSION, M, n, K, group, wfmt, epilogue, _DT[out.dtype], res_dt, *cfg, eps, x.data_ptr(), x.stride(0),
@@ -207,65 +211,19 @@ def gemv(
     return out
 
 
-def _gemv_tiled(x, w, wfmt, n, gamma, eps, epilogue, residual, out_dtype):
-    """gemv of up to 32 rows over a tiled weight where every argument is as the
-    library reads it, nothing to convert or copy: a decode step's calls, whose
-    host work is as long as their kernels.  None where that is not so, for the
-    caller to convert or to say what is wrong."""
-    index, shape = x.get_device(), x.shape
-    if index < 0 or len(shape) != 2 or not 0 < shape[0] <= 32 or x.dtype is not torch.bfloat16 \
-            or w.get_device() != index or out_dtype not in _DT or wfmt not in TILED_FORMATS:
-        return None
-    M, K = shape
-    norm = gamma is not None
-    table = _tuning.plans(index)
-    key = ("tiled", wfmt, n, K, epilogue, norm, M)
-    plan = table.get(key)
-    if plan is None:
-        plan = table[key] = _tiled_plan(x.device, *key[1:])
-    n_out, wbytes, cfg, need = plan
-    ld, inner = x.stride()
-    if inner != 1 or ld < K or ld & 7 or x.data_ptr() & 15 or w.numel() * w.element_size() != wbytes \
-            or not w.is_contiguous():
-        return None
-    gp = rp = res_dt = ldr = 0
-    if norm:
-        if gamma.get_device() != index or gamma.dtype is not torch.bfloat16 or gamma.numel() != K \
-                or not gamma.is_contiguous():
-            return None
-        gp = gamma.data_ptr()
-    if epilogue == EPI_RESIDUAL:
-        if residual is None or residual.get_device() != index or residual.shape != (M, n_out):
-            return None
-        res_dt = _DT.get(residual.dtype)
-        ldr, inner = residual.stride()
-        if res_dt is None or inner != 1:
-            return None
-        rp = residual.data_ptr()
-    out = torch.empty((M, n_out), dtype=out_dtype, device=x.device)
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    ws = 0
-    if need:
-        ws = _workspace(x.device, stream, need)
-        ws, need = ws.data_ptr(), ws.numel() * 4
-    d = _lib.gemv_desc(_lib.ABI_VERSION, M, n, K, 128, wfmt, epilogue, _DT[out_dtype], res_dt, *cfg, eps, x.data_ptr(),
-                       ld, w.data_ptr(), 0, 0, gp, rp, ldr, out.data_ptr(), n_out, ws, need, 0, 0, 0, 0)
-    rc = _lib.lib().bz_gemv(d, stream)
-    if rc != _lib.OK:
-        _lib.check(rc, "bz_gemv")
-    return out
-
-
-def _tiled_plan(dev, wfmt, n, k, epilogue, norm, m) -> tuple:
-    """(output columns, bytes of the weight, launch shape, workspace bytes) of a
-    tiled GEMV; -1 bytes where the shape cannot be tiled."""
+def _plan_tiled(dev, wfmt, n, k, epilogue, norm, m, cfg) -> None:
+    """What the next call of this shape needs to know, beside its launch shape in
+    the table: (output columns, bytes of the weight, launch shape, workspace
+    bytes)."""
+    table = _tuning.plans(dev.index)
+    key = ("tiled", wfmt, n, k, epilogue, norm, m)
+    if key in table:
+        return
     n_out = n // 2 if epilogue == EPI_SILU_GATE else n
-    cfg = _tuning.lookup(dev, n, k, wfmt, epilogue, norm, m) or _NO_CFG
-    cfg = (tuple(cfg) + _NO_CFG)[:5]
     at = 1 << 20  # (any aligned pointer: nothing is read)
     d = _lib.gemv_desc(_lib.ABI_VERSION, m, n, k, 128, wfmt, epilogue, DT_BF16, DT_BF16, *cfg, 1e-6, at, k, at, 0, 0,
                        at if norm else 0, at, n_out, at, n_out, 0, 0, 0, 0, 0, 0)
-    return n_out, tiled_bytes(wfmt, n, k) or -1, cfg, int(_lib.lib().bz_gemv_workspace(d))
+    table[key] = n_out, tiled_bytes(wfmt, n, k), cfg, int(_lib.lib().bz_gemv_workspace(d))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -385,6 +343,12 @@ def _workspace(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     stream run in order and may share it."""
     key = dev.index if dev.index is not None else torch.cuda.current_device()
     return _lib.stream_workspace(_GEMV_WS, (key,), nbytes, torch.device("cuda", key), stream, _GEMV_WS_RETIRED)
+
+
+def _raw_workspace(index: int, stream: int, nbytes: int) -> tuple:
+    """(address, bytes) of the same."""
+    ws = _workspace(torch.device("cuda", index), stream, nbytes)
+    return ws.data_ptr(), ws.numel() * 4
 
 
 # ---- custom-op registration (torch.compile / fake tensors) -----------------

@@ -106,6 +106,10 @@ def quantize_mx(x: torch.Tensor, elem: str = "e2m1") -> tuple[torch.Tensor, torc
     """(codes, scales) of x [M, K] (bf16, fp16 or fp32; K a multiple of 32):
     codes uint8 [M, K/2] with the even column in the low half (e2m1) or
     float8_e4m3fn [M, K]; scales uint8 [M, K/32]."""
+    if x.is_cuda:  # nothing to convert: checked and made in C++
+        held = (_lib._binding or _lib.binding()).quantize_mx(x, elem)
+        if held is not None:
+            return held
     code = _elem(elem)
     x, M, K, ld, dt, index = _rows(x, BLOCK)
     if code == MX_E2M1:
@@ -123,6 +127,10 @@ def dequantize_mx(codes: torch.Tensor, scales: torch.Tensor, elem: str = "e2m1",
                   dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values [M, K] (bf16 or fp32) that quantize_mx's codes and scales stand
     for: exact, in bf16 down to 2^-126."""
+    if codes.is_cuda:
+        out = (_lib._binding or _lib.binding()).dequantize_mx(codes, scales, elem, dtype)
+        if out is not None:
+            return out
     code, index, shape = _elem(elem), codes.get_device(), codes.shape
     if index < 0 or scales.get_device() != index:
         _gpu("codes", codes, index)
@@ -182,6 +190,7 @@ def _tiled_rows(x, M: int, K: int, ld: int, dt: int, code: int, index: int) -> t
 # each graph capture under way.
 _WS: dict = {}
 _WS_RETIRED: list = []
+_FEW_PLANS: dict = {}  # (element type, M, n, K) -> _plan's answer, for the binding
 _NO_WAY = (1 << 64) - 1  # what bz_mx_gemv_workspace gives for a shape it does not take
 
 
@@ -209,6 +218,10 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
     be out itself; out: [M, n] with unit column stride, apart from x and w.  cfg: a
     launch shape (include/bz_mx.h) instead of the built-in rule's."""
     rows = isinstance(x, MxRows)
+    if not (rows or cfg) and out is None and x.is_cuda:  # few rows, nothing to convert
+        y = (_lib._binding or _lib.binding()).mx_linear(_FEW_PLANS, _raw_workspace, x, w, n, elem, residual, out_dtype)
+        if y is not None:
+            return y
     if rows:
         src, (M, K), code = x.data, x.shape, _elem(x.elem)
         index, few = src.get_device(), False
@@ -222,6 +235,8 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
         # up to 32 rows that a launch can read as they are: quantised inside it
         few = dt == DT_BF16 and M <= FEW_ROWS and not (ld & 7 or src.data_ptr() & 15) and M * ld < 1 << 30
     weight, few, need = _plan(code, M, n, K, cfg, few)
+    if few and not cfg:
+        _FEW_PLANS[code, M, n, K] = weight, few, need
     if w.get_device() != index or w.numel() * w.element_size() != weight or not w.is_contiguous() or w.data_ptr() & 15:
         _gpu("w", w, index)
         raise ValueError(f"w must be a contiguous W_MXFP4_TILED weight of {n} x {K} (rows a multiple of 16), "
@@ -261,8 +276,7 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
     if not (few or rows):
         src = _tiled_rows(src, M, K, ld, dt, code, index)
     if need:
-        ws = _lib.stream_workspace(_WS, (index,), need, w.device, torch._C._cuda_getCurrentRawStream(index),
-                                   _WS_RETIRED).data_ptr()
+        ws, _ = _raw_workspace(index, torch._C._cuda_getCurrentRawStream(index), need)
     if few:
         _call(index, lib.bz_mx_gemv, code, src.data_ptr(), ld, M, w.data_ptr(), n, K, res, rdt, ldr, out.data_ptr(),
               odt, ldo, ws, need, cfg)
@@ -270,6 +284,12 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
         _call(index, lib.bz_mx_gemm, code, src.data_ptr(), M, w.data_ptr(), n, K, res, rdt, ldr, out.data_ptr(),
               odt, ldo, ws, need, cfg)
     return out
+
+
+def _raw_workspace(index: int, stream: int, nbytes: int) -> tuple:
+    """(address, bytes) of the workspace of products on this stream."""
+    ws = _lib.stream_workspace(_WS, (index,), nbytes, torch.device("cuda", index), stream, _WS_RETIRED)
+    return ws.data_ptr(), ws.numel() * 4
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:

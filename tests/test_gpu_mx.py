@@ -741,3 +741,87 @@ def test_rows_that_are_not_of_their_shape():
         mx.mx_linear(mx.MxRows(q.data, q.shape, O.E4M3), w.tiled, 32)
     with pytest.raises(RuntimeError, match="GPU tensor"):
         mx.mx_linear(mx.MxRows(q.data.cpu(), q.shape, q.elem), w.tiled.cpu(), 32)
+
+
+def test_calls_after_a_planned_one():
+    """The second call of a shape is made by the binding: what differs from the first is seen, or refused."""
+    n, k = 1024, 2048
+    w, x = Weight(n, k), _rows(2, k, 40)
+    res, gamma = _rows(2, n, 41), _rows(1, k, 42)[0]
+    first = G.gemv(x, w.tiled, w.fmt, n)
+    want = mx.mx_linear(x, w.tiled, n)
+    for _ in range(3):
+        assert torch.equal(G.gemv(x, w.tiled, w.fmt, n), first) and torch.equal(mx.mx_linear(x, w.tiled, n), want)
+    for bad in (w.tiled[:-16], w.tiled.cpu()):
+        for call in (lambda: G.gemv(x, bad, w.fmt, n), lambda: mx.mx_linear(x, bad, n)):
+            with pytest.raises((ValueError, RuntimeError)):
+                call()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        mx.mx_linear(x.clone().requires_grad_(), w.tiled, n)
+    with torch.no_grad():
+        assert torch.equal(mx.mx_linear(x.clone().requires_grad_(), w.tiled, n), want)
+    # rows to copy, to convert, of a wider tensor, of another type; types of the result and the residual
+    wide = torch.empty(2, k + 8, device="cuda", dtype=BF16)
+    wide[:, 8:] = x
+    odd = torch.empty(2, k + 1, device="cuda", dtype=BF16)
+    odd[:, 1:] = x
+    for view in (wide[:, 8:], odd[:, 1:], x.float(), x.t().contiguous().t(), torch.nn.Parameter(x, requires_grad=False)):
+        assert torch.equal(G.gemv(view, w.tiled, w.fmt, n), first) and torch.equal(mx.mx_linear(view, w.tiled, n), want)
+        for elem in ELEMS:
+            for a, b in zip(mx.quantize_mx(view, elem), mx.quantize_mx(x, elem)):
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    for r in (res, res.float(), res.t().contiguous().t(), res[:1].expand(2, n)):
+        for dt in (BF16, F32):
+            a = G.gemv(x, w.tiled, w.fmt, n, epilogue=G.EPI_RESIDUAL, residual=r.contiguous(), out_dtype=dt)
+            assert a.dtype == dt
+            if r.stride(0) >= n:
+                assert torch.equal(G.gemv(x, w.tiled, w.fmt, n, epilogue=G.EPI_RESIDUAL, residual=r, out_dtype=dt), a)
+            b = mx.mx_linear(x, w.tiled, n, residual=r.contiguous(), out_dtype=dt)
+            assert b.dtype == dt and torch.equal(mx.mx_linear(x, w.tiled, n, residual=r, out_dtype=dt), b)
+    for bad in (res[:1], res[:, :-1], res.cpu()):
+        for call in (lambda: G.gemv(x, w.tiled, w.fmt, n, epilogue=G.EPI_RESIDUAL, residual=bad),
+                     lambda: mx.mx_linear(x, w.tiled, n, residual=bad)):
+            with pytest.raises((ValueError, RuntimeError)):
+                call()
+    normed = G.gemv(x, w.tiled, w.fmt, n, gamma=gamma)
+    assert torch.equal(G.gemv(x, w.tiled, w.fmt, n, gamma=gamma.float()), normed)
+    with pytest.raises(ValueError):
+        G.gemv(x, w.tiled, w.fmt, n, gamma=gamma[:-1])
+    assert not torch.equal(G.gemv(x, w.tiled, w.fmt, n, gamma=gamma, eps=1), normed)
+
+
+def test_a_plan_goes_with_the_table(monkeypatch):
+    """A launch shape from a new table is taken, also for a shape that was called before."""
+    from breeze_amd import tuning
+
+    n, k = 1024, 2048
+    w, x = Weight(n, k), _rows(1, k, 43)
+    want = G.gemv(x, w.tiled, w.fmt, n)
+    arch = tuning.arch_of(x.device)
+    key = tuning.table_key(arch, n, k, w.fmt, G.EPI_NONE, False, 1)
+    monkeypatch.setitem(tuning._TABLES, arch, {key: [0, 0, 0, 9]})  # (no such path)
+    with pytest.raises(L.BzError):
+        G.gemv(x, w.tiled, w.fmt, n)
+    monkeypatch.setitem(tuning._TABLES, arch, {key: [0, 4, 0, 5]})
+    _close(G.gemv(x, w.tiled, w.fmt, n), *_gemv_reference(x, w, G.EPI_NONE, None, 0.0, None, BF16))
+    monkeypatch.undo()
+    assert torch.equal(G.gemv(x, w.tiled, w.fmt, n), want)
+
+
+def test_planned_calls_hold_no_memory():
+    n, k = 1024, 8192
+    w, x = Weight(n, k), _rows(5, k, 44)
+
+    def calls():
+        mx.mx_linear(x, w.tiled, n, elem="e4m3")  # (with a workspace)
+        G.gemv(x, w.tiled, w.fmt, n)
+        mx.dequantize_mx(*mx.quantize_mx(x))
+
+    for _ in range(3):
+        calls()
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    for _ in range(50):
+        calls()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == held

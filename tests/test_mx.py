@@ -225,3 +225,23 @@ def test_weight_buffers_are_checked():
         G._check_weight(w[:-1], G.W_MXFP4_TILED, 16, 128, 128, None, None)
     with pytest.raises(ValueError, match="sc0"):
         G._check_weight(w[:1024], G.W_MXFP4, 16, 128, 128, torch.zeros(63, dtype=torch.uint8), None)
+
+
+def test_the_binding_leaves_what_it_does_not_take(monkeypatch, tmp_path):
+    b = L.binding()
+    cpu = torch.zeros(2, 64, dtype=torch.bfloat16)
+    for args in ((), (cpu,), (cpu, "e2m1"), (None, "e2m1"), (1, 2, 3)):
+        assert b.quantize_mx(*args) is None
+    assert b.dequantize_mx(cpu, cpu, "e2m1", torch.bfloat16) is None
+    assert b.gemv({}, {}, None, cpu, cpu, 10, 16, None, 1e-6, 0, None, torch.bfloat16) is None
+    assert b.gemv(*[None] * 12) is None and b.gemv() is None
+    assert b.mx_linear({}, None, cpu, cpu, 16, "e2m1", None, torch.bfloat16) is None
+    assert b.mx_linear(*[None] * 8) is None
+    with pytest.raises(TypeError):
+        b.bind(1)
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        mx.quantize_mx(cpu)
+    monkeypatch.setattr(L, "_binding", None)
+    monkeypatch.setattr(L, "BINDING_PATH", tmp_path / "none.so")
+    with pytest.raises(RuntimeError, match="missing"):
+        L.binding()
