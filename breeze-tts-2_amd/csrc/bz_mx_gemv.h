@@ -3,10 +3,10 @@
 // launch that reads every weight byte once.
 //
 // Bound by the weight's bytes and by the latency of a launch.  Measured on
-// MI355X (graph replays, weights not in a cache): e2m1 N20480 K2560 M = 1 7.7 us
-// (3.6 TB/s of weight), M = 16 9.1; N2560 K10240 M = 5 8.1 us, e4m3 8.2; N1024
-// K2048 M = 1 3.7 us.  Quantising in a launch of its own, bz_mx_gemm behind
-// it, took 15.0 us for the third of these.
+// MI355X (graph replays, weights not in a cache): e2m1 N20480 K2560 M = 1 7.5 us
+// (3.7 TB/s of weight), M = 16 9.1; N2560 K10240 M = 5 7.8 us, e4m3 7.8; N1024
+// K2048 M = 1 3.4 us.  Quantising in a launch of its own, bz_mx_gemm behind it,
+// took 15.0 us for the third of these.
 //
 // Work decomposition (that of the several-block streaming kernel,
 // bz_gemv_wide.h, with the panel kernel's K slices, bz_gemv_panel.h)
@@ -20,6 +20,13 @@
 //     the elements with the scaled conversion.  No lane needs another's
 //     values, and quantising costs no launch (a launch of its own over a few
 //     rows takes 2.9 us on MI355X).
+//   * Up to 8 (4) rows leave half (three quarters) of an operand's rows free:
+//     these hold the same rows' next unit(s), so that all lanes quantise and 2
+//     (4) units share one operand.  Each unit's product is whole, into sums of
+//     its own, of which only its own rows count; they meet after the last
+//     unit.  Every workgroup quantises all the x it reads, so this is what
+//     took longest (N2560 K4096 M = 1 4.78 -> 4.20 us, N1024 K8192 M = 1 6.25 ->
+//     4.85 with the longer slices it allows, N20480 K2560 M = 5 7.97 -> 7.74).
 //   * The waves' sums are added through LDS in wave order; over K slices the
 //     last workgroup of a group to arrive adds the slices in their order.
 //
@@ -55,12 +62,26 @@ constexpr int kMxGemvRows = 32;
 constexpr int kMxGemvBlocks = 8;                        // most row blocks of a workgroup
 constexpr int kMxGemvUpw[] = {1, 2, 3, 4, 5, 6, 8};  // units per wave
 __host__ __device__ constexpr int mx_gemv_lds(int NW, int T, int MT) { return NW * T * MT * 1024 + 16; }
+// Units of a wave that share one operand of x: rows 16 / G and more of it belong
+// to the next unit.
+constexpr int mx_gemv_share(int M, int upw) { return M <= 4 && upw >= 3 ? 4 : M <= 8 && upw >= 2 ? 2 : 1; }
 // Most waves of a workgroup: 16 while two sets of tiles and the quantised x of
 // a wave's units leave room in 128 registers, else 8.
-__host__ __device__ constexpr int mx_gemv_waves(int elem, int mt, int upw) {
-    return upw * (10 + mt * (elem == BZ_MX_E2M1 ? 5 : 9)) <= 80 ? 16 : 8;
+__host__ __device__ constexpr int mx_gemv_waves(int elem, int mt, int upw, int G) {
+    return upw * 10 + (upw + G - 1) / G * mt * (elem == BZ_MX_E2M1 ? 5 : 9) <= 80 ? 16 : 8;
 }
-constexpr bool mx_gemv_built(int mt, int upw) { return mt == 1 || upw <= 5; }
+constexpr bool mx_gemv_built(int mt, int upw, int G) {
+    return mt == 1 ? G == 1 || (G == 2 && upw >= 2) || (G == 4 && upw >= 3) : G == 1 && upw <= 5;
+}
+
+// Lane j of 16 gets that of lane (j - N) % 16.
+template <int N>
+__device__ __forceinline__ mx_acc_t ror16(mx_acc_t v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        v[e] = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v[e]), 0x120 + N, 0xF, 0xF, false));
+    return v;
+}
 
 // A block of 32 bf16 values: its scale code and elements (e2m1: the first
 // four dwords; e4m3: eight).
@@ -90,8 +111,8 @@ __device__ __forceinline__ uint32_t mx_quantize_block(const u32x4 (&v)[4], u32x4
     return code;
 }
 
-template <int ELEM, int MT, int UPW>
-__global__ void __launch_bounds__(64 * mx_gemv_waves(ELEM, MT, UPW)) mx_gemv(MxGemvParams p) {
+template <int ELEM, int MT, int UPW, int G>
+__global__ void __launch_bounds__(64 * mx_gemv_waves(ELEM, MT, UPW, G)) mx_gemv(MxGemvParams p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     constexpr bool F8 = ELEM == BZ_MX_E4M3;
     const int nthr = blockDim.x, NW = nthr >> 6;
@@ -106,10 +127,11 @@ __global__ void __launch_bounds__(64 * mx_gemv_waves(ELEM, MT, UPW)) mx_gemv(MxG
     // x: rows past M and units past the slice read as zeros, without
     // requests; up to four units' rows are under way
     const __amdgpu_buffer_rsrc_t xrs = buffer_rsrc(p.x, (uint32_t)(((int64_t)(M - 1) * p.ldx + p.K) * 2));
-    constexpr int NX = UPW * MT, XD = NX < 4 ? NX : 4;
+    constexpr int R = 16 / G, NS = (UPW + G - 1) / G;  // rows of a unit in an operand, and operands
+    constexpr int NX = NS * MT, XD = NX < 4 ? NX : 4;
     u32x4 xv[XD][4];
-    auto x_load = [&](int i) __attribute__((always_inline)) {  // row group i % MT of unit i / MT
-        const int m = 16 * (i % MT) + j, u = u0 + i / MT;
+    auto x_load = [&](int i) __attribute__((always_inline)) {  // row group i % MT of operand i / MT
+        const int m = 16 * (i % MT) + j % R, u = u0 + i / MT * G + j / R;
         const uint32_t o = ((m < M ? (uint32_t)((m * (int)p.ldx + 32 * g) * 2) : 0x80000000u) + (uint32_t)u * 256u) |
                            (u < ue ? 0u : 0x80000000u);
 #pragma unroll
@@ -138,8 +160,8 @@ __global__ void __launch_bounds__(64 * mx_gemv_waves(ELEM, MT, UPW)) mx_gemv(MxG
     for (int q = 0; q < UPW; ++q) issue(0, q, wa, sa);
     __builtin_amdgcn_sched_barrier(0);
 
-    mx_op_t xq[UPW][MT];
-    uint32_t sx[UPW][MT];
+    mx_op_t xq[NS][MT];
+    uint32_t sx[NS][MT];
 #pragma unroll
     for (int i = 0; i < NX; ++i) {
         u32x4 lo, hi = {0u, 0u, 0u, 0u};
@@ -164,20 +186,29 @@ __global__ void __launch_bounds__(64 * mx_gemv_waves(ELEM, MT, UPW)) mx_gemv(MxG
     float* red = reinterpret_cast<float*>(smem);
     auto run_block = [&](int jb, const u32x4* cw, const uint32_t* cs, u32x4* nw2, uint32_t* ns2)
                          __attribute__((always_inline)) {
-        mx_acc_t acc[MT];
+        mx_acc_t acc[MT][G];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) acc[mt] = mx_acc_t{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int s = 0; s < G; ++s) acc[mt][s] = mx_acc_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int q = 0; q < UPW; ++q) {
             const mx_op_t w = mx_op(cw[q]);
             const uint32_t sw = cs[q] >> (8 * ((u0 + q) & 3));
             issue(jb + 1, q, nw2, ns2);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) acc[mt] = mx_mfma<ELEM, 0>(w, xq[q][mt], acc[mt], sw, sx[q][mt]);
+            for (int mt = 0; mt < MT; ++mt)
+                acc[mt][q % G] = mx_mfma<ELEM, 0>(w, xq[q / G][mt], acc[mt][q % G], sw, sx[q / G][mt]);
         }
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-            *reinterpret_cast<mx_acc_t*>(red + ((wave * T + jb) * MT + mt) * 256 + j * 16 + 4 * g) = acc[mt];
+        for (int mt = 0; mt < MT; ++mt) {
+            mx_acc_t a = acc[mt][0];
+#pragma unroll
+            for (int s = 1; s < G; ++s) a = j / R == s ? acc[mt][s] : a;
+            if (G >= 2) a += ror16<8>(a);
+            if (G >= 4) a += ror16<4>(a);
+            *reinterpret_cast<mx_acc_t*>(red + ((wave * T + jb) * MT + mt) * 256 + j * 16 + 4 * g) = a;
+        }
     };
     int jb = 0;
     for (; jb + 1 < nb; jb += 2) {
@@ -250,7 +281,7 @@ __global__ void __launch_bounds__(64 * mx_gemv_waves(ELEM, MT, UPW)) mx_gemv(MxG
 }
 
 struct MxGemvLaunch {
-    int nw, mt, upw;
+    int nw, mt, upw, share;
     unsigned grid;
     size_t lds;
 };

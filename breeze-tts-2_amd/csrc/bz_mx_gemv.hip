@@ -14,22 +14,31 @@ struct MxGemvPlan {
 };
 
 // Built-in rule (sweeps of blocks, units per wave and slices on MI355X, M = 1
-// .. 32, us): one slice and about one workgroup per CU while a row has up to
-// 32 units, 2 units per wave (e2m1 N20480 K2560 M = 5: 5 blocks x 2 units
-// 7.97, x 4 units 8.22, 3 blocks x 2 8.41); longer rows, whose x every
-// workgroup would read whole, in slices of about 20 units (N2560 K10240 M =
-// 5: 4 slices of 3 blocks 8.01, one slice 9.10); more than 16 rows in slices
-// of about 13, a unit per wave (N2560 K10240 M = 32: 6 slices of 4 blocks 11.2,
-// 4 of 3 12.2; e4m3 N10240 K2560: 2 slices of 5 11.0, one of 3 11.6).  8-bit
-// elements take a unit per wave over slices, whose longer conversion then runs in
-// more waves (N1024 K8192 M = 1: 6.48 us, 2 units 6.65; M = 5: 6.80, 6.90; 4-bit
-// 6.77, 6.27).
+// .. 32, us): about one workgroup per CU.  One slice while the x that every
+// workgroup then reads is short: up to 32 units, up to 48 for 8 rows, 64 for 5
+// and 96 for 2 (e4m3 N4096 K6144 M = 8 one slice 7.03, two 7.82; N1024 K8192 M =
+// 4 5.70, four 6.25, M = 8 7.0, three 6.65; N2560 K10240 M = 2 6.87, four 7.57; M
+// = 4 7.9, 7.79).  Beyond, slices of about 25 units, at most four, for up to 8
+// rows (N320 K16384 M = 5 four 6.20, seven 6.56), of 20, at least four, for up to
+// 16 (e4m3 N4096 K6144 M = 16 four 8.64, three 9.74) and of 13 for more (N2560
+// K10240 M = 32: 6 slices of 4 blocks
+// 11.2, 4 of 3 12.2).  Units per wave: 2 (N20480 K2560 M = 5: 5 blocks x 2 units
+// 7.97, x 4 8.22, 3 blocks x 2 8.41); 4, which share their operands of x, for up
+// to 8 rows where 2 would need 16 waves or more (N16384 K4096 M = 1 8.65, 2 units
+// 8.97) and for up to 4 over one or two blocks (N1024 K2048 M = 1 3.42, 3.54;
+// N10240 K2560 M = 4, three blocks, 5.97, 5.92); 1 for more than 16 rows in slices
+// (e4m3 N10240 K2560: 2 slices of 5 11.0, one of 3 11.6).
 static int mx_gemv_plan(int elem, int M, int N, int K, int cfg, MxGemvPlan& pl) {
     const int NU = K / 128, nblk = N / 16, mt = M > 16 ? 2 : 1;
     const int cT = cfg & 255, cu = (cfg >> 8) & 255, cs = cfg >> 16;
     if (cT > kMxGemvBlocks || cs > 64) return BZ_ERR_INVALID_ARG;
     auto blocks = [&](int slices) { return cT ? cT : (int)(((int64_t)nblk * slices + 255) / 256); };
-    int nsl = cs ? cs : mt == 2 ? std::max(1, (NU + 6) / 13) : NU <= 32 ? 1 : (NU + 19) / 20;
+    const bool whole = NU <= 32 || (NU <= 48 && M <= 8) || (NU <= 64 && M <= 5) || (NU <= 96 && M <= 2);
+    int nsl = cs        ? cs
+              : mt == 2 ? std::max(1, (NU + 6) / 13)
+              : whole   ? 1
+              : M <= 8  ? std::min(4, (NU + 24) / 25)
+                        : std::max(4, (NU + 19) / 20);
     if (!cs && blocks(nsl) > kMxGemvBlocks) nsl = 1;
     nsl = std::min(nsl, NU);
     const int T = std::min(kMxGemvBlocks, blocks(nsl));
@@ -39,15 +48,20 @@ static int mx_gemv_plan(int elem, int M, int N, int K, int cfg, MxGemvPlan& pl) 
         if (nsl > 64 || (nsl > 1 && (groups > kMxCounters || (int64_t)nsl * M * N * 4 >= (int64_t)1 << 31)))
             return BZ_ERR_UNSUPPORTED;
         pl.ups = (NU + nsl - 1) / nsl;
-        for (int u : kMxGemvUpw)
-            if (!upw && mx_gemv_built(mt, u) && (cu ? u == cu : u >= 2 || pl.ups == 1 || (nsl > 1 && (mt == 2 || elem == BZ_MX_E4M3))) &&
-                mx_gemv_waves(elem, mt, u) * u >= pl.ups)
+        const bool four = M <= 8 && (pl.ups >= 32 || (nsl == 1 && M <= 4 && T <= 2 && NU >= 16));
+        const int least = pl.ups == 1 || (nsl > 1 && mt == 2) ? 1 : four ? 4 : 2;
+        for (int u : kMxGemvUpw) {
+            const int share = mx_gemv_share(M, u);
+            if (!upw && mx_gemv_built(mt, u, share) && (cu ? u == cu : u >= least) &&
+                mx_gemv_waves(elem, mt, u, share) * u >= pl.ups)
                 upw = u;
+        }
         if (upw) break;
         if (cu || cs) return BZ_ERR_INVALID_ARG;
     }
     pl.nsl = (NU + pl.ups - 1) / pl.ups;
     pl.l.upw = upw;
+    pl.l.share = mx_gemv_share(M, upw);
     pl.l.nw = (pl.ups + upw - 1) / upw;
     pl.T = T;
     pl.l.mt = mt;
@@ -58,15 +72,23 @@ static int mx_gemv_plan(int elem, int M, int N, int K, int cfg, MxGemvPlan& pl) 
     return BZ_OK;
 }
 
-template <int ELEM, int MT, int UPW>
-static int launch_kernel(const MxGemvParams& p, const MxGemvLaunch& l, hipStream_t st) {
-    if constexpr (mx_gemv_built(MT, UPW)) {
-        auto kern = mx_gemv<ELEM, MT, UPW>;
+template <int ELEM, int MT, int UPW, int G>
+static int launch_share(const MxGemvParams& p, const MxGemvLaunch& l, hipStream_t st) {
+    if constexpr (mx_gemv_built(MT, UPW, G)) {
+        auto kern = mx_gemv<ELEM, MT, UPW, G>;
         if (l.lds > 65536 && raise_lds_limit(reinterpret_cast<const void*>(kern)) != BZ_OK) return BZ_ERR_LAUNCH;
         hipLaunchKernelGGL(kern, dim3(l.grid), dim3(64 * l.nw), l.lds, st, p);
         return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
     } else {
         return BZ_ERR_INVALID_ARG;
+    }
+}
+template <int ELEM, int MT, int UPW>
+static int launch_kernel(const MxGemvParams& p, const MxGemvLaunch& l, hipStream_t st) {
+    switch (l.share) {
+        case 1: return launch_share<ELEM, MT, UPW, 1>(p, l, st);
+        case 2: return launch_share<ELEM, MT, UPW, 2>(p, l, st);
+        default: return launch_share<ELEM, MT, UPW, 4>(p, l, st);
     }
 }
 template <int ELEM, int MT>

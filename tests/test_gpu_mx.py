@@ -825,3 +825,24 @@ def test_planned_calls_hold_no_memory():
         calls()
     torch.cuda.synchronize()
     assert torch.cuda.memory_allocated() == held
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+def test_few_rows_share_operands(elem):
+    """Up to 8 rows leave room for their next units: every row on its own, whatever the others hold."""
+    for n, k in ((48, 1664), (272, 640), (32, 1024)):
+        w = Weight(n, k)
+        for m in (1, 2, 3, 4, 5, 7, 8, 9):
+            x = _rows(m, k, 50 + m)
+            ref, bound = _mx_reference(x, w, elem, None, BF16)
+            for t, upw, nsl in ((0, 0, 0), (1, 2, 1), (2, 3, 1), (1, 3, 2), (3, 4, 1), (1, 5, 3), (2, 6, 1), (1, 8, 2)):
+                if upw * 8 < -(-k // 128) / max(nsl, 1):
+                    continue  # (more units than 8 waves hold)
+                cfg = t | upw << 8 | nsl << 16
+                out = mx.mx_linear(x, w.tiled, n, elem=elem, cfg=cfg)
+                _close(out, ref, bound)
+                for r in range(m):
+                    bad = x.clone()
+                    bad[r, ::128 * 3] = float("nan")
+                    got = mx.mx_linear(bad, w.tiled, n, elem=elem, cfg=cfg)
+                    assert got[r].isnan().all() and torch.equal(got[:r], out[:r]) and torch.equal(got[r + 1:], out[r + 1:])
