@@ -71,6 +71,8 @@ __all__ = [
 TILED_FORMATS = (W_INT4_TILED, W_INT4_TILED_PAIRED, W_FP8_TILED, W_FP8_TILED_PAIRED, W_MXFP4_TILED,
                  W_MXFP4_TILED_PAIRED)
 
+_INT4_TILED = (W_INT4_TILED, W_INT4_TILED_PAIRED)
+
 _DT = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
 _NO_CFG = (0, 0, 0, 0, 0)
 
@@ -130,7 +132,8 @@ def gemv(
     with ``n`` rows, optional RMSNorm gamma [K], epilogue NONE / SILU_GATE
     (N_out = n/2) / RESIDUAL (residual [M, N_out]).  Returns ``out``.
     """
-    plain = cfg is _NO_CFG and out is None and out2 is None and wfmt in TILED_FORMATS and x.is_cuda
+    plain = cfg is _NO_CFG and out is None and out2 is None and sc0 is None and sc1 is None and \
+        wfmt in TILED_FORMATS and (group == 128 or wfmt not in _INT4_TILED) and x.is_cuda
     if plain:  # a decode step's call: nothing to convert, checked and made in C++
         y = (_lib._binding or _lib.binding()).gemv(_tuning._TABLES, _tuning._ARCH, _raw_workspace, x, w, wfmt, n,
                                                    gamma, eps, epilogue, residual, out_dtype)

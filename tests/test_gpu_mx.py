@@ -846,3 +846,20 @@ def test_few_rows_share_operands(elem):
                     bad[r, ::128 * 3] = float("nan")
                     got = mx.mx_linear(bad, w.tiled, n, elem=elem, cfg=cfg)
                     assert got[r].isnan().all() and torch.equal(got[:r], out[:r]) and torch.equal(got[r + 1:], out[r + 1:])
+
+
+def test_a_refused_call_stays_refused():
+    """What the library or the checks refuse is refused the second time too."""
+    n, k = 64, 256
+    x, m = _rows(2, k, 60), Weight(n, k)
+    codes = torch.zeros(G.tiled_bytes(G.W_INT4_TILED, n, k), dtype=torch.uint8, device="cuda")
+    for _ in range(3):
+        G.gemv(x, codes, G.W_INT4_TILED, n)
+        for kw in ({"group": 64}, {"epilogue": G.EPI_SILU_GATE}, {"epilogue": 7}):
+            with pytest.raises((L.BzError, ValueError)):
+                G.gemv(x, codes, G.W_INT4_TILED, n, **kw)
+        for fmt in (G.W_MXFP4, 9, G.W_MXFP4_TILED_PAIRED):
+            with pytest.raises((L.BzError, ValueError)):
+                G.gemv(x, m.tiled, fmt, n)
+        with pytest.raises((L.BzError, ValueError)):
+            G.gemv(x, m.tiled, m.fmt, n - 8)
