@@ -50,7 +50,7 @@ HIP_FLAGS = [
 # kernel.  Attention over bf16 caches with D <= 256 (attn_bf16) is covered;
 # attn_kernel (fp32 caches, D = 512) is allowed scratch.
 NO_SCRATCH = (r"gemv_persist", r"gemv_mfma", r"gemv_i8mma", r"gemv_tile", r"gemv_stream", r"gemv_wide", r"gemv_panel",
-              r"gemm_tiled|mx_gemm|mx_quantize|mx_dequantize", r"gemv_rows", r"gemv_slab",
+              r"gemm_tiled|mx_gemm|mx_gemv|mx_quantize|mx_dequantize", r"gemv_rows", r"gemv_slab",
               r"head_f32", r"sample_cfg", r"step_tables", r"qkv_rope_cache", r"attn_bf16")
 
 

@@ -57,6 +57,13 @@ int64_t number(PyObject* o) {
 
 void* stream() { return c10::hip::getCurrentHIPStream().stream(); }
 
+// Allocation and launch can wait for the GPU, and what it waits for may need
+// the interpreter (a host function of a stream).
+struct NoGil {
+    PyThreadState* state = PyEval_SaveThread();
+    ~NoGil() { PyEval_RestoreThread(state); }
+};
+
 // Address and bytes of `need` bytes of workspace from f(device index, stream,
 // need), which Python keeps; false with an error set.
 bool workspace(PyObject* f, const at::Tensor& x, int64_t need, void*& at, size_t& bytes) {
@@ -128,7 +135,7 @@ PyObject* gemv(PyObject*, PyObject* const* a, Py_ssize_t count) {
         d.residual = r->data_ptr();
         d.ldr = r->stride(0);
     }
-    at::Tensor out = at::empty({M, n_out}, x->options().dtype(odt == BZ_DT_F32 ? at::kFloat : at::kBFloat16));
+    if (need && !workspace(a[2], *x, need, d.workspace, d.workspace_bytes)) return nullptr;
     d.abi_version = BZ_ABI_VERSION;
     d.M = (int32_t)M;
     d.N = (int32_t)n;
@@ -146,10 +153,16 @@ PyObject* gemv(PyObject*, PyObject* const* a, Py_ssize_t count) {
     d.x = x->data_ptr();
     d.ldx = ld;
     d.w = w->data_ptr();
-    d.out = out.data_ptr();
     d.ldo = n_out;
-    if (need && !workspace(a[2], *x, need, d.workspace, d.workspace_bytes)) return nullptr;
-    if (f_gemv(&d, stream()) != BZ_OK) Py_RETURN_NONE;
+    at::Tensor out;
+    int rc;
+    {
+        NoGil no_gil;
+        out = at::empty({M, n_out}, x->options().dtype(odt == BZ_DT_F32 ? at::kFloat : at::kBFloat16));
+        d.out = out.data_ptr();
+        rc = f_gemv(&d, stream());
+    }
+    if (rc != BZ_OK) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
 }
@@ -164,12 +177,17 @@ PyObject* quantize_mx(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const int64_t M = x->size(0), K = x->size(1), ld = M == 1 ? K : x->stride(0);
     if (dt < 0 || M < 1 || K < 1 || K % 32 || M > INT32_MAX || K > INT32_MAX || x->stride(1) != 1 || ld < K)
         Py_RETURN_NONE;
-    at::Tensor codes = el == BZ_MX_E2M1 ? at::empty({M, K / 2}, x->options().dtype(at::kByte))
-                                        : at::empty({M, K}, x->options().dtype(at::kFloat8_e4m3fn));
-    at::Tensor scales = at::empty({M, K / 32}, x->options().dtype(at::kByte));
-    if (f_quantize(x->data_ptr(), dt, ld, (int32_t)M, (int32_t)K, el, BZ_MX_ROWS, codes.data_ptr(), scales.data_ptr(),
-                   stream()) != BZ_OK)
-        Py_RETURN_NONE;
+    at::Tensor codes, scales;
+    int rc;
+    {
+        NoGil no_gil;
+        codes = el == BZ_MX_E2M1 ? at::empty({M, K / 2}, x->options().dtype(at::kByte))
+                                 : at::empty({M, K}, x->options().dtype(at::kFloat8_e4m3fn));
+        scales = at::empty({M, K / 32}, x->options().dtype(at::kByte));
+        rc = f_quantize(x->data_ptr(), dt, ld, (int32_t)M, (int32_t)K, el, BZ_MX_ROWS, codes.data_ptr(),
+                        scales.data_ptr(), stream());
+    }
+    if (rc != BZ_OK) Py_RETURN_NONE;
     PyObject* r = PyTuple_New(2);
     if (!r) return nullptr;
     PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(codes)));
@@ -192,10 +210,15 @@ PyObject* dequantize_mx(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const int64_t M = codes->size(0), K = codes->size(1) * (e4m3 ? 1 : 2);
     if (M < 1 || K < 1 || K % 32 || M > INT32_MAX || K > INT32_MAX || scales->size(0) != M || scales->size(1) != K / 32)
         Py_RETURN_NONE;
-    at::Tensor out = at::empty({M, K}, codes->options().dtype(dt == BZ_DT_F32 ? at::kFloat : at::kBFloat16));
-    if (f_dequantize(codes->data_ptr(), scales->data_ptr(), el, (int32_t)M, (int32_t)K, out.data_ptr(), dt, K,
-                     stream()) != BZ_OK)
-        Py_RETURN_NONE;
+    at::Tensor out;
+    int rc;
+    {
+        NoGil no_gil;
+        out = at::empty({M, K}, codes->options().dtype(dt == BZ_DT_F32 ? at::kFloat : at::kBFloat16));
+        rc = f_dequantize(codes->data_ptr(), scales->data_ptr(), el, (int32_t)M, (int32_t)K, out.data_ptr(), dt, K,
+                          stream());
+    }
+    if (rc != BZ_OK) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
 }
@@ -233,13 +256,19 @@ PyObject* mx_linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
             (M > 1 && r->stride(0) < n))
             Py_RETURN_NONE;
     }
-    at::Tensor out = at::empty({M, n}, x->options().dtype(odt == BZ_DT_F32 ? at::kFloat : at::kBFloat16));
     void* ws = nullptr;
     size_t bytes = 0;
     if (need && !workspace(a[1], *x, need, ws, bytes)) return nullptr;
-    if (f_mx_gemv(el, x->data_ptr(), ld, (int32_t)M, w->data_ptr(), (int32_t)n, (int32_t)K, r ? r->data_ptr() : nullptr,
-                  rdt, r && M > 1 ? r->stride(0) : n, out.data_ptr(), odt, n, ws, bytes, 0, stream()) != BZ_OK)
-        Py_RETURN_NONE;
+    at::Tensor out;
+    int rc;
+    {
+        NoGil no_gil;
+        out = at::empty({M, n}, x->options().dtype(odt == BZ_DT_F32 ? at::kFloat : at::kBFloat16));
+        rc = f_mx_gemv(el, x->data_ptr(), ld, (int32_t)M, w->data_ptr(), (int32_t)n, (int32_t)K,
+                       r ? r->data_ptr() : nullptr, rdt, r && M > 1 ? r->stride(0) : n, out.data_ptr(), odt, n, ws,
+                       bytes, 0, stream());
+    }
+    if (rc != BZ_OK) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
 }
