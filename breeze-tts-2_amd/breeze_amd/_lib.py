@@ -286,7 +286,8 @@ def binding():
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         module.bind(*(ctypes.cast(getattr(lib(), f), ctypes.c_void_p).value
-                      for f in ("bz_gemv", "bz_mx_gemv", "bz_mx_quantize", "bz_mx_dequantize")))
+                      for f in ("bz_gemv", "bz_mx_gemv", "bz_mx_gemm", "bz_mx_quantize", "bz_mx_dequantize",
+                                "bz_gemm_tiled", "bz_gemm_workspace", "bz_tiled_bytes")))
         _binding = module
     return _binding
 

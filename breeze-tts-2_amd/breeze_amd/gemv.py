@@ -535,12 +535,17 @@ def dequant_matmul(x: torch.Tensor, w: torch.Tensor, wfmt: int, n: int, k: int,
                    chunk_bytes: int = 16 << 20) -> torch.Tensor:
     """x [M, k] @ w_eff^T -> bf16 [M, n] for prefill-sized M, over an unpaired
     tiled weight (BZ_W_INT4_TILED, group 128, BZ_W_FP8_TILED or
-    BZ_W_MXFP4_TILED): one GEMM (bz_gemm_tiled) that decodes the weight in registers, so no decoded copy
-    exists; where it slices K, the slices' fp32 sums are held for the call.
+    BZ_W_MXFP4_TILED): one GEMM (bz_gemm_tiled) that decodes the weight in
+    registers, so no decoded copy exists; where it slices K, the slices' fp32
+    sums are held for the call.
     An x that autograd follows goes through torch's linear over the decoded
     weight instead (at most ``chunk_bytes`` of fp32 weight at a time)."""
     if wfmt not in (W_INT4_TILED, W_FP8_TILED, W_MXFP4_TILED):
         raise ValueError(f"dequant_matmul reads the unpaired tiled formats, not format {wfmt}")
+    if x.is_cuda and torch.autograd.forward_ad._current_level < 0:
+        y = (_lib._binding or _lib.binding()).dequant_matmul(x, w, wfmt, n, k)
+        if y is not None:
+            return y
     _require_gpu("x", x, x.device)
     _require_gpu("w", w, x.device)
     w = w.contiguous()

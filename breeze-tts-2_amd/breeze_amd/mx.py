@@ -190,7 +190,7 @@ def _tiled_rows(x, M: int, K: int, ld: int, dt: int, code: int, index: int) -> t
 # each graph capture under way.
 _WS: dict = {}
 _WS_RETIRED: list = []
-_FEW_PLANS: dict = {}  # (element type, M, n, K) -> _plan's answer, for the binding
+_PLANS: dict = {}  # (element type, M, n, K) -> _plan's answer and the bytes of the quantised rows, for the binding
 _NO_WAY = (1 << 64) - 1  # what bz_mx_gemv_workspace gives for a shape it does not take
 
 
@@ -218,8 +218,8 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
     be out itself; out: [M, n] with unit column stride, apart from x and w.  cfg: a
     launch shape (include/bz_mx.h) instead of the built-in rule's."""
     rows = isinstance(x, MxRows)
-    if not (rows or cfg) and out is None and x.is_cuda:  # few rows, nothing to convert
-        y = (_lib._binding or _lib.binding()).mx_linear(_FEW_PLANS, _raw_workspace, x, w, n, elem, residual, out_dtype)
+    if not (rows or cfg) and out is None and x.is_cuda:  # nothing to convert: checked and made in C++
+        y = (_lib._binding or _lib.binding()).mx_linear(_PLANS, _raw_workspace, x, w, n, elem, residual, out_dtype)
         if y is not None:
             return y
     if rows:
@@ -235,8 +235,8 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
         # up to 32 rows that a launch can read as they are: quantised inside it
         few = dt == DT_BF16 and M <= FEW_ROWS and not (ld & 7 or src.data_ptr() & 15) and M * ld < 1 << 30
     weight, few, need = _plan(code, M, n, K, cfg, few)
-    if few and not cfg:
-        _FEW_PLANS[code, M, n, K] = weight, few, need
+    if not cfg and not rows and few == (0 < M <= FEW_ROWS):  # (not the two launches of few rows that need a copy)
+        _PLANS[code, M, n, K] = weight, few, need, 0 if few else _rows_bytes(code, M, K)
     if w.get_device() != index or w.numel() * w.element_size() != weight or not w.is_contiguous() or w.data_ptr() & 15:
         _gpu("w", w, index)
         raise ValueError(f"w must be a contiguous W_MXFP4_TILED weight of {n} x {K} (rows a multiple of 16), "

@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "bz_gemm.h"
+#include "bz_plans.h"
 
 namespace bz {
 
@@ -86,7 +87,7 @@ static int gemm_shape(int M, int N, int K, int mt, int nt, int nsl, GemmPlan& pl
 constexpr int kGemmSlices[] = {1, 2, 3, 4, 6, 8, 12};
 constexpr unsigned kGemmSlicedGrid = 520;
 
-static int gemm_plan(int wf, int M, int N, int K, int cfg_mt, int cfg_nt, int cfg_nsl, GemmPlan& pl) {
+static int gemm_choose(int wf, int M, int N, int K, int cfg_mt, int cfg_nt, int cfg_nsl, GemmPlan& pl) {
     if (cfg_nsl > 64) return BZ_ERR_INVALID_ARG;
     float best = 0.0f;
     bool found = false;
@@ -110,6 +111,11 @@ static int gemm_plan(int wf, int M, int N, int K, int cfg_mt, int cfg_nt, int cf
     return found ? BZ_OK : BZ_ERR_INVALID_ARG;
 }
 
+static int gemm_plan(int wf, int M, int N, int K, int cfg, GemmPlan& pl) {
+    return planned(PlanKey{wf, M, N, K, cfg}, pl,
+                   [&](GemmPlan& q) { return gemm_choose(wf, M, N, K, cfg & 255, (cfg >> 8) & 255, cfg >> 16, q); });
+}
+
 static int gemm_check(int wf, int M, int N, int K) {
     if (M < 1 || N < 1 || K < 1) return BZ_ERR_INVALID_ARG;
     if (wf != BZ_W_INT4_TILED && wf != BZ_W_FP8_TILED && wf != BZ_W_MXFP4_TILED) return BZ_ERR_INVALID_ARG;
@@ -124,7 +130,7 @@ using namespace bz;
 extern "C" size_t bz_gemm_workspace(int32_t wfmt, int32_t M, int32_t N, int32_t K, int32_t cfg) {
     GemmPlan pl;
     if (gemm_check(wfmt, M, N, K) != BZ_OK || cfg < 0) return 0;
-    return gemm_plan(wfmt, M, N, K, cfg & 255, (cfg >> 8) & 255, cfg >> 16, pl) == BZ_OK ? pl.ws : 0;
+    return gemm_plan(wfmt, M, N, K, cfg, pl) == BZ_OK ? pl.ws : 0;
 }
 
 extern "C" int bz_gemm_tiled(int32_t wfmt, const void* x, int64_t ldx, int32_t M, const void* w, int32_t N, int32_t K,
@@ -139,7 +145,7 @@ extern "C" int bz_gemm_tiled(int32_t wfmt, const void* x, int64_t ldx, int32_t M
     if (off(x, 16) || ldx % 8 || off(w, 16) || off(out, out_dtype == BZ_DT_F32 ? 4 : 2)) return BZ_ERR_ALIGNMENT;
     if (ldx > (int64_t)1 << 22) return BZ_ERR_UNSUPPORTED;  // 32-bit offsets within a row tile
     GemmPlan pl;
-    const int prc = gemm_plan(wfmt, M, N, K, cfg & 255, (cfg >> 8) & 255, cfg >> 16, pl);
+    const int prc = gemm_plan(wfmt, M, N, K, cfg, pl);
     if (prc != BZ_OK) return prc;
     if (pl.ws && (!workspace || off(workspace, 16) || workspace_bytes < pl.ws)) return BZ_ERR_INVALID_ARG;
     GemmParams p{};

@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "bz_mx_gemm.h"
+#include "bz_plans.h"
 
 namespace bz {
 
@@ -83,7 +84,7 @@ static float mx_gemm_cost(int elem, int M, int N, int K, const MxGemmCost& c, co
 constexpr int kMxSlices[] = {1, 2, 3, 4, 6, 8};
 constexpr unsigned kMxSlicedGrid = 600;  // more workgroups than this never won with slices
 
-static int mx_gemm_plan(int elem, int M, int N, int K, int cfg, MxGemmPlan& pl) {
+static int mx_gemm_choose(int elem, int M, int N, int K, int cfg, MxGemmPlan& pl) {
     const int ctm = cfg & 255, ctn = (cfg >> 8) & 255, csl = cfg >> 16;
     if (csl > 64) return BZ_ERR_INVALID_ARG;
     float best = 0.0f;
@@ -112,6 +113,10 @@ static int mx_gemm_plan(int elem, int M, int N, int K, int cfg, MxGemmPlan& pl) 
     else
         for (const MxGemmCost& c : kMxCostE4m3) look(c);
     return found ? BZ_OK : rc;
+}
+
+static int mx_gemm_plan(int elem, int M, int N, int K, int cfg, MxGemmPlan& pl) {
+    return planned(PlanKey{elem, M, N, K, cfg}, pl, [&](MxGemmPlan& q) { return mx_gemm_choose(elem, M, N, K, cfg, q); });
 }
 
 static int mx_gemm_check(int elem, int M, int N, int K) {

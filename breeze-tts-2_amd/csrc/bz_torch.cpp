@@ -24,6 +24,10 @@ namespace {
 // entries of the library, which Python has loaded
 decltype(&bz_gemv) f_gemv;
 decltype(&bz_mx_gemv) f_mx_gemv;
+decltype(&bz_mx_gemm) f_mx_gemm;
+decltype(&bz_gemm_tiled) f_gemm;
+decltype(&bz_gemm_workspace) f_gemm_workspace;
+decltype(&bz_tiled_bytes) f_tiled_bytes;
 decltype(&bz_mx_quantize) f_quantize;
 decltype(&bz_mx_dequantize) f_dequantize;
 PyObject* tiled_key;  // "tiled"
@@ -41,6 +45,9 @@ bool aligned(const at::Tensor& t, uintptr_t to) { return reinterpret_cast<uintpt
 // bz_dtype of bf16 and fp32, else -1.
 int dtype_of(at::ScalarType t) { return t == at::kBFloat16 ? BZ_DT_BF16 : t == at::kFloat ? BZ_DT_F32 : -1; }
 int dtype_of(PyObject* o) { return THPDtype_Check(o) ? dtype_of(reinterpret_cast<THPDtype*>(o)->scalar_type) : -1; }
+
+// x type of bz_mx_quantize, else -1.
+int x_dtype(const at::Tensor& t) { return t.scalar_type() == at::kHalf ? BZ_MX_F16 : dtype_of(t.scalar_type()); }
 
 int elem(PyObject* o) {
     if (!PyUnicode_Check(o)) return -1;
@@ -173,7 +180,7 @@ PyObject* quantize_mx(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const at::Tensor* x = count == 2 ? gpu(a[0]) : nullptr;
     const int el = x ? elem(a[1]) : -1;
     if (el < 0 || x->dim() != 2) Py_RETURN_NONE;
-    const int dt = x->scalar_type() == at::kHalf ? BZ_MX_F16 : dtype_of(x->scalar_type());
+    const int dt = x_dtype(*x);
     const int64_t M = x->size(0), K = x->size(1), ld = M == 1 ? K : x->stride(0);
     if (dt < 0 || M < 1 || K < 1 || K % 32 || M > INT32_MAX || K > INT32_MAX || x->stride(1) != 1 || ld < K)
         Py_RETURN_NONE;
@@ -223,30 +230,31 @@ PyObject* dequantize_mx(PyObject*, PyObject* const* a, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
-// mx_linear(plans, workspace, x, w, n, elem, residual, out_dtype): up to 32 bf16
-// rows, quantised in the product's launch.  plans: (elem, M, n, K) -> (bytes of
-// the weight, whether one launch takes them, workspace bytes).
+// mx_linear(plans, workspace, x, w, n, elem, residual, out_dtype).  plans:
+// (elem, M, n, K) -> (bytes of the weight, whether one launch takes bf16 rows as
+// they are, workspace bytes, bytes of the quantised rows).
 PyObject* mx_linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
     HANDLE_TH_ERRORS
     if (count != 8 || !PyDict_Check(a[0])) Py_RETURN_NONE;
     const at::Tensor *x = gpu(a[2]), *w = gpu(a[3]);
     const int64_t n = number(a[4]);
     const int el = elem(a[5]), odt = dtype_of(a[7]);
-    if (!x || !w || n < 1 || el < 0 || odt < 0 || x->dim() != 2 || x->scalar_type() != at::kBFloat16 ||
-        (x->requires_grad() && c10::GradMode::is_enabled()))
+    if (!x || !w || n < 1 || el < 0 || odt < 0 || x->dim() != 2 || (x->requires_grad() && c10::GradMode::is_enabled()))
         Py_RETURN_NONE;
+    const int dt = x_dtype(*x);
     const int64_t M = x->size(0), K = x->size(1), ld = M == 1 ? K : x->stride(0);
-    if (M < 1 || M > 32 || x->stride(1) != 1 || ld < K || ld % 8 || M * ld >= 1 << 30 || !aligned(*x, 16)) Py_RETURN_NONE;
+    if (dt < 0 || M < 1 || M > INT32_MAX || x->stride(1) != 1 || ld < K) Py_RETURN_NONE;
     PyObject* key = Py_BuildValue("(iLLL)", el, (long long)M, (long long)n, (long long)K);
     PyObject* plan = key ? PyDict_GetItemWithError(a[0], key) : nullptr;
     Py_XDECREF(key);
-    if (!plan || !PyTuple_Check(plan) || PyTuple_GET_SIZE(plan) != 3) {
+    if (!plan || !PyTuple_Check(plan) || PyTuple_GET_SIZE(plan) != 4) {
         if (PyErr_Occurred()) return nullptr;
         Py_RETURN_NONE;
     }
-    const int64_t need = number(PyTuple_GET_ITEM(plan, 2));
-    if (!w->is_contiguous() || (int64_t)w->nbytes() != number(PyTuple_GET_ITEM(plan, 0)) ||
-        PyTuple_GET_ITEM(plan, 1) != Py_True || need < 0)
+    const bool few = PyTuple_GET_ITEM(plan, 1) == Py_True;
+    const int64_t need = number(PyTuple_GET_ITEM(plan, 2)), rows = number(PyTuple_GET_ITEM(plan, 3));
+    if (!w->is_contiguous() || (int64_t)w->nbytes() != number(PyTuple_GET_ITEM(plan, 0)) || need < 0 || rows < 0 ||
+        (few && (dt != BZ_DT_BF16 || ld % 8 || M * ld >= 1 << 30 || !aligned(*x, 16))))
         Py_RETURN_NONE;
     const at::Tensor* r = a[6] == Py_None ? nullptr : gpu(a[6]);
     int rdt = 0;
@@ -256,6 +264,8 @@ PyObject* mx_linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
             (M > 1 && r->stride(0) < n))
             Py_RETURN_NONE;
     }
+    const void* res = r ? r->data_ptr() : nullptr;
+    const int64_t ldr = r && M > 1 ? r->stride(0) : n;
     void* ws = nullptr;
     size_t bytes = 0;
     if (need && !workspace(a[1], *x, need, ws, bytes)) return nullptr;
@@ -264,29 +274,74 @@ PyObject* mx_linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
     {
         NoGil no_gil;
         out = at::empty({M, n}, x->options().dtype(odt == BZ_DT_F32 ? at::kFloat : at::kBFloat16));
-        rc = f_mx_gemv(el, x->data_ptr(), ld, (int32_t)M, w->data_ptr(), (int32_t)n, (int32_t)K,
-                       r ? r->data_ptr() : nullptr, rdt, r && M > 1 ? r->stride(0) : n, out.data_ptr(), odt, n, ws,
-                       bytes, 0, stream());
+        if (few) {
+            rc = f_mx_gemv(el, x->data_ptr(), ld, (int32_t)M, w->data_ptr(), (int32_t)n, (int32_t)K, res, rdt, ldr,
+                           out.data_ptr(), odt, n, ws, bytes, 0, stream());
+        } else {
+            at::Tensor q = at::empty({rows}, x->options().dtype(at::kByte));
+            rc = f_quantize(x->data_ptr(), dt, ld, (int32_t)M, (int32_t)K, el, BZ_MX_TILED, q.data_ptr(), nullptr,
+                            stream());
+            if (rc == BZ_OK)
+                rc = f_mx_gemm(el, q.data_ptr(), (int32_t)M, w->data_ptr(), (int32_t)n, (int32_t)K, res, rdt, ldr,
+                               out.data_ptr(), odt, n, ws, bytes, 0, stream());
+        }
     }
     if (rc != BZ_OK) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
 }
 
-// bind(gemv, mx_gemv, quantize, dequantize): addresses of the library's entries
+// dequant_matmul(x, w, wfmt, n, k) of an x without forward gradients
+PyObject* dequant_matmul(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    if (count != 5) Py_RETURN_NONE;
+    const at::Tensor *x = gpu(a[0]), *w = gpu(a[1]);
+    const int64_t wfmt = number(a[2]), n = number(a[3]), k = number(a[4]);
+    if (!x || !w || (wfmt != BZ_W_INT4_TILED && wfmt != BZ_W_FP8_TILED && wfmt != BZ_W_MXFP4_TILED) || n < 1 ||
+        n > INT32_MAX || k < 1 || k > INT32_MAX || x->dim() != 2 || x->size(1) != k ||
+        x->scalar_type() != at::kBFloat16 || (x->requires_grad() && c10::GradMode::is_enabled()))
+        Py_RETURN_NONE;
+    const int64_t M = x->size(0), ld = x->stride(0);
+    const size_t bytes = f_tiled_bytes((int32_t)wfmt, (int32_t)n, (int32_t)k);
+    if (M < 1 || M > INT32_MAX || x->stride(1) != 1 || ld < k || ld > 1 << 22 || ld % 8 || !aligned(*x, 16) || !bytes ||
+        !w->is_contiguous() || w->nbytes() != bytes)
+        Py_RETURN_NONE;
+    at::Tensor out;
+    int rc;
+    {
+        NoGil no_gil;
+        out = at::empty({M, n}, x->options());
+        const size_t need = f_gemm_workspace((int32_t)wfmt, (int32_t)M, (int32_t)n, (int32_t)k, 0);
+        // from the caching allocator: its memory is reused in stream order
+        at::Tensor sums;
+        if (need) sums = at::empty({(int64_t)need}, x->options().dtype(at::kByte));
+        rc = f_gemm((int32_t)wfmt, x->data_ptr(), ld, (int32_t)M, w->data_ptr(), (int32_t)n, (int32_t)k, out.data_ptr(), n,
+                    BZ_DT_BF16, need ? sums.data_ptr() : nullptr, need, 0, stream());
+    }
+    if (rc != BZ_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// bind(addresses): of the library's entries, in this order
 PyObject* bind(PyObject*, PyObject* args) {
-    unsigned long long g, m, q, r;
-    if (!PyArg_ParseTuple(args, "KKKK", &g, &m, &q, &r)) return nullptr;
-    f_mx_gemv = reinterpret_cast<decltype(f_mx_gemv)>(m);
-    f_gemv = reinterpret_cast<decltype(f_gemv)>(g);
-    f_quantize = reinterpret_cast<decltype(f_quantize)>(q);
-    f_dequantize = reinterpret_cast<decltype(f_dequantize)>(r);
+    unsigned long long p[8];
+    if (!PyArg_ParseTuple(args, "KKKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, p + 7)) return nullptr;
+    f_gemv = reinterpret_cast<decltype(f_gemv)>(p[0]);
+    f_mx_gemv = reinterpret_cast<decltype(f_mx_gemv)>(p[1]);
+    f_mx_gemm = reinterpret_cast<decltype(f_mx_gemm)>(p[2]);
+    f_quantize = reinterpret_cast<decltype(f_quantize)>(p[3]);
+    f_dequantize = reinterpret_cast<decltype(f_dequantize)>(p[4]);
+    f_gemm = reinterpret_cast<decltype(f_gemm)>(p[5]);
+    f_gemm_workspace = reinterpret_cast<decltype(f_gemm_workspace)>(p[6]);
+    f_tiled_bytes = reinterpret_cast<decltype(f_tiled_bytes)>(p[7]);
     Py_RETURN_NONE;
 }
 
 PyMethodDef methods[] = {
     {"gemv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gemv)), METH_FASTCALL, nullptr},
     {"mx_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx_linear)), METH_FASTCALL, nullptr},
+    {"dequant_matmul", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dequant_matmul)), METH_FASTCALL, nullptr},
     {"quantize_mx", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(quantize_mx)), METH_FASTCALL, nullptr},
     {"dequantize_mx", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dequantize_mx)), METH_FASTCALL, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},

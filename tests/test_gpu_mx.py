@@ -863,3 +863,60 @@ def test_a_refused_call_stays_refused():
                 G.gemv(x, m.tiled, fmt, n)
         with pytest.raises((L.BzError, ValueError)):
             G.gemv(x, m.tiled, m.fmt, n - 8)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_prompts_after_a_planned_one(dtype):
+    n, k, m = 256, 1024, 77
+    w, x = Weight(n, k), _rows(m, k, 70, dtype)
+    res = _rows(m, n, 71)
+    wide = torch.empty(m, k + 3, device="cuda", dtype=dtype)
+    wide[:, 3:] = x
+    for elem in ELEMS:
+        ref, bound = _mx_reference(x, w, elem, None, BF16)
+        first = mx.mx_linear(x, w.tiled, n, elem=elem)
+        _close(first, ref, bound)
+        for view in (x, wide[:, 3:], x.t().contiguous().t()):
+            for _ in range(2):
+                assert torch.equal(mx.mx_linear(view, w.tiled, n, elem=elem), first)
+        added = mx.mx_linear(x, w.tiled, n, elem=elem, residual=res, out_dtype=F32)
+        _close(added, *_mx_reference(x, w, elem, res, F32))
+        assert torch.equal(mx.mx_linear(x, w.tiled, n, elem=elem, residual=res.float(), out_dtype=F32), added)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            mx.mx_linear(x.clone().requires_grad_(), w.tiled, n, elem=elem)
+        with pytest.raises(ValueError):
+            mx.mx_linear(x, w.tiled[:-16], n, elem=elem)
+    xb = x.to(BF16)
+    first = G.dequant_matmul(xb, w.tiled, w.fmt, n, k)
+    _close(first, *_gemv_reference(xb, w, G.EPI_NONE, None, 0.0, None, BF16))
+    for view in (xb, wide[:, 3:], wide.to(BF16)[:, 3:], x):
+        assert torch.equal(G.dequant_matmul(view, w.tiled, w.fmt, n, k), first)
+    for args in ((xb, w.tiled[:-16], w.fmt, n, k), (xb, w.tiled, w.fmt, n, k - 128), (xb, w.tiled, w.fmt, n - 8, k),
+                 (xb, w.tiled, G.W_MXFP4_TILED_PAIRED, n, k)):
+        for _ in range(2):
+            with pytest.raises((ValueError, L.BzError)):
+                G.dequant_matmul(*args)
+    xg = xb.clone().requires_grad_()
+    G.dequant_matmul(xg, w.tiled, w.fmt, n, k).sum().backward()
+    assert xg.grad is not None
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(xb, torch.ones_like(xb))
+        out = G.dequant_matmul(dual, w.tiled, w.fmt, n, k)
+        assert torch.autograd.forward_ad.unpack_dual(out).tangent is not None
+    assert G.dequant_matmul(xb[:0], w.tiled, w.fmt, n, k).shape == (0, n)
+
+
+def test_launch_shapes_of_each_call():
+    """Plans that a thread keeps: the last of each place, whatever was asked for between."""
+    n, k = 256, 2048
+    w = Weight(n, k)
+    xs = {m: _rows(m, k, 80 + m) for m in range(33, 160, 9)}
+    first = {m: (mx.mx_linear(x, w.tiled, n), mx.mx_linear(x, w.tiled, n, elem="e4m3"),
+                 G.dequant_matmul(x, w.tiled, w.fmt, n, k)) for m, x in xs.items()}
+    for m, x in reversed(xs.items()):
+        ref, bound = _mx_reference(x, w, O.E2M1, None, BF16)
+        _close(mx.mx_linear(x, w.tiled, n, cfg=1 | 2 << 8 | 2 << 16), ref, bound)
+        again = (mx.mx_linear(x, w.tiled, n), mx.mx_linear(x, w.tiled, n, elem="e4m3"),
+                 G.dequant_matmul(x, w.tiled, w.fmt, n, k))
+        for a, b in zip(first[m], again):
+            assert torch.equal(a, b)
