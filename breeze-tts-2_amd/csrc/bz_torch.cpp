@@ -1,8 +1,8 @@
-// Torch binding of the calls whose host work would take longer than their
-// kernels: a decode step's products over tiled weights, and quantising a few
-// rows.  In Python the checks, the descriptor, the output and the library call
-// take 7.6 us; here they take 5.1 us, 2.6 of them HIP's launch (quantise 8.0 -> 4.8,
-// read back 6.7 -> 4.4, a product of quantised rows 7.9 -> 4.8).
+// Torch binding of the calls whose host work can take longer than their
+// kernels: products over tiled weights, and quantising rows.  In Python the
+// checks, the descriptor, the output and the library call of a decode step's
+// product take 7.6 us; here they take 5.1 us, 2.6 of them HIP's launch (quantise
+// 8.0 -> 4.8, read back 6.7 -> 4.4, a product of quantised rows 7.9 -> 4.8).
 //
 // Every function takes its arguments as the Python function of its name does
 // and returns None where one of them needs converting or copying, another
