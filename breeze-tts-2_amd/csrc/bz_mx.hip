@@ -9,6 +9,7 @@
 
 #include "bz_mx.h"
 #include "bz_mx_device.h"
+#include "bz_row_runs.h"
 
 namespace bz {
 
@@ -239,9 +240,6 @@ static bool mx_elem_ok(int elem) { return elem == BZ_MX_E2M1 || elem == BZ_MX_E4
 static bool off(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 static int launched() { return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH; }
 
-// Rows one launch takes: its items of eight values fit 32 bits.
-static int rows_per_launch(int M, int K) { return (int)std::min<int64_t>(M, ((int64_t)1 << 31) / (K / 8)); }
-
 template <int ELEM, class X>
 static int launch_quantize(const void* x, int64_t ldx, int M, int K, int layout, void* codes, void* scales,
                            hipStream_t st) {
@@ -256,18 +254,14 @@ static int launch_quantize(const void* x, int64_t ldx, int M, int K, int layout,
                            static_cast<uint8_t*>(codes), chunk, groups);
         return launched();
     }
-    const int rows = rows_per_launch(M, K);
     const int64_t row_codes = ELEM == BZ_MX_E2M1 ? K / 2 : K;
-    for (int m0 = 0; m0 < M; m0 += rows) {
-        const uint32_t items = (uint32_t)std::min(rows, M - m0) * (uint32_t)(K / 8);
+    return for_row_runs(M, K, [&](int64_t m0, int rows) {
+        const uint32_t items = (uint32_t)rows * (uint32_t)(K / 8);
         hipLaunchKernelGGL((mx_quantize_rows<ELEM, X>), dim3((items + 255) / 256), dim3(256), 0, st,
-                           xp + (int64_t)m0 * ldx * X::kBytes, ldx, items, K / 8, vec,
-                           static_cast<uint8_t*>(codes) + m0 * row_codes,
-                           static_cast<uint8_t*>(scales) + (int64_t)m0 * (K / 32));
-        const int rc = launched();
-        if (rc != BZ_OK) return rc;
-    }
-    return BZ_OK;
+                           xp + m0 * ldx * X::kBytes, ldx, items, K / 8, vec,
+                           static_cast<uint8_t*>(codes) + m0 * row_codes, static_cast<uint8_t*>(scales) + m0 * (K / 32));
+        return launched();
+    });
 }
 
 template <int ELEM>
@@ -310,16 +304,13 @@ extern "C" int bz_mx_dequantize(const void* codes, const void* scales, int32_t e
     if (off(codes, 4) || off(out, f32 ? 4 : 2)) return BZ_ERR_ALIGNMENT;
     const bool vec = !off(out, 16) && (ldo * (f32 ? 4 : 2)) % 16 == 0;
     const int64_t row_codes = elem == BZ_MX_E2M1 ? K / 2 : K;
-    const int rows = rows_per_launch(M, K);
-    for (int m0 = 0; m0 < M; m0 += rows) {
-        const uint32_t items = (uint32_t)std::min(rows, M - m0) * (uint32_t)(K / 8);
+    return for_row_runs(M, K, [&](int64_t m0, int rows) {
+        const uint32_t items = (uint32_t)rows * (uint32_t)(K / 8);
         auto kern = elem == BZ_MX_E2M1 ? mx_dequantize_rows<BZ_MX_E2M1> : mx_dequantize_rows<BZ_MX_E4M3>;
         hipLaunchKernelGGL(kern, dim3((items + 255) / 256), dim3(256), 0, static_cast<hipStream_t>(stream),
                            static_cast<const uint8_t*>(codes) + m0 * row_codes,
-                           static_cast<const uint8_t*>(scales) + (int64_t)m0 * (K / 32), items, K / 8,
-                           static_cast<uint8_t*>(out) + (int64_t)m0 * ldo * (f32 ? 4 : 2), ldo, f32, vec);
-        const int rc = launched();
-        if (rc != BZ_OK) return rc;
-    }
-    return BZ_OK;
+                           static_cast<const uint8_t*>(scales) + m0 * (K / 32), items, K / 8,
+                           static_cast<uint8_t*>(out) + m0 * ldo * (f32 ? 4 : 2), ldo, f32, vec);
+        return launched();
+    });
 }

@@ -1,0 +1,50 @@
+"""Calls of the microscaled operators at the edges of what they take, without a GPU."""
+
+from __future__ import annotations
+
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parents[1] / "breeze-tts-2_amd" / "csrc"
+
+
+# ---- rows cut into launches -------------------------------------------------------------------------
+
+
+ROW_RUNS = """
+#include <cstdio>
+#include "bz_row_runs.h"
+int main() {
+    const int cases[][2] = {%s};
+    for (auto& c : cases) {
+        int64_t next = 0;
+        int runs = 0;
+        const int rc = bz::for_row_runs(c[0], c[1], [&](int64_t m0, int rows) {
+            if (m0 != next || rows < 1 || (int64_t)rows * (c[1] / 8) > (int64_t)1 << 31) return 1;
+            next = m0 + rows;
+            return ++runs > 1000 ? 2 : 0;
+        });
+        std::printf("%%d %%lld %%d\\n", rc, (long long)next, runs);
+    }
+    return bz::for_row_runs(7, 32, [](int64_t, int) { return 5; }) == 5 ? 0 : 1;
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="no host compiler")
+def test_row_runs_cover_every_row_once(tmp_path):
+    """Up to 2^31 - 1 rows: a first row past 2^31 was a write 34 GB before the buffer."""
+    rows = [1, 2 ** 29, 2 ** 29 + 1, 3 * 2 ** 29, 3 * 2 ** 29 + 1, 2 ** 31 - 1]
+    cases = [(m, 32) for m in rows] + [(2 ** 31 - 1, 64), (9, 2 ** 31 - 32), (2 ** 20, 2 ** 16)]
+    (tmp_path / "runs.cpp").write_text(ROW_RUNS % ", ".join(f"{{{m}, {k}}}" for m, k in cases))
+    exe = tmp_path / "runs"
+    subprocess.run(["g++", "-std=c++17", "-O1", f"-I{CSRC}",
+                    str(tmp_path / "runs.cpp"), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split("\n")
+    for (m, k), line in zip(cases, out):
+        rc, end, runs = map(int, line.split())
+        per = min(m, 2 ** 31 // (k // 8))
+        assert rc == 0 and end == m and runs == -(-m // per), (m, k, line)
