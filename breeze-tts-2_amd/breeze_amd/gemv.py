@@ -300,6 +300,7 @@ def pack_tiled(src_wfmt: int, w: torch.Tensor, k: int, dst_wfmt: int, *, sc0: Op
         n = (w.numel() * w.element_size()) // row_bytes
         if sc0 is None:
             raise ValueError("a row-major source needs its scales (sc0)")
+        _require_gpu("sc0", sc0, w.device)
         _check_weight(w, src_wfmt, n, k, group, sc0, None)
     elif src_wfmt in (W_INT4_TILED, W_FP8_TILED, W_MXFP4_TILED):
         per16 = tiled_bytes(src_wfmt, 16, k)
@@ -314,8 +315,10 @@ def pack_tiled(src_wfmt: int, w: torch.Tensor, k: int, dst_wfmt: int, *, sc0: Op
         raise ValueError(f"a {n_total}x{k} weight cannot be tiled as format {dst_wfmt}")
     if out is None:
         out = torch.zeros(nbytes, device=w.device, dtype=torch.uint8)
-    elif out.numel() * out.element_size() != nbytes or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous buffer of {nbytes} bytes")
+    else:
+        _require_gpu("out", out, w.device)
+        if out.numel() * out.element_size() != nbytes or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous buffer of {nbytes} bytes")
     _lib.check(
         _lib.lib().bz_pack_tiled(src_wfmt, w.data_ptr(), _ptr(sc0), n, k, group, dst_wfmt, out.data_ptr(), n_total,
                                  row0, _lib.stream_of(w)),
@@ -521,6 +524,9 @@ def quantize_fp8_device(weight: torch.Tensor, amax_floor: float):
 def dequant(wfmt: int, w: torch.Tensor, n: int, k: int, *, sc0=None, sc1=None, group: int = 128) -> torch.Tensor:
     """w_eff float32 [n, k] decoded by the GPU path's own unpacking code."""
     _require_gpu("w", w, w.device)
+    for name, t in (("sc0", sc0), ("sc1", sc1)):
+        if t is not None:
+            _require_gpu(name, t, w.device)
     _check_weight(w, wfmt, n, k, group, sc0, sc1)
     out = torch.empty(n, k, device=w.device, dtype=torch.float32)
     _lib.check(

@@ -7,6 +7,9 @@ import subprocess
 from pathlib import Path
 
 import pytest
+import torch
+
+from breeze_amd import gemv as G
 
 CSRC = Path(__file__).resolve().parents[1] / "breeze-tts-2_amd" / "csrc"
 
@@ -48,3 +51,29 @@ def test_row_runs_cover_every_row_once(tmp_path):
         rc, end, runs = map(int, line.split())
         per = min(m, 2 ** 31 // (k // 8))
         assert rc == 0 and end == m and runs == -(-m // per), (m, k, line)
+
+
+# ---- buffers of another device ------------------------------------------------------------------------
+
+
+def test_scales_and_outputs_of_another_device_are_refused(monkeypatch):
+    """A kernel would read or write their host addresses.  The meta device stands for the GPU."""
+    def require(name, t, device):
+        if t.device != device:
+            raise RuntimeError(f"{name} is on {t.device}, expected {device}")
+
+    def zeros(*shape, device="meta", dtype=torch.uint8):
+        return torch.zeros(*shape, device=device, dtype=dtype)
+
+    monkeypatch.setattr(G, "_require_gpu", require)
+    w, sc, tiled = zeros(16, 64), zeros(16, 4), G.tiled_bytes(G.W_MXFP4_TILED, 16, 128)
+    for name, call in (
+            ("sc0", lambda: G.pack_tiled(G.W_MXFP4, w, 128, G.W_MXFP4_TILED, sc0=sc.new_zeros(16, 4, device="cpu"))),
+            ("out", lambda: G.pack_tiled(G.W_MXFP4, w, 128, G.W_MXFP4_TILED, sc0=sc, out=zeros(tiled, device="cpu"))),
+            ("out", lambda: G.pack_tiled(G.W_MXFP4_TILED, zeros(tiled), 128, G.W_MXFP4_TILED, n_total=32,
+                                         out=zeros(2 * tiled, device="cpu"))),
+            ("sc0", lambda: G.dequant(G.W_MXFP4, w, 16, 128, sc0=zeros(16, 4, device="cpu"))),
+            ("sc1", lambda: G.dequant(G.W_INT4_MIN, w, 16, 128, sc0=zeros(16, dtype=torch.bfloat16),
+                                      sc1=zeros(16, device="cpu", dtype=torch.bfloat16)))):
+        with pytest.raises(RuntimeError, match=f"{name} is on cpu"):
+            call()
