@@ -282,6 +282,8 @@ def _check_weight(w, wfmt, n, k, group, sc0, sc1) -> None:
 
 def tiled_bytes(wfmt: int, n: int, k: int) -> int:
     """Bytes of a tiled weight (bz_tiled_bytes); 0 when the shape cannot be tiled."""
+    if not (0 < n < 1 << 31 and 0 < k < 1 << 31):  # (ctypes would cut them to 32 bits)
+        return 0
     return int(_lib.lib().bz_tiled_bytes(wfmt, n, k))
 
 

@@ -81,6 +81,12 @@ def _call(index: int, f, *args) -> None:
         raise _lib.BzError(rc, f.__name__)
 
 
+def _counted(M: int, K: int) -> None:
+    """The library counts rows and columns in 32 bits (ctypes would cut them to that)."""
+    if M >= 1 << 31 or K >= 1 << 31:
+        raise ValueError(f"{M} rows of {K} columns: both have to be below 2^31")
+
+
 def _rows(x: torch.Tensor, unit: int) -> tuple:
     """(x with rows the kernels can read, M, K, row stride, type code, device
     index)."""
@@ -94,6 +100,7 @@ def _rows(x: torch.Tensor, unit: int) -> tuple:
     M, K = shape
     if K < 1 or K % unit:
         raise ValueError(f"{K} columns are not a positive multiple of {unit}")
+    _counted(M, K)
     ld, inner = x.stride()
     if M <= 1:
         ld = K
@@ -146,6 +153,7 @@ def dequantize_mx(codes: torch.Tensor, scales: torch.Tensor, elem: str = "e2m1",
         K *= 2
     if K < 1 or K % BLOCK or scales.shape != (M, K // BLOCK):
         raise ValueError(f"codes {list(shape)} and scales {list(scales.shape)} are not those of {elem} rows")
+    _counted(M, K)
     if not codes.is_contiguous() or codes.data_ptr() % 4:
         codes = codes.clone(memory_format=torch.contiguous_format)
     if not scales.is_contiguous():
@@ -199,7 +207,7 @@ def _plan(elem: int, M: int, n: int, k: int, cfg: int, rows: bool) -> tuple[int,
     """(bytes of the weight, whether one launch over bf16 rows takes the shape,
     workspace bytes)."""
     lib = _lib.lib()
-    weight = int(lib.bz_tiled_bytes(W_MXFP4_TILED, n, k)) or -1
+    weight = 0 < n < 1 << 31 and int(lib.bz_tiled_bytes(W_MXFP4_TILED, n, k)) or -1
     if rows and 0 < M <= FEW_ROWS:
         need = int(lib.bz_mx_gemv_workspace(elem, M, n, k, cfg))
         if need != _NO_WAY or cfg:  # (a forced shape it does not take is refused by the call)

@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from breeze_amd import gemv as G
+from breeze_amd import mx
 
 CSRC = Path(__file__).resolve().parents[1] / "breeze-tts-2_amd" / "csrc"
 
@@ -77,3 +78,33 @@ def test_scales_and_outputs_of_another_device_are_refused(monkeypatch):
                                       sc1=zeros(16, device="cpu", dtype=torch.bfloat16)))):
         with pytest.raises(RuntimeError, match=f"{name} is on cpu"):
             call()
+
+
+# ---- sizes past 32 bits -------------------------------------------------------------------------------
+
+
+def test_sizes_past_32_bits_are_refused(monkeypatch):
+    """ctypes cuts an int to 32 bits: a row of 2^32 + 128 columns was taken for one of 128.  The meta device stands
+    for the GPU."""
+    def meta(*shape, dtype=torch.bfloat16):
+        return torch.empty(*shape, device="meta", dtype=dtype)
+
+    launched = []
+    monkeypatch.setattr(mx, "_gpu", lambda *a: None)
+    monkeypatch.setattr(mx, "_call", lambda *a: launched.append(a))
+    u8 = torch.uint8
+    w = meta(1280, dtype=u8)
+    for m, k in ((1, 2 ** 32 + 128), (1, 2 ** 31), (2 ** 32 + 1, 128)):
+        for call in (lambda: mx.quantize_mx(meta(m, k)), lambda: mx.mx_rows(meta(m, k)),
+                     lambda: mx.mx_linear(meta(m, k), w, 16),
+                     lambda: mx.dequantize_mx(meta(m, k // 2, dtype=u8), meta(m, k // 32, dtype=u8))):
+            with pytest.raises(ValueError, match="2\\^31"):
+                call()
+    for n in (2 ** 32 + 16, 16 - 2 ** 32):
+        with pytest.raises(ValueError, match="W_MXFP4_TILED"):
+            mx.mx_linear(meta(1, 128), w, n)
+        for fmt, size in ((G.W_MXFP4_TILED, 1280), (G.W_INT4_TILED, 1152), (G.W_FP8_TILED, 2176)):
+            assert G.tiled_bytes(fmt, 16, 128) == size and G.tiled_bytes(fmt, n, 128) == G.tiled_bytes(fmt, 16, n) == 0
+            with pytest.raises(ValueError, match="cannot be tiled"):
+                G._check_weight(torch.zeros(size, dtype=u8), fmt, n, 128, 128, None, None)
+    assert not launched
