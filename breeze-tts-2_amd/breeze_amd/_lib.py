@@ -13,6 +13,7 @@ import ctypes
 import importlib.util
 import struct
 import os
+import threading
 from pathlib import Path
 
 import torch  # noqa: F401  (must precede loading the HIP library)
@@ -321,6 +322,9 @@ def capture_of(stream: int):
     return cid.value if active.value else None
 
 
+_WORKSPACE_LOCK = threading.RLock()
+
+
 def stream_workspace(table: dict, key: tuple, nbytes: int, device: torch.device, stream: int,
                      retired: list) -> torch.Tensor:
     """A zero-filled int32 buffer of at least ``nbytes`` owned by
@@ -338,10 +342,18 @@ def stream_workspace(table: dict, key: tuple, nbytes: int, device: torch.device,
     cap = capture_of(stream)
     full = key + (stream, cap)
     buf = table.get(full)
-    if buf is None or buf.numel() * 4 < nbytes:
-        n = max(nbytes, 2 * (buf.numel() * 4 if buf is not None else 0), 1 << 20)
-        if buf is not None:
-            retired.append(buf)
-        buf = torch.zeros(-(-n // 4), dtype=torch.int32, device=device)
-        table[full] = buf
+    if buf is not None and buf.numel() * 4 >= nbytes:
+        return buf
+    # one thread at a time: the allocation releases the interpreter lock, and of
+    # two threads' buffers the one that the table forgets would be freed while
+    # its thread is about to launch on it.  (Re-entrant: the allocation may
+    # run a finaliser that calls here; what it stores is retired.)
+    with _WORKSPACE_LOCK:
+        buf = table.get(full)
+        if buf is None or buf.numel() * 4 < nbytes:
+            n = max(nbytes, 2 * (buf.numel() * 4 if buf is not None else 0), 1 << 20)
+            buf = torch.zeros(-(-n // 4), dtype=torch.int32, device=device)
+            if full in table:
+                retired.append(table[full])
+            table[full] = buf
     return buf

@@ -4,11 +4,13 @@ from __future__ import annotations
 
 import shutil
 import subprocess
+import threading
 from pathlib import Path
 
 import pytest
 import torch
 
+from breeze_amd import _lib as L
 from breeze_amd import gemv as G
 from breeze_amd import mx
 
@@ -108,3 +110,54 @@ def test_sizes_past_32_bits_are_refused(monkeypatch):
             with pytest.raises(ValueError, match="cannot be tiled"):
                 G._check_weight(torch.zeros(size, dtype=u8), fmt, n, 128, 128, None, None)
     assert not launched
+
+
+# ---- workspaces of host threads -------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("held", [False, True])
+def test_threads_that_need_a_workspace_at_once(monkeypatch, held):
+    """No buffer that a thread was given is dropped while the other allocates: the thread is about to launch on it."""
+    zeros, inside = torch.zeros, threading.Barrier(2)
+
+    def slow(*args, **kw):  # the other thread gets as far as its own allocation, where nothing keeps it from that
+        try:
+            inside.wait(0.5)
+        except threading.BrokenBarrierError:
+            pass
+        return zeros(*args, **kw)
+
+    table, retired, given = {}, [], []
+    monkeypatch.setattr(L, "capture_of", lambda stream: None)
+    args = (torch.device("cpu"), 7, retired)
+    if held:
+        given.append(L.stream_workspace(table, ("key",), 100, *args).data_ptr())
+    monkeypatch.setattr(torch, "zeros", slow)
+
+    def work(nbytes):
+        buf = L.stream_workspace(table, ("key",), nbytes, *args)
+        assert buf.numel() * 4 >= nbytes
+        given.append(buf.data_ptr())
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in (3 << 20, (3 << 20) + 4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    kept = {b.data_ptr() for b in [*table.values(), *retired]}
+    assert len(table) == 1 and len(given) == 2 + held and set(given) <= kept
+
+
+def test_a_workspace_asked_for_inside_an_allocation(monkeypatch):
+    """A finaliser that runs in the allocation and asks for the same workspace: its buffer stays alive too."""
+    zeros, table, retired, given = torch.zeros, {}, [], []
+    monkeypatch.setattr(L, "capture_of", lambda stream: None)
+
+    def nested(*args, **kw):
+        monkeypatch.setattr(torch, "zeros", zeros)
+        given.append(L.stream_workspace(table, ("key",), 100, torch.device("cpu"), 7, retired).data_ptr())
+        return zeros(*args, **kw)
+
+    monkeypatch.setattr(torch, "zeros", nested)
+    given.append(L.stream_workspace(table, ("key",), 2 << 20, torch.device("cpu"), 7, retired).data_ptr())
+    assert [b.data_ptr() for b in retired] + [table["key", 7, None].data_ptr()] == given
