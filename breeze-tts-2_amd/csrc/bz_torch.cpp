@@ -142,7 +142,6 @@ PyObject* gemv(PyObject*, PyObject* const* a, Py_ssize_t count) {
         d.residual = r->data_ptr();
         d.ldr = r->stride(0);
     }
-    if (need && !workspace(a[2], *x, need, d.workspace, d.workspace_bytes)) return nullptr;
     d.abi_version = BZ_ABI_VERSION;
     d.M = (int32_t)M;
     d.N = (int32_t)n;
@@ -161,6 +160,9 @@ PyObject* gemv(PyObject*, PyObject* const* a, Py_ssize_t count) {
     d.ldx = ld;
     d.w = w->data_ptr();
     d.ldo = n_out;
+    // (last: it runs Python, where another thread may replace the table that
+    // plan and cfg are borrowed from)
+    if (need && !workspace(a[2], *x, need, d.workspace, d.workspace_bytes)) return nullptr;
     at::Tensor out;
     int rc;
     {
