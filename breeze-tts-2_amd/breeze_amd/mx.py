@@ -24,7 +24,8 @@ times such a weight, with nothing quantised on the way, are ``gemv.gemv`` and
 
 Calls follow torch's current stream of the tensors' device, do not synchronise,
 and may be captured into graphs and made from several streams at once.  None of
-them has a gradient.
+them has a gradient: rows, a residual or an ``out`` that autograd follows,
+backward or forward, are refused.
 """
 
 from __future__ import annotations
@@ -33,6 +34,7 @@ import functools
 from typing import Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import DT_BF16, DT_F32, MX_E2M1, MX_E4M3, MX_F16, MX_ROWS, MX_TILED, W_MXFP4_TILED
@@ -64,9 +66,17 @@ def _gpu(name: str, t: torch.Tensor, index: int) -> None:
         raise RuntimeError(f"{name} is on {t.device}, expected cuda:{index}")
 
 
-def _no_grad(x: torch.Tensor, what: str) -> None:
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on x.detach()")
+def followed(t: torch.Tensor) -> bool:
+    """Whether autograd follows t, backward or forward."""
+    if t.requires_grad and torch.is_grad_enabled():
+        return True
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
+def _no_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    for t in tensors:
+        if t is not None and followed(t):
+            raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on x.detach()")
 
 
 def _call(index: int, f, *args) -> None:
@@ -118,6 +128,7 @@ def quantize_mx(x: torch.Tensor, elem: str = "e2m1") -> tuple[torch.Tensor, torc
         if held is not None:
             return held
     code = _elem(elem)
+    _no_grad("quantize_mx", x)
     x, M, K, ld, dt, index = _rows(x, BLOCK)
     if code == MX_E2M1:
         codes = torch.empty((M, K // 2), dtype=torch.uint8, device=x.device)
@@ -183,7 +194,7 @@ def mx_rows(x: torch.Tensor, elem: str = "e2m1") -> MxRows:
     for mx_linear: once for all products that read the same rows."""
     code = _elem(elem)
     x, M, K, ld, dt, index = _rows(x, 128)
-    _no_grad(x, "mx_rows")
+    _no_grad("mx_rows", x)
     return MxRows(_tiled_rows(x, M, K, ld, dt, code, index), (M, K), elem)
 
 
@@ -239,9 +250,10 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
     else:
         code = _elem(elem)
         src, M, K, ld, dt, index = _rows(x, 128)
-        _no_grad(x, "mx_linear")
+        _no_grad("mx_linear", x)
         # up to 32 rows that a launch can read as they are: quantised inside it
         few = dt == DT_BF16 and M <= FEW_ROWS and not (ld & 7 or src.data_ptr() & 15) and M * ld < 1 << 30
+    _no_grad("mx_linear", residual, out)
     weight, few, need = _plan(code, M, n, K, cfg, few)
     if not cfg and not rows and few == (0 < M <= FEW_ROWS):  # (not the two launches of few rows that need a copy)
         _PLANS[code, M, n, K] = weight, few, need, 0 if few else _rows_bytes(code, M, K)

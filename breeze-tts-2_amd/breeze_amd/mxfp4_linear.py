@@ -56,6 +56,7 @@ def quantize_mxfp4(weight: torch.Tensor) -> torch.Tensor:
     """weight [N, K] (bf16, fp16 or fp32) -> weight_mxfp4, on the device the weight lives on
     (a CPU weight is quantized on the current GPU and the result moved back)."""
     n, k = weight.shape
+    weight = weight.detach()  # (a parameter is quantized as it is)
     w = weight if weight.device.type == "cuda" else weight.to(torch.device("cuda", torch.cuda.current_device()))
     if w.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         w = w.float()

@@ -55,6 +55,11 @@ int elem(PyObject* o) {
     return PyUnicode_CompareWithASCIIString(o, "e4m3") == 0 ? BZ_MX_E4M3 : -1;
 }
 
+// Whether autograd follows t, backward or forward.
+bool followed(const at::Tensor& t) {
+    return (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined();
+}
+
 // A non-negative int, else -1.
 int64_t number(PyObject* o) {
     if (!PyLong_Check(o)) return -1;
@@ -181,7 +186,7 @@ PyObject* quantize_mx(PyObject*, PyObject* const* a, Py_ssize_t count) {
     HANDLE_TH_ERRORS
     const at::Tensor* x = count == 2 ? gpu(a[0]) : nullptr;
     const int el = x ? elem(a[1]) : -1;
-    if (el < 0 || x->dim() != 2) Py_RETURN_NONE;
+    if (el < 0 || x->dim() != 2 || followed(*x)) Py_RETURN_NONE;
     const int dt = x_dtype(*x);
     const int64_t M = x->size(0), K = x->size(1), ld = M == 1 ? K : x->stride(0);
     if (dt < 0 || M < 1 || K < 1 || K % 32 || M > INT32_MAX || K > INT32_MAX || x->stride(1) != 1 || ld < K)
@@ -241,7 +246,7 @@ PyObject* mx_linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const at::Tensor *x = gpu(a[2]), *w = gpu(a[3]);
     const int64_t n = number(a[4]);
     const int el = elem(a[5]), odt = dtype_of(a[7]);
-    if (!x || !w || n < 1 || el < 0 || odt < 0 || x->dim() != 2 || (x->requires_grad() && c10::GradMode::is_enabled()))
+    if (!x || !w || n < 1 || el < 0 || odt < 0 || x->dim() != 2 || followed(*x))
         Py_RETURN_NONE;
     const int dt = x_dtype(*x);
     const int64_t M = x->size(0), K = x->size(1), ld = M == 1 ? K : x->stride(0);
@@ -263,7 +268,7 @@ PyObject* mx_linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (a[6] != Py_None) {
         rdt = r ? dtype_of(r->scalar_type()) : -1;
         if (rdt < 0 || r->dim() != 2 || r->size(0) != M || r->size(1) != n || r->stride(1) != 1 ||
-            (M > 1 && r->stride(0) < n))
+            (M > 1 && r->stride(0) < n) || followed(*r))
             Py_RETURN_NONE;
     }
     const void* res = r ? r->data_ptr() : nullptr;

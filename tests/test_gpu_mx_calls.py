@@ -6,8 +6,10 @@ import pytest
 import torch
 
 from breeze_amd import gemv as G
+from breeze_amd import mx
+from breeze_amd import mxfp4_linear as M4
 from breeze_amd import tuning
-from tests.test_gpu_mx import BF16, Weight, _close, _gemv_reference, _rows
+from tests.test_gpu_mx import BF16, ELEMS, Weight, _close, _gemv_reference, _rows
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +38,41 @@ def test_a_table_replaced_while_the_workspace_is_made(monkeypatch):
     assert torch.equal(G.gemv(x, w.tiled, w.fmt, n), want) and len(calls) == 1
     monkeypatch.undo()
     assert torch.equal(G.gemv(x, w.tiled, w.fmt, n), want)
+
+
+# ---- what autograd follows ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("m", [2, 40])
+def test_what_autograd_follows_is_refused(elem, m):
+    """Rows, residuals and outputs, followed backward or forward, the first time and after a planned call."""
+    n, k = 64, 256
+    w, x, res = Weight(n, k), _rows(m, k, 2), _rows(m, n, 3)
+    want, codes = mx.mx_linear(x, w.tiled, n, elem=elem, residual=res), mx.quantize_mx(x, elem)[0]
+    for _ in range(2):
+        p, r, o = x.clone().requires_grad_(), res.clone().requires_grad_(), res.clone().requires_grad_()
+        calls = [lambda: mx.quantize_mx(p, elem), lambda: mx.mx_rows(p, elem), lambda: mx.mx_linear(p, w.tiled, n, elem=elem),
+                 lambda: mx.mx_linear(x, w.tiled, n, elem=elem, residual=r),
+                 lambda: mx.mx_linear(mx.mx_rows(x, elem), w.tiled, n, residual=r),
+                 lambda: mx.mx_linear(x, w.tiled, n, elem=elem, residual=res, out=o)]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+        with torch.no_grad():
+            for call in calls:
+                call()
+            assert torch.equal(mx.mx_linear(p, w.tiled, n, elem=elem, residual=r), want) and torch.equal(o, want)
+        assert torch.equal(mx.quantize_mx(p.detach(), elem)[0].view(torch.uint8), codes.view(torch.uint8))
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual
+            p, r = dual(x, torch.ones_like(x)), dual(res, torch.ones_like(res))
+            for call in calls[:-1]:
+                with pytest.raises(RuntimeError, match="no gradient"):
+                    call()
+            assert torch.equal(mx.mx_linear(x, w.tiled, n, elem=elem, residual=res), want)
+
+
+def test_a_parameter_is_quantized_as_it_is():
+    p = torch.nn.Parameter(_rows(48, 256, 4))
+    assert torch.equal(M4.quantize_mxfp4(p), M4.quantize_mxfp4(p.data))

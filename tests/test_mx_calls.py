@@ -161,3 +161,23 @@ def test_a_workspace_asked_for_inside_an_allocation(monkeypatch):
     monkeypatch.setattr(torch, "zeros", nested)
     given.append(L.stream_workspace(table, ("key",), 2 << 20, torch.device("cpu"), 7, retired).data_ptr())
     assert [b.data_ptr() for b in retired] + [table["key", 7, None].data_ptr()] == given
+
+
+# ---- what autograd follows ------------------------------------------------------------------------------
+
+
+def test_what_autograd_follows():
+    x = torch.ones(2, 64)
+    assert not mx.followed(x)
+    p = x.clone().requires_grad_()
+    assert mx.followed(p) and mx.followed(2 * p) and not mx.followed(p.detach())
+    with torch.no_grad():
+        assert not mx.followed(p)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, x)
+        assert mx.followed(dual) and mx.followed(2 * dual) and not mx.followed(x)
+        with torch.no_grad():
+            assert mx.followed(dual)  # (no_grad is about the backward pass)
+        for f in (mx.quantize_mx, mx.mx_rows):
+            with pytest.raises(RuntimeError, match="no gradient|GPU tensor"):
+                f(dual)
