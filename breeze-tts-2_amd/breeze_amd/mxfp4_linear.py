@@ -26,7 +26,7 @@ from torch import nn
 
 from ._swap import swap_linears
 from .gemv import W_MXFP4, W_MXFP4_TILED, dequant_matmul, gemv_traceable, pack_tiled, tiled_bytes
-from .mx import BLOCK, mx_linear, quantize_mx
+from .mx import BLOCK, followed, mx_linear, quantize_mx
 
 MIN_QUANT_BYTES = 8 * 1024 * 1024
 
@@ -92,9 +92,9 @@ class Mxfp4Linear(nn.Module):
         if k_pad != k:
             flat = torch.nn.functional.pad(flat, (0, k_pad - k))
         # a traced call is a GEMV of any row count, as for the other modules; one
-        # that autograd follows goes the way of the prompts, which it can follow
-        grad = flat.requires_grad and torch.is_grad_enabled()
-        if torch.compiler.is_compiling() or (flat.shape[0] <= PREFILL_ROWS and not grad):
+        # that autograd follows, backward or forward, goes the way of the prompts,
+        # which it can follow
+        if torch.compiler.is_compiling() or (flat.shape[0] <= PREFILL_ROWS and not followed(flat)):
             out = gemv_traceable(flat, w, W_MXFP4_TILED, n_pad)
         elif self.act_bits == 16:
             out = dequant_matmul(flat, w, W_MXFP4_TILED, n_pad, k_pad)

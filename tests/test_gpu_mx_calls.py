@@ -2,14 +2,18 @@
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
+from torch import nn
+
+from oracle import bz_mx_oracle as O
 
 from breeze_amd import gemv as G
 from breeze_amd import mx
 from breeze_amd import mxfp4_linear as M4
 from breeze_amd import tuning
-from tests.test_gpu_mx import BF16, ELEMS, Weight, _close, _gemv_reference, _rows
+from tests.test_gpu_mx import BF16, ELEMS, Weight, _close, _gemv_reference, _np, _rows
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +80,23 @@ def test_what_autograd_follows_is_refused(elem, m):
 def test_a_parameter_is_quantized_as_it_is():
     p = torch.nn.Parameter(_rows(48, 256, 4))
     assert torch.equal(M4.quantize_mxfp4(p), M4.quantize_mxfp4(p.data))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 32, 40])
+@pytest.mark.parametrize("n,k", [(48, 256), (50, 200)])
+def test_module_keeps_forward_tangents(rows, n, k):
+    lin = nn.Linear(k, n, bias=False).cuda()
+    x, t = torch.randn(rows, k, device="cuda"), torch.randn(rows, k, device="cuda").to(BF16)
+    wq = O.rounded(np.pad(_np(lin.weight), ((0, 0), (0, -k % 32))), O.E2M1)[:, :k]
+    ref = _np(t) @ wq.T
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, t.float())
+        out = M4.Mxfp4Linear(lin)(dual)
+        value, tangent = torch.autograd.forward_ad.unpack_dual(out)
+        # the tangent of a bf16 product, rounded once to bf16
+        _close(tangent, ref, 2.0 ** -8 * np.abs(ref) + k * 2.0 ** -24 * (np.abs(_np(t)) @ np.abs(wq).T))
+        for bits in (4, 8):
+            mod = M4.Mxfp4Linear(lin, act_bits=bits)
+            with pytest.raises(RuntimeError, match="no gradient"):
+                mod(dual)
+            assert mod(x).shape == (rows, n)
