@@ -25,7 +25,7 @@ import torch
 from torch import nn
 
 from ._swap import swap_linears
-from .gemv import W_MXFP4, W_MXFP4_TILED, dequant_matmul, gemv_traceable, pack_tiled, tiled_bytes
+from .gemv import W_MXFP4, W_MXFP4_TILED, dequant_matmul, gemv, pack_tiled, tiled_bytes
 from .mx import BLOCK, followed, mx_linear, quantize_mx
 
 MIN_QUANT_BYTES = 8 * 1024 * 1024
@@ -68,6 +68,29 @@ def quantize_mxfp4(weight: torch.Tensor) -> torch.Tensor:
     return tiled if weight.device.type == "cuda" else tiled.to(weight.device)
 
 
+def _product(x: torch.Tensor, w: torch.Tensor, n: int, act_bits: int) -> torch.Tensor:
+    """x [M, K] bf16 times a weight of n rows, in the way of its row count; a call
+    that autograd follows, backward or forward, goes the way of the prompts,
+    which it can follow."""
+    if x.shape[0] <= PREFILL_ROWS and not followed(x):
+        return gemv(x, w, W_MXFP4_TILED, n)
+    if act_bits == 16:
+        return dequant_matmul(x, w, W_MXFP4_TILED, n, x.shape[1])
+    return mx_linear(x, w, n, elem=_ACT_ELEM[act_bits])
+
+
+@torch.library.custom_op("breeze_amd::mxfp4_linear", mutates_args=())
+def mxfp4_linear_op(x: torch.Tensor, w: torch.Tensor, n: int, act_bits: int) -> torch.Tensor:
+    """_product where torch.compile traces: the row count decides when the call
+    runs, so a compiled prompt multiplies what an eager one does."""
+    return _product(x, w, n, act_bits)
+
+
+@mxfp4_linear_op.register_fake
+def _mxfp4_linear_fake(x, w, n, act_bits):
+    return x.new_empty((x.shape[0], n), dtype=torch.bfloat16)
+
+
 class Mxfp4Linear(nn.Module):
     """Drop-in replacement for a bias-free nn.Linear using microscaled 4-bit weights."""
 
@@ -91,15 +114,10 @@ class Mxfp4Linear(nn.Module):
             flat = flat.to(torch.bfloat16)
         if k_pad != k:
             flat = torch.nn.functional.pad(flat, (0, k_pad - k))
-        # a traced call is a GEMV of any row count, as for the other modules; one
-        # that autograd follows, backward or forward, goes the way of the prompts,
-        # which it can follow
-        if torch.compiler.is_compiling() or (flat.shape[0] <= PREFILL_ROWS and not followed(flat)):
-            out = gemv_traceable(flat, w, W_MXFP4_TILED, n_pad)
-        elif self.act_bits == 16:
-            out = dequant_matmul(flat, w, W_MXFP4_TILED, n_pad, k_pad)
+        if torch.compiler.is_compiling():
+            out = torch.ops.breeze_amd.mxfp4_linear(flat, w, n_pad, self.act_bits)
         else:
-            out = mx_linear(flat, w, n_pad, elem=_ACT_ELEM[self.act_bits])
+            out = _product(flat, w, n_pad, self.act_bits)
         if n_pad != n:
             out = out[:, :n].contiguous()
         if x.dtype != torch.bfloat16:

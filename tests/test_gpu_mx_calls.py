@@ -100,3 +100,26 @@ def test_module_keeps_forward_tangents(rows, n, k):
             with pytest.raises(RuntimeError, match="no gradient"):
                 mod(dual)
             assert mod(x).shape == (rows, n)
+
+
+@pytest.mark.parametrize("act_bits", [16, 8, 4])
+@pytest.mark.parametrize("n,k", [(64, 256), (50, 200)])
+def test_a_compiled_module_multiplies_what_an_eager_one_does(act_bits, n, k):
+    """Row counts on either side of a prompt's, one compilation for all of them."""
+    mod = M4.Mxfp4Linear(nn.Linear(k, n, bias=False).cuda(), act_bits=act_bits)
+    torch._dynamo.reset()
+    compiled = torch.compile(mod, fullgraph=True, backend="eager", dynamic=True)
+    with torch.no_grad():
+        for rows in (5, 32, 33, 70, 200, 2):
+            x = _rows(rows, k, rows)
+            assert torch.equal(compiled(x), mod(x)), rows
+        x = _rows(60, k, 7).view(3, 20, k)
+        assert torch.equal(compiled(x), mod(x))
+    torch._dynamo.reset()
+
+
+def test_the_traced_modules_operator():
+    mod = M4.Mxfp4Linear(nn.Linear(256, 48, bias=False).cuda(), act_bits=8)
+    for rows in (4, 40):
+        torch.library.opcheck(M4.mxfp4_linear_op, (_rows(rows, 256, 5), mod.weight_mxfp4, 48, 8),
+                              test_utils=("test_schema", "test_faketensor"))

@@ -13,6 +13,7 @@ import torch
 from breeze_amd import _lib as L
 from breeze_amd import gemv as G
 from breeze_amd import mx
+from breeze_amd import mxfp4_linear as M4  # noqa: F401  (registers its operator)
 
 CSRC = Path(__file__).resolve().parents[1] / "breeze-tts-2_amd" / "csrc"
 
@@ -181,3 +182,12 @@ def test_what_autograd_follows():
         for f in (mx.quantize_mx, mx.mx_rows):
             with pytest.raises(RuntimeError, match="no gradient|GPU tensor"):
                 f(dual)
+
+
+# ---- traced calls ---------------------------------------------------------------------------------------
+
+
+def test_the_traced_modules_operator_has_a_shape():
+    x = torch.empty(77, 256, device="meta", dtype=torch.bfloat16)
+    out = torch.ops.breeze_amd.mxfp4_linear(x, torch.empty(3, 2304, device="meta", dtype=torch.uint8), 48, 8)
+    assert out.shape == (77, 48) and out.dtype == torch.bfloat16
