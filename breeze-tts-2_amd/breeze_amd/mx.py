@@ -209,7 +209,11 @@ def _tiled_rows(x, M: int, K: int, ld: int, dt: int, code: int, index: int) -> t
 # each graph capture under way.
 _WS: dict = {}
 _WS_RETIRED: list = []
-_PLANS: dict = {}  # (element type, M, n, K) -> _plan's answer and the bytes of the quantised rows, for the binding
+# (element type, M, n, K) -> _plan's answer and the bytes of the quantised rows, for
+# the binding.  Forgotten when there are too many: a server that sees prompts of
+# every length adds one for each of them and each weight.
+_PLANS: dict = {}
+_MOST_PLANS = 4096
 _NO_WAY = (1 << 64) - 1  # what bz_mx_gemv_workspace gives for a shape it does not take
 
 
@@ -255,8 +259,6 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
         few = dt == DT_BF16 and M <= FEW_ROWS and not (ld & 7 or src.data_ptr() & 15) and M * ld < 1 << 30
     _no_grad("mx_linear", residual, out)
     weight, few, need = _plan(code, M, n, K, cfg, few)
-    if not cfg and not rows and few == (0 < M <= FEW_ROWS):  # (not the two launches of few rows that need a copy)
-        _PLANS[code, M, n, K] = weight, few, need, 0 if few else _rows_bytes(code, M, K)
     if w.get_device() != index or w.numel() * w.element_size() != weight or not w.is_contiguous() or w.data_ptr() & 15:
         _gpu("w", w, index)
         raise ValueError(f"w must be a contiguous W_MXFP4_TILED weight of {n} x {K} (rows a multiple of 16), "
@@ -292,6 +294,10 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
             ldr = n
     if M == 0:
         return out
+    if not cfg and not rows and few == (M <= FEW_ROWS):  # (not the two launches of few rows that need a copy)
+        if len(_PLANS) >= _MOST_PLANS:
+            _PLANS.clear()
+        _PLANS[code, M, n, K] = weight, few, need, 0 if few else _rows_bytes(code, M, K)
     lib, ws = _lib.lib(), 0
     if not (few or rows):
         src = _tiled_rows(src, M, K, ld, dt, code, index)

@@ -123,3 +123,31 @@ def test_the_traced_modules_operator():
     for rows in (4, 40):
         torch.library.opcheck(M4.mxfp4_linear_op, (_rows(rows, 256, 5), mod.weight_mxfp4, 48, 8),
                               test_utils=("test_schema", "test_faketensor"))
+
+
+# ---- plans that calls leave behind --------------------------------------------------------------------
+
+
+def test_plans_are_few_and_of_calls_that_were_made(monkeypatch):
+    n, k = 64, 256
+    w = Weight(n, k)
+    monkeypatch.setattr(mx, "_PLANS", {})
+    for m in (2, 40):
+        x = _rows(m, k, m)
+        for kw in ({"residual": x}, {"out_dtype": torch.float16}, {"out": x[:, :n]}, {"cfg": 1 | 2 << 8}):
+            try:
+                mx.mx_linear(x, w.tiled, n, **kw)
+            except (ValueError, TypeError):
+                pass
+        with pytest.raises(ValueError):
+            mx.mx_linear(x, w.tiled[:-16], n)
+        assert mx.mx_linear(x[:0], w.tiled, n).shape == (0, n)
+    assert not mx._PLANS
+    monkeypatch.setattr(mx, "_MOST_PLANS", 20)
+    base = _rows(150, k, 9)
+    want = mx.mx_linear(base, w.tiled, n)
+    for _ in range(2):
+        for m in range(1, 151):
+            out = mx.mx_linear(base[:m], w.tiled, n)
+            assert len(mx._PLANS) <= 20 and torch.equal(mx.mx_linear(base[:m], w.tiled, n), out)
+    assert torch.equal(out, want)
