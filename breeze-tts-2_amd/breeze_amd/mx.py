@@ -43,8 +43,13 @@ __all__ = ["BLOCK", "MxRows", "quantize_mx", "dequantize_mx", "mx_rows", "mx_lin
 
 BLOCK = 32
 
-# Up to this many rows mx_linear is one launch over the rows themselves.
+# Up to this many rows mx_linear is one launch over the rows themselves; not for
+# more than 16 rows over a weight of more than ONE_ROUND rows, which takes a second
+# round of workgroups of eight row blocks, each quantising x (N40960 K2560 M = 17 e2m1
+# 22.6 us, two launches 18.6; N151936 72.3 and 48.7 for 32; N28672 K4096 17.4 and 21.9 for
+# 17, 19.7 and 19.7 for 32; N32768 K2560 13.9 and 16.3, 15.7 and 15.3).
 FEW_ROWS = 32
+ONE_ROUND = 32768
 
 _ELEM = {"e2m1": MX_E2M1, "e4m3": MX_E4M3}
 _X = {torch.bfloat16: DT_BF16, torch.float32: DT_F32, torch.float16: MX_F16}
@@ -223,7 +228,7 @@ def _plan(elem: int, M: int, n: int, k: int, cfg: int, rows: bool) -> tuple[int,
     workspace bytes)."""
     lib = _lib.lib()
     weight = 0 < n < 1 << 31 and int(lib.bz_tiled_bytes(W_MXFP4_TILED, n, k)) or -1
-    if rows and 0 < M <= FEW_ROWS:
+    if rows and 0 < M <= FEW_ROWS and (M <= 16 or n <= ONE_ROUND or cfg):
         need = int(lib.bz_mx_gemv_workspace(elem, M, n, k, cfg))
         if need != _NO_WAY or cfg:  # (a forced shape it does not take is refused by the call)
             return weight, True, 0 if need == _NO_WAY else need
@@ -258,6 +263,7 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
         # up to 32 rows that a launch can read as they are: quantised inside it
         few = dt == DT_BF16 and M <= FEW_ROWS and not (ld & 7 or src.data_ptr() & 15) and M * ld < 1 << 30
     _no_grad("mx_linear", residual, out)
+    fits = few
     weight, few, need = _plan(code, M, n, K, cfg, few)
     if w.get_device() != index or w.numel() * w.element_size() != weight or not w.is_contiguous() or w.data_ptr() & 15:
         _gpu("w", w, index)
@@ -294,7 +300,7 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
             ldr = n
     if M == 0:
         return out
-    if not cfg and not rows and few == (M <= FEW_ROWS):  # (not the two launches of few rows that need a copy)
+    if not cfg and not rows and fits == (M <= FEW_ROWS):  # (not the two launches of few rows that need a copy)
         if len(_PLANS) >= _MOST_PLANS:
             _PLANS.clear()
         _PLANS[code, M, n, K] = weight, few, need, 0 if few else _rows_bytes(code, M, K)

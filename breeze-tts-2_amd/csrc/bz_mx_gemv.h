@@ -62,6 +62,7 @@ constexpr int kMxGemvRows = 32;
 constexpr int kMxGemvBlocks = 8;                        // most row blocks of a workgroup
 constexpr int kMxGemvUpw[] = {1, 2, 3, 4, 5, 6, 8};  // units per wave
 __host__ __device__ constexpr int mx_gemv_lds(int NW, int T, int MT) { return NW * T * MT * 1024 + 16; }
+constexpr int kMxGemvMostLds = 160 * 1024;
 // Units of a wave that share one operand of x: rows 16 / G and more of it belong
 // to the next unit.
 constexpr int mx_gemv_share(int M, int upw) { return M <= 4 && upw >= 3 ? 4 : M <= 8 && upw >= 2 ? 2 : 1; }

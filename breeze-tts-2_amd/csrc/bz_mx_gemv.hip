@@ -28,6 +28,11 @@ struct MxGemvPlan {
 // 8.97) and for up to 4 over one or two blocks (N1024 K2048 M = 1 3.42, 3.54;
 // N10240 K2560 M = 4, three blocks, 5.97, 5.92); 1 for more than 16 rows in slices
 // (e4m3 N10240 K2560: 2 slices of 5 11.0, one of 3 11.6).
+// More than 16 rows keep up to 16 KiB of sums a wave, which may not fit LDS:
+// then fewer slices, so fewer blocks a workgroup (N4096 K10240 M = 17: 4 slices
+// of 4 blocks 11.4, 6 of 6 with two units a wave 16.2, quantising in a launch of
+// its own 15.4; N8192 K5120 M = 32 12.8, 18.6, 13.6), and over one slice more units
+// a wave (N20480 K4096 M = 17 3 units 14.0, 2 units over 4 blocks 16.6).
 static int mx_gemv_plan(int elem, int M, int N, int K, int cfg, MxGemvPlan& pl) {
     const int NU = K / 128, nblk = N / 16, mt = M > 16 ? 2 : 1;
     const int cT = cfg & 255, cu = (cfg >> 8) & 255, cs = cfg >> 16;
@@ -41,33 +46,50 @@ static int mx_gemv_plan(int elem, int M, int N, int K, int cfg, MxGemvPlan& pl) 
                         : std::max(4, (NU + 19) / 20);
     if (!cs && blocks(nsl) > kMxGemvBlocks) nsl = 1;
     nsl = std::min(nsl, NU);
-    const int T = std::min(kMxGemvBlocks, blocks(nsl));
-    const int groups = (nblk + T - 1) / T;
-    int upw = 0;
-    for (;; ++nsl) {  // more slices where the waves do not hold the row
-        if (nsl > 64 || (nsl > 1 && (groups > kMxCounters || (int64_t)nsl * M * N * 4 >= (int64_t)1 << 31)))
-            return BZ_ERR_UNSUPPORTED;
-        pl.ups = (NU + nsl - 1) / nsl;
-        const bool four = M <= 8 && (pl.ups >= 32 || (nsl == 1 && M <= 4 && T <= 2 && NU >= 16));
-        const int least = pl.ups == 1 || (nsl > 1 && mt == 2) ? 1 : four ? 4 : 2;
+    auto most = [&](int slices) { return std::min(kMxGemvBlocks, blocks(slices)); };
+    bool over = false;  // the waves hold some shape that LDS or the workspace does not
+    // The fewest units per wave with which the waves of workgroups of t blocks
+    // hold a slice, or, where their sums do not fit LDS and `more`, the fewest
+    // with which they do; 0: none.
+    auto units = [&](int slices, int t, bool more) {
+        const int ups = (NU + slices - 1) / slices;
+        const bool four = M <= 8 && (ups >= 32 || (slices == 1 && M <= 4 && t <= 2 && NU >= 16));
+        const int least = ups == 1 || (slices > 1 && mt == 2) ? 1 : four ? 4 : 2;
+        const bool counted = slices == 1 || ((nblk + t - 1) / t <= kMxCounters && (int64_t)slices * M * N * 4 < (int64_t)1 << 31);
         for (int u : kMxGemvUpw) {
             const int share = mx_gemv_share(M, u);
-            if (!upw && mx_gemv_built(mt, u, share) && (cu ? u == cu : u >= least) &&
-                mx_gemv_waves(elem, mt, u, share) * u >= pl.ups)
-                upw = u;
+            if (!mx_gemv_built(mt, u, share) || (cu ? u != cu : u < least) || mx_gemv_waves(elem, mt, u, share) * u < ups)
+                continue;
+            if (counted && mx_gemv_lds((ups + u - 1) / u, t, mt) <= kMxGemvMostLds) return u;
+            over = true;
+            if (!more) break;
         }
+        return 0;
+    };
+    const int T0 = most(nsl);
+    int s = nsl, T = T0, upw = units(s, T, s == 1 || cs);
+    if (!cs)
+        while (!upw && over && s > 1) {
+            --s;
+            T = most(s);
+            upw = units(s, T, s == 1);
+        }
+    if (!upw) s = nsl;
+    while (!upw) {  // more slices where the waves do not hold the row, fewer blocks where their sums never fit
+        for (T = T0; !(upw = units(s, T, true)) && T > 1 && !cT;) --T;
         if (upw) break;
-        if (cu || cs) return BZ_ERR_INVALID_ARG;
+        if (cu || cs) return over ? BZ_ERR_UNSUPPORTED : BZ_ERR_INVALID_ARG;
+        if (++s > 64) return BZ_ERR_UNSUPPORTED;
     }
+    pl.ups = (NU + s - 1) / s;
     pl.nsl = (NU + pl.ups - 1) / pl.ups;
     pl.l.upw = upw;
     pl.l.share = mx_gemv_share(M, upw);
     pl.l.nw = (pl.ups + upw - 1) / upw;
     pl.T = T;
     pl.l.mt = mt;
-    pl.l.grid = (unsigned)(groups * pl.nsl);
+    pl.l.grid = (unsigned)((nblk + T - 1) / T * pl.nsl);
     pl.l.lds = (size_t)mx_gemv_lds(pl.l.nw, T, mt);
-    if (pl.l.lds > 160 * 1024) return BZ_ERR_UNSUPPORTED;
     pl.ws = pl.nsl > 1 ? kMxPartOffset + (size_t)pl.nsl * M * N * 4 : 0;
     return BZ_OK;
 }

@@ -84,7 +84,9 @@ int bz_mx_gemm(int32_t elem, const void* xq, int32_t M, const void* w, int32_t N
  * x [M][ldx] bf16, 16-byte aligned rows (ldx % 8 == 0).  The result is that of
  * bz_mx_quantize and bz_mx_gemm up to the order of its fp32 sums.  Workspace
  * as for bz_mx_gemm; bz_mx_gemv_workspace is (size_t)-1 where the call is
- * refused (K above 2^22 or too long for 64 K slices).  cfg = 0 takes the built-in launch
+ * refused: K above 2^22 or too long for 64 K slices, slices of more than 4096
+ * workgroups' columns or whose sums reach 2^31 bytes, a forced shape that is
+ * not built or whose sums do not fit LDS.  cfg = 0 takes the built-in launch
  * shape, else row blocks per workgroup (1 .. 8) | units of 128 columns per
  * wave (1 .. 6, 8) << 8 | K slices << 16 (a part left 0 keeps the rule's
  * choice). */

@@ -9,11 +9,12 @@ from torch import nn
 
 from oracle import bz_mx_oracle as O
 
+from breeze_amd import _lib as L
 from breeze_amd import gemv as G
 from breeze_amd import mx
 from breeze_amd import mxfp4_linear as M4
 from breeze_amd import tuning
-from tests.test_gpu_mx import BF16, ELEMS, Weight, _close, _gemv_reference, _np, _rows
+from tests.test_gpu_mx import BF16, ELEMS, Weight, _close, _gemv_reference, _mx_reference, _np, _rows
 
 pytestmark = pytest.mark.gpu
 
@@ -151,3 +152,25 @@ def test_plans_are_few_and_of_calls_that_were_made(monkeypatch):
             out = mx.mx_linear(base[:m], w.tiled, n)
             assert len(mx._PLANS) <= 20 and torch.equal(mx.mx_linear(base[:m], w.tiled, n), out)
     assert torch.equal(out, want)
+
+
+# ---- few rows in one launch -------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n,k", [(4096, 10240), (8192, 5120), (14336, 4096), (20480, 4096), (32768, 2560), (32784, 128),
+                                 (2624, 16384)])
+def test_few_rows_whose_sums_would_not_fit(n, k):
+    w = Weight(n, k)
+    for m in (17, 32):
+        x, res = _rows(m, k, m), _rows(m, n, 6)
+        for elem in ELEMS:
+            ref, bound = _mx_reference(x, w, elem, res, BF16)
+            for cfg in (0, 4, 3 << 16):
+                if elem == O.E4M3 and k == 16384 and cfg == 3 << 16:  # 8 waves hold 40 units, a slice has 43
+                    with pytest.raises(L.BzError):
+                        mx.mx_linear(x, w.tiled, n, elem=elem, residual=res, cfg=cfg)
+                    continue
+                out = mx.mx_linear(x, w.tiled, n, elem=elem, residual=res, cfg=cfg)
+                _close(out, ref, bound)
+                assert torch.equal(mx.mx_linear(x, w.tiled, n, elem=elem, residual=res, cfg=cfg), out)
+            assert mx._PLANS[mx._ELEM[elem], m, n, k][1] == (n <= mx.ONE_ROUND)

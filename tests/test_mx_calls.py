@@ -191,3 +191,23 @@ def test_the_traced_modules_operator_has_a_shape():
     x = torch.empty(77, 256, device="meta", dtype=torch.bfloat16)
     out = torch.ops.breeze_amd.mxfp4_linear(x, torch.empty(3, 2304, device="meta", dtype=torch.uint8), 48, 8)
     assert out.shape == (77, 48) and out.dtype == torch.bfloat16
+
+
+# ---- few rows in one launch -------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("elem", [L.MX_E2M1, L.MX_E4M3])
+def test_the_built_in_shape_of_few_rows_fits(elem):
+    """17 .. 32 rows: the rule's shape did not fit LDS at about one in eight sizes, and the call was refused."""
+    need = L.lib().bz_mx_gemv_workspace
+    for m in (1, 5, 8, 9, 16, 17, 25, 32):
+        for n, k in ((4096, 10240), (3584, 10240), (8192, 5120), (14336, 4096), (20480, 4096), (32768, 2560),
+                     (151936, 2560), (576, 65536)):
+            assert need(elem, m, n, k, 0) < 1 << 31, (m, n, k)
+        for n in [*range(16, 20481, 1040), 32768]:
+            for k in range(128, 10241, 640):
+                assert need(elem, m, n, k, 0) < 1 << 31, (m, n, k)
+        assert need(elem, m, 64, (1 << 22) + 128, 0) == (1 << 64) - 1
+    for cfg in (8 | 1 << 8 | 1 << 16, 8 | 2 << 8 | 1 << 16):  # 16 waves over eight blocks of 32 rows: 256 KiB of sums
+        assert need(elem, 32, 512, 2048 * (cfg >> 8 & 255), cfg) == (1 << 64) - 1
+    assert need(elem, 32, 512, 2048, 8 | 1 << 16) == 0  # (the rule's units, more of them)
