@@ -330,8 +330,18 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether a and b may share memory; matrices of one row stride are compared
+    column range by column range, as views of one wider tensor have them."""
     (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
+    if not (a0 < b1 and b0 < a1):
+        return False
+    if a.dim() != 2 or b.dim() != 2 or a.stride(1) != 1 or b.stride(1) != 1:
+        return True
+    step, wide_a, wide_b = (a.stride(0) * a.element_size(), a.shape[1] * a.element_size(), b.shape[1] * b.element_size())
+    if b.stride(0) * b.element_size() != step or max(wide_a, wide_b) > step:
+        return True
+    at = (b0 - a0) % step  # of b's rows, from the last start of one of a's
+    return at < wide_a or at + wide_b > step
 
 
 def _same(a: torch.Tensor, b: torch.Tensor) -> bool:

@@ -174,3 +174,22 @@ def test_few_rows_whose_sums_would_not_fit(n, k):
                 _close(out, ref, bound)
                 assert torch.equal(mx.mx_linear(x, w.tiled, n, elem=elem, residual=res, cfg=cfg), out)
             assert mx._PLANS[mx._ELEM[elem], m, n, k][1] == (n <= mx.ONE_ROUND)
+
+
+@pytest.mark.parametrize("elem", ELEMS)
+@pytest.mark.parametrize("m", [1, 3, 40])
+def test_rows_residual_and_output_in_one_buffer(elem, m):
+    """Column ranges of one tensor that share no element."""
+    n, k = 144, 256
+    w = Weight(n, k)
+    buf = torch.randn(m, n + k + n + 8).to(BF16).cuda()
+    out, x, res = buf[:, :n], buf[:, n:n + k], buf[:, n + k:n + k + n]
+    before = buf.clone()
+    ref, bound = _mx_reference(x, w, elem, res, BF16)
+    mx.mx_linear(x, w.tiled, n, elem=elem, residual=res, out=out)
+    _close(out, ref, bound)
+    before[:, :n] = out
+    assert torch.equal(buf, before)
+    for wrong in (buf[:, 1:n + 1], buf[:, n + k - 1:n + k - 1 + n]):
+        with pytest.raises(ValueError, match="overlap"):
+            mx.mx_linear(x, w.tiled, n, elem=elem, out=wrong)

@@ -211,3 +211,24 @@ def test_the_built_in_shape_of_few_rows_fits(elem):
     for cfg in (8 | 1 << 8 | 1 << 16, 8 | 2 << 8 | 1 << 16):  # 16 waves over eight blocks of 32 rows: 256 KiB of sums
         assert need(elem, 32, 512, 2048 * (cfg >> 8 & 255), cfg) == (1 << 64) - 1
     assert need(elem, 32, 512, 2048, 8 | 1 << 16) == 0  # (the rule's units, more of them)
+
+
+# ---- views that share memory ------------------------------------------------------------------------------
+
+
+def test_views_overlap_where_they_share_an_element():
+    buf = torch.zeros(6, 20)
+    marks = torch.arange(120).view(6, 20)
+    views = [lambda t: t[:, :8], lambda t: t[:, 8:], lambda t: t[:, 7:12], lambda t: t[:, 12:], lambda t: t[1:4, 2:9],
+             lambda t: t[4:, :8], lambda t: t[:1, 3:15], lambda t: t.view(-1)[15:115].view(5, 20)[:, :8],
+             lambda t: t.view(-1)[15:115].view(5, 20)[:, 9:], lambda t: t[:, 2:9:2], lambda t: t.t()[:, 1:3],
+             lambda t: t[::2, :8], lambda t: t[1::2, :8], lambda t: t.view(-1), lambda t: t[2:2]]
+    for f in views:
+        for g in views:
+            share = bool(set(f(marks).flatten().tolist()) & set(g(marks).flatten().tolist()))
+            said = mx._overlap(f(buf), g(buf))
+            rows = all(v.dim() == 2 and v.stride(1) == 1 and v.stride(0) == 20 for v in (f(buf), g(buf)))
+            assert said >= share and (not rows or said == share), (f(marks), g(marks))
+    half = torch.zeros(6, 40, dtype=torch.bfloat16)
+    assert not mx._overlap(half[:, :32], half.view(torch.float32)[:, 16:])
+    assert mx._overlap(half[:, :33], half.view(torch.float32)[:, 16:])
