@@ -50,8 +50,10 @@ HIP_FLAGS = [
 # kernel.  Attention over bf16 caches with D <= 256 (attn_bf16) is covered;
 # attn_kernel (fp32 caches, D = 512) is allowed scratch.
 NO_SCRATCH = (r"gemv_persist", r"gemv_mfma", r"gemv_i8mma", r"gemv_tile", r"gemv_stream", r"gemv_wide", r"gemv_panel",
-              r"gemm_tiled|mx_gemm|mx_gemv|mx_quantize|mx_dequantize", r"gemv_rows", r"gemv_slab",
+              r"gemm_tiled", r"gemv_rows", r"gemv_slab",
               r"head_f32", r"sample_cfg", r"step_tables", r"qkv_rope_cache", r"attn_bf16")
+# The same of the kernels over microscaled blocks.
+NO_SCRATCH_MX = (r"mx_gemm", r"mx_gemv", r"mx_quantize_rows", r"mx_quantize_tiled", r"mx_dequantize_rows")
 
 
 def kernel_resources(remarks: str) -> list[tuple[str, int, int]]:
@@ -73,13 +75,13 @@ def kernel_resources(remarks: str) -> list[tuple[str, int, int]]:
     return out
 
 
-def check_scratch(kernels: list[tuple[str, int, int]]) -> None:
-    """RuntimeError for a decode kernel that uses scratch memory, and for a
-    pattern that matches no kernel (a renamed or removed one)."""
-    spilled = [name for name, _, sc in kernels if sc and any(re.search(t, name) for t in NO_SCRATCH)]
+def check_scratch(kernels: list[tuple[str, int, int]], patterns: tuple[str, ...] = NO_SCRATCH) -> None:
+    """RuntimeError for a kernel of ``patterns`` that uses scratch memory, and for
+    a pattern that matches no kernel (a renamed or removed one)."""
+    spilled = [name for name, _, sc in kernels if sc and any(re.search(t, name) for t in patterns)]
     if spilled:
         raise RuntimeError("decode kernels using scratch memory:\n  " + "\n  ".join(spilled))
-    unused = [t for t in NO_SCRATCH if not any(re.search(t, name) for name, _, _ in kernels)]
+    unused = [t for t in patterns if not any(re.search(t, name) for name, _, _ in kernels)]
     if unused:
         raise RuntimeError("no compiled kernel matches: " + ", ".join(unused))
 
@@ -146,7 +148,7 @@ def build(verbose: bool = False) -> Path:
     kernels = sorted({k for _, ks in done for k in ks})
     (obj_dir / "kernel_resources.txt").write_text(
         "".join(f"{vg:4d} vgpr {sc:6d} scratch  {name}\n" for name, vg, sc in kernels))
-    check_scratch(kernels)
+    check_scratch(kernels, NO_SCRATCH + NO_SCRATCH_MX)
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
     if verbose:

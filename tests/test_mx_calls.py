@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from breeze_amd import _lib as L
+from breeze_amd import build as B
 from breeze_amd import gemv as G
 from breeze_amd import mx
 from breeze_amd import mxfp4_linear as M4  # noqa: F401  (registers its operator)
@@ -232,3 +233,23 @@ def test_views_overlap_where_they_share_an_element():
     half = torch.zeros(6, 40, dtype=torch.bfloat16)
     assert not mx._overlap(half[:, :32], half.view(torch.float32)[:, 16:])
     assert mx._overlap(half[:, :33], half.view(torch.float32)[:, 16:])
+
+
+# ---- the build's scratch guard ------------------------------------------------------------------------------
+
+
+def test_the_scratch_guard_names_each_kernel():
+    """One pattern a kernel: an alternative of several would pass while any one of them is compiled."""
+    assert not [p for p in B.NO_SCRATCH + B.NO_SCRATCH_MX if "|" in p]
+    kernels = [(f"_ZN2bz{len(p)}{p}ILi0EEEv", 64, 0) for p in B.NO_SCRATCH_MX]
+    assert {p for p in B.NO_SCRATCH_MX} == {"mx_gemm", "mx_gemv", "mx_quantize_rows", "mx_quantize_tiled", "mx_dequantize_rows"}
+    B.check_scratch(kernels, B.NO_SCRATCH_MX)
+    for i, (name, vgpr, _) in enumerate(kernels):
+        with pytest.raises(RuntimeError, match="no compiled kernel"):
+            B.check_scratch(kernels[:i] + kernels[i + 1:], B.NO_SCRATCH_MX)
+        with pytest.raises(RuntimeError, match="scratch"):
+            B.check_scratch(kernels[:i] + [(name, vgpr, 16)] + kernels[i + 1:], B.NO_SCRATCH_MX)
+    built = B.PKG_DIR / "_build" / "kernel_resources.txt"
+    if built.exists():  # (the names of the last build)
+        names = [(line.split()[-1], 0, 0) for line in built.read_text().splitlines()]
+        B.check_scratch(names, B.NO_SCRATCH + B.NO_SCRATCH_MX)
