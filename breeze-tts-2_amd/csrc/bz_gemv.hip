@@ -257,7 +257,7 @@ static int stream_plan(const bz_gemv_desc* d, int rows, StreamLaunch& l) {
     l.upw = upw;
     l.mm = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
     l.grid = (unsigned)(d->N / 16);
-    l.lds = (size_t)stream_lds(wf, rows, d->K, nw).total;
+    l.lds = (size_t)stream_lds(wf, rows, d->K, nw, upw).total;
     return l.lds <= (size_t)device_lds_limit() ? BZ_OK : BZ_ERR_UNSUPPORTED;
 }
 
@@ -321,7 +321,7 @@ static int wide_plan(const bz_gemv_desc* d, int rows, int T, WideLaunch& l) {
     l.mm = mm;
     l.T = T;
     l.grid = (unsigned)((nblk + T - 1) / T);
-    l.lds = (size_t)wide_lds(wf, rows, d->K, T).total;
+    l.lds = (size_t)wide_lds(wf, rows, d->K, T, nw * upw).total;
     return l.lds <= (size_t)device_lds_limit() ? BZ_OK : BZ_ERR_UNSUPPORTED;
 }
 

@@ -125,17 +125,24 @@ struct StreamParams {
 };
 
 // LDS carve-up (bytes), shared with the host launcher: x rows as bf16 (row
-// stride 2K + 16 bytes), the int4 per-unit sums X [row][unit], the sums of x^2
-// of each wave's four 16-lane rows [wave][row][4] and the partial dot
+// stride stream_x_row_bytes), the int4 per-unit sums X [row][unit], the sums of
+// x^2 of each wave's four 16-lane rows [wave][row][4] and the partial dot
 // products [row][column][wave].
 struct StreamLds {
     int xs, xst, sq, red, total;
 };
-__host__ __device__ inline int stream_x_row_bytes(int K) { return 2 * K + 16; }
-__host__ __device__ inline StreamLds stream_lds(int wf, int M, int K, int NW) {
+// Bytes from one x row to the next.  Where the last wave has units past the
+// row (units = waves x units per wave > NU), fp8 and MXFP4 rows end with a unit
+// of zeros that these multiply: the row's last unit, as int4 takes it, may
+// hold an infinity, which a weight of zero turns into a NaN.  (int4's sums
+// with zero points are NaN for such a row anyway.)
+__host__ __device__ inline int stream_x_row_bytes(int wf, int K, int units) {
+    return 2 * K + 16 + (!tiled_i4(wf) && units * tiled_unit_k(wf) > K ? 256 : 0);
+}
+__host__ __device__ inline StreamLds stream_lds(int wf, int M, int K, int NW, int UPW) {
     StreamLds L;
     L.xs = 0;
-    L.xst = align16(M * stream_x_row_bytes(K));
+    L.xst = align16(M * stream_x_row_bytes(wf, K, NW * UPW));
     L.sq = L.xst + align16(tiled_i4(wf) ? M * (K / 128) * 4 : 0);
     L.red = L.sq + align16(NW * M * 16);
     L.total = L.red + align16(M * 16 * 16 * 4);  // 16 wave slots
@@ -201,12 +208,12 @@ __global__ void __launch_bounds__(1024) gemv_stream(const uint8_t* hw, const uin
     const int b = blockIdx.x;
     const uint8_t* chunk = p.w + (int64_t)b * p.chunk;
 
-    const StreamLds L = stream_lds(WF, M, K, NW);
+    const StreamLds L = stream_lds(WF, M, K, NW, UPW);
     uint8_t* xs = smem + L.xs;
     float* xst = reinterpret_cast<float*>(smem + L.xst);
     float* sq = reinterpret_cast<float*>(smem + L.sq);
     float* red = reinterpret_cast<float*>(smem + L.red);
-    const int xrow = stream_x_row_bytes(K);
+    const int xrow = stream_x_row_bytes(WF, K, NW * UPW);
 
     // this wave's units [u0, u0 + nu) and blocks of x [kb0, kb0 + nkb)
     const int u0 = wave * UPW;
@@ -359,21 +366,24 @@ __global__ void __launch_bounds__(1024) gemv_stream(const uint8_t* hw, const uin
             if (j == 0 && m < M) sq[(wave * M + m) * 4 + kq] = t;
         }
     }
+    if (!I4 && nu < UPW && lane < 16) {  // the unit of zeros behind each row
+        for (int m = 0; m < M; ++m) *reinterpret_cast<u32x4*>(xs + m * xrow + 2 * K + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+    }
     // the wave reads back only what it wrote: LDS operations of one wave
     // complete in order, so no workgroup barrier is needed here
     __builtin_amdgcn_wave_barrier();
 
     // 2. the wave's units: consume tile q, issue tile q + D, without run-time
     //    conditions, so each wait counts exactly the loads in flight.  A unit
-    //    past the block reads x and X at the block's last unit, which the
-    //    same wave staged (every wave owns at least one unit), so it
-    //    multiplies finite values by its zero weights.
+    //    past the block multiplies its zero weights by the zeros behind the
+    //    row (fp8, MXFP4) or by x and X of the block's last unit (int4), which
+    //    the same wave staged (every wave owns at least one unit).
     float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     f32x4_t facc = {0.0f, 0.0f, 0.0f, 0.0f};
     const uint8_t* xa = xs + min(j, M - 1) * xrow;  // the x row this lane supplies to A
     const NibbleConsts nc;
     auto consume = [&](int q, bool next) {
-        const int u = min(u0 + q, NU - 1);
+        const int u = min(u0 + q, I4 ? NU - 1 : NU);
         if (I4) {
             u32x4 bq[4];
 #pragma unroll

@@ -38,16 +38,16 @@
 
 namespace bz {
 
-// LDS carve-up (bytes): x rows as bf16 (row stride 2K + 16), the int4
-// per-unit sums X [row][unit], each wave's sum of x^2 per row [row][16 wave
+// LDS carve-up (bytes): x rows as bf16 (row stride stream_x_row_bytes), the
+// int4 per-unit sums X [row][unit], each wave's sum of x^2 per row [row][16 wave
 // slots] and the partial dot products [block][row][column][16 wave slots].
 struct WideLds {
     int xs, xst, sq, red, total;
 };
-__host__ __device__ inline WideLds wide_lds(int wf, int M, int K, int T) {
+__host__ __device__ inline WideLds wide_lds(int wf, int M, int K, int T, int units) {
     WideLds L;
     L.xs = 0;
-    L.xst = align16(M * stream_x_row_bytes(K));
+    L.xst = align16(M * stream_x_row_bytes(wf, K, units));
     L.sq = L.xst + align16(tiled_i4(wf) ? M * (K / 128) * 4 : 0);
     L.red = L.sq + align16(M * 16 * 4);
     L.total = L.red + align16(T * M * 16 * 16 * 4);
@@ -86,12 +86,12 @@ __global__ void __launch_bounds__(1024) gemv_wide(const uint8_t* hw, const uint1
     const int nb = TC > 0 ? TC : min(T, nblk - b0);
     const int ocols = PAIR ? 8 : 16;
 
-    const WideLds L = wide_lds(WF, M, K, T);
+    const WideLds L = wide_lds(WF, M, K, T, NW * UPW);
     uint8_t* xs = smem + L.xs;
     float* xst = reinterpret_cast<float*>(smem + L.xst);
     float* sq = reinterpret_cast<float*>(smem + L.sq);
     float* red = reinterpret_cast<float*>(smem + L.red);
-    const int xrow = stream_x_row_bytes(K);
+    const int xrow = stream_x_row_bytes(WF, K, NW * UPW);
 
     const int u0 = wave * UPW;
     const int nu = max(0, min(UPW, NU - u0));
@@ -232,14 +232,16 @@ __global__ void __launch_bounds__(1024) gemv_wide(const uint8_t* hw, const uint1
             }
         }
     }
+    if (!I4 && nu < UPW && lane < 16) {  // the unit of zeros behind each row
+        for (int m = 0; m < M; ++m) *reinterpret_cast<u32x4*>(xs + m * xrow + 2 * K + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+    }
     // the wave reads back only what it wrote (LDS operations of one wave
     // complete in order): no workgroup barrier here
     __builtin_amdgcn_wave_barrier();
 
     // 2. the blocks in order; slot q's tile is unpacked, refilled with unit q
-    //    of the next block, then multiplied.  A unit past the row reads x and
-    //    X at the row's last unit (staged by this wave) and multiplies them by
-    //    zero weights.
+    //    of the next block, then multiplied.  A unit past the row multiplies
+    //    zero weights, as in the one-block kernel.
     const uint8_t* xa = xs + min(j, M - 1) * xrow;  // the x row this lane supplies to A
     const NibbleConsts nc;
     // block jb from set (cw, cs); slot q refilled with unit q of block jb + 1
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(1024) gemv_wide(const uint8_t* hw, const uint1
         f32x4_t facc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int q = 0; q < UPW; ++q) {
-            const int u = min(u0 + q, NU - 1);
+            const int u = min(u0 + q, I4 ? NU - 1 : NU);
             if (I4) {
                 u32x4 bq[4];
 #pragma unroll

@@ -193,3 +193,69 @@ def test_rows_residual_and_output_in_one_buffer(elem, m):
     for wrong in (buf[:, 1:n + 1], buf[:, n + k - 1:n + k - 1 + n]):
         with pytest.raises(ValueError, match="overlap"):
             mx.mx_linear(x, w.tiled, n, elem=elem, out=wrong)
+
+
+# ---- scale codes at the ends, rows with infinities ----------------------------------------------------------
+
+
+def _product(x, w):
+    """bf16 rows times the weight, by the call of their number."""
+    if x.shape[0] <= 32:
+        return G.gemv(x, w.tiled, w.fmt, w.n, out_dtype=torch.float32)
+    return G.dequant_matmul(x, w.tiled, w.fmt, w.n, w.k)
+
+
+MS = [1, 2, 5, 9, 17, 40]
+
+
+@pytest.mark.parametrize("m", MS)
+@pytest.mark.parametrize("n,k", [(48, 640), (272, 1280), (4112, 512), (64, 8192)])
+def test_bf16_rows_with_nan_and_infinity(m, n, k):
+    """An infinity times a weight of zero is a NaN, times another one of that one's sign; rows are independent."""
+    w, x = Weight(n, k), _rows(m, k, 11)
+    clean = _product(x, w)
+    for r in sorted({0, m // 2, m - 1}):
+        for bad in (float("inf"), -float("inf"), float("nan")):
+            for col in (0, k // 2 + 3, k - 1):
+                y = x.clone()
+                y[r, col] = bad
+                out = _product(y, w)
+                assert torch.equal(out[:r], clean[:r]) and torch.equal(out[r + 1:], clean[r + 1:])
+                weight = torch.from_numpy(w.values[:, col]).cuda()
+                want = bad * weight
+                assert torch.equal(out[r].isnan(), want.isnan()) and (out[r][~want.isnan()] == want[~want.isnan()]).all()
+
+
+@pytest.mark.parametrize("m", [1, 2, 5, 9])
+@pytest.mark.parametrize("epi", [G.EPI_NONE, G.EPI_SILU_GATE])
+def test_normed_rows_with_nan_and_infinity(m, epi):
+    n, k = 272, 640
+    w, x, gamma = Weight(n, k, paired=epi == G.EPI_SILU_GATE), _rows(m, k, 12), _rows(1, k, 13)[0].abs() + 1
+
+    def run(x):
+        return G.gemv(x, w.tiled, w.fmt, n, gamma=gamma, epilogue=epi)
+
+    clean = run(x)
+    for r in sorted({0, m - 1}):
+        for bad in (float("inf"), float("nan")):
+            y = x.clone()
+            y[r, 100] = bad
+            out = run(y)
+            assert out[r].isnan().all() and torch.equal(out[:r], clean[:r]) and torch.equal(out[r + 1:], clean[r + 1:])
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("n,k", [(48, 640), (272, 1280), (64, 2176), (4112, 192), (64, 4160), (2560, 1280)])
+def test_fp8_rows_with_infinity_in_the_last_unit(m, n, k):
+    """The waves' units past a row multiply their zero weights by zeros, not by its last columns."""
+    codes, scale = G.quantize_fp8_device(_rows(n, k, 14), 1e-12)
+    w = G.pack_tiled(G.W_FP8, codes.view(torch.uint8), k, G.W_FP8_TILED, sc0=scale)
+    values, x = G.dequant(G.W_FP8_TILED, w, n, k), _rows(m, k, 15)
+    clean = G.gemv(x, w, G.W_FP8_TILED, n)
+    for bad in (float("inf"), -float("inf")):
+        y = x.clone()
+        y[m - 1, k - 1] = bad
+        out = G.gemv(y, w, G.W_FP8_TILED, n)
+        want = bad * values[:, k - 1]
+        assert torch.equal(out[:m - 1], clean[:m - 1]) and torch.equal(out[m - 1].isnan(), want.isnan())
+        assert (out[m - 1][~want.isnan()] == want[~want.isnan()]).all()
