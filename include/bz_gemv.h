@@ -84,8 +84,9 @@ typedef enum bz_status {
  *   block (block g of row r at byte 256 g + 16 r), and the scales follow the
  *   tiles, per four units 256 bytes (unit u, block g, row r at byte 64 g +
  *   4 r + u % 4; the bytes of units past the last are zero).  Runs on
- *   paths 5 and 6; w_eff is exact in bf16, so the products equal those of the
- *   bf16 weight.
+ *   paths 5 and 6; w_eff is exact in bf16 (an infinity from 2^128 on, which
+ *   codes 253 and 254 reach; NaN for code 255), so the products equal those of
+ *   the bf16 weight.
  * The tiled formats run on GEMV path 5, the streaming kernel (M <= 8 rows
  * per launch; more rows run as several launches), and the unpaired ones also
  * on the several-row paths 4 (int4, fp8) and 6 (see below).  They need K %

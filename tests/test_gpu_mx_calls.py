@@ -205,7 +205,63 @@ def _product(x, w):
     return G.dequant_matmul(x, w.tiled, w.fmt, w.n, w.k)
 
 
+def _scaled(n, k, codes):
+    """A weight whose blocks take these scale codes in turn along a row."""
+    w = Weight(n, k)
+    w.scales[:] = np.resize(np.asarray(codes, np.uint8), w.scales.shape)
+    w.tiled = torch.from_numpy(O.tile(w.codes, w.scales, O.E2M1)).cuda()
+    w.values = O.values(w.codes, w.scales, O.E2M1)
+    return w
+
+
 MS = [1, 2, 5, 9, 17, 40]
+
+
+@pytest.mark.parametrize("m", MS)
+@pytest.mark.parametrize("n,k", [(48, 640), (272, 1280), (4112, 512)])
+def test_products_of_the_smallest_scales(m, n, k):
+    """Codes 0, 1 and 2: weights from 2^-128 up, some of them subnormal bf16, times rows about 2^100."""
+    w = _scaled(n, k, [0, 1, 0, 2])
+    x = (_rows(m, k, 8).float() * 2.0 ** 100).to(BF16)
+    out_dtype = torch.float32 if m <= 32 else BF16
+    _close(_product(x, w), *_gemv_reference(x, w, G.EPI_NONE, None, 0.0, None, out_dtype))
+    for elem in ELEMS:
+        _close(mx.mx_linear(x, w.tiled, n, elem=elem, out_dtype=torch.float32), *_mx_reference(x, w, elem, None, torch.float32))
+
+
+@pytest.mark.parametrize("m", MS)
+@pytest.mark.parametrize("n,k", [(48, 640), (272, 1280)])
+def test_products_of_the_largest_scales(m, n, k):
+    """Codes 252 to 254 times rows about 2^-110.  bf16 holds a weight below 2^128; a larger one is an infinity to the
+    products of bf16 rows, and itself to those of quantised rows, whose scales the matrix cores add."""
+    w = _scaled(n, k, [252, 254, 253, 254])
+    x = (_rows(m, k, 9).float().abs() * 2.0 ** -110 + 2.0 ** -112).to(BF16)
+    for elem in ELEMS:
+        _close(mx.mx_linear(x, w.tiled, n, elem=elem, out_dtype=torch.float32), *_mx_reference(x, w, elem, None, torch.float32))
+    got = _np(_product(x, w))
+    with np.errstate(invalid="ignore"):
+        want = _np(x) @ np.where(np.abs(w.values) < 2.0 ** 128, w.values, np.copysign(np.inf, w.values)).T
+    assert (np.isnan(got) == np.isnan(want)).all() and (got[np.isinf(want)] == want[np.isinf(want)]).all()
+    w.codes[:] = w.codes & 0xB  # elements up to 1.5
+    w.tiled = torch.from_numpy(O.tile(w.codes, w.scales, O.E2M1)).cuda()
+    w.values = O.values(w.codes, w.scales, O.E2M1)
+    _close(_product(x, w), *_gemv_reference(x, w, G.EPI_NONE, None, 0.0, None, torch.float32 if m <= 32 else BF16))
+
+
+@pytest.mark.parametrize("m", MS)
+@pytest.mark.parametrize("n,k", [(48, 640), (272, 1280), (4112, 512)])
+def test_products_of_blocks_that_are_nan(m, n, k):
+    """Code 255: the columns of the result whose weight row has such a block, and no others."""
+    w, x = Weight(n, k), _rows(m, k, 10)
+    clean = [_product(x, w)] + [mx.mx_linear(x, w.tiled, n, elem=e) for e in ELEMS]
+    bad = np.zeros(n, bool)
+    for row, block in ((0, 0), (5, k // 32 - 1), (n - 1, 7), (n // 2, 3)):
+        w.scales[row, block] = 255
+        bad[row] = True
+    w.tiled = torch.from_numpy(O.tile(w.codes, w.scales, O.E2M1)).cuda()
+    bad = torch.from_numpy(bad).cuda()
+    for out, was in zip([_product(x, w)] + [mx.mx_linear(x, w.tiled, n, elem=e) for e in ELEMS], clean):
+        assert out[:, bad].isnan().all() and torch.equal(out[:, ~bad], was[:, ~bad])
 
 
 @pytest.mark.parametrize("m", MS)
