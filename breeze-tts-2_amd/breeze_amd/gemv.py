@@ -130,7 +130,8 @@ def gemv(
 
     x [M, K] (any float dtype; computed as bf16), weight of format ``wfmt``
     with ``n`` rows, optional RMSNorm gamma [K], epilogue NONE / SILU_GATE
-    (N_out = n/2) / RESIDUAL (residual [M, N_out]).  Returns ``out``.
+    (N_out = n/2) / RESIDUAL (residual [M, N_out]).  Returns ``out``, which
+    autograd does not follow.
     """
     plain = cfg is _NO_CFG and out is None and out2 is None and sc0 is None and sc1 is None and \
         wfmt in TILED_FORMATS and (group == 128 or wfmt not in _INT4_TILED) and x.is_cuda

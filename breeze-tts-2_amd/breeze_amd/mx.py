@@ -240,11 +240,16 @@ def mx_linear(x: Union[torch.Tensor, MxRows], w: torch.Tensor, n: int, *, elem: 
               out_dtype: torch.dtype = torch.bfloat16, cfg: int = 0) -> torch.Tensor:
     """q(x) @ w_eff^T (+ residual) -> [M, n]: x [M, K] (bf16, fp16 or fp32), quantised to
     blocks of ``elem`` on the way, or the MxRows of it; w a W_MXFP4_TILED weight of n
-    rows and K columns.  Products are exact, sums fp32 (with e4m3 after a first sum
-    of eight products on the matrix core's grid, include/bz_mx.h); the result is
-    rounded once, to out's dtype (bf16 or fp32).  residual: [M, n] bf16 or fp32, may
-    be out itself; out: [M, n] with unit column stride, apart from x and w.  cfg: a
-    launch shape (include/bz_mx.h) instead of the built-in rule's."""
+    rows and K columns.  e2m1 products are exact and their sums fp32; e4m3's are
+    first added by eights on the matrix core's grid (include/bz_mx.h), which leaves
+    an fp32 result 2e-5 of its norm off, bf16's rounding being 1.7e-3.  The result
+    is rounded once, to out's dtype (bf16 or fp32).  residual: [M, n] bf16 or fp32,
+    may be out itself; out: [M, n] with unit column stride, apart from x and w.
+    cfg: a launch shape (include/bz_mx.h) instead of the built-in rule's.
+
+    Few rows are for a step that has to round its activations as the prompt
+    before it did; gemv.gemv over the same weight rounds none and takes less at one
+    or two (N2560 K10240 M = 2 5.3 us against 6.9, N1024 K2048 M = 1 2.7 and 3.4)."""
     rows = isinstance(x, MxRows)
     if not (rows or cfg) and out is None and x.is_cuda:  # nothing to convert: checked and made in C++
         y = (_lib._binding or _lib.binding()).mx_linear(_PLANS, _raw_workspace, x, w, n, elem, residual, out_dtype)

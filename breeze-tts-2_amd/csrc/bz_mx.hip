@@ -3,8 +3,9 @@
 // Both are one pass over memory and bound by it; a few rows by the launch.
 // Measured on MI355X (kernel trace, three tensors in turn; a copy of 1 GiB
 // reaches 5.2 TB/s): 10240 x 2560 fp32 to e2m1 21.3 us (5.6 TB/s), 2011 x 10240
-// bf16 to e4m3 11.8 us (5.3) and back 11.2 us (5.6), tiled 12.3 us (5.1); 2 x
-// 2560 1.5 us and back 1.6 us.
+// bf16 to e4m3 11.8 us (5.3) and back 11.2 us (5.6), tiled 12.3 us (5.1); 8192 x
+// 2560 bf16 to e2m1, tiled, 10.8 us by itself (4.9), 20 behind a product whose
+// 335 MB are still on their way to memory; 2 x 2560 1.5 us and back 1.6 us.
 #include <algorithm>
 
 #include "bz_mx.h"

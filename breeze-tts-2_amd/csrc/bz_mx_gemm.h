@@ -28,15 +28,17 @@
 //   * K slices where the tiles would leave CUs idle: fp32 sums to the
 //     workspace, added in slice order by the last workgroup to arrive.
 //
-// Bound by the LDS reads in the narrower tiles, by power in large products: the
-// card lowers its clock to 1.75 .. 1.9 GHz under the block-scaled instructions
-// (over zeros the same kernel keeps 2.38 GHz: e2m1 8192 cubed 184 us, 242 over
-// random values).  Two workgroups a CU of smaller tiles, wave priorities, waves
+// Bound by the LDS reads in the narrower tiles, by power and LDS reads in large
+// products: the card lowers its clock to 1.75 .. 1.9 GHz under the block-scaled
+// instructions (over zeros the same kernel keeps 2.38 GHz: e2m1 8192 cubed 184
+// us, 242 over random values).  The instruction alone, operands in registers,
+// reaches 7400 TFLOP/s over random e2m1 (9800 over zeros) and 4700 over e4m3 x
+// e2m1 (5000).  Two workgroups a CU of smaller tiles, wave priorities, waves
 // half a unit apart and deeper stages changed nothing there.
-// Measured on MI355X (graph replays): e2m1 8192 cubed 242 us (4550 TFLOP/s),
-// 8192 x 20480 x 2560 226 us (3800), 611 x 10240 x 2560 15.5 us (2070); e4m3 8192
-// cubed 369 us (2980), 2011 x 2560 x 10240 45.1 us (2340).  The card's large
-// bf16 matmul reaches 1269.
+// Measured on MI355X (graph replays; the ranges over cards and runs): e2m1 8192
+// cubed 242 us (4550 TFLOP/s), 8192 x 20480 x 2560 226 .. 235 us (3800 .. 3650),
+// 611 x 10240 x 2560 15.5 .. 15.8 us (2070); e4m3 8192 cubed 369 us (2980), 2011 x
+// 2560 x 10240 45.1 .. 46.8 us (2340).  The card's large bf16 matmul reaches 1269.
 #pragma once
 
 #include <type_traits>
