@@ -93,7 +93,7 @@ bool is_tiled(int64_t wfmt) {
            wfmt == BZ_W_MXFP4_TILED_PAIRED;
 }
 
-// The plan of a product that gemv._tiled_plan has put into the launch-shape
+// The plan of a product that gemv._plan_tiled has put into the launch-shape
 // table of the device: (output columns, bytes of the weight, launch shape,
 // workspace bytes).  Borrowed; null without an error where there is none.
 PyObject* plan_of(PyObject* tables, PyObject* archs, int64_t index, int64_t wfmt, int64_t n, int64_t k, int64_t epi,
